@@ -30,19 +30,6 @@
 
 namespace motif {
 
-// Keys and query start of a decode launch: from the host arguments, or from the
-// device cursor (clamped so the window stays inside the capacity).
-struct DecodeWindow { int S, q_start; };
-__device__ __forceinline__ DecodeWindow decode_window(const ChordArgs &a) {
-  if (!a.len_dev) return {min(a.S, a.q_start + a.L), a.q_start};
-  const int cached = min(max(__builtin_amdgcn_readfirstlane(*a.len_dev), 0), a.S - a.L);
-  return {cached + a.L, cached};
-}
-
-__device__ __forceinline__ float log_n_at(const ChordArgs &a, int b, int i, int q_start) {
-  return a.log_n ? a.log_n[b * a.ln_sb + int64_t(i) * a.ln_st] : a.log_tab[q_start + i];
-}
-
 constexpr int kD = 64;        // head dim
 constexpr int kBN = 64;       // keys per tile
 

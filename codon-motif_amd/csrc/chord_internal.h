@@ -28,7 +28,64 @@ struct ChordArgs {
   // merge pass advances *len_dev by L
   int *len_dev;
   const float *log_tab;  // ln(1 .. n) when log_n is NULL: log_n[b, i] = log_tab[q_start + i]
+  // sliding window (windowed kernels): a query at position p sees the keys j <= p with
+  // j > p - window or j < sinks
+  int window, sinks;
 };
+
+// Longest window and most first tokens a launch takes (positions stay below it as well), so that
+// no sum of two positions leaves 32 bits.
+constexpr int kMaxWindow = 1 << 29;
+
+// A 4-bit cache: for each (batch row, kv head) rows of D / 2 bytes (feature 2 m in the low half of
+// byte m) and rows of D / min(32, D) bf16 pairs (scale, base), value = code * scale + base.
+struct KV4Args {
+  const uint8_t *kc; int64_t kc_sb, kc_sh;  // strides in bytes
+  const uint32_t *kp; int64_t kp_sb, kp_sh;  // strides in pairs
+  const uint8_t *vc; int64_t vc_sb, vc_sh;
+  const uint32_t *vp; int64_t vp_sb, vp_sh;
+};
+inline KV4Args kv4_args(const void *kc, int64_t kc_sb, int64_t kc_sh, const void *kp, int64_t kp_sb, int64_t kp_sh,
+                        const void *vc, int64_t vc_sb, int64_t vc_sh, const void *vp, int64_t vp_sb, int64_t vp_sh) {
+  return {static_cast<const uint8_t *>(kc), kc_sb, kc_sh, static_cast<const uint32_t *>(kp), kp_sb, kp_sh,
+          static_cast<const uint8_t *>(vc), vc_sb, vc_sh, static_cast<const uint32_t *>(vp), vp_sb, vp_sh};
+}
+inline bool kv4_head_dim(int D) { return D == 16 || D == 32 || D == 64 || D == 128; }
+const char *kv4_check(const KV4Args &kv, int D);  // what is wrong with a cache's pointers, or null
+// the two halves of a (scale, base) pair
+__device__ __forceinline__ float kv4_scale(uint32_t p) { return __uint_as_float(p << 16); }
+__device__ __forceinline__ float kv4_base(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
+
+// The tiles of TS keys that queries at positions [first, last] meet under a window: those that hold
+// first tokens, then those of the windows, up to key `end` (exclusive).  Tiles between them hold no
+// key that any of these queries sees.
+template <int TS> struct KeyWalk {
+  int lo, ns, t0, count;  // the lowest key in a window, tiles of first tokens, first window tile, all tiles
+  __host__ __device__ KeyWalk(int first, int end, int window, int sinks) {
+    lo = first - window + 1;
+    lo = lo > 0 ? lo : 0;
+    t0 = lo / TS;
+    const int se = sinks < end ? sinks : end;
+    ns = (se + TS - 1) / TS;
+    ns = ns < t0 ? ns : t0;
+    const int tend = (end + TS - 1) / TS;
+    count = ns + (tend > t0 ? tend - t0 : 0);
+  }
+  __host__ __device__ int tile(int i) const { return i < ns ? i : t0 + i - ns; }
+};
+
+// Keys and query start of a decode launch: from the host arguments, or from the
+// device cursor (clamped so the window stays inside the capacity).
+struct DecodeWindow { int S, q_start; };
+__device__ __forceinline__ DecodeWindow decode_window(const ChordArgs &a) {
+  if (!a.len_dev) return {min(a.S, a.q_start + a.L), a.q_start};
+  const int cached = min(max(__builtin_amdgcn_readfirstlane(*a.len_dev), 0), a.S - a.L);
+  return {cached + a.L, cached};
+}
+
+__device__ __forceinline__ float log_n_at(const ChordArgs &a, int b, int i, int q_start) {
+  return a.log_n ? a.log_n[b * a.ln_sb + int64_t(i) * a.ln_st] : a.log_tab[q_start + i];
+}
 
 __device__ __forceinline__ float ggd_bias(float dist, float alpha, float beta, float mu, float eps) {
   // -alpha * (|d - mu| + eps)^beta, the power through exp2(beta * log2(.)).
@@ -40,6 +97,10 @@ __device__ __forceinline__ float ggd_bias(float dist, float alpha, float beta, f
 // not take: fp32, fp16 and bf16 at head dims 16, 32, 64, 128, padded batches.
 bool chord_wide_serves(const ChordArgs &a);
 int launch_chord_wide(const ChordArgs &a, int dtype, int D, hipStream_t s);
+// The same kernel with a window (k / v rows), and over a 4-bit cache (`kv`; a.k / a.v unused),
+// with the host's q_start or the device cursor (which the launch then advances).
+int launch_chord_wide_window(const ChordArgs &a, int dtype, int D, hipStream_t s);
+int launch_chord_wide_kv4(const ChordArgs &a, const KV4Args &kv, int dtype, int D, hipStream_t s);
 
 // Chord decode over a device cursor, shared by the C-ABI entry points that take
 // a caller workspace and those that use the library's own scratch.

@@ -27,6 +27,7 @@
 // tokens 34.5 (151), 4096 tokens 325 (1355), 3 tokens over 4096 82 (101); fp16 1023 tokens 22 (148);
 // bf16 D = 128 1000 tokens 36 (381).  Error against 64 bits, fp32: 3.7e-7 (4.1e-7).
 #include <algorithm>
+#include <type_traits>
 
 #include "capi_internal.h"
 #include "chord_internal.h"
@@ -115,6 +116,10 @@ template <typename T, int N> struct Piece {
       w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
     }
   }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int x = 0; x < kW; ++x) w[x] = 0u;
+  }
   __device__ __forceinline__ float get(int e) const {
     if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
     const uint16_t b = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
@@ -123,19 +128,75 @@ template <typename T, int N> struct Piece {
   }
 };
 
-template <typename T, int D, int NW>
+// What the keys and values are, and which a query sees
+enum { kCausal = 0, kWindow = 1, k4Bit = 2 };  // k4Bit: rows of a 4-bit cache, with a window
+
+// One row of a 4-bit cache as loaded: D codes (word j: features 8 j ..) and the (scale, base) pairs
+template <int D> struct Row4 {
+  static constexpr int kG = D >= 32 ? D / 32 : 1;
+  uint32_t w[D / 8], p[kG];
+  __device__ __forceinline__ void load(buf_t c, buf_t pr, int row) {
+    const uint32_t co = static_cast<uint32_t>(row) * (D / 2), po = static_cast<uint32_t>(row) * (4 * kG);
+    if constexpr (D == 16) {
+      const uint2 u = buf_ld8(c, co);
+      w[0] = u.x; w[1] = u.y;
+    } else {
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        const uint4 u = buf_ld16(c, co + 16 * j);
+        w[4 * j] = u.x; w[4 * j + 1] = u.y; w[4 * j + 2] = u.z; w[4 * j + 3] = u.w;
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < kG; ++g) p[g] = __builtin_amdgcn_raw_buffer_load_b32(pr, po + 4 * g, 0, 0);
+  }
+  // the values of lane half h's features 8 j + 4 h + 0..3
+  __device__ __forceinline__ void expand(RowOp<float, D> &k, int h) const {
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) {
+      const uint32_t n = w[j] >> (16 * h), pr = p[j * 8 / (D / kG)];
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        k.x[j][t] = fmaf(static_cast<float>((n >> (4 * t)) & 15u), kv4_scale(pr), kv4_base(pr));
+    }
+  }
+};
+// N consecutive values of one 4-bit row, features f .. f + N - 1 (f a multiple of N)
+template <int D, int N> struct Piece4 {
+  uint32_t c, p;
+  __device__ __forceinline__ void load(buf_t cb, buf_t pb, int row, int f) {
+    const uint32_t co = static_cast<uint32_t>(row) * (D / 2) + static_cast<uint32_t>(f) / 2;
+    if constexpr (N == 4) c = __builtin_amdgcn_raw_buffer_load_b16(cb, co, 0, 0);
+    else c = __builtin_amdgcn_raw_buffer_load_b8(cb, co, 0, 0);
+    if constexpr (N == 1) c >>= 4 * (f & 1);
+    p = __builtin_amdgcn_raw_buffer_load_b32(pb, 4u * static_cast<uint32_t>(row * Row4<D>::kG + f / (D / Row4<D>::kG)), 0, 0);
+  }
+  __device__ __forceinline__ void clear() { c = p = 0u; }
+  __device__ __forceinline__ float get(int e) const {
+    return fmaf(static_cast<float>((c >> (4 * e)) & 15u), kv4_scale(p), kv4_base(p));
+  }
+};
+
+template <typename T, int D, int NW, int MODE>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4)))
-chord_wide_kernel(ChordArgs a) {
+chord_wide_kernel(ChordArgs a, KV4Args kv) {
   constexpr int VD = D >= 32 ? D / 32 : 1;  // output tiles, and features of a V piece
-  constexpr int ES = sizeof(T), NS = ES == 4 ? 2 : 1;
+  // the scores' operand type: a 4-bit cache's values are fp32
+  using KT = std::conditional_t<MODE == k4Bit, float, T>;
+  constexpr int ES = sizeof(T), KS = sizeof(KT), NS = KS == 4 ? 2 : 1;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 31, h = lane >> 5;
   // (the heads vary fastest, the latest -- longest -- query blocks first)
   const int head = blockIdx.x, qb = gridDim.y - 1 - blockIdx.y, b = blockIdx.z;
   const int kvh = head / (a.H / a.Hkv);
-  const int q0 = 32 * qb, my_q = q0 + i, q_abs = a.q_start + my_q;
-  const int kv_end = min(a.S, a.q_start + min(a.L, q0 + 32));  // keys any query of the block sees
-  const int ntiles = (kv_end + 31) / 32;
+  const DecodeWindow cur = MODE == kCausal ? DecodeWindow{a.S, a.q_start} : decode_window(a);
+  const int q_start = cur.q_start;
+  const int q0 = 32 * qb, my_q = q0 + i, q_abs = q_start + my_q;
+  const int kv_end = min(cur.S, q_start + min(a.L, q0 + 32));  // keys any query of the block sees
+  const KeyWalk<32> walk = MODE == kCausal ? KeyWalk<32>(0, kv_end, kMaxWindow, 0)
+                                           : KeyWalk<32>(q_start + q0, kv_end, a.window, a.sinks);
+  const int ntiles = MODE == kCausal ? (kv_end + 31) / 32 : walk.count;
+  auto tile_at = [&](int x) { return MODE == kCausal ? x : walk.tile(x); };
 
   const T *kp = static_cast<const T *>(a.k) + b * a.k_sb + kvh * a.k_sh;
   const T *vp = static_cast<const T *>(a.v) + b * a.v_sb + kvh * a.v_sh;
@@ -144,20 +205,51 @@ chord_wide_kernel(ChordArgs a) {
     const int rows = min(32, kv_end - 32 * t);
     return make_buf(p + int64_t(32 * t) * st, rows > 0 ? static_cast<uint32_t>(((rows - 1) * st + D) * ES) : 0u);
   };
+  // (4-bit rows: codes and pairs of tile t)
+  auto code_buf = [&](const uint8_t *p, int t) {
+    const int rows = min(32, kv_end - 32 * t);
+    return make_buf(p + int64_t(32 * t) * (D / 2), rows > 0 ? static_cast<uint32_t>(rows) * (D / 2) : 0u);
+  };
+  auto pair_buf = [&](const uint32_t *p, int t) {
+    const int rows = min(32, kv_end - 32 * t);
+    return make_buf(p + int64_t(32 * t) * Row4<D>::kG, rows > 0 ? static_cast<uint32_t>(rows) * (4 * Row4<D>::kG) : 0u);
+  };
+  const uint8_t *kcp = nullptr, *vcp = nullptr;
+  const uint32_t *kpp = nullptr, *vpp = nullptr;
+  if constexpr (MODE == k4Bit) {
+    kcp = kv.kc + b * kv.kc_sb + kvh * kv.kc_sh;
+    vcp = kv.vc + b * kv.vc_sb + kvh * kv.vc_sh;
+    kpp = kv.kp + b * kv.kp_sb + kvh * kv.kp_sh;
+    vpp = kv.vp + b * kv.vp_sb + kvh * kv.vp_sh;
+  }
   const uint32_t koff = static_cast<uint32_t>(i * a.k_st) * ES;
   const uint32_t voff = static_cast<uint32_t>(4 * h * a.v_st + VD * (D < 32 ? i & (D - 1) : i)) * ES;
   const uint32_t vrow = static_cast<uint32_t>(a.v_st) * ES;
 
-  RowOp<T, D> q, k;
+  RowOp<KT, D> q, k;
+  Row4<D> k4;
   {
     const T *qp = static_cast<const T *>(a.q) + b * a.q_sb + head * a.q_sh + int64_t(q0) * a.q_st;
     const int rows = min(32, a.L - q0);
-    q.load(make_buf(qp, static_cast<uint32_t>(((rows - 1) * a.q_st + D) * ES)),
-           static_cast<uint32_t>(min(i, rows - 1) * a.q_st) * ES, h);
+    if constexpr (MODE == k4Bit) {
+      const T *qr = qp + min(i, rows - 1) * a.q_st + 4 * h;
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) q.x[j][t] = ld(qr + 8 * j + t);
+    } else {
+      q.load(make_buf(qp, static_cast<uint32_t>(((rows - 1) * a.q_st + D) * ES)),
+             static_cast<uint32_t>(min(i, rows - 1) * a.q_st) * ES, h);
+    }
   }
-  if (w < ntiles) k.load(tile_buf(kp, a.k_st, w), koff, h);
+  auto load_k = [&](int t) {  // (past the last tile: an empty buffer, zeros)
+    if constexpr (MODE == k4Bit) k4.load(code_buf(kcp, t), pair_buf(kpp, t), i);
+    else k.load(tile_buf(kp, a.k_st, t), koff, h);
+  };
+  if (w < ntiles) load_k(tile_at(w));
 
-  const float mul = a.ssmax[head] * a.log_n[b * a.ln_sb + int64_t(min(my_q, a.L - 1)) * a.ln_st];
+  const float mul = a.ssmax[head] * (MODE == kCausal ? a.log_n[b * a.ln_sb + int64_t(min(my_q, a.L - 1)) * a.ln_st]
+                                                     : log_n_at(a, b, min(my_q, a.L - 1), q_start));
   const float c_qk = mul * a.scale * kLog2e, c_b = mul * kLog2e;  // logits in log2 units
   const float al = a.alpha[head], be = a.beta[head], mu = a.mu[head];
 
@@ -172,34 +264,51 @@ chord_wide_kernel(ChordArgs a) {
 #pragma unroll
   for (int t = 0; t < VD; ++t) o[t] = f32x16{};
 
-  for (int t = w; t < ntiles; t += NW) {
-    const int n0 = 32 * t;
-    Piece<T, VD> v[16];
-    const buf_t vb = tile_buf(vp, a.v_st, t);
+  for (int x = w; x < ntiles; x += NW) {
+    const int t = tile_at(x), n0 = 32 * t;
+    std::conditional_t<MODE == k4Bit, Piece4<D, VD>, Piece<T, VD>> v[16];
+    if constexpr (MODE == k4Bit) {
+      const buf_t vcb = code_buf(vcp, t), vpb = pair_buf(vpp, t);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) v[r].load(vb, voff + static_cast<uint32_t>(8 * (r >> 2) + (r & 3)) * vrow);
-    win[lane] = ggd_bias(static_cast<float>(n0 - a.q_start - q0 - 31 + lane), al, be, mu, a.eps);
+      for (int r = 0; r < 16; ++r) v[r].load(vcb, vpb, 8 * (r >> 2) + 4 * h + (r & 3), VD * (D < 32 ? i & (D - 1) : i));
+    } else {
+      const buf_t vb = tile_buf(vp, a.v_st, t);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) v[r].load(vb, voff + static_cast<uint32_t>(8 * (r >> 2) + (r & 3)) * vrow);
+    }
+    win[lane] = ggd_bias(static_cast<float>(n0 - q_start - q0 - 31 + lane), al, be, mu, a.eps);
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (MODE == k4Bit) k4.expand(k, h);
     f32x16 sc[NS];
     score<D>(k, q, sc);
     float bias[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) bias[r] = winr[8 * (r >> 2) + (r & 3)];
     __builtin_amdgcn_sched_barrier(0);
-    k.load(tile_buf(kp, a.k_st, t + NW), koff, h);  // (past the last tile: an empty buffer, zeros)
+    load_k(tile_at(x + NW));  // (past the last tile: an empty buffer, zeros)
     __builtin_amdgcn_sched_barrier(0);
-    const bool masked = n0 + 31 > a.q_start + q0 || n0 + 32 > kv_end;  // the diagonal and the last tiles
+    // the diagonal and the last tiles, and with a window those that not every query of the block sees whole
+    const bool masked = n0 + 31 > q_start + q0 || n0 + 32 > kv_end ||
+                        (MODE != kCausal && n0 <= q_start + q0 + 31 - a.window && n0 + 32 > a.sinks);
     auto keep = [&](int r) {
       const int key = n0 + 8 * (r >> 2) + 4 * h + (r & 3);
-      return key <= q_abs && key < kv_end;
+      return key <= q_abs && key < kv_end && (MODE == kCausal || key > q_abs - a.window || key < a.sinks);
     };
+    // rows that no query of the block sees may hold anything (0 * NaN in the products below)
+    if (MODE != kCausal && n0 < walk.lo && n0 + 32 > a.sinks) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int key = n0 + 8 * (r >> 2) + 4 * h + (r & 3);
+        if (key < walk.lo && key >= a.sinks) v[r].clear();
+      }
+    }
     // a logit plus `off`: the fp32 form adds the large terms first, so with off = -max they cancel
     // before the small result is rounded
     auto logit = [&](int r, float off) {
-      float x = ES == 4 ? fmaf(c_b, bias[r], off) : c_b * bias[r];
+      float x = KS == 4 ? fmaf(c_b, bias[r], off) : c_b * bias[r];
 #pragma unroll
       for (int n = 0; n < NS; ++n) x = fmaf(sc[n][r], c_qk, x);
-      return ES == 4 ? x : x + off;
+      return KS == 4 ? x : x + off;
     };
     float mx = -INFINITY, s[16];
     if (masked) {
@@ -300,23 +409,35 @@ chord_wide_kernel(ChordArgs a) {
   if (a.lse && w == 0 && h == 0) a.lse[(static_cast<size_t>(b) * a.H + head) * a.L + my_q] = M + fast_log2(Ls);
 }
 
-template <typename T, int D, int NW>
-int launch_wide(const ChordArgs &a, hipStream_t s) {
+// *len_dev += L behind the launch that read it
+__global__ void chord_advance_kernel(int *len_dev, int L, int capacity) { *len_dev = min(*len_dev + L, capacity); }
+
+template <typename T, int D, int NW, int MODE>
+int launch_wide(const ChordArgs &a, const KV4Args &kv, hipStream_t s) {
   constexpr int smem = (2 * 64 * NW + NW * 16 * 64) * static_cast<int>(sizeof(float));
   const dim3 grid(a.H, (a.L + 31) / 32, a.B), block(64 * NW);
-  chord_wide_kernel<T, D, NW><<<grid, block, smem, s>>>(a);
-  return check_launch("chord_wide_kernel");
+  chord_wide_kernel<T, D, NW, MODE><<<grid, block, smem, s>>>(a, kv);
+  if (const int rc = check_launch("chord_wide_kernel"); rc || MODE == kCausal || !a.len_dev) return rc;
+  chord_advance_kernel<<<dim3(1), dim3(1), 0, s>>>(a.len_dev, a.L, a.S);
+  return check_launch("chord_advance_kernel");
 }
 
-template <typename T>
-int launch_wide_t(const ChordArgs &a, int D, hipStream_t s) {
+template <typename T, int MODE>
+int launch_wide_t(const ChordArgs &a, const KV4Args &kv, int D, hipStream_t s) {
   switch (D) {
-    case 16: return launch_wide<T, 16, 8>(a, s);
-    case 32: return launch_wide<T, 32, 8>(a, s);
-    case 64: return launch_wide<T, 64, 8>(a, s);
+    case 16: return launch_wide<T, 16, 8, MODE>(a, kv, s);
+    case 32: return launch_wide<T, 32, 8, MODE>(a, kv, s);
+    case 64: return launch_wide<T, 64, 8, MODE>(a, kv, s);
     // (fp32 rows of 128 features leave no registers for a second wave per SIMD)
-    default: return launch_wide<T, 128, sizeof(T) == 4 ? 4 : 8>(a, s);
+    default: return launch_wide<T, 128, sizeof(T) == 4 || MODE == k4Bit ? 4 : 8, MODE>(a, kv, s);
   }
+}
+
+template <int MODE>
+int launch_wide_m(const ChordArgs &a, const KV4Args &kv, int dtype, int D, hipStream_t s) {
+  if (dtype == MOTIF_BF16) return launch_wide_t<bf16_t, MODE>(a, kv, D, s);
+  if (dtype == MOTIF_F16) return launch_wide_t<f16_t, MODE>(a, kv, D, s);
+  return launch_wide_t<float, MODE>(a, kv, D, s);
 }
 
 }  // namespace
@@ -329,9 +450,13 @@ bool chord_wide_serves(const ChordArgs &a) {
 }
 
 int launch_chord_wide(const ChordArgs &a, int dtype, int D, hipStream_t s) {
-  if (dtype == MOTIF_BF16) return launch_wide_t<bf16_t>(a, D, s);
-  if (dtype == MOTIF_F16) return launch_wide_t<f16_t>(a, D, s);
-  return launch_wide_t<float>(a, D, s);
+  return launch_wide_m<kCausal>(a, KV4Args{}, dtype, D, s);
+}
+int launch_chord_wide_window(const ChordArgs &a, int dtype, int D, hipStream_t s) {
+  return launch_wide_m<kWindow>(a, KV4Args{}, dtype, D, s);
+}
+int launch_chord_wide_kv4(const ChordArgs &a, const KV4Args &kv, int dtype, int D, hipStream_t s) {
+  return launch_wide_m<k4Bit>(a, kv, dtype, D, s);
 }
 
 }  // namespace motif

@@ -4,6 +4,7 @@ The library is loaded after `torch` so that it binds to the HIP runtime torch
 already loaded (both are `libamdhip64.so.7`): one runtime per process, so the
 hipStream_t handles and device pointers torch hands out are valid for it.
 '''
+import contextlib
 import ctypes
 import os
 
@@ -80,6 +81,16 @@ _SIGNATURES = {
     'motif_chord_decode_noalloc': (
         _T4 * 3 + [_P, _I32] + [_P] * 4 + [_P, _I64, _I64, _P, _I32] + _T4 + [_I32] * 5 + [_F32, _F32]
         + [_I32, _P], _I32),
+    'motif_chord_window_workspace_bytes': ([_I32] * 9, _SZ),
+    'motif_chord_window_fwd': (
+        _T4 * 3 + [_P] * 4 + [_P, _I64, _I64, _P, _I32] + _T4 + [_P, _P] + [_I32] * 7 + [_F32, _F32]
+        + [_I32, _I32, _P, _SZ, _I32, _P], _I32),
+    'motif_kv4_append': (_T4 * 2 + [_P, _I64, _I64] * 4 + [_P] + [_I32] * 7 + [_P], _I32),
+    'motif_kv4_read': ([_P, _I64, _I64] * 4 + _T4 * 2 + [_I32] * 7 + [_P], _I32),
+    'motif_chord_kv4_workspace_bytes': ([_I32] * 9, _SZ),
+    'motif_chord_kv4_fwd': (
+        _T4 + [_P, _I64, _I64] * 4 + [_P] * 4 + [_P, _I64, _I64, _P, _I32] + _T4 + [_P] + [_I32] * 7 + [_F32, _F32]
+        + [_I32, _I32, _P, _SZ, _I32, _P], _I32),
     'motif_probe_copy': ([_P, _P, _SZ, _I32, _P], _I32),
     'motif_probe_read': ([_P, _P, _SZ, _I32, _P], _I32),
     'motif_probe_mfma_bf16': ([_P, _I32, _I32, _I32, _P], _I32),
@@ -175,6 +186,17 @@ def stream_ptr(device) -> int:
     if index is None:
         return torch.cuda.current_stream(device).cuda_stream
     return torch._C._cuda_getCurrentRawStream(index)
+
+
+def on_device(device):
+    '''A context in which `device` is the current one (launches go to the current device;
+    switching costs a few us, so only where it is another).'''
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def as_type(t, dt):

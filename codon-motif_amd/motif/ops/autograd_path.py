@@ -99,11 +99,13 @@ def short_conv_silu_torch(x, weight, cache=None, head_dim=None, scale=1.0):
     return y.to(x.dtype), xc[..., xc.shape[-1] - (K - 1):]
 
 
-def chord_attention_torch(q, k, v, alpha, beta, mu, ssmax, log_n, q_start=None, softmax_scale=None, eps=1e-5):
+def chord_attention_torch(q, k, v, alpha, beta, mu, ssmax, log_n, q_start=None, softmax_scale=None, eps=1e-5,
+                          window=None, sinks=0):
     '''Chord attention with the gated geometric-decay bias (chord_attention.py:74-244):
     logit = (s q_i.k_j - alpha_h (|j - i_abs - mu_h| + eps)^beta_h) ssmax_h log_n[b, i],
     keys j <= i_abs = q_start + i, softmax over keys.  q [B, H, L, D], k / v
-    [B, Hkv, S, D]; returns [B, H, L, D] in q's dtype.'''
+    [B, Hkv, S, D]; returns [B, H, L, D] in q's dtype.  With a window only the keys
+    j > i_abs - window or j < sinks of those; a row that sees none gives zeros.'''
     B, H, L, D = q.shape
     Hkv, S = k.shape[1], k.shape[2]
     scale = D ** -0.5 if softmax_scale is None else softmax_scale
@@ -118,17 +120,23 @@ def chord_attention_torch(q, k, v, alpha, beta, mu, ssmax, log_n, q_start=None, 
     logits = (scale * (c(q) @ kf.transpose(-1, -2)) + bias[None]) * c(ssmax)[None, :, None, None] \
         * c(log_n)[:, None, :, None]
     visible = torch.arange(S, device=q.device)[None, :] <= i_abs[:, None]
-    logits = logits.masked_fill(~visible, -math.inf)
-    return (logits.softmax(-1) @ vf).to(q.dtype)
+    if window is None:
+        logits = logits.masked_fill(~visible, -math.inf)
+        return (logits.softmax(-1) @ vf).to(q.dtype)
+    j = torch.arange(S, device=q.device)[None, :]
+    visible = visible & ((j > i_abs[:, None] - window) | (j < sinks))
+    logits = logits.masked_fill(~visible, torch.finfo(cdt).min)  # (finite: an empty row stays free of NaN)
+    return ((logits.softmax(-1) * visible) @ vf).to(q.dtype)
 
 
-def chord_attention_varlen_torch(q, k, v, alpha, beta, mu, ssmax, log_n, cu_seqlens, softmax_scale=None, eps=1e-5):
+def chord_attention_varlen_torch(q, k, v, alpha, beta, mu, ssmax, log_n, cu_seqlens, softmax_scale=None, eps=1e-5,
+                                 window=None, sinks=0):
     '''Packed-sequence Chord attention as separate differentiable runs: sequence i
     (rows cu[i]:cu[i+1] of q [1, H, T, D] / k, v [1, Hkv, T, D]) attends causally within
     itself from position 0 with its slice of log_n [1, T].'''
     cu = [int(x) for x in cu_seqlens.detach().to('cpu')]
     outs = [chord_attention_torch(q[:, :, a:b], k[:, :, a:b], v[:, :, a:b], alpha, beta, mu, ssmax,
-                                  log_n[:, a:b], 0, softmax_scale, eps)
+                                  log_n[:, a:b], 0, softmax_scale, eps, window, sinks)
             for a, b in zip(cu[:-1], cu[1:]) if b > a]
     if not outs:
         return q.new_empty(q.shape)

@@ -18,6 +18,7 @@ dv and the four per-head parameter gradients, the reference's custom backward
 :1348-1554).  Other gradient calls take the differentiable torch forms
 (motif/ops/autograd_path.py).
 '''
+import numbers
 from typing import Optional
 
 import torch
@@ -28,12 +29,26 @@ from .autograd_path import chord_attention_torch, chord_attention_varlen_torch, 
 
 HEAD_DIM = 64                  # the model's head dim: bf16 runs on the MFMA kernels
 HEAD_DIMS = (16, 32, 64, 128)  # head dims the kernels serve
+NO_WINDOW = 2 ** 31 - 1        # window argument of the kernels that always take one
 
 
 def serves_head_dim(D: int) -> bool:
     '''Head dims apply_chord_attention takes: the kernels' own (HEAD_DIMS) and every
     size between them (zero-padded to the next one).'''
     return HEAD_DIMS[0] <= D <= HEAD_DIMS[-1]
+
+
+def check_window(window, sinks):
+    '''(window, sinks) as ints (window None: every key up to the query's own), checked.'''
+    if isinstance(sinks, bool) or not isinstance(sinks, numbers.Integral) or sinks < 0:
+        raise ValueError(f'sinks must be an int >= 0, got {sinks!r}')
+    if window is None:
+        if sinks:
+            raise ValueError('sinks (first tokens that stay visible) need a window')
+        return None, 0
+    if isinstance(window, bool) or not isinstance(window, numbers.Integral) or window < 1:
+        raise ValueError(f'window must be an int >= 1 or None, got {window!r}')
+    return min(int(window), NO_WINDOW), min(int(sinks), NO_WINDOW)
 
 
 def _grad_kernels_serve(q, k, v, alpha, beta, mu, ssmax, log_n, q_start):
@@ -209,6 +224,48 @@ def _launch(q, k, v, alpha, beta, mu, ssmax, log_n, q_start, scale, eps, out, ls
     return out
 
 
+def _launch_window(q, k, v, params, log_n, q_start, scale, eps, window, sinks, out, lse=None, length_dev=None,
+                   log_table=None, workspace=None):
+    '''motif_chord_window_fwd into `out`: host positions (log_n), or the device cursor over a
+    fixed-capacity cache (length_dev and log_table; the launch advances it).'''
+    B, H, L, D = q.shape
+    Hkv, S = k.shape[1], k.shape[2]
+    if D not in HEAD_DIMS:  # zero-padded to the next size, as in _launch
+        Dp = next((d for d in HEAD_DIMS if d > D), None)
+        if Dp is None or length_dev is not None:
+            raise NotImplementedError(f'windowed Chord attention: head_dim {D} unsupported')
+        pad = lambda t: torch.nn.functional.pad(t, (0, Dp - D))
+        out_p = torch.empty((B, H, L, Dp), dtype=out.dtype, device=out.device)
+        _launch_window(pad(q), pad(k), pad(v), params, log_n, q_start, scale, eps, window, sinks, out_p, lse)
+        out.copy_(out_p[..., :D])
+        return out
+    lib = _lib.lib()
+    code = _lib.chord_dtype_code(q.dtype)
+    with _lib.on_device(q.device):
+        if length_dev is None:  # (a cache that is written in place is never copied)
+            q, k, v = (_near(_aligned(t)) for t in (q, k, v))
+        else:
+            q = _aligned(q)
+        if workspace is None:
+            n = int(lib.motif_chord_window_workspace_bytes(B, H, Hkv, L, S, D, window, sinks, code))
+            workspace = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        ln = (log_n.data_ptr(), log_n.stride(0), log_n.stride(1)) if log_n is not None else (None, 0, 0)
+        table = (None, 0) if log_table is None else (log_table.data_ptr(), log_table.numel())
+        rc = lib.motif_chord_window_fwd(
+            *_lib.t4(q), *_lib.t4(k), *_lib.t4(v), *[t.data_ptr() for t in params], *ln, *table, *_lib.t4(out),
+            _lib.ptr(lse), _lib.ptr(length_dev), B, H, Hkv, L, S, D, int(q_start), float(scale), float(eps),
+            window, sinks, _lib.ptr(workspace), 0 if workspace is None else workspace.numel(), code,
+            _lib.stream_ptr(q.device))
+    _lib.check(rc, 'motif_chord_window_fwd')
+    return out
+
+
+def _near(t):
+    '''t, copied where its rows lie further apart than the windowed kernels' 32-bit offsets
+    hold, or run backwards.'''
+    return t if t.shape[2] <= 1 or 0 <= t.stride(2) < 2 ** 24 else t.contiguous()
+
+
 def apply_chord_attention(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -222,6 +279,8 @@ def apply_chord_attention(
     softmax_scale: Optional[float] = None,
     eps: float = 1e-5,
     out: Optional[torch.Tensor] = None,
+    window: Optional[int] = None,
+    sinks: int = 0,
 ) -> torch.Tensor:
     '''Chord attention forward on the HIP kernels.
 
@@ -239,6 +298,10 @@ def apply_chord_attention(
         out: optional [B, H, L, D] destination in q's dtype with unit feature stride (a
             strided view, e.g. the transpose of a [B, L, H, D] buffer, so the heads come
             out already merged); not a reference argument.
+        window: a query at position p sees only the keys j > p - window of those up to its
+            own (None: all of them), and
+        sinks: the first `sinks` keys besides; a row that sees no key gives zeros.  Not
+            reference arguments.
 
     Returns:
         [B, H, L, D] in q's dtype (`out` when given).
@@ -249,10 +312,13 @@ def apply_chord_attention(
             differentiable torch form).
         RuntimeError: when the HIP library is unavailable or a launch fails.
     '''
+    window, sinks = check_window(window, sinks)
     if wants_grad(q, k, v, alpha, beta, mu, ssmax, log_n):
         if q_start is not None and int(q_start) < 0:
             raise ValueError(f'q_start must not be negative, got {q_start}')
-        if _grad_kernels_serve(q, k, v, alpha, beta, mu, ssmax, log_n, q_start):
+        if window is not None:
+            res = chord_attention_torch(q, k, v, alpha, beta, mu, ssmax, log_n, q_start, softmax_scale, eps, window, sinks)
+        elif _grad_kernels_serve(q, k, v, alpha, beta, mu, ssmax, log_n, q_start):
             scale = q.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale)
             qs = k.shape[2] - q.shape[2] if q_start is None else int(q_start)
             res = ChordFunction.apply(q, k, v, alpha, beta, mu, ssmax, log_n, qs, scale, float(eps))
@@ -273,11 +339,15 @@ def apply_chord_attention(
     out = _out_for(out, q)
     if L == 0:
         return out
+    if window is not None:
+        if out.numel() == 0 or S == 0:
+            return out.zero_()
+        return _launch_window(q, k, v, (alpha, beta, mu, ssmax), log_n, q_start, softmax_scale, eps, window, sinks, out)
     return _launch(q, k, v, alpha, beta, mu, ssmax, log_n, q_start, softmax_scale, eps, out)
 
 
 def apply_chord_attention_varlen(q, k, v, alpha, beta, mu, ssmax, log_n, cu_seqlens,
-                                 softmax_scale=None, eps=1e-5, out=None):
+                                 softmax_scale=None, eps=1e-5, out=None, window=None, sinks=0):
     '''Packed-sequence Chord attention (no reference counterpart).
 
     B == 1; q [1, H, T, D], k/v [1, H_kv, T, D] hold the sequences back to back,
@@ -288,19 +358,23 @@ def apply_chord_attention_varlen(q, k, v, alpha, beta, mu, ssmax, log_n, cu_seql
     metadata then spares the call every read back from the device).
     Calls that need gradients run the sequences separately: through the HIP forward /
     backward pair (`ChordFunction`) where it serves, else as differentiable torch runs.
-    `out` is an optional destination, as for apply_chord_attention.
+    `out` is an optional destination and `window` / `sinks` limit what a query sees of its
+    own sequence, as for apply_chord_attention.
     '''
+    window, sinks = check_window(window, sinks)
     if wants_grad(q, k, v, alpha, beta, mu, ssmax, log_n):
         if (q.shape[0] == 1 and q.shape[2] > 0 and k.shape[2] == q.shape[2]
                 and _grad_kernels_serve(q, k, v, alpha, beta, mu, ssmax, log_n, 0)):
             cu = PackedSeqs.of(cu_seqlens, q.shape[2], q.device).cu_host.tolist()
             outs = [apply_chord_attention(q[:, :, a:b], k[:, :, a:b], v[:, :, a:b], alpha, beta, mu, ssmax,
-                                          log_n[:, a:b], q_start=0, softmax_scale=softmax_scale, eps=eps)
+                                          log_n[:, a:b], q_start=0, softmax_scale=softmax_scale, eps=eps,
+                                          window=window, sinks=sinks)
                     for a, b in zip(cu[:-1], cu[1:]) if b > a]
             res = torch.cat(outs, dim=2)
         else:
             cu_t = cu_seqlens.cu_host if isinstance(cu_seqlens, PackedSeqs) else cu_seqlens
-            res = chord_attention_varlen_torch(q, k, v, alpha, beta, mu, ssmax, log_n, cu_t, softmax_scale, eps)
+            res = chord_attention_varlen_torch(q, k, v, alpha, beta, mu, ssmax, log_n, cu_t, softmax_scale, eps,
+                                               window, sinks)
         return res if out is None else _check_out(out, res.shape, res.dtype, res.device).copy_(res)
     if not _lib.available():
         raise RuntimeError('there is no usable HIP backend in the current environment')
@@ -314,6 +388,12 @@ def apply_chord_attention_varlen(q, k, v, alpha, beta, mu, ssmax, log_n, cu_seql
     out = _out_for(out, q)
     if L == 0:
         return out
+    if window is not None:
+        for a, b in ps.bounds():
+            if b > a:
+                _launch_window(q[:, :, a:b], k[:, :, a:b], v[:, :, a:b], (alpha, beta, mu, ssmax), log_n[:, a:b], 0,
+                               softmax_scale, eps, window, sinks, out[:, :, a:b])
+        return out
     return _launch(q, k, v, alpha, beta, mu, ssmax, log_n, 0, softmax_scale, eps, out,
                    cu_dev=ps.cu, nseq=ps.nseq, max_seqlen=ps.max_len, cu_host=ps.cu_host)
 
@@ -322,6 +402,15 @@ def chord_decode_workspace(B, H, Hkv, L, capacity, D, dtype, device) -> torch.Te
     '''A workspace for chord_decode_cursor at these sizes.'''
     n = _lib.lib().motif_chord_decode_workspace_bytes(B, H, Hkv, L, capacity, D, _lib.chord_dtype_code(dtype), None)
     return torch.empty(max(int(n), 1), dtype=torch.uint8, device=device)
+
+
+def chord_window_workspace(B, H, Hkv, L, capacity, D, dtype, device, window, sinks=0) -> Optional[torch.Tensor]:
+    '''A workspace for chord_decode_cursor with a window at these sizes (None where it needs
+    none).'''
+    window, sinks = check_window(window, sinks)
+    n = int(_lib.lib().motif_chord_window_workspace_bytes(B, H, Hkv, L, capacity, D, window, sinks,
+                                                          _lib.chord_dtype_code(dtype)))
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
 def chord_decode_step_serves(proj, H, Hkv, D) -> bool:
@@ -365,7 +454,7 @@ def chord_decode_step(proj, offsets, q_norm_weight, k_norm_weight, norm_eps, k_c
 
 
 def chord_decode_cursor(q, k_cache, v_cache, length_dev, alpha, beta, mu, ssmax, log_table, softmax_scale=None,
-                        eps=1e-5, log_n=None, workspace=None, library_scratch=False):
+                        eps=1e-5, log_n=None, workspace=None, library_scratch=False, window=None, sinks=0):
     '''Chord attention of L new queries over a fixed-capacity cache (new).
 
     k_cache / v_cache [B, Hkv, capacity, D] hold `length_dev[0]` cached positions and
@@ -375,7 +464,10 @@ def chord_decode_cursor(q, k_cache, v_cache, length_dev, alpha, beta, mu, ssmax,
     a captured launch replays token after token.  Returns [B, H, L, D].
     `library_scratch=True` takes the allocation-free entry point
     (motif_chord_decode_noalloc: the library's own per-device scratch, no workspace).
+    `window` / `sinks` limit what a query sees, as for apply_chord_attention (then
+    `workspace` is chord_window_workspace's).
     '''
+    window, sinks = check_window(window, sinks)
     B, H, L, D = q.shape
     Hkv, cap = k_cache.shape[1], k_cache.shape[2]
     if length_dev.dtype != torch.int32 or length_dev.device != q.device:
@@ -386,6 +478,15 @@ def chord_decode_cursor(q, k_cache, v_cache, length_dev, alpha, beta, mu, ssmax,
         softmax_scale = D ** -0.5
     q = _aligned(q)
     out = torch.empty((B, H, L, D), dtype=q.dtype, device=q.device)
+    if window is not None:
+        if library_scratch:
+            raise ValueError('chord_decode_cursor: a window and library_scratch do not go together')
+        if L > cap:
+            raise ValueError('chord_decode_cursor: more queries than the capacity')
+        if out.numel() == 0:
+            return out
+        return _launch_window(q, k_cache, v_cache, (alpha, beta, mu, ssmax), log_n, 0, softmax_scale, eps, window, sinks,
+                              out, length_dev=length_dev, log_table=log_table, workspace=workspace)
     ln_sb, ln_st = (log_n.stride(0), log_n.stride(1)) if log_n is not None else (0, 0)
     if library_scratch:
         rc = _lib.lib().motif_chord_decode_noalloc(

@@ -470,6 +470,75 @@ int motif_chord_qkv_prep(const void *proj, int64_t p_sb, int64_t p_st, int q_off
                          void *stream);
 
 /*
+ * Chord attention under a sliding window with visible first tokens (no reference
+ * counterpart): motif_chord_fwd's formula with a query at position p seeing the keys
+ * j <= p with j > p - window or j < sinks (window >= 1, sinks >= 0).  A row that sees no
+ * key (q_start + i - window >= S without first tokens) gives zeros.  Rows of k / v that no
+ * query of the launch's 32-query blocks sees are not used, whatever they hold.
+ *   q [B,H,L,D], k / v [B,Hkv,S,D], out [B,H,L,D]: fp32, fp16 or bf16, D 16, 32, 64, 128,
+ *   rows on 16-byte boundaries, row strides below 2^24 elements.
+ *   log_n [B,L] fp32, or NULL: log_table[q_start + i].
+ *   lse: optional [B,H,L] fp32 base-2 log-sum-exp (-inf for a row that sees no key).
+ *   length_dev: NULL, or the device cursor: S is then the cache's capacity, *length_dev
+ *   positions are cached with the L new rows behind them, q_start = *length_dev
+ *   (the argument must be 0), and the launch advances *length_dev by L.
+ *   workspace: motif_chord_window_workspace_bytes(...) bytes (may be 0), 16-byte aligned.
+ */
+size_t motif_chord_window_workspace_bytes(int B, int H, int Hkv, int L, int S, int D, int window, int sinks, int dtype);
+int motif_chord_window_fwd(
+    const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st,
+    const void *k, int64_t k_sb, int64_t k_sh, int64_t k_st,
+    const void *v, int64_t v_sb, int64_t v_sh, int64_t v_st,
+    const float *alpha, const float *beta, const float *mu, const float *ssmax,
+    const float *log_n, int64_t ln_sb, int64_t ln_st, const float *log_table, int log_table_len,
+    void *out, int64_t o_sb, int64_t o_sh, int64_t o_st, float *lse,
+    int *length_dev, int B, int H, int Hkv, int L, int S, int D, int q_start, float scale, float eps,
+    int window, int sinks, void *workspace, size_t workspace_bytes, int dtype, void *stream);
+
+/*
+ * Rows of a 4-bit key / value cache (no reference counterpart).  For each (batch row, kv head,
+ * position) and for keys and values alike:
+ *   codes  [B,Hkv,capacity,D/2] bytes: feature 2 m in the low half of byte m, 2 m + 1 in the high;
+ *   params [B,Hkv,capacity,D/min(32,D)] pairs of bf16 (scale, base), one per group of min(32, D)
+ *          features: value = code * scale + base.
+ * Positions lie back to back (D/2 bytes, D/min(32,D) pairs); the batch and head strides are in
+ * bytes for codes and in pairs for params; rows start on 4-byte boundaries.
+ *
+ * motif_kv4_append writes n rows of k / v [B,Hkv,n,D] (fp32, fp16 or bf16, 16-byte aligned rows)
+ * at `position`, or at *position_dev (read, not advanced; rows at or past `capacity` are dropped):
+ *   base = bf16(min), scale = bf16((max - min) / 15), code = rint((x - base) / scale) held to
+ *   0 .. 15, over each group; a group with an infinity or a NaN reads back NaN.
+ * motif_kv4_read gives the values of n rows from `position` on as k / v [B,Hkv,n,D].
+ */
+int motif_kv4_append(const void *k, int64_t k_sb, int64_t k_sh, int64_t k_st,
+                     const void *v, int64_t v_sb, int64_t v_sh, int64_t v_st,
+                     void *k_codes, int64_t kc_sb, int64_t kc_sh, void *k_params, int64_t kp_sb, int64_t kp_sh,
+                     void *v_codes, int64_t vc_sb, int64_t vc_sh, void *v_params, int64_t vp_sb, int64_t vp_sh,
+                     const int *position_dev, int position, int capacity, int B, int n, int Hkv, int D,
+                     int dtype, void *stream);
+int motif_kv4_read(const void *k_codes, int64_t kc_sb, int64_t kc_sh, const void *k_params, int64_t kp_sb, int64_t kp_sh,
+                   const void *v_codes, int64_t vc_sb, int64_t vc_sh, const void *v_params, int64_t vp_sb, int64_t vp_sh,
+                   void *k, int64_t k_sb, int64_t k_sh, int64_t k_st, void *v, int64_t v_sb, int64_t v_sh, int64_t v_st,
+                   int position, int capacity, int B, int n, int Hkv, int D, int dtype, void *stream);
+
+/*
+ * Chord attention over a 4-bit cache: motif_chord_window_fwd's formula and arguments with the
+ * keys and values that the first S rows (or, with length_dev, the first *length_dev + L rows)
+ * of the cache stand for; window INT_MAX: every key up to the query's own.  q / out fp32, fp16
+ * or bf16.
+ */
+size_t motif_chord_kv4_workspace_bytes(int B, int H, int Hkv, int L, int S, int D, int window, int sinks, int dtype);
+int motif_chord_kv4_fwd(
+    const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st,
+    const void *k_codes, int64_t kc_sb, int64_t kc_sh, const void *k_params, int64_t kp_sb, int64_t kp_sh,
+    const void *v_codes, int64_t vc_sb, int64_t vc_sh, const void *v_params, int64_t vp_sb, int64_t vp_sh,
+    const float *alpha, const float *beta, const float *mu, const float *ssmax,
+    const float *log_n, int64_t ln_sb, int64_t ln_st, const float *log_table, int log_table_len,
+    void *out, int64_t o_sb, int64_t o_sh, int64_t o_st,
+    int *length_dev, int B, int H, int Hkv, int L, int S, int D, int q_start, float scale, float eps,
+    int window, int sinks, void *workspace, size_t workspace_bytes, int dtype, void *stream);
+
+/*
  * Workspace bytes of motif_chord_decode for a cache of `capacity` positions (the
  * split partials, plus the fp32 path's bias table); *splits (may be NULL) receives
  * the key-range split count.
