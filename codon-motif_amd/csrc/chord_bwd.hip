@@ -40,6 +40,7 @@
 #include <string>
 
 #include "capi_internal.h"
+#include "chord_internal.h"
 #include "common.h"
 
 namespace motif {
@@ -73,6 +74,10 @@ struct ChordBwdArgs {
   int B, H, Hkv, L, S, q_start, nqb, nkb;
   int cq, nsq, ckv, nskv, kv_direct;
   float scale, eps;
+  // window (WIN kernels): key blocks that hold first tokens, the chunks of `csink` query tiles behind
+  // their windows, those chunks' partials [nsc][H][B][nsb * 128][64], and the key rows of pk / pv
+  int window, sinks, nsb, nsc, csink, prows;
+  float *pks, *pvs;
 };
 
 // Key tiles the dQ workgroup of query block qb visits, and query tiles the dK / dV
@@ -82,6 +87,11 @@ __host__ __device__ inline int dq_tiles(int qb, int L, int q_start) {
   return (q_start + last + 1 + kT - 1) / kT;
 }
 __host__ __device__ inline int kv_first_tile(int kb, int q_start) { return std::max(0, kb * kBlk - q_start) / kT; }
+// End of the query tiles whose windows reach key block kb.
+__host__ __device__ inline int kv_window_end(int kb, int L, int q_start, int window) {
+  const int last = kb * kBlk + kBlk - 1 + window - 1 - q_start;  // the last query that sees its last key
+  return last < 0 ? 0 : std::min((L + kT - 1) / kT, last / kT + 1);
+}
 
 __device__ __forceinline__ f32x16 mma32(const bf16x8 &a, const bf16x8 &b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -149,13 +159,16 @@ __device__ __forceinline__ void stage_store(const Stage2 &g, int t, bf16_t *rows
 }
 
 // ------------------------------------------------------------------ dQ (+ Delta, parameter sums)
-template <bool ANY>
+template <bool ANY, bool WIN>
 __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
   const int h = blockIdx.x, qb = a.nqb - 1 - static_cast<int>(blockIdx.y);  // heaviest blocks first
   const int b = blockIdx.z / a.nsq, chunk = blockIdx.z - b * a.nsq;
-  const int ntiles = dq_tiles(qb, a.L, a.q_start);
-  const int t_begin = chunk * a.cq, t_end = min(ntiles, t_begin + a.cq);
-  if (t_begin >= t_end) return;
+  const int kv_end = min(a.S, a.q_start + min(a.L, qb * kBlk + kBlk));
+  // (a window's loop is one chunk, run over the tiles of the first tokens and of the block's windows)
+  const KeyWalk<kT> walk(WIN ? a.q_start + qb * kBlk : 0, kv_end, WIN ? a.window : kMaxWindow, WIN ? a.sinks : 0);
+  const int t_begin = WIN ? 0 : chunk * a.cq, t_end = WIN ? walk.count : min(dq_tiles(qb, a.L, a.q_start), t_begin + a.cq);
+  if (!WIN && t_begin >= t_end) return;
+  auto tile_at = [&](int x) { return WIN ? walk.tile(x) : x; };
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lc = lane & 31, hh = lane >> 5;
@@ -163,12 +176,11 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
   const int q0 = qb * kBlk + 32 * w;
   const int my_q = q0 + lc;
   const bool qv = my_q < a.L;
-  const int kv_end = min(a.S, a.q_start + min(a.L, qb * kBlk + kBlk));
   // waves 0, 1 stage K (rows and K^T), 2, 3 V (rows); the first tile's loads go ahead of the rest
   const bool kside = w < 2;
   const StageSrc<ANY> src(kside ? a.k + b * a.k_sb + kvh * a.k_sh : a.v + b * a.v_sb + kvh * a.v_sh, kside ? a.k_st : a.v_st,
                      kv_end, tid & 127);
-  Stage2 stg = src.load(t_begin * kT);
+  Stage2 stg = src.load(tile_at(t_begin) * kT);
   const int qr = min(my_q, a.L - 1);
 
   // this lane's query row: Q and dO as B operands (d = 16 ds + 8 hh .. +8), Delta
@@ -195,9 +207,10 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
   const float lam = a.log_n[b * a.ln_sb + int64_t(qr) * a.ln_st];
   const float sig = a.ssmax[h], al = a.alpha[h], be = a.beta[h], mu = a.mu[h];
   const float s = a.scale, c = sig * lam, cl = c * kLog2e, cs = c * s;
-  if (chunk == 0 && qv && hh == 0) a.rows[ri] = float4{lse2, delta, cl, cs};
+  if (!WIN && chunk == 0 && qv && hh == 0) a.rows[ri] = float4{lse2, delta, cl, cs};
   const int q_abs = a.q_start + my_q;
   const int wave_kv_end = a.q_start + min(a.L, q0 + 32);  // keys this wave sees: < wave_kv_end
+  const int k_max = WIN ? min(q_abs, a.S - 1) : q_abs;    // this query's last key
 
   __shared__ __attribute__((aligned(16))) bf16_t sK[2][kT * kRowP];    // K rows of the tile
   __shared__ __attribute__((aligned(16))) bf16_t sV[2][kT * kRowP];    // V rows
@@ -209,19 +222,34 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
   dqacc[0] = f32x16{};
   dqacc[1] = f32x16{};
   float sa = 0.f, sb = 0.f, sm = 0.f, ss = 0.f;
+  // WIN: sums of P (dP - Delta), P x, P r and P K, see below
+  float rho = 0.f, ea = 0.f, eb = 0.f, em = 0.f, es = 0.f;
+  f32x16 pkacc[2];
+  pkacc[0] = pkacc[1] = f32x16{};
 
-  auto store_kv = [&](const Stage2 &g, int buf) { stage_store(g, tid & 127, kside ? sK[buf] : sV[buf], kside ? sKT[buf] : nullptr); };
-  store_kv(stg, 0);
-  stg = src.load((t_begin + 1) * kT);  // (past the last tile: zeros)
+  auto store_kv = [&](Stage2 g, int buf, int x) {
+    if constexpr (WIN) {  // rows that no query of the block sees may hold anything: 0 * NaN
+      const int n0 = tile_at(x) * kT;
+      if (n0 < walk.lo && n0 + kT > a.sinks) {
+        const int r0 = n0 + 2 * (tid & 15);
+        const uint4 z = {0u, 0u, 0u, 0u};
+        if (r0 < walk.lo && r0 >= a.sinks) g.a = z;
+        if (r0 + 1 < walk.lo && r0 + 1 >= a.sinks) g.b = z;
+      }
+    }
+    stage_store(g, tid & 127, kside ? sK[buf] : sV[buf], kside ? sKT[buf] : nullptr);
+  };
+  store_kv(stg, 0, t_begin);
+  stg = src.load(tile_at(t_begin + 1) * kT);  // (past the last tile: zeros)
   __syncthreads();
 
   for (int kt = t_begin; kt < t_end; ++kt) {
-    const int n0 = kt * kT, buf = (kt - t_begin) & 1;
+    const int n0 = tile_at(kt) * kT, buf = (kt - t_begin) & 1;
     if (kt + 1 < t_end) {  // the next tile into the other buffer (free since the last barrier)
-      store_kv(stg, buf ^ 1);
-      stg = src.load(n0 + 2 * kT);
+      store_kv(stg, buf ^ 1, kt + 1);
+      stg = src.load(tile_at(kt + 2) * kT);
     }
-    if (n0 < wave_kv_end) {
+    if (n0 < wave_kv_end && (!WIN || n0 + kT - 1 > a.q_start + q0 - a.window || n0 < a.sinks)) {
       // window entry j (lane j < 63): distance d = key - q_abs = n0 - q_start - q0 - 31 + j
       {
         const int d = n0 - a.q_start - q0 - 31 + lane;
@@ -245,7 +273,7 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
         sacc = mma32(ko, qreg[ds], sacc);
         pacc = mma32(vo, dreg[ds], pacc);
       }
-      float dz[16];
+      float dz[16], pr[WIN ? 16 : 1];
       auto body = [&](auto masked) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -253,8 +281,17 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
           const float4 wv = sW[w][kk - lc + 31];
           const float rr = fmaf(s, sacc[r], wv.x);
           float p = fast_exp2(fmaf(cl, rr, -lse2));
-          if constexpr (decltype(masked)::value) p = (qv && n0 + kk <= q_abs) ? p : 0.f;
+          if constexpr (decltype(masked)::value)
+            p = (qv && n0 + kk <= k_max && (!WIN || n0 + kk > q_abs - a.window || n0 + kk < a.sinks)) ? p : 0.f;
           const float g = p * (pacc[r] - delta);
+          if constexpr (WIN) {
+            rho += g;
+            ea = fmaf(p, wv.y, ea);
+            eb = fmaf(p, wv.z, eb);
+            em = fmaf(p, wv.w, em);
+            es = fmaf(p, rr, es);
+            pr[r] = p;
+          }
           ss = fmaf(g, rr, ss);
           sa = fmaf(g, wv.y, sa);
           sb = fmaf(g, wv.z, sb);
@@ -262,8 +299,10 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
           dz[r] = g * cs;  // (rounded to bf16 with its factor, as the dK / dV kernel rounds it)
         }
       };
-      // every key of the tile at or before every query of the wave, all queries valid
-      if (n0 + kT - 1 <= a.q_start + q0 && q0 + 32 <= a.L) body(std::false_type{});
+      // every key of the tile at or before every query of the wave (and in its window), all queries valid
+      if (n0 + kT - 1 <= a.q_start + q0 && q0 + 32 <= a.L &&
+          (!WIN || (n0 + kT <= a.S && (n0 > a.q_start + q0 + 31 - a.window || n0 + kT <= a.sinks))))
+        body(std::false_type{});
       else body(std::true_type{});
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
@@ -272,10 +311,30 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
         for (int dt = 0; dt < 2; ++dt) {
           const bf16x8 kto = *reinterpret_cast<const bf16x8 *>(sKT[buf] + (32 * dt + lc) * kTRow + 16 * ks + 8 * hh);
           dqacc[dt] = mma32(kto, zb, dqacc[dt]);
+          if constexpr (WIN) pkacc[dt] = mma32(kto, pack8(pr + 8 * ks), pkacc[dt]);
         }
       }
     }
     __syncthreads();  // this tile's reads done, the next tile's stores visible
+  }
+
+  // Delta = dO . O carries O's rounding (2^-8 of a term).  The sum over a row's keys of P (dP - Delta)
+  // is 0, so what is left of it, rho, is the error of Delta: every sum of P (dP - Delta) x is put
+  // right by rho times that of P x, and the second kernel is given Delta + rho.  (2 x 2048 tokens, a
+  // window of 512, against 64 bits: dq and dk 4.6e-3 off without, 2e-3 with; alpha's gradient 1e-2
+  // and 2e-6.)
+  if constexpr (WIN) {
+    const auto s32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(rho), __float_as_uint(rho), false, false);
+    const float r = __uint_as_float(s32[0]) + __uint_as_float(s32[1]);
+    sa = fmaf(-r, ea, sa);
+    sb = fmaf(-r, eb, sb);
+    sm = fmaf(-r, em, sm);
+    ss = fmaf(-r, es, ss);
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dqacc[dt][i] = fmaf(-r * cs, pkacc[dt][i], dqacc[dt][i]);
+    if (qv && hh == 0) a.rows[ri] = float4{lse2, delta + r, cl, cs};
   }
 
   if (qv) {
@@ -311,14 +370,27 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
 }
 
 // ------------------------------------------------------------------ dK, dV
-template <bool ANY>
+template <bool ANY, bool WIN>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) chord_bwd_dkdv_kernel(ChordBwdArgs a) {
-  const int h = blockIdx.x, kb = blockIdx.y;
-  const int b = blockIdx.z / a.nskv, chunk = blockIdx.z - b * a.nskv;
+  // WIN: first the chunks behind the windows of the blocks that hold first tokens (the longest loops)
+  const int h = blockIdx.x, nsx = WIN ? a.nsb * a.nsc : 0;
+  const bool behind = WIN && static_cast<int>(blockIdx.y) < nsx;
+  const int kb = behind ? blockIdx.y / a.nsc : blockIdx.y - nsx;
+  const int b = WIN ? blockIdx.z : blockIdx.z / a.nskv;
+  const int chunk = !WIN ? blockIdx.z - b * a.nskv : behind ? blockIdx.y - kb * a.nsc : 0;
   const int qt_end = (a.L + kT - 1) / kT;
-  const int t_begin = kv_first_tile(kb, a.q_start) + chunk * a.ckv, t_end = min(qt_end, t_begin + a.ckv);
-  // a chunk with no tiles writes nothing, except that direct writes must cover every key
-  if (t_begin >= t_end && !(a.kv_direct && chunk == 0)) return;
+  int t_begin, t_end;
+  if constexpr (WIN) {
+    const int w_end = kv_window_end(kb, a.L, a.q_start, a.window);
+    t_begin = behind ? max(w_end, kv_first_tile(kb, a.q_start)) + chunk * a.csink : kv_first_tile(kb, a.q_start);
+    t_end = behind ? min(qt_end, t_begin + a.csink) : w_end;
+    if (behind && t_begin >= t_end) return;
+  } else {
+    t_begin = kv_first_tile(kb, a.q_start) + chunk * a.ckv;
+    t_end = min(qt_end, t_begin + a.ckv);
+    // a chunk with no tiles writes nothing, except that direct writes must cover every key
+    if (t_begin >= t_end && !(a.kv_direct && chunk == 0)) return;
+  }
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lc = lane & 31, hh = lane >> 5;
@@ -377,7 +449,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       rowv = load_row(i0 + 2 * kT);
     }
     // a wave whose keys all lie past the tile's last query (or past S) skips it
-    if (k0w < a.S && a.q_start + i0 + kT - 1 >= k0w) {
+    if (k0w < a.S && a.q_start + i0 + kT - 1 >= k0w &&
+        (!WIN || k0w + kT - 1 > a.q_start + i0 - a.window || k0w < a.sinks)) {
       {  // window entry j: distance key - q_abs = k0w - q_start - i0 - 31 + j
         const int d = k0w - a.q_start - i0 - 31 + lane;
         const float x = fabsf(static_cast<float>(d) - mu) + a.eps;
@@ -398,7 +471,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       float pv[16], dz[16];
       // the tile's queries that see this lane's key: q_lo .. q_lo + q_n - 1 (one compare per element)
       const int q_lo = max(0, my_k - a.q_start - i0);
-      const uint32_t q_n = kvld ? max(0, min(kT, a.L - i0) - q_lo) : 0;
+      const int q_hi = WIN && my_k >= a.sinks ? min(min(kT, a.L - i0), my_k + a.window - a.q_start - i0) : min(kT, a.L - i0);
+      const uint32_t q_n = kvld ? max(0, q_hi - q_lo) : 0;
       auto body = [&](auto masked) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -406,13 +480,17 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
           const float4 rw = sRow[buf][qq];
           const float rr = fmaf(s, sacc[r], sW[w][lc - qq + 31]);
           float p = fast_exp2(fmaf(rw.z, rr, -rw.x));
-          if constexpr (decltype(masked)::value) p = static_cast<uint32_t>(qq - q_lo) < q_n ? p : 0.f;
+          const bool ok = !decltype(masked)::value || static_cast<uint32_t>(qq - q_lo) < q_n;
+          p = ok ? p : 0.f;
           pv[r] = p;
           dz[r] = p * (pacc[r] - rw.y) * rw.w;
+          if constexpr (WIN) dz[r] = ok ? dz[r] : 0.f;  // (a row that no query sees may hold anything)
         }
       };
-      // every key of the wave at or before every query of the tile, all queries valid
-      if (k0w + 31 <= a.q_start + i0 && i0 + kT <= a.L) body(std::false_type{});
+      // every key of the wave at or before every query of the tile (and in its window), all queries valid
+      if (k0w + 31 <= a.q_start + i0 && i0 + kT <= a.L &&
+          (!WIN || (k0w + kT <= a.S && (k0w > a.q_start + i0 + kT - 1 - a.window || k0w + kT <= a.sinks))))
+        body(std::false_type{});
       else body(std::true_type{});
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
@@ -430,7 +508,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   }
 
   if (!kvld) return;
-  if (a.kv_direct) {
+  if (a.kv_direct && (!WIN || kb >= a.nsb)) {
     bf16_t *dk = a.dk + b * a.dk_sb + kvh * a.dk_sh + int64_t(my_k) * a.dk_st;
     bf16_t *dv = a.dv + b * a.dv_sb + kvh * a.dv_sh + int64_t(my_k) * a.dv_st;
 #pragma unroll
@@ -445,15 +523,17 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       }
     return;
   }
-  const size_t o = (((static_cast<size_t>(chunk) * a.H + h) * a.B + b) * a.S + my_k) * kBD;
+  const int rows = !WIN ? a.S : behind ? a.nsb * kBlk : a.prows;
+  const size_t o = (((static_cast<size_t>(chunk) * a.H + h) * a.B + b) * rows + my_k) * kBD;
+  float *pk = WIN && behind ? a.pks : a.pk, *pv = WIN && behind ? a.pvs : a.pv;
 #pragma unroll
   for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
     for (int q4 = 0; q4 < 4; ++q4) {
       const int d0 = 32 * dt + 8 * q4 + 4 * hh;
-      *reinterpret_cast<f32x4 *>(a.pk + o + d0) =
+      *reinterpret_cast<f32x4 *>(pk + o + d0) =
           f32x4{dkacc[dt][4 * q4], dkacc[dt][4 * q4 + 1], dkacc[dt][4 * q4 + 2], dkacc[dt][4 * q4 + 3]};
-      *reinterpret_cast<f32x4 *>(a.pv + o + d0) =
+      *reinterpret_cast<f32x4 *>(pv + o + d0) =
           f32x4{dvacc[dt][4 * q4], dvacc[dt][4 * q4 + 1], dvacc[dt][4 * q4 + 2], dvacc[dt][4 * q4 + 3]};
     }
 }
@@ -489,6 +569,46 @@ __device__ __forceinline__ void reduce_kv(const ChordBwdArgs &a, int block) {
   *reinterpret_cast<uint2 *>(dv) = uint2{pk2bf(vs[0], vs[1]), pk2bf(vs[2], vs[3])};
 }
 
+// The same for a window: the first a.prows keys' window partials (every key, or with kv_direct those
+// of the blocks that hold first tokens), then the chunks behind those blocks' windows, in order.
+__device__ __forceinline__ void reduce_kv_window(const ChordBwdArgs &a, int block) {
+  const int rows = min(a.prows, a.S);
+  const int64_t n4 = static_cast<int64_t>(a.B) * a.Hkv * rows * (kBD / 4);
+  const int64_t e = static_cast<int64_t>(block) * 256 + threadIdx.x;
+  if (e >= n4) return;
+  const int d0 = 4 * static_cast<int>(e % (kBD / 4));
+  const int64_t rest = e / (kBD / 4);
+  const int sk = static_cast<int>(rest % rows);
+  const int kvh = static_cast<int>((rest / rows) % a.Hkv), b = static_cast<int>(rest / (static_cast<int64_t>(rows) * a.Hkv));
+  const int G = a.H / a.Hkv, kb = sk / kBlk, qt_end = (a.L + kT - 1) / kT;
+  int ns = 0;
+  if (kb < a.nsb) {
+    const int first = max(kv_window_end(kb, a.L, a.q_start, a.window), kv_first_tile(kb, a.q_start));
+    ns = (max(0, qt_end - first) + a.csink - 1) / a.csink;
+  }
+  f32x4 ks = {0.f, 0.f, 0.f, 0.f}, vs = {0.f, 0.f, 0.f, 0.f};
+  for (int g = 0; g < G; ++g) {
+    const int h = kvh * G + g;
+    const size_t o = ((static_cast<size_t>(h) * a.B + b) * a.prows + sk) * kBD + d0;
+    f32x4 pk = *reinterpret_cast<const f32x4 *>(a.pk + o), pv = *reinterpret_cast<const f32x4 *>(a.pv + o);
+    for (int c = 0;; ++c) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ks[i] += pk[i];
+        vs[i] += pv[i];
+      }
+      if (c == ns) break;
+      const size_t oc = (((static_cast<size_t>(c) * a.H + h) * a.B + b) * (a.nsb * kBlk) + sk) * kBD + d0;
+      pk = *reinterpret_cast<const f32x4 *>(a.pks + oc);
+      pv = *reinterpret_cast<const f32x4 *>(a.pvs + oc);
+    }
+  }
+  bf16_t *dk = a.dk + b * a.dk_sb + kvh * a.dk_sh + int64_t(sk) * a.dk_st + d0;
+  bf16_t *dv = a.dv + b * a.dv_sb + kvh * a.dv_sh + int64_t(sk) * a.dv_st + d0;
+  *reinterpret_cast<uint2 *>(dk) = uint2{pk2bf(ks[0], ks[1]), pk2bf(ks[2], ks[3])};
+  *reinterpret_cast<uint2 *>(dv) = uint2{pk2bf(vs[0], vs[1]), pk2bf(vs[2], vs[3])};
+}
+
 // dQ = the sum over the chunks of the query's block, in order, rounded to bf16.
 __device__ __forceinline__ void reduce_q(const ChordBwdArgs &a, int block) {
   const int64_t n4 = static_cast<int64_t>(a.B) * a.H * a.L * (kBD / 4);
@@ -512,12 +632,13 @@ __device__ __forceinline__ void reduce_q(const ChordBwdArgs &a, int block) {
 
 // dparam[k][h] = the sum of the dQ workgroups' partials (batch rows, query blocks, chunks):
 // one wave per (k, h), lanes over (batch row, query block) in a fixed order.
+template <bool WIN>
 __device__ __forceinline__ void reduce_param(const ChordBwdArgs &a, int t) {
   const int h = t % a.H, k = t / a.H, lane = threadIdx.x & 63;
   float acc = 0.f;
   for (int e = lane; e < a.B * a.nqb; e += 64) {
     const int b = e / a.nqb, qb = e - b * a.nqb;
-    const int ns = (dq_tiles(qb, a.L, a.q_start) + a.cq - 1) / a.cq;
+    const int ns = WIN ? 1 : (dq_tiles(qb, a.L, a.q_start) + a.cq - 1) / a.cq;
     for (int c = 0; c < ns; ++c) acc += a.pparam[(((static_cast<size_t>(c) * a.B + b) * a.nqb + qb) * a.H + h) * 4 + k];
   }
   acc = wave_sum(acc);
@@ -527,12 +648,13 @@ __device__ __forceinline__ void reduce_param(const ChordBwdArgs &a, int t) {
 // Every reduction in one launch (three apart took 12.5 + 7.7 + 4.7 us at B = 2, 12 heads, 2048
 // tokens, most of it launch and tail): workgroups [0, nkv) dK / dV, then nq of dQ, then one of four
 // waves per four parameter sums.
+template <bool WIN>
 __global__ void __launch_bounds__(256) chord_bwd_reduce_kernel(ChordBwdArgs a, int nkv, int nq) {
   const int block = blockIdx.x;
-  if (block < nkv) return reduce_kv(a, block);
+  if (block < nkv) return WIN ? reduce_kv_window(a, block) : reduce_kv(a, block);
   if (block < nkv + nq) return reduce_q(a, block - nkv);
   const int t = 4 * (block - nkv - nq) + (threadIdx.x >> 6);
-  if (t < 4 * a.H) reduce_param(a, t);
+  if (t < 4 * a.H) reduce_param<WIN>(a, t);
 }
 
 }  // namespace
@@ -594,6 +716,41 @@ static BwdPlan plan_bwd(int B, int H, int Hkv, int L, int S, int q_start) {
   return p;
 }
 
+// The windowed backward: one chunk per query block and per key block (every block's loop is about as
+// long as its window), and for the blocks that hold first tokens chunks of the queries behind.
+struct WinBwdPlan {
+  int nqb, nkb, nsb, nsc, csink, prows;
+  bool kv_direct;
+  size_t off_param, off_pk, off_pv, off_pks, off_pvs, bytes;
+};
+
+static WinBwdPlan plan_bwd_window(int B, int H, int Hkv, int L, int S, int q_start, int window, int sinks) {
+  WinBwdPlan p{};
+  p.nqb = (L + kBlk - 1) / kBlk;
+  p.nkb = (S + kBlk - 1) / kBlk;
+  p.nsb = (std::min(sinks, S) + kBlk - 1) / kBlk;
+  const int qt_end = (L + kT - 1) / kT;
+  int most = 0;  // query tiles behind a window that see first tokens
+  for (int kb = 0; kb < p.nsb; ++kb)
+    most = std::max(most, qt_end - std::max(kv_window_end(kb, L, q_start, window), kv_first_tile(kb, q_start)));
+  // chunks about as long as a window's loop, at most 16 of them
+  p.csink = std::max({8, (window + kBlk) / kT, (most + 15) / 16});
+  p.nsc = (most + p.csink - 1) / p.csink;
+  p.kv_direct = H == Hkv;
+  p.prows = p.kv_direct ? p.nsb * kBlk : S;
+  auto al = [](size_t x) { return (x + 255) / 256 * 256; };
+  size_t off = al(static_cast<size_t>(B) * H * L * sizeof(float4));
+  p.off_param = off;
+  off += al(static_cast<size_t>(B) * p.nqb * H * 4 * sizeof(float));
+  const size_t row = static_cast<size_t>(H) * B * kBD * sizeof(float);
+  p.off_pk = off;
+  p.off_pv = off += al(row * p.prows);
+  p.off_pks = off += al(row * p.prows);
+  p.off_pvs = off += al(row * p.nsc * p.nsb * kBlk);
+  p.bytes = off + al(row * p.nsc * p.nsb * kBlk);
+  return p;
+}
+
 }  // namespace motif
 
 extern "C" size_t motif_chord_bwd_workspace_bytes(int B, int H, int Hkv, int L, int S, int q_start) {
@@ -628,7 +785,7 @@ extern "C" int motif_chord_bwd(
     z.H = H;
     z.cq = 1;
     z.dparam = dparam;
-    chord_bwd_reduce_kernel<<<dim3(H), dim3(256), 0, s>>>(z, 0, 0);
+    chord_bwd_reduce_kernel<false><<<dim3(H), dim3(256), 0, s>>>(z, 0, 0);
     return check_launch("chord_bwd_reduce_kernel");
   }
   if (!q || !k || !v || !out || !dout || !lse || !alpha || !beta || !mu || !ssmax || !log_n || !dq || !dk || !dv)
@@ -670,15 +827,109 @@ extern "C" int motif_chord_bwd(
   for (int64_t x : {k_st, v_st}) any |= S > 1 && (x < kBD || x >= kBufStride);
   int rc = MOTIF_OK;
   if (L > 0) {  // with no queries dK and dV are zero (the dK / dV pass below writes them)
-    (any ? chord_bwd_dq_kernel<true> : chord_bwd_dq_kernel<false>)<<<dim3(H, pl.nqb, B * pl.nsq), dim3(256), 0, s>>>(a);
+    (any ? chord_bwd_dq_kernel<true, false> : chord_bwd_dq_kernel<false, false>)<<<dim3(H, pl.nqb, B * pl.nsq), dim3(256), 0, s>>>(a);
     if ((rc = check_launch("chord_bwd_dq_kernel"))) return rc;
   }
-  (any ? chord_bwd_dkdv_kernel<true> : chord_bwd_dkdv_kernel<false>)<<<dim3(H, pl.nkb, B * pl.nskv), dim3(256), 0, s>>>(a);
+  (any ? chord_bwd_dkdv_kernel<true, false> : chord_bwd_dkdv_kernel<false, false>)<<<dim3(H, pl.nkb, B * pl.nskv), dim3(256), 0, s>>>(a);
   if ((rc = check_launch("chord_bwd_dkdv_kernel"))) return rc;
   auto blocks = [](int64_t rows) { return static_cast<int>((rows * (kBD / 4) + 255) / 256); };
   const int nkv = pl.kv_direct ? 0 : blocks(static_cast<int64_t>(B) * Hkv * S);
   const int nq = L > 0 && pl.nsq > 1 ? blocks(static_cast<int64_t>(B) * H * L) : 0;
-  chord_bwd_reduce_kernel<<<dim3(nkv + nq + H), dim3(256), 0, s>>>(a, nkv, nq);
+  chord_bwd_reduce_kernel<false><<<dim3(nkv + nq + H), dim3(256), 0, s>>>(a, nkv, nq);
   if ((rc = check_launch("chord_bwd_reduce_kernel"))) return rc;
   return MOTIF_OK;
+}
+
+extern "C" size_t motif_chord_window_bwd_workspace_bytes(int B, int H, int Hkv, int L, int S, int q_start, int window,
+                                                         int sinks) {
+  using namespace motif;
+  if (B <= 0 || H <= 0 || Hkv <= 0 || L < 0 || S < 0 || q_start < 0 || window < 1 || sinks < 0) return 0;
+  if (std::max<int64_t>(S, static_cast<int64_t>(q_start) + L) >= kMaxWindow) return 0;
+  return plan_bwd_window(B, H, Hkv, L, S, q_start, std::min(window, kMaxWindow), std::min(sinks, kMaxWindow)).bytes + 16;
+}
+
+extern "C" int motif_chord_window_bwd(
+    const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st,
+    const void *k, int64_t k_sb, int64_t k_sh, int64_t k_st,
+    const void *v, int64_t v_sb, int64_t v_sh, int64_t v_st,
+    const void *out, int64_t o_sb, int64_t o_sh, int64_t o_st,
+    const void *dout, int64_t d_sb, int64_t d_sh, int64_t d_st,
+    const float *lse, const float *alpha, const float *beta, const float *mu, const float *ssmax,
+    const float *log_n, int64_t ln_sb, int64_t ln_st,
+    void *dq, int64_t dq_sb, int64_t dq_sh, int64_t dq_st,
+    void *dk, int64_t dk_sb, int64_t dk_sh, int64_t dk_st,
+    void *dv, int64_t dv_sb, int64_t dv_sh, int64_t dv_st,
+    float *dparam, int B, int H, int Hkv, int L, int S, int D, int q_start, float scale, float eps,
+    int window, int sinks, void *workspace, size_t workspace_bytes, int dtype, void *stream) {
+  using namespace motif;
+  if (B < 0 || H <= 0 || Hkv <= 0 || L < 0 || S < 0 || H % Hkv != 0)
+    return set_error(MOTIF_ERR_INVALID, "chord_window_bwd: bad sizes");
+  if (dtype != MOTIF_BF16 || D != kBD)
+    return set_error(MOTIF_ERR_UNSUPPORTED, "chord_window_bwd: bf16 with head_dim 64 only");
+  if (q_start < 0 || window < 1 || sinks < 0)
+    return set_error(MOTIF_ERR_INVALID, "chord_window_bwd: need q_start >= 0, window >= 1 and sinks >= 0");
+  if (std::max<int64_t>(S, static_cast<int64_t>(q_start) + L) >= kMaxWindow || B > 65535)
+    return set_error(MOTIF_ERR_UNSUPPORTED, "chord_window_bwd: sequence too long or too many batch rows");
+  window = std::min(window, kMaxWindow);
+  sinks = std::min(sinks, kMaxWindow);
+  if (!dparam) return set_error(MOTIF_ERR_INVALID, "chord_window_bwd: NULL pointer");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (B == 0 || S == 0 || L == 0) {  // nothing to differentiate: zero parameter gradients (dq, dk, dv: the caller's)
+    ChordBwdArgs z{};
+    z.H = H;
+    z.cq = 1;
+    z.dparam = dparam;
+    chord_bwd_reduce_kernel<true><<<dim3(H), dim3(256), 0, s>>>(z, 0, 0);
+    return check_launch("chord_bwd_reduce_kernel");
+  }
+  if (!q || !k || !v || !out || !dout || !lse || !alpha || !beta || !mu || !ssmax || !log_n || !dq || !dk || !dv)
+    return set_error(MOTIF_ERR_INVALID, "chord_window_bwd: NULL pointer");
+  const int64_t st = q_sb | q_sh | q_st | k_sb | k_sh | k_st | v_sb | v_sh | v_st | o_sb | o_sh | o_st | d_sb | d_sh |
+                     d_st | dq_sb | dq_sh | dq_st | dk_sb | dk_sh | dk_st | dv_sb | dv_sh | dv_st;
+  const uintptr_t al = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+                       reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(dout) |
+                       reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv);
+  if ((st & 7) != 0 || (al & 15) != 0) return set_error(MOTIF_ERR_UNSUPPORTED, "chord_window_bwd: need 16-byte aligned rows");
+  const WinBwdPlan pl = plan_bwd_window(B, H, Hkv, L, S, q_start, window, sinks);
+  if (pl.nkb + pl.nsb * pl.nsc > 65535)
+    return set_error(MOTIF_ERR_UNSUPPORTED, "chord_window_bwd: sequence too long");
+  const size_t pad = -reinterpret_cast<uintptr_t>(workspace) & 15;  // (the size asked for holds it)
+  if (!workspace || workspace_bytes < pl.bytes + pad)
+    return set_error(MOTIF_ERR_INVALID, "chord_window_bwd: workspace too small (need " + std::to_string(pl.bytes + pad) + " bytes)");
+  ChordBwdArgs a{};
+  a.q = static_cast<const bf16_t *>(q); a.q_sb = q_sb; a.q_sh = q_sh; a.q_st = q_st;
+  a.k = static_cast<const bf16_t *>(k); a.k_sb = k_sb; a.k_sh = k_sh; a.k_st = k_st;
+  a.v = static_cast<const bf16_t *>(v); a.v_sb = v_sb; a.v_sh = v_sh; a.v_st = v_st;
+  a.o = static_cast<const bf16_t *>(out); a.o_sb = o_sb; a.o_sh = o_sh; a.o_st = o_st;
+  a.dout = static_cast<const bf16_t *>(dout); a.d_sb = d_sb; a.d_sh = d_sh; a.d_st = d_st;
+  a.lse = lse; a.alpha = alpha; a.beta = beta; a.mu = mu; a.ssmax = ssmax;
+  a.log_n = log_n; a.ln_sb = ln_sb; a.ln_st = ln_st;
+  a.dq = static_cast<bf16_t *>(dq); a.dq_sb = dq_sb; a.dq_sh = dq_sh; a.dq_st = dq_st;
+  a.dk = static_cast<bf16_t *>(dk); a.dk_sb = dk_sb; a.dk_sh = dk_sh; a.dk_st = dk_st;
+  a.dv = static_cast<bf16_t *>(dv); a.dv_sb = dv_sb; a.dv_sh = dv_sh; a.dv_st = dv_st;
+  a.dparam = dparam;
+  char *ws = static_cast<char *>(workspace) + pad;
+  a.rows = reinterpret_cast<float4 *>(ws);
+  a.pparam = reinterpret_cast<float *>(ws + pl.off_param);
+  a.pk = reinterpret_cast<float *>(ws + pl.off_pk);
+  a.pv = reinterpret_cast<float *>(ws + pl.off_pv);
+  a.B = B; a.H = H; a.Hkv = Hkv; a.L = L; a.S = S; a.q_start = q_start;
+  a.nqb = pl.nqb; a.nkb = pl.nkb;
+  a.nsq = a.nskv = 1; a.kv_direct = pl.kv_direct ? 1 : 0;
+  a.window = window; a.sinks = sinks; a.nsb = pl.nsb; a.nsc = pl.nsc; a.csink = pl.csink; a.prows = pl.prows;
+  a.pks = reinterpret_cast<float *>(ws + pl.off_pks);
+  a.pvs = reinterpret_cast<float *>(ws + pl.off_pvs);
+  a.scale = scale; a.eps = eps;
+  bool any = false;  // (a single row's stride is not used)
+  for (int64_t x : {q_st, d_st}) any |= L > 1 && (x < kBD || x >= kBufStride);
+  for (int64_t x : {k_st, v_st}) any |= S > 1 && (x < kBD || x >= kBufStride);
+  int rc = MOTIF_OK;
+  (any ? chord_bwd_dq_kernel<true, true> : chord_bwd_dq_kernel<false, true>)<<<dim3(H, pl.nqb, B), dim3(256), 0, s>>>(a);
+  if ((rc = check_launch("chord_bwd_dq_kernel"))) return rc;
+  (any ? chord_bwd_dkdv_kernel<true, true> : chord_bwd_dkdv_kernel<false, true>)<<<dim3(H, pl.nkb + pl.nsb * pl.nsc, B), dim3(256), 0, s>>>(a);
+  if ((rc = check_launch("chord_bwd_dkdv_kernel"))) return rc;
+  const int64_t red = static_cast<int64_t>(B) * Hkv * std::min(pl.prows, S) * (kBD / 4);
+  const int nkv = static_cast<int>((red + 255) / 256);
+  chord_bwd_reduce_kernel<true><<<dim3(nkv + H), dim3(256), 0, s>>>(a, nkv, 0);
+  return check_launch("chord_bwd_reduce_kernel");
 }

@@ -1,6 +1,20 @@
-// Entry points of Chord attention under a sliding window with visible first tokens, and over a 4-bit
-// cache: argument checks and the choice of kernel.  A query at position p sees the keys j <= p with
-// j > p - window or j < sinks; a row that sees none gives zeros.
+// Chord attention under a sliding window with visible first tokens (gfx950): the bf16 head-dim-64
+// prefill kernel, and the entry points of the windowed and the 4-bit forwards with the choice of
+// kernel.  A query at position p sees the keys j <= p with j > p - window or j < sinks; a row that
+// sees none gives zeros.
+//
+// chord_window_kernel: flash attention whose key loop visits the tiles that hold first tokens and
+// those that the block's windows reach, and no others.  With a window every query block has the same
+// work, so the workgroups are small and even: PARTS parts of two waves, a part taking its run of the
+// 32-key tiles.  A wave owns 32 score columns (16 queries of two heads that share a kv head, or 32 of
+// one head): S^T = K Q^T on v_mfma_f32_32x32x16_bf16, lane l column l % 32, register r of lane half h
+// key 8 (r / 4) + 4 h + r % 4; P^T enters O^T += V^T P^T from the same registers, V^T stored in LDS in
+// that key order.  K / V tiles are double buffered in LDS, one barrier a tile, the tile after next in
+// registers.  The distance bias, the diagonal and the window's edge are one value per distance: 47
+// (two heads) or 63 distances meet in a tile, 32 of them new, so each lane evaluates one per tile
+// (-inf where the distance is masked) into its wave's LDS row, and the score accumulators start from
+// it.  Tiles with first tokens are masked by key instead.  The row sums take P before its rounding to
+// bf16, so that the log-sum-exp the backward rebuilds P from is exact to fp32.
 #include <algorithm>
 #include <string>
 
@@ -11,6 +25,295 @@
 namespace motif {
 
 namespace {
+
+constexpr int kBD = 64;    // head dim
+constexpr int kT = 32;     // keys per tile
+constexpr int kRowK = 72;  // padded LDS row of 64 bf16: row-per-lane 16-byte reads without bank conflicts
+constexpr int kRowV = 40;  // padded LDS row of a V^T tile (32 keys)
+
+__device__ __forceinline__ f32x16 mma32(const bf16x8 &a, const bf16x8 &b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+// Position of key k (0..31) in a V^T row: the eight keys a lane half holds of each 16-key group together
+__device__ __forceinline__ int vperm(int k) { return (k & ~15) | ((k & 4) << 1) | ((k & 8) >> 1) | (k & 3); }
+typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
+typedef float f32x2v __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pk2bf(float x0, float x1) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2v){x0, x1}, bf16x2v));
+}
+
+template <int HPW, int PARTS>  // query heads per workgroup (of one kv head), key parts
+__global__ void __launch_bounds__(128 * PARTS) __attribute__((amdgpu_waves_per_eu(4, 4))) chord_window_kernel(ChordArgs a) {
+  constexpr int RH = HPW >= 2 ? 2 : 1;  // heads per wave
+  constexpr int RQ = 32 / RH;           // queries per wave
+  constexpr int HGW = HPW / RH;         // head groups per part
+  constexpr int QW = (2 / HGW) * RQ;    // queries per workgroup
+  constexpr int kWin = kT + RQ;         // bias row of a head (>= 31 + RQ entries)
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int part = wv >> 1, w = wv & 1;
+  const int htid = tid & 127;  // thread inside the part
+  const int lc = lane & 31, hh = lane >> 5;
+  const int hg = blockIdx.x, sq = blockIdx.z;
+
+  int batch = sq, tok0 = 0, Lq = a.L, Skv = a.S, q_start = a.q_start;
+  if (a.cu) {  // a packed sequence
+    batch = 0; tok0 = a.cu[sq]; Lq = a.cu[sq + 1] - tok0; Skv = Lq; q_start = 0;
+  }
+  const int qb0 = blockIdx.y * QW;
+  if (qb0 >= Lq) return;
+
+  const int head0 = hg * HPW + (w % HGW) * RH;  // the wave's first head
+  const int cq = lc % RQ, head = head0 + lc / RQ;
+  const int kvh = (hg * HPW) / (a.H / a.Hkv);
+  const int q0 = qb0 + (w / HGW) * RQ, my_q = q0 + cq, q_last = q0 + RQ - 1;
+  const bool q_valid = my_q < Lq;
+  const int kv_end = min(Skv, q_start + min(Lq, qb0 + QW));
+  const KeyWalk<kT> walk(q_start + qb0, kv_end, a.window, a.sinks);
+  const int nsteps = (walk.count + PARTS - 1) / PARTS;
+  const int t_first = part * nsteps, t_count = max(0, min(nsteps, walk.count - t_first));
+  const int wave_kv_end = min(Skv, q_start + min(Lq, q0 + RQ));
+
+  const bf16_t *kp = static_cast<const bf16_t *>(a.k) + batch * a.k_sb + kvh * a.k_sh + int64_t(tok0) * a.k_st;
+  const bf16_t *vp = static_cast<const bf16_t *>(a.v) + batch * a.v_sb + kvh * a.v_sh + int64_t(tok0) * a.v_st;
+
+  // logit = a_row acc with acc = rho q.k + kappa GGD, rho = sign(ssmax scale) (0 when scale is 0), kappa =
+  // sign(ssmax) / |scale| (sign(ssmax) when scale is 0), a_row = |ssmax log_n scale| (|ssmax log_n|);
+  // p = exp2(A (acc - m)), A = log2e a_row > 0 so that a masked key's -inf stays one
+  const float ssm = a.ssmax[head], sg = ssm < 0.f ? -1.f : 1.f;
+  const float rho = a.scale > 0.f ? sg : a.scale < 0.f ? -sg : 0.f;
+  const float lnv = a.log_n ? a.log_n[batch * a.ln_sb + int64_t(tok0 + min(my_q, Lq - 1)) * a.ln_st]
+                            : a.log_tab[q_start + min(my_q, Lq - 1)];
+  const float A = q_valid ? fmaxf(fabsf(ssm) * (a.scale != 0.f ? fabsf(a.scale) : 1.f) * lnv * kLog2e, 1e-30f) : 1.f;
+
+  bf16x8 qreg[4];  // rho Q^T, the B operand: features 16 ds + 8 hh .. of this lane's row
+  {
+    const bf16_t *qrow = static_cast<const bf16_t *>(a.q) + batch * a.q_sb + head * a.q_sh + int64_t(tok0 + min(my_q, Lq - 1)) * a.q_st;
+#pragma unroll
+    for (int ds = 0; ds < 4; ++ds) {
+      uint4 u = *reinterpret_cast<const uint4 *>(qrow + 16 * ds + 8 * hh);
+      if (rho < 0.f) { u.x ^= 0x80008000u; u.y ^= 0x80008000u; u.z ^= 0x80008000u; u.w ^= 0x80008000u; }
+      if (rho == 0.f || !q_valid) u = uint4{0u, 0u, 0u, 0u};
+      qreg[ds] = __builtin_bit_cast(bf16x8, u);
+    }
+  }
+
+  constexpr int kTileK = kT * kRowK, kTileV = kBD * kRowV;
+  constexpr int kStage = PARTS * 2 * (kTileK + kTileV), kMerge = (PARTS - 1) * 2 * 32 * 64 * 2;  // in bf16 elements
+  __shared__ __attribute__((aligned(16))) bf16_t sKV[kStage > kMerge ? kStage : kMerge];
+  __shared__ float sB[2 * PARTS][RH * kWin > 128 ? RH * kWin : 128];
+  auto sK = [&](int buf) { return sKV + (part * 2 + buf) * (kTileK + kTileV); };
+  auto sV = [&](int buf) { return sKV + (part * 2 + buf) * (kTileK + kTileV) + kTileK; };
+
+  // Bias rows: entry j of a head is distance key - q_abs = n0 - q_start - q0 - (RQ - 1) + j.  Lane l
+  // (head l / 32 of two) holds entry RQ - 1 + l % 32 of its tile in `bnew`; the first RQ - 1 entries are
+  // the last ones of the tile before (`bold`, 32 distances less), evaluated anew where that tile is not
+  // the one before or was masked by key.
+  const int bh = RH == 2 ? lane >> 5 : 0;
+  const float gal = a.alpha[head0 + bh], gbe = a.beta[head0 + bh], gmu = a.mu[head0 + bh];
+  const float gka = (a.ssmax[head0 + bh] < 0.f ? -1.f : 1.f) / (a.scale != 0.f ? fabsf(a.scale) : 1.f);
+  auto eval = [&](int t, int d) {  // for tile t
+    return d <= 0 && (d > -a.window || t * kT < a.sinks) ? gka * ggd_bias(static_cast<float>(d), gal, gbe, gmu, a.eps) : -INFINITY;
+  };
+  const int d0 = lc - q_start - q0;
+  float *bw = &sB[wv][bh * kWin];
+  auto store_bias = [&](float bnew, float bold) {
+    bw[RQ - 1 + lc] = bnew;
+    if (lc >= kT + 1 - RQ) bw[RQ - 1 + lc - kT] = bold;
+  };
+  // this lane's entries for keys 8 q4 + 4 hh + (0..3): j = 8 q4 + p + 4 hh - cq + RQ - 1
+  const float *bwr = &sB[wv][(lc / RQ) * kWin] + 4 * hh - cq + RQ - 1;
+
+  // Staging by the part's 128 threads: K rows htid / 8 and + 16; V rows 2 (htid % 16) and + 1 (8 features)
+  uint4 kst[2], vst[2];
+  const int krow = htid >> 3, vpair = htid & 15, vseg = htid >> 4;
+  const uint32_t koff = static_cast<uint32_t>((krow * a.k_st + (htid & 7) * 8) * 2), koff2 = koff + static_cast<uint32_t>(32 * a.k_st);
+  const uint32_t voff = static_cast<uint32_t>((2 * vpair * a.v_st + 8 * vseg) * 2), voff2 = voff + static_cast<uint32_t>(2 * a.v_st);
+  auto load_tile = [&](int t) {  // rows from kv_end on read zeros
+    const int rows = min(kT, kv_end - t * kT);
+    const buf_t kr = make_buf(kp + int64_t(t) * kT * a.k_st, rows > 0 ? static_cast<uint32_t>(((rows - 1) * a.k_st + kBD) * 2) : 0u);
+    const buf_t vr = make_buf(vp + int64_t(t) * kT * a.v_st, rows > 0 ? static_cast<uint32_t>(((rows - 1) * a.v_st + kBD) * 2) : 0u);
+    kst[0] = buf_ld16(kr, koff);
+    kst[1] = buf_ld16(kr, koff2);
+    vst[0] = buf_ld16(vr, voff);
+    vst[1] = buf_ld16(vr, voff2);
+  };
+  auto store_tile = [&](int t, int buf) {
+    const int n0 = t * kT;
+    if (n0 < walk.lo && n0 + kT > a.sinks) {  // rows that no query of the block sees may hold anything
+      auto dead = [&](int row) { return n0 + row < walk.lo && n0 + row >= a.sinks; };
+      const uint4 z{0u, 0u, 0u, 0u};
+      if (dead(krow)) kst[0] = z;
+      if (dead(krow + 16)) kst[1] = z;
+      if (dead(2 * vpair)) vst[0] = z;
+      if (dead(2 * vpair + 1)) vst[1] = z;
+    }
+    bf16_t *kd = sK(buf) + krow * kRowK + (htid & 7) * 8;
+    *reinterpret_cast<uint4 *>(kd) = kst[0];
+    *reinterpret_cast<uint4 *>(kd + 16 * kRowK) = kst[1];
+    const uint32_t v0[4] = {vst[0].x, vst[0].y, vst[0].z, vst[0].w}, v1[4] = {vst[1].x, vst[1].y, vst[1].z, vst[1].w};
+    bf16_t *vd = sV(buf) + 8 * vseg * kRowV + vperm(2 * vpair);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      *reinterpret_cast<uint32_t *>(vd + (2 * i) * kRowV) = (v0[i] & 0xffffu) | (v1[i] << 16);
+      *reinterpret_cast<uint32_t *>(vd + (2 * i + 1) * kRowV) = (v0[i] >> 16) | (v1[i] & 0xffff0000u);
+    }
+  };
+
+  float m_run = -INFINITY, l_run = 0.f;  // per column (m: acc units; l: this lane's share)
+  f32x16 oacc[2] = {f32x16{}, f32x16{}};  // O^T rows d = 32 dt + 8 (r / 4) + 4 hh + r % 4, column lc
+
+  load_tile(walk.tile(t_first));
+  store_tile(walk.tile(t_first), 0);
+  float bnew = eval(walk.tile(t_first), walk.tile(t_first) * kT + d0);
+  store_bias(bnew, eval(walk.tile(t_first), walk.tile(t_first) * kT + d0 - kT));
+  load_tile(walk.tile(t_first + 1));
+  __syncthreads();
+
+  for (int i = 0; i < nsteps; ++i) {
+    const int t = walk.tile(t_first + i), n0 = t * kT, buf = i & 1;
+    const int tn = walk.tile(t_first + i + 1);
+    // the next tile's new distances ahead of this tile's work
+    float bold = bnew;
+    bnew = eval(tn, tn * kT + d0);
+    if (tn != t + 1 || n0 < a.sinks) bold = eval(tn, tn * kT + d0 - kT);
+    if (i < t_count && n0 < wave_kv_end && (n0 + kT - 1 > q_start + q0 - a.window || n0 < a.sinks)) {
+      f32x16 acc;
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4)
+#pragma unroll
+        for (int p4 = 0; p4 < 4; ++p4) acc[4 * q4 + p4] = bwr[8 * q4 + p4];
+#pragma unroll
+      for (int ds = 0; ds < 4; ++ds) {
+        const bf16x8 kop = *reinterpret_cast<const bf16x8 *>(sK(buf) + lc * kRowK + 16 * ds + 8 * hh);
+        acc = mma32(kop, qreg[ds], acc);
+      }
+      // by key: tiles of first tokens at the window's edge, and the end of the keys
+      if ((n0 < a.sinks && n0 + kT > a.sinks && n0 <= q_start + q_last - a.window) || n0 + kT > Skv) {
+        const int q_abs = q_start + my_q;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = n0 + 8 * (r >> 2) + 4 * hh + (r & 3);
+          if (key >= Skv || (key <= q_abs - a.window && key >= a.sinks)) acc[r] = -INFINITY;
+        }
+      }
+      float mx = acc[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, acc[r]);
+      {
+        const auto s32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+        mx = fmaxf(__uint_as_float(s32[0]), __uint_as_float(s32[1]));
+      }
+      // the running max moves only when a tile passes it by more than 8 (log2 units), so p <= 2^8
+      const bool grow = A * (mx - m_run) > 8.f || m_run == -INFINITY;
+      const float m_new = grow ? mx : m_run;
+      const float m_use = m_new == -INFINITY ? 0.f : m_new;
+      if (__builtin_amdgcn_read_exec() & __ballot(grow)) {
+        const float resc = m_run == -INFINITY ? 0.f : fast_exp2(A * (m_run - m_use));
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          oacc[0][r] *= resc;
+          oacc[1][r] *= resc;
+        }
+        l_run *= resc;
+      }
+      m_run = m_new;
+      const float nb = -A * m_use;
+#pragma unroll
+      for (int hk = 0; hk < 2; ++hk) {
+        uint32_t pw[4];
+        float ps[2] = {0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p0 = fast_exp2(fmaf(acc[8 * hk + 2 * e], A, nb)), p1 = fast_exp2(fmaf(acc[8 * hk + 2 * e + 1], A, nb));
+          ps[0] += p0;
+          ps[1] += p1;
+          pw[e] = pk2bf(p0, p1);
+        }
+        l_run += ps[0] + ps[1];
+        const bf16x8 pb = __builtin_bit_cast(bf16x8, uint4{pw[0], pw[1], pw[2], pw[3]});
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt) {
+          const bf16x8 va = *reinterpret_cast<const bf16x8 *>(sV(buf) + (32 * dt + lc) * kRowV + 16 * hk + 8 * hh);
+          oacc[dt] = mma32(va, pb, oacc[dt]);
+        }
+      }
+    }
+    // the next tile's bias rows (this wave's own; its reads above come first) and rows into LDS (the
+    // other buffer, last read before the previous barrier), the tile after into flight
+    store_bias(bnew, bold);
+    store_tile(tn, buf ^ 1);
+    load_tile(walk.tile(t_first + i + 2));
+    __syncthreads();
+  }
+
+  {
+    const auto s32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
+    l_run = __uint_as_float(s32[0]) + __uint_as_float(s32[1]);
+  }
+
+  // Merge: parts 1 .. leave O^T over the tiles and (l, m) in their bias rows; part 0 writes the rows.
+  float *mo = reinterpret_cast<float *>(sKV) + lane;
+  if (part > 0) {
+    float *dst = mo + ((part - 1) * 2 + w) * 32 * 64;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      dst[r * 64] = oacc[0][r];
+      dst[(16 + r) * 64] = oacc[1][r];
+    }
+    sB[wv][lane] = l_run;
+    sB[wv][64 + lane] = m_run;
+  }
+  __syncthreads();
+  if (part == 0 && q_valid) {
+    float m = m_run;
+#pragma unroll
+    for (int p = 1; p < PARTS; ++p) m = fmaxf(m, sB[2 * p + w][64 + lane]);
+    float f[PARTS];
+    f[0] = m_run == -INFINITY ? 0.f : fast_exp2(A * (m_run - m));
+    float l = l_run * f[0];
+#pragma unroll
+    for (int p = 1; p < PARTS; ++p) {
+      const float mp = sB[2 * p + w][64 + lane];
+      f[p] = mp == -INFINITY ? 0.f : fast_exp2(A * (mp - m));
+      l = fmaf(sB[2 * p + w][lane], f[p], l);
+    }
+    const float inv = 1.f / fmaxf(l, 1e-20f);
+    bf16_t *op = static_cast<bf16_t *>(a.out) + batch * a.o_sb + head * a.o_sh + int64_t(tok0 + my_q) * a.o_st;
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        float o[4];
+#pragma unroll
+        for (int p4 = 0; p4 < 4; ++p4) {
+          const int r = 4 * q4 + p4;
+          float x = oacc[dt][r] * f[0];
+#pragma unroll
+          for (int p = 1; p < PARTS; ++p) x = fmaf(mo[(((p - 1) * 2 + w) * 32 + 16 * dt + r) * 64], f[p], x);
+          o[p4] = x * inv;
+        }
+        *reinterpret_cast<uint2 *>(op + 32 * dt + 8 * q4 + 4 * hh) = uint2{pk2bf(o[0], o[1]), pk2bf(o[2], o[3])};
+      }
+    if (a.lse && hh == 0)
+      a.lse[(static_cast<size_t>(batch) * a.H + head) * a.L + tok0 + my_q] = A * (m == -INFINITY ? 0.f : m) + fast_log2(l);
+  }
+}
+
+template <int HPW>
+int launch_window_h(const ChordArgs &a, int nseq, int max_len, hipStream_t s) {
+  constexpr int kQ = HPW == 4 ? 16 : HPW == 2 ? 32 : 64;
+  const dim3 grid(a.H / HPW, (max_len + kQ - 1) / kQ, nseq);
+  chord_window_kernel<HPW, 2><<<grid, dim3(256), 0, s>>>(a);
+  return check_launch("chord_window_kernel");
+}
+
+int launch_window(const ChordArgs &a, int nseq, int max_len, hipStream_t s) {
+  const int group = a.H / a.Hkv;
+  if (group % 4 == 0) return launch_window_h<4>(a, nseq, max_len, s);
+  if (group % 2 == 0) return launch_window_h<2>(a, nseq, max_len, s);
+  return launch_window_h<1>(a, nseq, max_len, s);
+}
 
 // Everything the three forward entries share: sizes, types, pointers, alignment; fills a.
 struct Call {
@@ -103,7 +406,9 @@ extern "C" int motif_chord_window_fwd(
   if (rc || B == 0 || L == 0) return rc;
   if ((rc = fill_rows(c, a, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st))) return rc;
   (void)workspace; (void)workspace_bytes;
-  return launch_chord_wide_window(a, dtype, D, static_cast<hipStream_t>(stream));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == MOTIF_BF16 && D == kBD && !length_dev && L <= 65535 * 16) return launch_window(a, B, L, st);
+  return launch_chord_wide_window(a, dtype, D, st);
 }
 
 extern "C" size_t motif_chord_window_workspace_bytes(int B, int H, int Hkv, int L, int S, int D, int window, int sinks,

@@ -111,6 +111,64 @@ class ChordFunction(torch.autograd.Function):
         return (*grads, None, None, None, None)
 
 
+class ChordWindowFunction(torch.autograd.Function):
+    '''ChordFunction under a window (no reference counterpart): the windowed forward with its
+    log-sum-exp, then motif_chord_window_bwd.  The inputs keep their strides.'''
+
+    @staticmethod
+    def forward(ctx, q, k, v, alpha, beta, mu, ssmax, log_n, q_start, scale, eps, window, sinks):
+        q, k, v = (_near(_aligned(t if t.stride(-1) == 1 else t.contiguous())) for t in (q, k, v))
+        params = [t.detach().contiguous() for t in (alpha, beta, mu, ssmax)]
+        ln = log_n.detach()
+        B, H, L, D = q.shape
+        out = torch.empty((B, L, H, D), dtype=q.dtype, device=q.device).transpose(1, 2)
+        lse = torch.empty((B, H, L), dtype=torch.float32, device=q.device)
+        _launch_window(q, k, v, params, ln, q_start, scale, eps, window, sinks, out, lse)
+        ctx.save_for_backward(q, k, v, out, lse, *params, ln)
+        ctx.args = q_start, scale, eps, window, sinks
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, out, lse, alpha, beta, mu, ssmax, ln = ctx.saved_tensors
+        q_start, scale, eps, window, sinks = ctx.args
+        B, H, L, D = q.shape
+        Hkv, S = k.shape[1], k.shape[2]
+        # (the kernels read dout's own rows, expanded ones too)
+        dout = _aligned(dout if dout.stride(-1) == 1 else dout.contiguous())
+        # gradients in storage of their own (an expanded input's would share elements)
+        dq = torch.empty((B, L, H, D), dtype=q.dtype, device=q.device).transpose(1, 2)
+        dk, dv = (torch.empty((B, Hkv, S, D), dtype=q.dtype, device=q.device) for _ in range(2))
+        d_params = torch.empty((4, H), dtype=torch.float32, device=q.device)
+        lib = _lib.lib()
+        with _lib.on_device(q.device):
+            n = int(lib.motif_chord_window_bwd_workspace_bytes(B, H, Hkv, L, S, q_start, window, sinks))
+            ws = torch.empty(max(n, 1), dtype=torch.uint8, device=q.device)
+            rc = lib.motif_chord_window_bwd(
+                *_lib.t4(q), *_lib.t4(k), *_lib.t4(v), *_lib.t4(out), *_lib.t4(dout),
+                lse.data_ptr(), alpha.data_ptr(), beta.data_ptr(), mu.data_ptr(), ssmax.data_ptr(),
+                ln.data_ptr(), ln.stride(0), ln.stride(1),
+                *_lib.t4(dq), *_lib.t4(dk), *_lib.t4(dv), d_params.data_ptr(),
+                B, H, Hkv, L, S, D, q_start, float(scale), float(eps), window, sinks,
+                ws.data_ptr(), ws.numel(), _lib.chord_dtype_code(q.dtype), _lib.stream_ptr(q.device))
+        _lib.check(rc, 'motif_chord_window_bwd')
+        grads = [dq, dk, dv, *d_params.unbind(0)]
+        grads = [g if need else None for g, need in zip(grads, ctx.needs_input_grad)]
+        return (*grads, *[None] * 6)
+
+
+def _window_grad_kernels_serve(q, k, v, alpha, beta, mu, ssmax, log_n):
+    '''As _grad_kernels_serve, for a window (any q_start >= 0; something to differentiate).'''
+    if not (q.is_cuda and q.dtype == torch.bfloat16 and k.dtype == q.dtype and v.dtype == q.dtype
+            and q.dim() == 4 and k.dim() == 4 and q.shape[-1] == HEAD_DIM and k.shape == v.shape
+            and k.shape[-1] == HEAD_DIM and q.shape[0] == k.shape[0] and q.shape[1] % max(k.shape[1], 1) == 0
+            and q.numel() and k.numel() and _lib.available()):
+        return False
+    if log_n.requires_grad or any(t.dtype != torch.float32 or t.dim() != 1 for t in (alpha, beta, mu, ssmax)):
+        return False
+    return log_n.dtype == torch.float32 and log_n.shape == (q.shape[0], q.shape[2])
+
+
 def _check_tensors(q, k, v, log_n):
     for name, t in (('q', q), ('k', k), ('v', v)):
         if not t.is_cuda:
@@ -316,7 +374,15 @@ def apply_chord_attention(
     if wants_grad(q, k, v, alpha, beta, mu, ssmax, log_n):
         if q_start is not None and int(q_start) < 0:
             raise ValueError(f'q_start must not be negative, got {q_start}')
-        if window is not None:
+        if window is not None and _window_grad_kernels_serve(q, k, v, alpha, beta, mu, ssmax, log_n):
+            _check_tensors(q, k, v, log_n)
+            _check_params(alpha, beta, mu, ssmax, q.shape[1])
+            scale = q.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale)
+            qs = k.shape[2] - q.shape[2] if q_start is None else int(q_start)
+            if qs < 0:
+                raise ValueError(f'q_start must not be negative, got {qs}')
+            res = ChordWindowFunction.apply(q, k, v, alpha, beta, mu, ssmax, log_n, qs, scale, float(eps), window, sinks)
+        elif window is not None:
             res = chord_attention_torch(q, k, v, alpha, beta, mu, ssmax, log_n, q_start, softmax_scale, eps, window, sinks)
         elif _grad_kernels_serve(q, k, v, alpha, beta, mu, ssmax, log_n, q_start):
             scale = q.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale)

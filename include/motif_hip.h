@@ -496,6 +496,28 @@ int motif_chord_window_fwd(
     int window, int sinks, void *workspace, size_t workspace_bytes, int dtype, void *stream);
 
 /*
+ * Gradients of motif_chord_window_fwd (bf16, head_dim 64, host positions): motif_chord_bwd's
+ * arguments and outputs with a window; q_start + L may pass S.  `lse` is the forward's.  A row
+ * that sees no key has a zero gradient and adds none.  The parameter gradients are fp32 sums
+ * that do not carry the rounding of `out` (the row sums of the softmax's gradient, which are
+ * 0, are used to take it out).  With L == 0 or S == 0 only dparam is written.
+ */
+size_t motif_chord_window_bwd_workspace_bytes(int B, int H, int Hkv, int L, int S, int q_start, int window, int sinks);
+int motif_chord_window_bwd(
+    const void *q, int64_t q_sb, int64_t q_sh, int64_t q_st,
+    const void *k, int64_t k_sb, int64_t k_sh, int64_t k_st,
+    const void *v, int64_t v_sb, int64_t v_sh, int64_t v_st,
+    const void *out, int64_t o_sb, int64_t o_sh, int64_t o_st,
+    const void *dout, int64_t d_sb, int64_t d_sh, int64_t d_st,
+    const float *lse, const float *alpha, const float *beta, const float *mu, const float *ssmax,
+    const float *log_n, int64_t ln_sb, int64_t ln_st,
+    void *dq, int64_t dq_sb, int64_t dq_sh, int64_t dq_st,
+    void *dk, int64_t dk_sb, int64_t dk_sh, int64_t dk_st,
+    void *dv, int64_t dv_sb, int64_t dv_sh, int64_t dv_st,
+    float *dparam, int B, int H, int Hkv, int L, int S, int D, int q_start, float scale, float eps,
+    int window, int sinks, void *workspace, size_t workspace_bytes, int dtype, void *stream);
+
+/*
  * Rows of a 4-bit key / value cache (no reference counterpart).  For each (batch row, kv head,
  * position) and for keys and values alike:
  *   codes  [B,Hkv,capacity,D/2] bytes: feature 2 m in the low half of byte m, 2 m + 1 in the high;
