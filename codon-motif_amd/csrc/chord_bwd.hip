@@ -38,6 +38,7 @@
 // 71 -> 45, 16 x 512 tokens 125 -> 88.
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "capi_internal.h"
 #include "chord_internal.h"
@@ -78,6 +79,9 @@ struct ChordBwdArgs {
   // their windows, those chunks' partials [nsc][H][B][nsb * 128][64], and the key rows of pk / pv
   int window, sinks, nsb, nsc, csink, prows;
   float *pks, *pvs;
+  const float2 *dist;  // [H][dist_n] {x^beta, x^beta log2 x} of distances 0, -1, .. (motif_chord_distances)
+  const float *dmu;    // [H][dist_n] x^(beta - 1) sign
+  int dist_n;
 };
 
 // Key tiles the dQ workgroup of query block qb visits, and query tiles the dK / dV
@@ -159,7 +163,9 @@ __device__ __forceinline__ void stage_store(const Stage2 &g, int t, bf16_t *rows
 }
 
 // ------------------------------------------------------------------ dQ (+ Delta, parameter sums)
-template <bool ANY, bool WIN>
+// WIN: with a window; MU: mu's gradient too (the layer's is frozen; it costs a window kernel 2 of 13
+// instructions per score).
+template <bool ANY, bool WIN, bool MU>
 __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
   const int h = blockIdx.x, qb = a.nqb - 1 - static_cast<int>(blockIdx.y);  // heaviest blocks first
   const int b = blockIdx.z / a.nsq, chunk = blockIdx.z - b * a.nsq;
@@ -207,6 +213,7 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
   const float lam = a.log_n[b * a.ln_sb + int64_t(qr) * a.ln_st];
   const float sig = a.ssmax[h], al = a.alpha[h], be = a.beta[h], mu = a.mu[h];
   const float s = a.scale, c = sig * lam, cl = c * kLog2e, cs = c * s;
+  const float cls = cl * s, cla = -cl * al;
   if (!WIN && chunk == 0 && qv && hh == 0) a.rows[ri] = float4{lse2, delta, cl, cs};
   const int q_abs = a.q_start + my_q;
   const int wave_kv_end = a.q_start + min(a.L, q0 + 32);  // keys this wave sees: < wave_kv_end
@@ -215,15 +222,17 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
   __shared__ __attribute__((aligned(16))) bf16_t sK[2][kT * kRowP];    // K rows of the tile
   __shared__ __attribute__((aligned(16))) bf16_t sV[2][kT * kRowP];    // V rows
   __shared__ __attribute__((aligned(16))) bf16_t sKT[2][kBD * kTRow];  // K^T, keys in tperm order
-  __shared__ float4 sW[4][64];  // per wave: {b, d/d alpha, d/d beta, d/d mu} per distance
+  // per wave and distance: {b, d/d alpha, d/d beta, d/d mu}; WIN: {x^beta, x^beta log2 x, d x^beta / d x sign}
+  using DistV = std::conditional_t<WIN && !MU, float2, float4>;
+  __shared__ DistV sW[4][64];
   __shared__ float sRed[4][4];
 
   f32x16 dqacc[2];
   dqacc[0] = f32x16{};
   dqacc[1] = f32x16{};
   float sa = 0.f, sb = 0.f, sm = 0.f, ss = 0.f;
-  // WIN: sums of P (dP - Delta), P x, P r and P K, see below
-  float rho = 0.f, ea = 0.f, eb = 0.f, em = 0.f, es = 0.f;
+  // WIN: sums of P (dP - Delta), P x, P S and P K, see below
+  float rho = 0.f, psum = 0.f, ea = 0.f, eb = 0.f, em = 0.f, es = 0.f;
   f32x16 pkacc[2];
   pkacc[0] = pkacc[1] = f32x16{};
 
@@ -239,6 +248,20 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
     }
     stage_store(g, tid & 127, kside ? sK[buf] : sV[buf], kside ? sKT[buf] : nullptr);
   };
+  // WIN: this lane's entry of tile x's window, d = key - q_abs = 32 x - q_start - q0 - 31 + lane, loaded a
+  // tile ahead (outside the table, where no query of the wave sees a key: zeros)
+  const buf_t dbuf = make_buf(WIN ? a.dist + static_cast<size_t>(h) * a.dist_n : nullptr, WIN ? a.dist_n * 8u : 0u);
+  const buf_t mbuf = make_buf(WIN ? a.dmu + static_cast<size_t>(h) * a.dist_n : nullptr, WIN && MU ? a.dist_n * 4u : 0u);
+  auto dist_at = [&](int x) {
+    const uint32_t i = static_cast<uint32_t>(a.q_start + q0 + 31 - lane - tile_at(x) * kT);
+    const uint32_t o = i < static_cast<uint32_t>(a.dist_n) ? i : 0x10000000u;
+    const uint2 u = buf_ld8(dbuf, 8u * o);
+    float4 r{__uint_as_float(u.x), __uint_as_float(u.y), 0.f, 0.f};
+    if constexpr (MU) r.z = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(mbuf, 4u * o, 0, 0));
+    return r;
+  };
+  float4 dnext{};
+  if constexpr (WIN) dnext = dist_at(t_begin);
   store_kv(stg, 0, t_begin);
   stg = src.load(tile_at(t_begin + 1) * kT);  // (past the last tile: zeros)
   __syncthreads();
@@ -249,9 +272,13 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
       store_kv(stg, buf ^ 1, kt + 1);
       stg = src.load(tile_at(kt + 2) * kT);
     }
+    const float4 dcur = dnext;
+    if constexpr (WIN) dnext = dist_at(kt + 1);
     if (n0 < wave_kv_end && (!WIN || n0 + kT - 1 > a.q_start + q0 - a.window || n0 < a.sinks)) {
       // window entry j (lane j < 63): distance d = key - q_abs = n0 - q_start - q0 - 31 + j
-      {
+      if constexpr (WIN && !MU) sW[w][lane] = float2{dcur.x, dcur.y};
+      else if constexpr (WIN) sW[w][lane] = dcur;
+      else {
         const int d = n0 - a.q_start - q0 - 31 + lane;
         const float x = fabsf(static_cast<float>(d) - mu) + a.eps;
         const float l2 = fast_log2(x);
@@ -274,29 +301,45 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
         pacc = mma32(vo, dreg[ds], pacc);
       }
       float dz[16], pr[WIN ? 16 : 1];
+      // WIN: the tile's keys that this query sees, kk <= m_hi and (kk > m_lo or kk < m_first)
+      const int m_hi = qv ? k_max - n0 : -1, m_lo = q_abs - a.window - n0, m_first = a.sinks - n0;
       auto body = [&](auto masked) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int kk = 8 * (r >> 2) + 4 * hh + (r & 3);
-          const float4 wv = sW[w][kk - lc + 31];
-          const float rr = fmaf(s, sacc[r], wv.x);
-          float p = fast_exp2(fmaf(cl, rr, -lse2));
-          if constexpr (decltype(masked)::value)
-            p = (qv && n0 + kk <= k_max && (!WIN || n0 + kk > q_abs - a.window || n0 + kk < a.sinks)) ? p : 0.f;
-          const float g = p * (pacc[r] - delta);
+          const DistV wv = sW[w][kk - lc + 31];
           if constexpr (WIN) {
+            // log2e c r = cls S + cla x^beta; the sums of g r, g b and g b ln x follow from those of g S,
+            // g x^beta and g x^beta log2 x
+            // (the two large terms that cancel first: what is left is of the bias's size)
+            float p = fast_exp2(fmaf(cla, wv.x, fmaf(cls, sacc[r], -lse2)));
+            if constexpr (decltype(masked)::value) p = ((kk <= m_hi) & ((kk > m_lo) | (kk < m_first))) ? p : 0.f;
+            const float g = p * (pacc[r] - delta);
+            psum += p;
             rho += g;
-            ea = fmaf(p, wv.y, ea);
-            eb = fmaf(p, wv.z, eb);
-            em = fmaf(p, wv.w, em);
-            es = fmaf(p, rr, es);
+            ss = fmaf(g, sacc[r], ss);
+            sa = fmaf(g, wv.x, sa);
+            sb = fmaf(g, wv.y, sb);
+            es = fmaf(p, sacc[r], es);
+            ea = fmaf(p, wv.x, ea);
+            eb = fmaf(p, wv.y, eb);
+            if constexpr (MU) {
+              sm = fmaf(g, wv.z, sm);
+              em = fmaf(p, wv.z, em);
+            }
             pr[r] = p;
+            dz[r] = g * cs;
+          } else {
+            const float rr = fmaf(s, sacc[r], wv.x);
+            float p = fast_exp2(fmaf(cl, rr, -lse2));
+            if constexpr (decltype(masked)::value) p = (qv && n0 + kk <= q_abs) ? p : 0.f;
+            const float g = p * (pacc[r] - delta);
+            ss = fmaf(g, rr, ss);
+            sa = fmaf(g, wv.y, sa);
+            sb = fmaf(g, wv.z, sb);
+            sm = fmaf(g, wv.w, sm);
+            dz[r] = g * cs;  // (rounded to bf16 with its factor, as the dK / dV kernel rounds it)
           }
-          ss = fmaf(g, rr, ss);
-          sa = fmaf(g, wv.y, sa);
-          sb = fmaf(g, wv.z, sb);
-          sm = fmaf(g, wv.w, sm);
-          dz[r] = g * cs;  // (rounded to bf16 with its factor, as the dK / dV kernel rounds it)
         }
       };
       // every key of the tile at or before every query of the wave (and in its window), all queries valid
@@ -320,16 +363,23 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
 
   // Delta = dO . O carries O's rounding (2^-8 of a term).  The sum over a row's keys of P (dP - Delta)
   // is 0, so what is left of it, rho, is the error of Delta: every sum of P (dP - Delta) x is put
-  // right by rho times that of P x, and the second kernel is given Delta + rho.  (2 x 2048 tokens, a
-  // window of 512, against 64 bits: dq and dk 4.6e-3 off without, 2e-3 with; alpha's gradient 1e-2
-  // and 2e-6.)
+  // right by rho times that of P x, and the second kernel is given Delta + rho.  The weights' own sum
+  // takes the log-sum-exp's fp32 rounding (1e-6 of a weight) out of the parameter sums.  (2 x 2048
+  // tokens, a window of 512, against 64 bits: dq and dk 4.6e-3 off without, 2.4e-3 with; alpha's
+  // gradient 1e-2 and 1e-6.)
   if constexpr (WIN) {
-    const auto s32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(rho), __float_as_uint(rho), false, false);
-    const float r = __uint_as_float(s32[0]) + __uint_as_float(s32[1]);
-    sa = fmaf(-r, ea, sa);
-    sb = fmaf(-r, eb, sb);
-    sm = fmaf(-r, em, sm);
-    ss = fmaf(-r, es, ss);
+    auto both = [](float x) {  // over the two lane halves
+      const auto s32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+      return __uint_as_float(s32[0]) + __uint_as_float(s32[1]);
+    };
+    const float ps = both(psum), inv = ps > 0.f ? 1.f / ps : 0.f, r = both(rho) * inv;
+    sa = fmaf(-r, ea, sa) * inv;
+    sb = fmaf(-r, eb, sb) * inv;
+    ss = fmaf(-r, es, ss) * inv;
+    ss = fmaf(s, ss, -al * sa);             // r = s S + b, b = -alpha x^beta
+    sa = -sa;                               // d b / d alpha
+    sb = sb * (-al * 0.6931471805599453f);  // d b / d beta = b ln x
+    if constexpr (MU) sm = fmaf(-r, em, sm) * inv * (al * be);
 #pragma unroll
     for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
@@ -436,6 +486,15 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     stage_store(g, tid & 127, qside ? sQ[buf] : sD[buf], qside ? sQT[buf] : sDT[buf]);
     if (tid < kT) sRow[buf][tid] = rv;
   };
+  // WIN: this lane's entry of the window of query tile qt, distance k0w - q_start - 32 qt - 31 + lane
+  const buf_t dbuf = make_buf(WIN ? a.dist + static_cast<size_t>(h) * a.dist_n : nullptr, WIN ? a.dist_n * 8u : 0u);
+  auto dist_at = [&](int qt) {
+    const uint32_t i = static_cast<uint32_t>(a.q_start + qt * kT + 31 - lane - k0w);
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+                                         dbuf, 8u * (i < static_cast<uint32_t>(a.dist_n) ? i : 0x10000000u), 0, 0));
+  };
+  float dnext = 0.f;
+  if constexpr (WIN) dnext = dist_at(t_begin);
   store_q(stg, rowv, 0);
   stg = src.load((t_begin + 1) * kT);
   rowv = load_row((t_begin + 1) * kT);
@@ -448,10 +507,15 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       stg = src.load(i0 + 2 * kT);
       rowv = load_row(i0 + 2 * kT);
     }
+    const float dcur = dnext;
+    if constexpr (WIN) dnext = dist_at(qt + 1);
     // a wave whose keys all lie past the tile's last query (or past S) skips it
     if (k0w < a.S && a.q_start + i0 + kT - 1 >= k0w &&
         (!WIN || k0w + kT - 1 > a.q_start + i0 - a.window || k0w < a.sinks)) {
-      {  // window entry j: distance key - q_abs = k0w - q_start - i0 - 31 + j
+      // window entry j: distance key - q_abs = k0w - q_start - i0 - 31 + j
+      if constexpr (WIN) {
+        sW[w][lane] = -al * dcur;
+      } else {
         const int d = k0w - a.q_start - i0 - 31 + lane;
         const float x = fabsf(static_cast<float>(d) - mu) + a.eps;
         sW[w][lane] = d <= 0 ? -al * fast_exp2(be * fast_log2(x)) : 0.f;
@@ -827,7 +891,7 @@ extern "C" int motif_chord_bwd(
   for (int64_t x : {k_st, v_st}) any |= S > 1 && (x < kBD || x >= kBufStride);
   int rc = MOTIF_OK;
   if (L > 0) {  // with no queries dK and dV are zero (the dK / dV pass below writes them)
-    (any ? chord_bwd_dq_kernel<true, false> : chord_bwd_dq_kernel<false, false>)<<<dim3(H, pl.nqb, B * pl.nsq), dim3(256), 0, s>>>(a);
+    (any ? chord_bwd_dq_kernel<true, false, true> : chord_bwd_dq_kernel<false, false, true>)<<<dim3(H, pl.nqb, B * pl.nsq), dim3(256), 0, s>>>(a);
     if ((rc = check_launch("chord_bwd_dq_kernel"))) return rc;
   }
   (any ? chord_bwd_dkdv_kernel<true, false> : chord_bwd_dkdv_kernel<false, false>)<<<dim3(H, pl.nkb, B * pl.nskv), dim3(256), 0, s>>>(a);
@@ -860,7 +924,8 @@ extern "C" int motif_chord_window_bwd(
     void *dk, int64_t dk_sb, int64_t dk_sh, int64_t dk_st,
     void *dv, int64_t dv_sb, int64_t dv_sh, int64_t dv_st,
     float *dparam, int B, int H, int Hkv, int L, int S, int D, int q_start, float scale, float eps,
-    int window, int sinks, void *workspace, size_t workspace_bytes, int dtype, void *stream) {
+    int window, int sinks, int need_mu, const float *distances, int distances_len,
+    void *workspace, size_t workspace_bytes, int dtype, void *stream) {
   using namespace motif;
   if (B < 0 || H <= 0 || Hkv <= 0 || L < 0 || S < 0 || H % Hkv != 0)
     return set_error(MOTIF_ERR_INVALID, "chord_window_bwd: bad sizes");
@@ -882,8 +947,10 @@ extern "C" int motif_chord_window_bwd(
     chord_bwd_reduce_kernel<true><<<dim3(H), dim3(256), 0, s>>>(z, 0, 0);
     return check_launch("chord_bwd_reduce_kernel");
   }
-  if (!q || !k || !v || !out || !dout || !lse || !alpha || !beta || !mu || !ssmax || !log_n || !dq || !dk || !dv)
+  if (!q || !k || !v || !out || !dout || !lse || !alpha || !beta || !mu || !ssmax || !log_n || !dq || !dk || !dv || !distances)
     return set_error(MOTIF_ERR_INVALID, "chord_window_bwd: NULL pointer");
+  if (distances_len < motif_chord_distances_len(L, q_start, window, sinks) || distances_len >= (1 << 28))
+    return set_error(MOTIF_ERR_INVALID, "chord_window_bwd: distance table too short (or too long)");
   const int64_t st = q_sb | q_sh | q_st | k_sb | k_sh | k_st | v_sb | v_sh | v_st | o_sb | o_sh | o_st | d_sb | d_sh |
                      d_st | dq_sb | dq_sh | dq_st | dk_sb | dk_sh | dk_st | dv_sb | dv_sh | dv_st;
   const uintptr_t al = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
@@ -916,6 +983,9 @@ extern "C" int motif_chord_window_bwd(
   a.B = B; a.H = H; a.Hkv = Hkv; a.L = L; a.S = S; a.q_start = q_start;
   a.nqb = pl.nqb; a.nkb = pl.nkb;
   a.nsq = a.nskv = 1; a.kv_direct = pl.kv_direct ? 1 : 0;
+  a.dist = reinterpret_cast<const float2 *>(distances);
+  a.dmu = distances + 2 * static_cast<size_t>(H) * distances_len;
+  a.dist_n = distances_len;
   a.window = window; a.sinks = sinks; a.nsb = pl.nsb; a.nsc = pl.nsc; a.csink = pl.csink; a.prows = pl.prows;
   a.pks = reinterpret_cast<float *>(ws + pl.off_pks);
   a.pvs = reinterpret_cast<float *>(ws + pl.off_pvs);
@@ -924,7 +994,9 @@ extern "C" int motif_chord_window_bwd(
   for (int64_t x : {q_st, d_st}) any |= L > 1 && (x < kBD || x >= kBufStride);
   for (int64_t x : {k_st, v_st}) any |= S > 1 && (x < kBD || x >= kBufStride);
   int rc = MOTIF_OK;
-  (any ? chord_bwd_dq_kernel<true, true> : chord_bwd_dq_kernel<false, true>)<<<dim3(H, pl.nqb, B), dim3(256), 0, s>>>(a);
+  const dim3 grid_q(H, pl.nqb, B);
+  if (any) (need_mu ? chord_bwd_dq_kernel<true, true, true> : chord_bwd_dq_kernel<true, true, false>)<<<grid_q, dim3(256), 0, s>>>(a);
+  else (need_mu ? chord_bwd_dq_kernel<false, true, true> : chord_bwd_dq_kernel<false, true, false>)<<<grid_q, dim3(256), 0, s>>>(a);
   if ((rc = check_launch("chord_bwd_dq_kernel"))) return rc;
   (any ? chord_bwd_dkdv_kernel<true, true> : chord_bwd_dkdv_kernel<false, true>)<<<dim3(H, pl.nkb + pl.nsb * pl.nsc, B), dim3(256), 0, s>>>(a);
   if ((rc = check_launch("chord_bwd_dkdv_kernel"))) return rc;

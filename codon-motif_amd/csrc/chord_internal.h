@@ -31,6 +31,9 @@ struct ChordArgs {
   // sliding window (windowed kernels): a query at position p sees the keys j <= p with
   // j > p - window or j < sinks
   int window, sinks;
+  // distances 0, -1, ... -(dist_n - 1) of each head: {x^beta, x^beta log2 x}, or null
+  const float2 *dist;
+  int dist_n;
 };
 
 // Longest window and most first tokens a launch takes (positions stay below it as well), so that

@@ -42,7 +42,21 @@ __device__ __forceinline__ uint32_t pk2bf(float x0, float x1) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2v){x0, x1}, bf16x2v));
 }
 
-template <int HPW, int PARTS>  // query heads per workgroup (of one kv head), key parts
+// x^beta and its derivatives' factors at distances d = 0, -1, .. of a head, x = |d - mu| + eps:
+// dist[h][-d] = {x^beta, x^beta log2 x}, dmu[h][-d] = x^(beta - 1) sign(d - mu).  In 64 bits and rounded
+// once: through fp32 log2 and exp2 the power is 3e-7 off, which the scaled logits turn into 1e-5 of a
+// weight, and the parameter gradients are small differences of sums over weights.
+__global__ void __launch_bounds__(256) chord_distance_kernel(const float *beta, const float *mu, float eps, float2 *dist,
+                                                             float *dmu, int n) {
+  const int h = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const double e = -static_cast<double>(i) - mu[h], x = fabs(e) + eps, l = log2(x), p = exp2(beta[h] * l);
+  const size_t o = static_cast<size_t>(h) * n + i;
+  dist[o] = float2{static_cast<float>(p), static_cast<float>(p * l)};
+  dmu[o] = e == 0. ? 0.f : static_cast<float>(e > 0. ? p / x : -p / x);
+}
+
+template <int HPW, int PARTS, bool TAB>  // query heads per workgroup (of one kv head), key parts, distances from a.dist
 __global__ void __launch_bounds__(128 * PARTS) __attribute__((amdgpu_waves_per_eu(4, 4))) chord_window_kernel(ChordArgs a) {
   constexpr int RH = HPW >= 2 ? 2 : 1;  // heads per wave
   constexpr int RQ = 32 / RH;           // queries per wave
@@ -112,8 +126,18 @@ __global__ void __launch_bounds__(128 * PARTS) __attribute__((amdgpu_waves_per_e
   const int bh = RH == 2 ? lane >> 5 : 0;
   const float gal = a.alpha[head0 + bh], gbe = a.beta[head0 + bh], gmu = a.mu[head0 + bh];
   const float gka = (a.ssmax[head0 + bh] < 0.f ? -1.f : 1.f) / (a.scale != 0.f ? fabsf(a.scale) : 1.f);
+  const buf_t dbuf = make_buf(a.dist, TAB ? static_cast<uint32_t>(a.H) * static_cast<uint32_t>(a.dist_n) * 8u : 0u);
+  const uint32_t dhead = static_cast<uint32_t>(head0 + bh) * static_cast<uint32_t>(a.dist_n);
   auto eval = [&](int t, int d) {  // for tile t
-    return d <= 0 && (d > -a.window || t * kT < a.sinks) ? gka * ggd_bias(static_cast<float>(d), gal, gbe, gmu, a.eps) : -INFINITY;
+    const bool ok = d <= 0 && (d > -a.window || t * kT < a.sinks);
+    float bias;
+    if constexpr (TAB) {  // (a masked distance may lie past the table: entry 0 is read instead)
+      bias = -gal * __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+                        dbuf, 8u * (dhead + static_cast<uint32_t>(ok ? -d : 0)), 0, 0));
+    } else {
+      bias = ggd_bias(static_cast<float>(d), gal, gbe, gmu, a.eps);
+    }
+    return ok ? gka * bias : -INFINITY;
   };
   const int d0 = lc - q_start - q0;
   float *bw = &sB[wv][bh * kWin];
@@ -190,11 +214,12 @@ __global__ void __launch_bounds__(128 * PARTS) __attribute__((amdgpu_waves_per_e
       }
       // by key: tiles of first tokens at the window's edge, and the end of the keys
       if ((n0 < a.sinks && n0 + kT > a.sinks && n0 <= q_start + q_last - a.window) || n0 + kT > Skv) {
-        const int q_abs = q_start + my_q;
+        // (kk from Skv on, or outside the window without being a first token)
+        const int e = Skv - n0 - 4 * hh, lo = q_start + my_q - a.window - n0 - 4 * hh, first = a.sinks - n0 - 4 * hh;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int key = n0 + 8 * (r >> 2) + 4 * hh + (r & 3);
-          if (key >= Skv || (key <= q_abs - a.window && key >= a.sinks)) acc[r] = -INFINITY;
+          const int kk = 8 * (r >> 2) + (r & 3);
+          acc[r] = (kk < e) & ((kk > lo) | (kk < first)) ? acc[r] : -INFINITY;
         }
       }
       float mx = acc[0];
@@ -304,7 +329,7 @@ template <int HPW>
 int launch_window_h(const ChordArgs &a, int nseq, int max_len, hipStream_t s) {
   constexpr int kQ = HPW == 4 ? 16 : HPW == 2 ? 32 : 64;
   const dim3 grid(a.H / HPW, (max_len + kQ - 1) / kQ, nseq);
-  chord_window_kernel<HPW, 2><<<grid, dim3(256), 0, s>>>(a);
+  (a.dist ? chord_window_kernel<HPW, 2, true> : chord_window_kernel<HPW, 2, false>)<<<grid, dim3(256), 0, s>>>(a);
   return check_launch("chord_window_kernel");
 }
 
@@ -314,6 +339,9 @@ int launch_window(const ChordArgs &a, int nseq, int max_len, hipStream_t s) {
   if (group % 2 == 0) return launch_window_h<2>(a, nseq, max_len, s);
   return launch_window_h<1>(a, nseq, max_len, s);
 }
+
+// Distances that the queries of a call meet: those of a window, or with first tokens all of them.
+int distance_count(int L, int q_start, int window, int sinks) { return sinks > 0 ? q_start + L : std::min(window, q_start + L); }
 
 // Everything the three forward entries share: sizes, types, pointers, alignment; fills a.
 struct Call {
@@ -397,7 +425,8 @@ extern "C" int motif_chord_window_fwd(
     const float *log_n, int64_t ln_sb, int64_t ln_st, const float *log_table, int log_table_len,
     void *out, int64_t o_sb, int64_t o_sh, int64_t o_st, float *lse,
     int *length_dev, int B, int H, int Hkv, int L, int S, int D, int q_start, float scale, float eps,
-    int window, int sinks, void *workspace, size_t workspace_bytes, int dtype, void *stream) {
+    int window, int sinks, const float *distances, int distances_len, void *workspace, size_t workspace_bytes, int dtype,
+    void *stream) {
   const Call c{"chord_window_fwd", q, q_sb, q_sh, q_st, alpha, beta, mu, ssmax, log_n, ln_sb, ln_st, log_table,
                log_table_len, out, o_sb, o_sh, o_st, lse, length_dev, B, H, Hkv, L, S, D, q_start, scale, eps,
                window, sinks, dtype};
@@ -407,8 +436,28 @@ extern "C" int motif_chord_window_fwd(
   if ((rc = fill_rows(c, a, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st))) return rc;
   (void)workspace; (void)workspace_bytes;
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (distances && distances_len < distance_count(L, q_start, window, sinks))
+    return set_error(MOTIF_ERR_INVALID, "chord_window_fwd: distance table too short");
+  a.dist = reinterpret_cast<const float2 *>(distances);
+  a.dist_n = distances_len;
+  if (static_cast<int64_t>(H) * distances_len >= (int64_t(1) << 29)) a.dist = nullptr;  // (past 32-bit offsets: evaluated)
   if (dtype == MOTIF_BF16 && D == kBD && !length_dev && L <= 65535 * 16) return launch_window(a, B, L, st);
   return launch_chord_wide_window(a, dtype, D, st);
+}
+
+extern "C" int motif_chord_distances_len(int L, int q_start, int window, int sinks) {
+  if (L <= 0 || q_start < 0 || window < 1 || sinks < 0 || static_cast<int64_t>(q_start) + L >= kMaxWindow) return 0;
+  return distance_count(L, q_start, window, sinks);
+}
+
+extern "C" int motif_chord_distances(const float *beta, const float *mu, int H, int n, float eps, float *out, void *stream) {
+  if (H < 0 || n < 0 || H > 65535) return set_error(MOTIF_ERR_INVALID, "chord_distances: bad size");
+  if (H == 0 || n == 0) return MOTIF_OK;
+  if (!beta || !mu || !out) return set_error(MOTIF_ERR_INVALID, "chord_distances: NULL pointer");
+  if (reinterpret_cast<uintptr_t>(out) & 7) return set_error(MOTIF_ERR_INVALID, "chord_distances: out must be 8-byte aligned");
+  chord_distance_kernel<<<dim3((n + 255) / 256, H), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
+      beta, mu, eps, reinterpret_cast<float2 *>(out), out + 2 * static_cast<size_t>(H) * n, n);
+  return check_launch("chord_distance_kernel");
 }
 
 extern "C" size_t motif_chord_window_workspace_bytes(int B, int H, int Hkv, int L, int S, int D, int window, int sinks,

@@ -123,14 +123,21 @@ class ChordWindowFunction(torch.autograd.Function):
         B, H, L, D = q.shape
         out = torch.empty((B, L, H, D), dtype=q.dtype, device=q.device).transpose(1, 2)
         lse = torch.empty((B, H, L), dtype=torch.float32, device=q.device)
-        _launch_window(q, k, v, params, ln, q_start, scale, eps, window, sinks, out, lse)
-        ctx.save_for_backward(q, k, v, out, lse, *params, ln)
+        lib = _lib.lib()
+        n = lib.motif_chord_distances_len(L, q_start, window, sinks)
+        distances = torch.empty(3 * H * n, dtype=torch.float32, device=q.device)
+        with _lib.on_device(q.device):
+            rc = lib.motif_chord_distances(params[1].data_ptr(), params[2].data_ptr(), H, n, eps, distances.data_ptr(),
+                                           _lib.stream_ptr(q.device))
+        _lib.check(rc, 'motif_chord_distances')
+        _launch_window(q, k, v, params, ln, q_start, scale, eps, window, sinks, out, lse, distances=distances)
+        ctx.save_for_backward(q, k, v, out, lse, *params, ln, distances)
         ctx.args = q_start, scale, eps, window, sinks
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        q, k, v, out, lse, alpha, beta, mu, ssmax, ln = ctx.saved_tensors
+        q, k, v, out, lse, alpha, beta, mu, ssmax, ln, distances = ctx.saved_tensors
         q_start, scale, eps, window, sinks = ctx.args
         B, H, L, D = q.shape
         Hkv, S = k.shape[1], k.shape[2]
@@ -149,8 +156,8 @@ class ChordWindowFunction(torch.autograd.Function):
                 lse.data_ptr(), alpha.data_ptr(), beta.data_ptr(), mu.data_ptr(), ssmax.data_ptr(),
                 ln.data_ptr(), ln.stride(0), ln.stride(1),
                 *_lib.t4(dq), *_lib.t4(dk), *_lib.t4(dv), d_params.data_ptr(),
-                B, H, Hkv, L, S, D, q_start, float(scale), float(eps), window, sinks,
-                ws.data_ptr(), ws.numel(), _lib.chord_dtype_code(q.dtype), _lib.stream_ptr(q.device))
+                B, H, Hkv, L, S, D, q_start, float(scale), float(eps), window, sinks, int(ctx.needs_input_grad[5]),
+                distances.data_ptr(), distances.numel() // (3 * H), ws.data_ptr(), ws.numel(), _lib.chord_dtype_code(q.dtype), _lib.stream_ptr(q.device))
         _lib.check(rc, 'motif_chord_window_bwd')
         grads = [dq, dk, dv, *d_params.unbind(0)]
         grads = [g if need else None for g, need in zip(grads, ctx.needs_input_grad)]
@@ -283,7 +290,7 @@ def _launch(q, k, v, alpha, beta, mu, ssmax, log_n, q_start, scale, eps, out, ls
 
 
 def _launch_window(q, k, v, params, log_n, q_start, scale, eps, window, sinks, out, lse=None, length_dev=None,
-                   log_table=None, workspace=None):
+                   log_table=None, workspace=None, distances=None):
     '''motif_chord_window_fwd into `out`: host positions (log_n), or the device cursor over a
     fixed-capacity cache (length_dev and log_table; the launch advances it).'''
     B, H, L, D = q.shape
@@ -312,7 +319,8 @@ def _launch_window(q, k, v, params, log_n, q_start, scale, eps, window, sinks, o
         rc = lib.motif_chord_window_fwd(
             *_lib.t4(q), *_lib.t4(k), *_lib.t4(v), *[t.data_ptr() for t in params], *ln, *table, *_lib.t4(out),
             _lib.ptr(lse), _lib.ptr(length_dev), B, H, Hkv, L, S, D, int(q_start), float(scale), float(eps),
-            window, sinks, _lib.ptr(workspace), 0 if workspace is None else workspace.numel(), code,
+            window, sinks, _lib.ptr(distances), 0 if distances is None else distances.numel() // (3 * H),
+            _lib.ptr(workspace), 0 if workspace is None else workspace.numel(), code,
             _lib.stream_ptr(q.device))
     _lib.check(rc, 'motif_chord_window_fwd')
     return out

@@ -482,6 +482,8 @@ int motif_chord_qkv_prep(const void *proj, int64_t p_sb, int64_t p_st, int q_off
  *   length_dev: NULL, or the device cursor: S is then the cache's capacity, *length_dev
  *   positions are cached with the L new rows behind them, q_start = *length_dev
  *   (the argument must be 0), and the launch advances *length_dev by L.
+ *   distances: NULL (the bias is evaluated in fp32), or motif_chord_distances' table, which a
+ *   forward whose gradients follow is given so that both use the same weights.
  *   workspace: motif_chord_window_workspace_bytes(...) bytes (may be 0), 16-byte aligned.
  */
 size_t motif_chord_window_workspace_bytes(int B, int H, int Hkv, int L, int S, int D, int window, int sinks, int dtype);
@@ -493,14 +495,25 @@ int motif_chord_window_fwd(
     const float *log_n, int64_t ln_sb, int64_t ln_st, const float *log_table, int log_table_len,
     void *out, int64_t o_sb, int64_t o_sh, int64_t o_st, float *lse,
     int *length_dev, int B, int H, int Hkv, int L, int S, int D, int q_start, float scale, float eps,
-    int window, int sinks, void *workspace, size_t workspace_bytes, int dtype, void *stream);
+    int window, int sinks, const float *distances, int distances_len,
+    void *workspace, size_t workspace_bytes, int dtype, void *stream);
+
+/*
+ * Table of the bias's distances for motif_chord_window_fwd / _bwd: n = motif_chord_distances_len(..)
+ * entries per head (3 * H * n floats, 8-byte aligned) in 64-bit arithmetic, with
+ * x_d = |-d - mu_h| + eps: out[h][d] = {x_d^beta, x_d^beta log2 x_d} for d = 0 .. n - 1, then
+ * x_d^(beta - 1) sign(-d - mu_h).
+ */
+int motif_chord_distances_len(int L, int q_start, int window, int sinks);
+int motif_chord_distances(const float *beta, const float *mu, int H, int n, float eps, float *out, void *stream);
 
 /*
  * Gradients of motif_chord_window_fwd (bf16, head_dim 64, host positions): motif_chord_bwd's
  * arguments and outputs with a window; q_start + L may pass S.  `lse` is the forward's.  A row
  * that sees no key has a zero gradient and adds none.  The parameter gradients are fp32 sums
- * that do not carry the rounding of `out` (the row sums of the softmax's gradient, which are
- * 0, are used to take it out).  With L == 0 or S == 0 only dparam is written.
+ * (given `distances`, the table the forward had) that do not carry the rounding of `out` (the row sums of the softmax's gradient, which are
+ * 0, are used to take it out).  need_mu 0: mu's row of dparam is 0.  With L == 0 or S == 0
+ * only dparam is written.
  */
 size_t motif_chord_window_bwd_workspace_bytes(int B, int H, int Hkv, int L, int S, int q_start, int window, int sinks);
 int motif_chord_window_bwd(
@@ -515,7 +528,8 @@ int motif_chord_window_bwd(
     void *dk, int64_t dk_sb, int64_t dk_sh, int64_t dk_st,
     void *dv, int64_t dv_sb, int64_t dv_sh, int64_t dv_st,
     float *dparam, int B, int H, int Hkv, int L, int S, int D, int q_start, float scale, float eps,
-    int window, int sinks, void *workspace, size_t workspace_bytes, int dtype, void *stream);
+    int window, int sinks, int need_mu, const float *distances, int distances_len,
+    void *workspace, size_t workspace_bytes, int dtype, void *stream);
 
 /*
  * Rows of a 4-bit key / value cache (no reference counterpart).  For each (batch row, kv head,
