@@ -34,7 +34,7 @@ FLAGS = [
 # the default: their register budgets rely on the accumulator file (the VGPR form made the
 # per-chunk gradient kernel of gdn_bwd_chunk.hip 19% slower).
 _VGPR_FORM = ['-mllvm', '-amdgpu-mfma-vgpr-form']
-EXTRA = {f: _VGPR_FORM for f in ('chord.hip', 'chord_bwd.hip', 'chord_window.hip', 'gdn_bwd.hip', 'gdn_chunk.hip')}
+EXTRA = {f: _VGPR_FORM for f in ('chord.hip', 'chord_bwd.hip', 'chord_window.hip', 'chord_kv4.hip', 'gdn_bwd.hip', 'gdn_chunk.hip')}
 
 
 def _run(cmd, verbose):

@@ -1174,6 +1174,26 @@ static void launch_decode_d(const ChordArgs &a, int R, const float *tab, int tab
   else chord_decode_kernel<T, 8, D><<<grid, block, 0, s>>>(a, tab, tab_n);
 }
 
+int chord_cu_count() { return device_cu_count(); }
+
+template <typename T>
+static int launch_merge_t(const ChordArgs &a, int D, hipStream_t s) {
+  const dim3 grid((a.H / a.Hkv) * a.L, a.Hkv, a.B);
+  switch (D) {
+    case 16: chord_merge_kernel<T, 16><<<grid, dim3(16), 0, s>>>(a); break;
+    case 32: chord_merge_kernel<T, 32><<<grid, dim3(32), 0, s>>>(a); break;
+    case 64: chord_merge_kernel<T, 64><<<grid, dim3(64), 0, s>>>(a); break;
+    default: chord_merge_kernel<T, 128><<<grid, dim3(128), 0, s>>>(a); break;
+  }
+  return check_launch("chord_merge_kernel");
+}
+
+int launch_chord_merge(const ChordArgs &a, int dtype, int D, hipStream_t s) {
+  if (dtype == MOTIF_BF16) return launch_merge_t<bf16_t>(a, D, s);
+  if (dtype == MOTIF_F16) return launch_merge_t<f16_t>(a, D, s);
+  return launch_merge_t<float>(a, D, s);
+}
+
 // The vector kernel and (with splits) its merge, for head dim D in {16, 32, 64, 128}.
 template <typename T>
 static int launch_vector(const ChordArgs &a, int R, int D, const float *tab, int tab_n, hipStream_t s) {
@@ -1185,14 +1205,7 @@ static int launch_vector(const ChordArgs &a, int R, int D, const float *tab, int
   }
   int rc = check_launch("chord_decode_kernel");
   if (rc || !a.part) return rc;  // partials (split keys, or the cursor decode): merge them
-  const dim3 grid((a.H / a.Hkv) * a.L, a.Hkv, a.B);
-  switch (D) {
-    case 16: chord_merge_kernel<T, 16><<<grid, dim3(16), 0, s>>>(a); break;
-    case 32: chord_merge_kernel<T, 32><<<grid, dim3(32), 0, s>>>(a); break;
-    case 64: chord_merge_kernel<T, 64><<<grid, dim3(64), 0, s>>>(a); break;
-    default: chord_merge_kernel<T, 128><<<grid, dim3(128), 0, s>>>(a); break;
-  }
-  return check_launch("chord_merge_kernel");
+  return launch_merge_t<T>(a, D, s);
 }
 
 static int launch_vector_dt(int dtype, const ChordArgs &a, int R, int D, const float *tab, int tab_n, hipStream_t s) {

@@ -105,6 +105,15 @@ int launch_chord_wide(const ChordArgs &a, int dtype, int D, hipStream_t s);
 int launch_chord_wide_window(const ChordArgs &a, int dtype, int D, hipStream_t s);
 int launch_chord_wide_kv4(const ChordArgs &a, const KV4Args &kv, int dtype, int D, hipStream_t s);
 
+// Few rows over a 4-bit cache (chord_kv4.hip; (H / Hkv) L <= 16, bf16 or fp16, head dim 64), a.splits
+// key ranges: partials and a merge where a.part is set (with the cursor always), else straight to out.
+bool chord_kv4_serves(int H, int Hkv, int L, int D, int dtype);
+int chord_kv4_splits(int B, int Hkv, int L, int S, int window, int sinks);
+int launch_chord_kv4(const ChordArgs &a, const KV4Args &kv, int dtype, hipStream_t s);
+// The merge of split partials (and the cursor's advance).
+int launch_chord_merge(const ChordArgs &a, int dtype, int D, hipStream_t s);
+int chord_cu_count();
+
 // Chord decode over a device cursor, shared by the C-ABI entry points that take
 // a caller workspace and those that use the library's own scratch.
 // The body of motif_chord_decode (same arguments and status codes).

@@ -468,8 +468,10 @@ extern "C" size_t motif_chord_window_workspace_bytes(int B, int H, int Hkv, int 
 
 extern "C" size_t motif_chord_kv4_workspace_bytes(int B, int H, int Hkv, int L, int S, int D, int window, int sinks,
                                                   int dtype) {
-  (void)B; (void)H; (void)Hkv; (void)L; (void)S; (void)D; (void)window; (void)sinks; (void)dtype;
-  return 0;
+  if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || L <= 0 || S <= 0 || window < 1 || sinks < 0 ||
+      !chord_kv4_serves(H, Hkv, L, D, dtype))
+    return 0;
+  return static_cast<size_t>(B) * H * L * chord_kv4_splits(B, Hkv, L, S, window, sinks) * (D + 2) * sizeof(float);
 }
 
 extern "C" int motif_chord_kv4_fwd(
@@ -490,6 +492,15 @@ extern "C" int motif_chord_kv4_fwd(
   const KV4Args kv = kv4_args(k_codes, kc_sb, kc_sh, k_params, kp_sb, kp_sh, v_codes, vc_sb, vc_sh, v_params, vp_sb, vp_sh);
   if (const char *bad = kv4_check(kv, D)) return set_error(MOTIF_ERR_INVALID, std::string("chord_kv4_fwd: ") + bad);
   if (a.q_st < 0 || a.q_st >= (int64_t(1) << 24)) return set_error(MOTIF_ERR_UNSUPPORTED, "chord_kv4_fwd: row stride out of range");
-  (void)workspace; (void)workspace_bytes;
-  return launch_chord_wide_kv4(a, kv, dtype, D, static_cast<hipStream_t>(stream));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  // more rows, fp32 and other head dims: the fp32-accumulating flash kernel, which expands the codes
+  if (!chord_kv4_serves(H, Hkv, L, D, dtype)) return launch_chord_wide_kv4(a, kv, dtype, D, st);
+  a.splits = chord_kv4_splits(B, Hkv, L, S, window, sinks);
+  if (a.splits > 1 || length_dev) {  // (the merge advances the cursor)
+    const size_t need = motif_chord_kv4_workspace_bytes(B, H, Hkv, L, S, D, window, sinks, dtype);
+    if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 3))
+      return set_error(MOTIF_ERR_INVALID, "chord_kv4_fwd: workspace too small (need " + std::to_string(need) + " bytes) or not aligned");
+    a.part = static_cast<float *>(workspace);
+  }
+  return launch_chord_kv4(a, kv, dtype, st);
 }

@@ -122,6 +122,7 @@ EXPORTED = tuple(_SIGNATURES)
 
 _lib = None
 _load_error = None
+_found = False
 
 
 def _load():
@@ -141,8 +142,11 @@ def _load():
 
 def available() -> bool:
     '''True when the kernel library loaded and a ROCm device is visible.'''
-    _load()
-    return _lib is not None and torch.cuda.is_available()
+    global _found
+    if not _found:  # (a device that was seen stays: asking again costs a few us a call)
+        _load()
+        _found = _lib is not None and torch.cuda.is_available()
+    return _found
 
 
 def lib():

@@ -18,6 +18,7 @@ dv and the four per-head parameter gradients, the reference's custom backward
 :1348-1554).  Other gradient calls take the differentiable torch forms
 (motif/ops/autograd_path.py).
 '''
+import functools
 import numbers
 from typing import Optional
 
@@ -40,6 +41,10 @@ def serves_head_dim(D: int) -> bool:
 
 def check_window(window, sinks):
     '''(window, sinks) as ints (window None: every key up to the query's own), checked.'''
+    if type(window) is int and type(sinks) is int and 1 <= window <= NO_WINDOW and 0 <= sinks <= NO_WINDOW:
+        return window, sinks
+    if window is None and type(sinks) is int and sinks == 0:
+        return None, 0
     if isinstance(sinks, bool) or not isinstance(sinks, numbers.Integral) or sinks < 0:
         raise ValueError(f'sinks must be an int >= 0, got {sinks!r}')
     if window is None:
@@ -117,51 +122,59 @@ class ChordWindowFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, alpha, beta, mu, ssmax, log_n, q_start, scale, eps, window, sinks):
-        q, k, v = (_near(_aligned(t if t.stride(-1) == 1 else t.contiguous())) for t in (q, k, v))
-        params = [t.detach().contiguous() for t in (alpha, beta, mu, ssmax)]
-        ln = log_n.detach()
+        q, k, v = _rows4(q)[0], _rows4(k)[0], _rows4(v)[0]
         B, H, L, D = q.shape
-        out = torch.empty((B, L, H, D), dtype=q.dtype, device=q.device).transpose(1, 2)
-        lse = torch.empty((B, H, L), dtype=torch.float32, device=q.device)
+        dev = q.device
+        out = torch.empty((B, L, H, D), dtype=q.dtype, device=dev).transpose(1, 2)
+        lse = torch.empty((B, H, L), dtype=torch.float32, device=dev)
         lib = _lib.lib()
         n = lib.motif_chord_distances_len(L, q_start, window, sinks)
-        distances = torch.empty(3 * H * n, dtype=torch.float32, device=q.device)
-        with _lib.on_device(q.device):
-            rc = lib.motif_chord_distances(params[1].data_ptr(), params[2].data_ptr(), H, n, eps, distances.data_ptr(),
-                                           _lib.stream_ptr(q.device))
-        _lib.check(rc, 'motif_chord_distances')
-        _launch_window(q, k, v, params, ln, q_start, scale, eps, window, sinks, out, lse, distances=distances)
-        ctx.save_for_backward(q, k, v, out, lse, *params, ln, distances)
+        distances = torch.empty(3 * H * n, dtype=torch.float32, device=dev)
+        with _lib.on_device(dev):
+            rc = lib.motif_chord_distances(beta.data_ptr(), mu.data_ptr(), H, n, eps, distances.data_ptr(),
+                                           _lib.stream_ptr(dev))
+        if rc:
+            _lib.check(rc, 'motif_chord_distances')
+        _launch_window(q, k, v, (alpha, beta, mu, ssmax), log_n, q_start, scale, eps, window, sinks, out, lse,
+                       distances=distances)
+        ctx.save_for_backward(q, k, v, out, lse, alpha, beta, mu, ssmax, log_n, distances)
         ctx.args = q_start, scale, eps, window, sinks
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        q, k, v, out, lse, alpha, beta, mu, ssmax, ln, distances = ctx.saved_tensors
+        q, k, v, out, lse, alpha, beta, mu, ssmax, log_n, distances = ctx.saved_tensors
         q_start, scale, eps, window, sinks = ctx.args
+        needs = ctx.needs_input_grad
         B, H, L, D = q.shape
         Hkv, S = k.shape[1], k.shape[2]
+        dev = q.device
         # (the kernels read dout's own rows, expanded ones too)
         dout = _aligned(dout if dout.stride(-1) == 1 else dout.contiguous())
         # gradients in storage of their own (an expanded input's would share elements)
-        dq = torch.empty((B, L, H, D), dtype=q.dtype, device=q.device).transpose(1, 2)
-        dk, dv = (torch.empty((B, Hkv, S, D), dtype=q.dtype, device=q.device) for _ in range(2))
-        d_params = torch.empty((4, H), dtype=torch.float32, device=q.device)
-        lib = _lib.lib()
-        with _lib.on_device(q.device):
-            n = int(lib.motif_chord_window_bwd_workspace_bytes(B, H, Hkv, L, S, q_start, window, sinks))
-            ws = torch.empty(max(n, 1), dtype=torch.uint8, device=q.device)
-            rc = lib.motif_chord_window_bwd(
-                *_lib.t4(q), *_lib.t4(k), *_lib.t4(v), *_lib.t4(out), *_lib.t4(dout),
+        dq = torch.empty((B, L, H, D), dtype=q.dtype, device=dev).transpose(1, 2)
+        dk = torch.empty((B, Hkv, S, D), dtype=q.dtype, device=dev)
+        dv = torch.empty((B, Hkv, S, D), dtype=q.dtype, device=dev)
+        d_params = torch.empty((4, H), dtype=torch.float32, device=dev)
+        ws = torch.empty(_window_bwd_workspace_bytes(B, H, Hkv, L, S, q_start, window, sinks), dtype=torch.uint8, device=dev)
+        with _lib.on_device(dev):
+            rc = _lib.lib().motif_chord_window_bwd(
+                q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3],
+                out.data_ptr(), *out.stride()[:3], dout.data_ptr(), *dout.stride()[:3],
                 lse.data_ptr(), alpha.data_ptr(), beta.data_ptr(), mu.data_ptr(), ssmax.data_ptr(),
-                ln.data_ptr(), ln.stride(0), ln.stride(1),
-                *_lib.t4(dq), *_lib.t4(dk), *_lib.t4(dv), d_params.data_ptr(),
-                B, H, Hkv, L, S, D, q_start, float(scale), float(eps), window, sinks, int(ctx.needs_input_grad[5]),
-                distances.data_ptr(), distances.numel() // (3 * H), ws.data_ptr(), ws.numel(), _lib.chord_dtype_code(q.dtype), _lib.stream_ptr(q.device))
-        _lib.check(rc, 'motif_chord_window_bwd')
-        grads = [dq, dk, dv, *d_params.unbind(0)]
-        grads = [g if need else None for g, need in zip(grads, ctx.needs_input_grad)]
-        return (*grads, *[None] * 6)
+                log_n.data_ptr(), *log_n.stride(), dq.data_ptr(), *dq.stride()[:3], dk.data_ptr(), *dk.stride()[:3],
+                dv.data_ptr(), *dv.stride()[:3], d_params.data_ptr(), B, H, Hkv, L, S, D, q_start, scale, eps,
+                window, sinks, 1 if needs[5] else 0, distances.data_ptr(), distances.numel() // (3 * H), ws.data_ptr(),
+                ws.numel(), _lib.MOTIF_BF16, _lib.stream_ptr(dev))
+        if rc:
+            _lib.check(rc, 'motif_chord_window_bwd')
+        return (dq if needs[0] else None, dk if needs[1] else None, dv if needs[2] else None,
+                *(d_params[i] if needs[3 + i] else None for i in range(4)), None, None, None, None, None, None)
+
+
+@functools.lru_cache(maxsize=256)
+def _window_bwd_workspace_bytes(*sizes) -> int:
+    return int(_lib.lib().motif_chord_window_bwd_workspace_bytes(*sizes))
 
 
 def _window_grad_kernels_serve(q, k, v, alpha, beta, mu, ssmax, log_n):
@@ -297,39 +310,55 @@ def _launch_window(q, k, v, params, log_n, q_start, scale, eps, window, sinks, o
     Hkv, S = k.shape[1], k.shape[2]
     if D not in HEAD_DIMS:  # zero-padded to the next size, as in _launch
         Dp = next((d for d in HEAD_DIMS if d > D), None)
-        if Dp is None or length_dev is not None:
+        if Dp is None or lse is not None or length_dev is not None:
             raise NotImplementedError(f'windowed Chord attention: head_dim {D} unsupported')
         pad = lambda t: torch.nn.functional.pad(t, (0, Dp - D))
         out_p = torch.empty((B, H, L, Dp), dtype=out.dtype, device=out.device)
-        _launch_window(pad(q), pad(k), pad(v), params, log_n, q_start, scale, eps, window, sinks, out_p, lse)
+        _launch_window(pad(q), pad(k), pad(v), params, log_n, q_start, scale, eps, window, sinks, out_p)
         out.copy_(out_p[..., :D])
         return out
-    lib = _lib.lib()
     code = _lib.chord_dtype_code(q.dtype)
+    q, q4 = _rows4(q)
+    if length_dev is None:
+        k, k4 = _rows4(k)
+        v, v4 = _rows4(v)
+    else:  # (a cache that is written in place is never copied)
+        k4, v4 = _lib.t4(k), _lib.t4(v)
     with _lib.on_device(q.device):
-        if length_dev is None:  # (a cache that is written in place is never copied)
-            q, k, v = (_near(_aligned(t)) for t in (q, k, v))
-        else:
-            q = _aligned(q)
         if workspace is None:
-            n = int(lib.motif_chord_window_workspace_bytes(B, H, Hkv, L, S, D, window, sinks, code))
+            n = _window_workspace_bytes(B, H, Hkv, L, S, D, window, sinks, code)
             workspace = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-        ln = (log_n.data_ptr(), log_n.stride(0), log_n.stride(1)) if log_n is not None else (None, 0, 0)
-        table = (None, 0) if log_table is None else (log_table.data_ptr(), log_table.numel())
-        rc = lib.motif_chord_window_fwd(
-            *_lib.t4(q), *_lib.t4(k), *_lib.t4(v), *[t.data_ptr() for t in params], *ln, *table, *_lib.t4(out),
-            _lib.ptr(lse), _lib.ptr(length_dev), B, H, Hkv, L, S, D, int(q_start), float(scale), float(eps),
-            window, sinks, _lib.ptr(distances), 0 if distances is None else distances.numel() // (3 * H),
-            _lib.ptr(workspace), 0 if workspace is None else workspace.numel(), code,
+        ln = (None, 0, 0) if log_n is None else (log_n.data_ptr(), *log_n.stride())
+        alpha, beta, mu, ssmax = params
+        rc = _lib.lib().motif_chord_window_fwd(
+            *q4, *k4, *v4, alpha.data_ptr(), beta.data_ptr(), mu.data_ptr(), ssmax.data_ptr(), *ln,
+            None if log_table is None else log_table.data_ptr(), 0 if log_table is None else log_table.numel(),
+            out.data_ptr(), *out.stride()[:3], None if lse is None else lse.data_ptr(),
+            None if length_dev is None else length_dev.data_ptr(), B, H, Hkv, L, S, D, q_start, scale, eps,
+            window, sinks, None if distances is None else distances.data_ptr(),
+            0 if distances is None else distances.numel() // (3 * H),
+            None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel(), code,
             _lib.stream_ptr(q.device))
-    _lib.check(rc, 'motif_chord_window_fwd')
+    if rc:
+        _lib.check(rc, 'motif_chord_window_fwd')
     return out
 
 
-def _near(t):
-    '''t, copied where its rows lie further apart than the windowed kernels' 32-bit offsets
-    hold, or run backwards.'''
-    return t if t.shape[2] <= 1 or 0 <= t.stride(2) < 2 ** 24 else t.contiguous()
+@functools.lru_cache(maxsize=256)
+def _window_workspace_bytes(*sizes) -> int:
+    return int(_lib.lib().motif_chord_window_workspace_bytes(*sizes))
+
+
+def _rows4(t):
+    '''(t, (pointer, batch, head and time stride)) for the windowed kernels: t itself where its
+    rows have unit feature stride, start on 16-byte boundaries and lie less than 2^24
+    elements apart, else a copy.'''
+    s, p = t.stride(), t.data_ptr()
+    if s[3] == 1 and not p & 15 and not (s[0] | s[1] | s[2]) & (16 // t.element_size() - 1) \
+            and (s[2] < 2 ** 24 or t.shape[2] <= 1):
+        return t, (p, s[0], s[1], s[2])
+    t = torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+    return t, _lib.t4(t)
 
 
 def apply_chord_attention(
@@ -416,7 +445,8 @@ def apply_chord_attention(
     if window is not None:
         if out.numel() == 0 or S == 0:
             return out.zero_()
-        return _launch_window(q, k, v, (alpha, beta, mu, ssmax), log_n, q_start, softmax_scale, eps, window, sinks, out)
+        return _launch_window(q, k, v, (alpha, beta, mu, ssmax), log_n, q_start, float(softmax_scale), float(eps), window,
+                              sinks, out)
     return _launch(q, k, v, alpha, beta, mu, ssmax, log_n, q_start, softmax_scale, eps, out)
 
 
@@ -466,7 +496,7 @@ def apply_chord_attention_varlen(q, k, v, alpha, beta, mu, ssmax, log_n, cu_seql
         for a, b in ps.bounds():
             if b > a:
                 _launch_window(q[:, :, a:b], k[:, :, a:b], v[:, :, a:b], (alpha, beta, mu, ssmax), log_n[:, a:b], 0,
-                               softmax_scale, eps, window, sinks, out[:, :, a:b])
+                               float(softmax_scale), float(eps), window, sinks, out[:, :, a:b])
         return out
     return _launch(q, k, v, alpha, beta, mu, ssmax, log_n, 0, softmax_scale, eps, out,
                    cu_dev=ps.cu, nseq=ps.nseq, max_seqlen=ps.max_len, cu_host=ps.cu_host)
@@ -482,8 +512,7 @@ def chord_window_workspace(B, H, Hkv, L, capacity, D, dtype, device, window, sin
     '''A workspace for chord_decode_cursor with a window at these sizes (None where it needs
     none).'''
     window, sinks = check_window(window, sinks)
-    n = int(_lib.lib().motif_chord_window_workspace_bytes(B, H, Hkv, L, capacity, D, window, sinks,
-                                                          _lib.chord_dtype_code(dtype)))
+    n = _window_workspace_bytes(B, H, Hkv, L, capacity, D, window, sinks, _lib.chord_dtype_code(dtype))
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
@@ -559,8 +588,8 @@ def chord_decode_cursor(q, k_cache, v_cache, length_dev, alpha, beta, mu, ssmax,
             raise ValueError('chord_decode_cursor: more queries than the capacity')
         if out.numel() == 0:
             return out
-        return _launch_window(q, k_cache, v_cache, (alpha, beta, mu, ssmax), log_n, 0, softmax_scale, eps, window, sinks,
-                              out, length_dev=length_dev, log_table=log_table, workspace=workspace)
+        return _launch_window(q, k_cache, v_cache, (alpha, beta, mu, ssmax), log_n, 0, float(softmax_scale), float(eps),
+                              window, sinks, out, length_dev=length_dev, log_table=log_table, workspace=workspace)
     ln_sb, ln_st = (log_n.stride(0), log_n.stride(1)) if log_n is not None else (0, 0)
     if library_scratch:
         rc = _lib.lib().motif_chord_decode_noalloc(

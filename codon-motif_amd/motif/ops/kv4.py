@@ -14,13 +14,14 @@ nearest to (x - base) / scale, ties to even), `kv4_read` gives the values back, 
 expanding it in memory: 40 bytes a row at head dim 64 where bf16 takes 128.  All of them
 are forward-only: calls that would need a gradient raise.
 '''
+import functools
 from typing import NamedTuple, Optional, Tuple
 
 import torch
 
 from . import _lib
 from .autograd_path import wants_grad
-from .chord_attention import (HEAD_DIMS, NO_WINDOW, _aligned, _check_params, _out_for, check_window)
+from .chord_attention import HEAD_DIMS, NO_WINDOW, _check_params, _out_for, _rows4, check_window
 
 GROUP = 32  # features that share a (scale, base) pair
 
@@ -52,39 +53,35 @@ def kv4_alloc(batch: int, kv_heads: int, capacity: int, head_dim: int, device) -
 
 
 def _check_slab(slab: KV4Slab, what: str):
+    '''((B, Hkv, capacity, D), the entry points' arguments), or ValueError.'''
     kc, kp, vc, vp = slab
-    if kc.dim() != 4 or kc.dtype != torch.uint8 or vc.dtype != torch.uint8:
+    shape = kc.shape
+    if len(shape) != 4 or kc.dtype != torch.uint8 or vc.dtype != torch.uint8:
         raise ValueError(f'{what}: codes must be uint8 [B, Hkv, capacity, D / 2]')
-    B, Hkv, cap, half = kc.shape
+    B, Hkv, cap, half = shape
     D = 2 * half
     if D not in HEAD_DIMS:
         raise ValueError(f'{what}: head_dim must be one of {HEAD_DIMS}, got {D}')
-    G = D // min(GROUP, D)
-    shape = (B, Hkv, cap, G, 2)
-    if vc.shape != kc.shape or kp.shape != shape or vp.shape != shape \
+    G = D // GROUP if D > GROUP else 1
+    pshape = (B, Hkv, cap, G, 2)
+    if vc.shape != shape or kp.shape != pshape or vp.shape != pshape \
             or kp.dtype != torch.bfloat16 or vp.dtype != torch.bfloat16:
-        raise ValueError(f'{what}: codes of keys and values must have one shape, params must be bfloat16 {shape}')
-    if not kc.is_cuda:
+        raise ValueError(f'{what}: codes of keys and values must have one shape, params must be bfloat16 {pshape}')
+    dev = kc.device
+    if dev.type != 'cuda':
         raise ValueError(f'{what}: the cache must live on CUDA')
-    for t in (kp, vc, vp):
-        if t.device != kc.device:
-            raise ValueError(f'{what}: the cache tensors must live on one device')
-    if kc.numel():
-        for t in (kc, vc):
-            if t.stride(3) != 1 or (cap > 1 and t.stride(2) != half) or t.data_ptr() % 4 \
-                    or t.stride(0) % 4 or t.stride(1) % 4:
+    if kp.device != dev or vc.device != dev or vp.device != dev:
+        raise ValueError(f'{what}: the cache tensors must live on one device')
+    args = []
+    for c, p in ((kc, kp), (vc, vp)):
+        cs, ps, cp, pp = c.stride(), p.stride(), c.data_ptr(), p.data_ptr()
+        if B and Hkv and cap:
+            if cs[3] != 1 or (cap > 1 and cs[2] != half) or (cp | cs[0] | cs[1]) & 3:
                 raise ValueError(f'{what}: rows of codes must lie back to back on 4-byte boundaries')
-        for t in (kp, vp):
-            if t.stride(4) != 1 or (G > 1 and t.stride(3) != 2) or (cap > 1 and t.stride(2) != 2 * G) \
-                    or t.data_ptr() % 4 or t.stride(0) % 2 or t.stride(1) % 2:
+            if ps[4] != 1 or (G > 1 and ps[3] != 2) or (cap > 1 and ps[2] != 2 * G) or pp & 3 or (ps[0] | ps[1]) & 1:
                 raise ValueError(f'{what}: rows of params must lie back to back on 4-byte boundaries')
-    return B, Hkv, cap, D
-
-
-def _slab_args(slab: KV4Slab):
-    kc, kp, vc, vp = slab
-    return (kc.data_ptr(), kc.stride(0), kc.stride(1), kp.data_ptr(), kp.stride(0) // 2, kp.stride(1) // 2,
-            vc.data_ptr(), vc.stride(0), vc.stride(1), vp.data_ptr(), vp.stride(0) // 2, vp.stride(1) // 2)
+        args += (cp, cs[0], cs[1], pp, ps[0] >> 1, ps[1] >> 1)
+    return (B, Hkv, cap, D), args
 
 
 def _need_backend():
@@ -99,7 +96,7 @@ def kv4_append(slab: KV4Slab, k: torch.Tensor, v: torch.Tensor, start) -> None:
     dropped).  A group of features that holds an infinity or a NaN reads back as NaN.'''
     if wants_grad(k, v):
         raise RuntimeError('kv4_append is forward-only: detach the rows or call it under no_grad')
-    B, Hkv, cap, D = _check_slab(slab, 'kv4_append')
+    (B, Hkv, cap, D), args = _check_slab(slab, 'kv4_append')
     if k.shape != v.shape or k.dim() != 4 or k.shape[:2] != (B, Hkv) or k.shape[3] != D:
         raise ValueError(f'kv4_append: k / v must be [{B}, {Hkv}, n, {D}], got {tuple(k.shape)} and {tuple(v.shape)}')
     if k.dtype != v.dtype or k.device != slab.k_codes.device or v.device != k.device:
@@ -116,64 +113,76 @@ def kv4_append(slab: KV4Slab, k: torch.Tensor, v: torch.Tensor, start) -> None:
     _need_backend()
     if k.numel() == 0:
         return
-    k, v = (_aligned(t if t.stride(-1) == 1 else t.contiguous()) for t in (k, v))
+    k4, v4 = _rows4(k), _rows4(v)
     with _lib.on_device(k.device):
-        rc = _lib.lib().motif_kv4_append(*_lib.t4(k), *_lib.t4(v), *_slab_args(slab), dev, pos, cap, B, n, Hkv, D,
+        rc = _lib.lib().motif_kv4_append(*k4[1], *v4[1], *args, dev, pos, cap, B, n, Hkv, D,
                                          _lib.chord_dtype_code(k.dtype), _lib.stream_ptr(k.device))
-    _lib.check(rc, 'motif_kv4_append')
+    if rc:
+        _lib.check(rc, 'motif_kv4_append')
 
 
 def kv4_read(slab: KV4Slab, start: int, n: int, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     '''The values of positions [start, start + n) as (k, v), new [B, Hkv, n, D] tensors of
     `dtype` (fp16, bf16 or fp32; the fp32 value rounded once).'''
-    B, Hkv, cap, D = _check_slab(slab, 'kv4_read')
+    (B, Hkv, cap, D), args = _check_slab(slab, 'kv4_read')
     start, n = int(start), int(n)
     if start < 0 or n < 0 or start + n > cap:
         raise ValueError(f'kv4_read: positions [{start}, {start + n}) outside a cache of {cap}')
     code = _lib.chord_dtype_code(dtype)
     _need_backend()
     k = torch.empty(B, Hkv, n, D, dtype=dtype, device=slab.k_codes.device)
-    v = torch.empty_like(k)
+    v = torch.empty(B, Hkv, n, D, dtype=dtype, device=slab.k_codes.device)
     if k.numel():
+        s0, s1, s2, _ = k.stride()
         with _lib.on_device(k.device):
-            rc = _lib.lib().motif_kv4_read(*_slab_args(slab), *_lib.t4(k), *_lib.t4(v), start, cap, B, n, Hkv, D, code,
-                                           _lib.stream_ptr(k.device))
-        _lib.check(rc, 'motif_kv4_read')
+            rc = _lib.lib().motif_kv4_read(*args, k.data_ptr(), s0, s1, s2, v.data_ptr(), s0, s1, s2, start, cap, B, n, Hkv,
+                                           D, code, _lib.stream_ptr(k.device))
+        if rc:
+            _lib.check(rc, 'motif_kv4_read')
     return k, v
 
 
 def _check_query(q, slab, params, what):
-    B, Hkv, cap, D = _check_slab(slab, what)
-    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D or q.shape[1] % Hkv:
-        raise ValueError(f'{what}: q {tuple(q.shape)} does not fit a cache of {B} rows, {Hkv} kv heads of {D}')
-    if q.dtype not in (torch.float16, torch.bfloat16, torch.float32) or q.stride(-1) != 1:
+    (B, Hkv, cap, D), args = _check_slab(slab, what)
+    shape, dev = q.shape, q.device
+    if len(shape) != 4 or shape[0] != B or shape[3] != D or shape[1] % Hkv:
+        raise ValueError(f'{what}: q {tuple(shape)} does not fit a cache of {B} rows, {Hkv} kv heads of {D}')
+    if q.dtype not in (torch.float16, torch.bfloat16, torch.float32) or q.stride(3) != 1:
         raise ValueError(f'{what}: q must be fp16 / bf16 / fp32 and contiguous along the last dimension')
-    if q.device != slab.k_codes.device:
+    if dev != slab[0].device:
         raise ValueError(f'{what}: q and the cache must live on one device')
-    _check_params(*params, q.shape[1])
-    if any(t.device != q.device for t in params):
+    _check_params(*params, shape[1])
+    if any(t.device != dev for t in params):
         raise ValueError(f'{what}: the head parameters must live on q\'s device')
-    return B, q.shape[1], Hkv, q.shape[2], D, cap
+    return B, shape[1], Hkv, shape[2], D, cap, args
 
 
-def _launch_kv4(q, slab, params, log_n, log_table, length_dev, S, q_start, scale, eps, window, sinks, out, workspace):
+def _launch_kv4(q, args, Hkv, params, log_n, log_table, length_dev, S, q_start, scale, eps, window, sinks, out, workspace):
     B, H, L, D = q.shape
-    Hkv = slab.k_codes.shape[1]
-    q = _aligned(q)
-    lib = _lib.lib()
+    q, q4 = _rows4(q)
     code = _lib.chord_dtype_code(q.dtype)
-    with _lib.on_device(q.device):
+    dev = q.device
+    with _lib.on_device(dev):
         if workspace is None:
-            n = int(lib.motif_chord_kv4_workspace_bytes(B, H, Hkv, L, S, D, window, sinks, code))
-            workspace = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-        ln = (log_n.data_ptr(), log_n.stride(0), log_n.stride(1)) if log_n is not None else (None, 0, 0)
-        table = (None, 0) if log_table is None else (log_table.data_ptr(), log_table.numel())
-        rc = lib.motif_chord_kv4_fwd(
-            *_lib.t4(q), *_slab_args(slab), *[t.data_ptr() for t in params], *ln, *table, *_lib.t4(out),
-            _lib.ptr(length_dev), B, H, Hkv, L, S, D, q_start, float(scale), float(eps), window, sinks,
-            _lib.ptr(workspace), 0 if workspace is None else workspace.numel(), code, _lib.stream_ptr(q.device))
-    _lib.check(rc, 'motif_chord_kv4_fwd')
+            n = _kv4_workspace_bytes(B, H, Hkv, L, S, D, window, sinks, code)
+            workspace = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        alpha, beta, mu, ssmax = params
+        rc = _lib.lib().motif_chord_kv4_fwd(
+            *q4, *args, alpha.data_ptr(), beta.data_ptr(), mu.data_ptr(), ssmax.data_ptr(),
+            *((None, 0, 0) if log_n is None else (log_n.data_ptr(), *log_n.stride())),
+            *((None, 0) if log_table is None else (log_table.data_ptr(), log_table.numel())),
+            out.data_ptr(), *out.stride()[:3], None if length_dev is None else length_dev.data_ptr(),
+            B, H, Hkv, L, S, D, q_start, scale, eps, window, sinks,
+            None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel(), code,
+            _lib.stream_ptr(dev))
+    if rc:
+        _lib.check(rc, 'motif_chord_kv4_fwd')
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _kv4_workspace_bytes(*sizes) -> int:
+    return int(_lib.lib().motif_chord_kv4_workspace_bytes(*sizes))
 
 
 def chord_attention_kv4(q: torch.Tensor, slab: KV4Slab, alpha, beta, mu, ssmax, log_n: torch.Tensor, length: int,
@@ -190,7 +199,7 @@ def chord_attention_kv4(q: torch.Tensor, slab: KV4Slab, alpha, beta, mu, ssmax, 
         raise RuntimeError('chord_attention_kv4 is forward-only: call it under no_grad')
     window, sinks = check_window(window, sinks)
     params = (alpha, beta, mu, ssmax)
-    B, H, Hkv, L, D, cap = _check_query(q, slab, params, 'chord_attention_kv4')
+    B, H, Hkv, L, D, cap, args = _check_query(q, slab, params, 'chord_attention_kv4')
     length = int(length)
     if not L <= length <= cap:
         raise ValueError(f'chord_attention_kv4: length {length} must lie between the {L} queries and the capacity {cap}')
@@ -200,16 +209,16 @@ def chord_attention_kv4(q: torch.Tensor, slab: KV4Slab, alpha, beta, mu, ssmax, 
     out = _out_for(out, q)
     if out.numel() == 0:
         return out
-    return _launch_kv4(q, slab, params, log_n, None, None, length, length - L,
-                       D ** -0.5 if softmax_scale is None else softmax_scale, eps,
+    return _launch_kv4(q, args, Hkv, params, log_n, None, None, length, length - L,
+                       D ** -0.5 if softmax_scale is None else float(softmax_scale), float(eps),
                        NO_WINDOW if window is None else window, sinks, out, None)
 
 
 def chord_decode_kv4_workspace(B, H, Hkv, L, capacity, D, dtype, device, window=None, sinks=0) -> Optional[torch.Tensor]:
     '''A workspace for chord_decode_kv4_cursor at these sizes (None where it needs none).'''
     window, sinks = check_window(window, sinks)
-    n = int(_lib.lib().motif_chord_kv4_workspace_bytes(B, H, Hkv, L, capacity, D, NO_WINDOW if window is None else window,
-                                                       sinks, _lib.chord_dtype_code(dtype)))
+    n = _kv4_workspace_bytes(B, H, Hkv, L, capacity, D, NO_WINDOW if window is None else window, sinks,
+                             _lib.chord_dtype_code(dtype))
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
@@ -224,7 +233,7 @@ def chord_decode_kv4_cursor(q, slab: KV4Slab, length_dev, alpha, beta, mu, ssmax
         raise RuntimeError('chord_decode_kv4_cursor is forward-only: call it under no_grad')
     window, sinks = check_window(window, sinks)
     params = (alpha, beta, mu, ssmax)
-    B, H, Hkv, L, D, cap = _check_query(q, slab, params, 'chord_decode_kv4_cursor')
+    B, H, Hkv, L, D, cap, args = _check_query(q, slab, params, 'chord_decode_kv4_cursor')
     if length_dev.dtype != torch.int32 or length_dev.device != q.device or length_dev.numel() != 1:
         raise ValueError('chord_decode_kv4_cursor: length_dev must be one int32 on q\'s device')
     if log_table.dtype != torch.float32 or log_table.device != q.device or log_table.numel() < cap \
@@ -236,6 +245,6 @@ def chord_decode_kv4_cursor(q, slab: KV4Slab, length_dev, alpha, beta, mu, ssmax
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if out.numel() == 0:
         return out
-    return _launch_kv4(q, slab, params, None, log_table, length_dev, cap, 0,
-                       D ** -0.5 if softmax_scale is None else softmax_scale, eps,
+    return _launch_kv4(q, args, Hkv, params, None, log_table, length_dev, cap, 0,
+                       D ** -0.5 if softmax_scale is None else float(softmax_scale), float(eps),
                        NO_WINDOW if window is None else window, sinks, out, workspace)

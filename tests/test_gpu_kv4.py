@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from support import gen
-from window_ref import (check_attention, inputs, log_n_of, quantise64, random_slab, slab_values64, values64)
+from window_ref import (check_attention, code_sizes64, inputs, log_n_of, quantise64, random_slab, slab_values64, values64)
 
 pytestmark = pytest.mark.gpu
 
@@ -132,7 +132,8 @@ def test_attention(shape, dtype):
     log_n = log_n_of(B, L, length - L)
     got = chord_attention_kv4(q.to(DEV), slab, *(t.to(DEV) for t in par), log_n.to(DEV), length, window=window, sinks=sinks)
     k, v = (t[:, :, :length] for t in slab_values64(slab))
-    check_attention(got, q, k, v, par, log_n, length - L, window, sinks, what=str(shape))
+    check_attention(got, q, k, v, par, log_n, length - L, window, sinks, what=str(shape),
+                    rounded=code_sizes64(slab)[:, :, :length])
 
 
 @TYPES
@@ -177,7 +178,8 @@ def test_cursor_steps_equal_host_steps(dtype, window, sinks, D):
         got = chord_decode_kv4_cursor(q, slab, cursor, *par, table, window=window, sinks=sinks, workspace=ws)
         assert int(cursor) == pos + L
         kk, vv = (t[:, :, :pos + L] for t in slab_values64(slab))
-        check_attention(got, q, kk, vv, par, table[None, pos:pos + L].expand(B, L), pos, window, sinks, what=f'pos {pos}')
+        check_attention(got, q, kk, vv, par, table[None, pos:pos + L].expand(B, L), pos, window, sinks, what=f'pos {pos}',
+                        rounded=code_sizes64(slab)[:, :, :pos + L])
         pos += L if pos < 75 else 9 if pos + 9 < cap else 1
         cursor.fill_(pos)
         kv4_append(slab, k[:, :, :min(pos, cap)], v[:, :, :min(pos, cap)], 0)

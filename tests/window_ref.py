@@ -72,10 +72,12 @@ def assert_near(got, out, allowed, v_abs_mean, dtype, what=''):
     assert not bad.any(), f'{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((d / lim).max()):.2f} of the limit'
 
 
-def check_attention(got, q, k, v, par, log_n, q_start, window=None, sinks=0, scale=None, what=''):
+def check_attention(got, q, k, v, par, log_n, q_start, window=None, sinks=0, scale=None, what='', rounded=None):
+    '''`rounded` (default |v|): the sizes that a weight's rounding to a 16-bit type multiplies.'''
     dt = q.dtype
     out, _, allowed = attention64(q, k, v, par, log_n, q_start, window, sinks, scale)
-    mean, _, _ = attention64(q, k, v.detach().cpu().double().abs(), par, log_n, q_start, window, sinks, scale)
+    rounded = (v if rounded is None else rounded).detach().cpu().double().abs()
+    mean, _, _ = attention64(q, k, rounded, par, log_n, q_start, window, sinks, scale)
     assert_near(got, out, allowed, mean, dt, what)
 
 
@@ -105,6 +107,18 @@ def slab_values64(slab):
         codes = torch.stack([c & 15, c >> 4], -1).flatten(-2)
         out.append(values64(codes, p[..., 0], p[..., 1]))
     return out
+
+
+def code_sizes64(slab):
+    '''max(|v|, scale |code - 8|) of every value of a KV4Slab: over 4-bit rows the product with the
+    weights runs on v = scale (code - 8) + (base + 8 scale), the weight p scale rounded to the
+    matrix instructions' type and multiplied by code - 8, the rest in fp32; so a weight's
+    rounding h moves the output by h p scale |code - 8|, where expanded values would give h p |v|.'''
+    c, p = slab.v_codes.cpu(), slab.v_params.cpu()
+    codes = torch.stack([c & 15, c >> 4], -1).flatten(-2)
+    scale = p[..., 0].double().abs()
+    off = (codes.double() - 8).abs().unflatten(-1, (scale.shape[-1], -1)) * scale[..., None]
+    return torch.maximum(values64(codes, p[..., 0], p[..., 1]).abs(), off.flatten(-2))
 
 
 def random_slab(B, Hkv, cap, D, device, seed=0):
