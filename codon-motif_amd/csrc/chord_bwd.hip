@@ -132,8 +132,8 @@ struct StageSrc {
   __device__ __forceinline__ StageSrc(const bf16_t *p, int64_t s, int n, int t)
       : base(p), st(s), nrows(n), off(static_cast<uint32_t>((2 * (t & 15) * s + 8 * (t >> 4)) * 2)),
         off1(off + static_cast<uint32_t>(2 * s)) {}
-  __device__ __forceinline__ Stage2 load(int row0) const {
-    const int rows = min(kT, nrows - row0);
+  __device__ __forceinline__ Stage2 load(int row0) const { return load(row0, min(kT, nrows - row0)); }
+  __device__ __forceinline__ Stage2 load(int row0, int rows) const {
     if constexpr (ANY) {
       const int r0 = 2 * (threadIdx.x & 15);
       const bf16_t *p = base + (row0 + r0) * st + 8 * ((threadIdx.x & 127) >> 4);
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
   const KeyWalk<kT> walk(WIN ? a.q_start + qb * kBlk : 0, kv_end, WIN ? a.window : kMaxWindow, WIN ? a.sinks : 0);
   const int t_begin = WIN ? 0 : chunk * a.cq, t_end = WIN ? walk.count : min(dq_tiles(qb, a.L, a.q_start), t_begin + a.cq);
   if (!WIN && t_begin >= t_end) return;
-  auto tile_at = [&](int x) { return WIN ? walk.tile(x) : x; };
+  auto key_at = [&](int x) { return WIN ? walk.start(x) : x * kT; };
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lc = lane & 31, hh = lane >> 5;
@@ -186,7 +186,8 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
   const bool kside = w < 2;
   const StageSrc<ANY> src(kside ? a.k + b * a.k_sb + kvh * a.k_sh : a.v + b * a.v_sb + kvh * a.v_sh, kside ? a.k_st : a.v_st,
                      kv_end, tid & 127);
-  Stage2 stg = src.load(tile_at(t_begin) * kT);
+  auto load_tile = [&](int x) { return WIN ? src.load(walk.start(x), walk.rows(x)) : src.load(x * kT); };
+  Stage2 stg = load_tile(t_begin);
   const int qr = min(my_q, a.L - 1);
 
   // this lane's query row: Q and dO as B operands (d = 16 ds + 8 hh .. +8), Delta
@@ -236,24 +237,13 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
   f32x16 pkacc[2];
   pkacc[0] = pkacc[1] = f32x16{};
 
-  auto store_kv = [&](Stage2 g, int buf, int x) {
-    if constexpr (WIN) {  // rows that no query of the block sees may hold anything: 0 * NaN
-      const int n0 = tile_at(x) * kT;
-      if (n0 < walk.lo && n0 + kT > a.sinks) {
-        const int r0 = n0 + 2 * (tid & 15);
-        const uint4 z = {0u, 0u, 0u, 0u};
-        if (r0 < walk.lo && r0 >= a.sinks) g.a = z;
-        if (r0 + 1 < walk.lo && r0 + 1 >= a.sinks) g.b = z;
-      }
-    }
-    stage_store(g, tid & 127, kside ? sK[buf] : sV[buf], kside ? sKT[buf] : nullptr);
-  };
-  // WIN: this lane's entry of tile x's window, d = key - q_abs = 32 x - q_start - q0 - 31 + lane, loaded a
+  auto store_kv = [&](const Stage2 &g, int buf) { stage_store(g, tid & 127, kside ? sK[buf] : sV[buf], kside ? sKT[buf] : nullptr); };
+  // WIN: this lane's entry of tile x's window, d = key - q_abs = key_at(x) - q_start - q0 - 31 + lane, loaded a
   // tile ahead (outside the table, where no query of the wave sees a key: zeros)
   const buf_t dbuf = make_buf(WIN ? a.dist + static_cast<size_t>(h) * a.dist_n : nullptr, WIN ? a.dist_n * 8u : 0u);
   const buf_t mbuf = make_buf(WIN ? a.dmu + static_cast<size_t>(h) * a.dist_n : nullptr, WIN && MU ? a.dist_n * 4u : 0u);
   auto dist_at = [&](int x) {
-    const uint32_t i = static_cast<uint32_t>(a.q_start + q0 + 31 - lane - tile_at(x) * kT);
+    const uint32_t i = static_cast<uint32_t>(a.q_start + q0 + 31 - lane - key_at(x));
     const uint32_t o = i < static_cast<uint32_t>(a.dist_n) ? i : 0x10000000u;
     const uint2 u = buf_ld8(dbuf, 8u * o);
     float4 r{__uint_as_float(u.x), __uint_as_float(u.y), 0.f, 0.f};
@@ -262,15 +252,15 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
   };
   float4 dnext{};
   if constexpr (WIN) dnext = dist_at(t_begin);
-  store_kv(stg, 0, t_begin);
-  stg = src.load(tile_at(t_begin + 1) * kT);  // (past the last tile: zeros)
+  store_kv(stg, 0);
+  stg = load_tile(t_begin + 1);  // (past the last tile: zeros)
   __syncthreads();
 
   for (int kt = t_begin; kt < t_end; ++kt) {
-    const int n0 = tile_at(kt) * kT, buf = (kt - t_begin) & 1;
+    const int n0 = key_at(kt), buf = (kt - t_begin) & 1;
     if (kt + 1 < t_end) {  // the next tile into the other buffer (free since the last barrier)
-      store_kv(stg, buf ^ 1, kt + 1);
-      stg = src.load(tile_at(kt + 2) * kT);
+      store_kv(stg, buf ^ 1);
+      stg = load_tile(kt + 2);
     }
     const float4 dcur = dnext;
     if constexpr (WIN) dnext = dist_at(kt + 1);
@@ -301,9 +291,10 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
         pacc = mma32(vo, dreg[ds], pacc);
       }
       float dz[16], pr[WIN ? 16 : 1];
-      // WIN: the tile's keys that this query sees, kk <= m_hi and (kk > m_lo or kk < m_first)
-      const int m_hi = qv ? k_max - n0 : -1, m_lo = q_abs - a.window - n0, m_first = a.sinks - n0;
       auto body = [&](auto masked) {
+        uint32_t seen = 0u;  // WIN: the tile's keys that this query sees
+        if constexpr (WIN && decltype(masked)::value)
+          seen = qv ? seen_keys(min(k_max - n0, walk.rows(kt) - 1), q_abs - a.window - n0, a.sinks - n0) >> (4 * hh) : 0u;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int kk = 8 * (r >> 2) + 4 * hh + (r & 3);
@@ -313,7 +304,7 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
             // g x^beta and g x^beta log2 x
             // (the two large terms that cancel first: what is left is of the bias's size)
             float p = fast_exp2(fmaf(cla, wv.x, fmaf(cls, sacc[r], -lse2)));
-            if constexpr (decltype(masked)::value) p = ((kk <= m_hi) & ((kk > m_lo) | (kk < m_first))) ? p : 0.f;
+            if constexpr (decltype(masked)::value) p = seen & (1u << (8 * (r >> 2) + (r & 3))) ? p : 0.f;
             const float g = p * (pacc[r] - delta);
             psum += p;
             rho += g;

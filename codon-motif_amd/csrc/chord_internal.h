@@ -59,22 +59,25 @@ const char *kv4_check(const KV4Args &kv, int D);  // what is wrong with a cache'
 __device__ __forceinline__ float kv4_scale(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float kv4_base(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
-// The tiles of TS keys that queries at positions [first, last] meet under a window: those that hold
-// first tokens, then those of the windows, up to key `end` (exclusive).  Tiles between them hold no
-// key that any of these queries sees.
+// The tiles of TS keys that queries at positions [first, ..], whose last key is end - 1, meet under a
+// window: those of the first tokens, then those from the lowest key in a window on.  No tile holds a
+// row that none of these queries sees (first tokens end at `se`, windows start at `lo`): what lies
+// between may be anything.  A tile ends after its rows: keys behind them belong to another tile.
 template <int TS> struct KeyWalk {
-  int lo, ns, t0, count;  // the lowest key in a window, tiles of first tokens, first window tile, all tiles
-  __host__ __device__ KeyWalk(int first, int end, int window, int sinks) {
+  int lo, se, end, ns, count;  // tiles of first tokens, all tiles
+  __host__ __device__ KeyWalk(int first, int end_, int window, int sinks) : end(end_) {
     lo = first - window + 1;
     lo = lo > 0 ? lo : 0;
-    t0 = lo / TS;
-    const int se = sinks < end ? sinks : end;
+    se = sinks < end ? sinks : end;
+    if (lo <= se) lo = se = 0;  // one run from the start
     ns = (se + TS - 1) / TS;
-    ns = ns < t0 ? ns : t0;
-    const int tend = (end + TS - 1) / TS;
-    count = ns + (tend > t0 ? tend - t0 : 0);
+    count = ns + (end > lo ? (end - lo + TS - 1) / TS : 0);
   }
-  __host__ __device__ int tile(int i) const { return i < ns ? i : t0 + i - ns; }
+  __host__ __device__ int start(int i) const { return i < ns ? i * TS : lo + (i - ns) * TS; }
+  __host__ __device__ int rows(int i) const {  // of tile i that may be read (none past the last tile)
+    const int n = (i < ns ? se : end) - start(i);
+    return n < 0 ? 0 : n < TS ? n : TS;
+  }
 };
 
 // Keys and query start of a decode launch: from the host arguments, or from the
@@ -88,6 +91,13 @@ __device__ __forceinline__ DecodeWindow decode_window(const ChordArgs &a) {
 
 __device__ __forceinline__ float log_n_at(const ChordArgs &a, int b, int i, int q_start) {
   return a.log_n ? a.log_n[b * a.ln_sb + int64_t(i) * a.ln_st] : a.log_tab[q_start + i];
+}
+
+// Keys of a 32-key tile (bit k: key k) that are <= last, and > out or < first: one register for a lane's
+// masks, a test per key.
+__device__ __forceinline__ uint32_t keys_upto(int x) { return x < 0 ? 0u : x >= 31 ? ~0u : (2u << x) - 1u; }
+__device__ __forceinline__ uint32_t seen_keys(int last, int out, int first) {
+  return keys_upto(last) & (~keys_upto(out) | keys_upto(first - 1));
 }
 
 __device__ __forceinline__ float ggd_bias(float dist, float alpha, float beta, float mu, float eps) {

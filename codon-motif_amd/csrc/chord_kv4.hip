@@ -135,8 +135,8 @@ __global__ void __launch_bounds__(256) chord_kv4_kernel(ChordArgs a, KV4Args kv)
   }
   const uint32_t po = lane < 32 ? 16u * lane : 0x40000000u;
   auto stage = [&](int x) {
-    const int n0 = walk.tile(x) * kStep;
-    const uint32_t n = static_cast<uint32_t>(max(0, min(kStep, k_end - n0)));
+    const int n0 = walk.start(x);
+    const uint32_t n = static_cast<uint32_t>(walk.rows(x));
     const buf_t kb = make_buf(kc + int64_t(n0) * 32, n * 32u), vb = make_buf(vc + int64_t(n0) * 32, n * 32u);
     const buf_t kpb = make_buf(kp + int64_t(n0) * 2, n * 8u), vpb = make_buf(vp + int64_t(n0) * 2, n * 8u);
     buf_ld16_lds<2>(kb, sk, ko[0], 0);
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(256) chord_kv4_kernel(ChordArgs a, KV4Args kv)
       vq[j] = *reinterpret_cast<const uint4 *>(svp + 8 * (16 * g + NK * u) + 16 * j);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and out of it again
-    const int n0 = walk.tile(x) * kStep;
+    const int n0 = walk.start(x);
     if (x + 4 < x_end) stage(x + 4);
     __builtin_amdgcn_sched_barrier(0);
 
@@ -218,12 +218,13 @@ __global__ void __launch_bounds__(256) chord_kv4_kernel(ChordArgs a, KV4Args kv)
       z[e] = fmaf(s, c_qk, c_b * fast_exp2(gbe * fast_log2(d)));
     }
     // the step's last keys, the diagonal, the window's edges: by key (their values' pairs may hold anything)
+    const int n_end = n0 + walk.rows(x);
     const bool masked = n0 + kStep - 1 > q_start || n0 + kStep > k_end || (n0 <= q_start + a.L - 1 - a.window && n0 + kStep > a.sinks);
     if (masked) {
 #pragma unroll
       for (int e = 0; e < NK; ++e) {
         const int key = key0 + e;
-        const bool ok = (key <= q_abs) & (key < k_end) & ((key > q_abs - a.window) | (key < a.sinks));
+        const bool ok = (key <= q_abs) & (key < n_end) & ((key > q_abs - a.window) | (key < a.sinks));
         z[e] = ok ? z[e] : -INFINITY;
         uint4 &pr = vq[e >> 1];
         if (e & 1) { pr.z = ok ? pr.z : 0u; pr.w = ok ? pr.w : 0u; }

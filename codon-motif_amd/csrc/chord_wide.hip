@@ -116,10 +116,6 @@ template <typename T, int N> struct Piece {
       w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
     }
   }
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int x = 0; x < kW; ++x) w[x] = 0u;
-  }
   __device__ __forceinline__ float get(int e) const {
     if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
     const uint16_t b = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
@@ -171,7 +167,6 @@ template <int D, int N> struct Piece4 {
     if constexpr (N == 1) c >>= 4 * (f & 1);
     p = __builtin_amdgcn_raw_buffer_load_b32(pb, 4u * static_cast<uint32_t>(row * Row4<D>::kG + f / (D / Row4<D>::kG)), 0, 0);
   }
-  __device__ __forceinline__ void clear() { c = p = 0u; }
   __device__ __forceinline__ float get(int e) const {
     return fmaf(static_cast<float>((c >> (4 * e)) & 15u), kv4_scale(p), kv4_base(p));
   }
@@ -196,23 +191,24 @@ chord_wide_kernel(ChordArgs a, KV4Args kv) {
   const KeyWalk<32> walk = MODE == kCausal ? KeyWalk<32>(0, kv_end, kMaxWindow, 0)
                                            : KeyWalk<32>(q_start + q0, kv_end, a.window, a.sinks);
   const int ntiles = MODE == kCausal ? (kv_end + 31) / 32 : walk.count;
-  auto tile_at = [&](int x) { return MODE == kCausal ? x : walk.tile(x); };
+  const int q_max = min(q_abs, kv_end - 1);  // this query's last key
+  // the first key of tile x and the rows of it that are read (none past the last tile)
+  auto key_at = [&](int x) { return MODE == kCausal ? 32 * x : walk.start(x); };
+  auto rows_at = [&](int x) { return MODE == kCausal ? min(32, kv_end - 32 * x) : walk.rows(x); };
 
   const T *kp = static_cast<const T *>(a.k) + b * a.k_sb + kvh * a.k_sh;
   const T *vp = static_cast<const T *>(a.v) + b * a.v_sb + kvh * a.v_sh;
-  // the buffer of tile t: its rows below kv_end (rows past it read zeros)
-  auto tile_buf = [&](const T *p, int64_t st, int t) {
-    const int rows = min(32, kv_end - 32 * t);
-    return make_buf(p + int64_t(32 * t) * st, rows > 0 ? static_cast<uint32_t>(((rows - 1) * st + D) * ES) : 0u);
+  // the buffer of tile x: rows past its own read zeros
+  auto tile_buf = [&](const T *p, int64_t st, int x) {
+    const int rows = rows_at(x);
+    return make_buf(p + int64_t(key_at(x)) * st, rows > 0 ? static_cast<uint32_t>(((rows - 1) * st + D) * ES) : 0u);
   };
-  // (4-bit rows: codes and pairs of tile t)
-  auto code_buf = [&](const uint8_t *p, int t) {
-    const int rows = min(32, kv_end - 32 * t);
-    return make_buf(p + int64_t(32 * t) * (D / 2), rows > 0 ? static_cast<uint32_t>(rows) * (D / 2) : 0u);
+  // (4-bit rows: codes and pairs of tile x)
+  auto code_buf = [&](const uint8_t *p, int x) {
+    return make_buf(p + int64_t(key_at(x)) * (D / 2), static_cast<uint32_t>(rows_at(x)) * (D / 2));
   };
-  auto pair_buf = [&](const uint32_t *p, int t) {
-    const int rows = min(32, kv_end - 32 * t);
-    return make_buf(p + int64_t(32 * t) * Row4<D>::kG, rows > 0 ? static_cast<uint32_t>(rows) * (4 * Row4<D>::kG) : 0u);
+  auto pair_buf = [&](const uint32_t *p, int x) {
+    return make_buf(p + int64_t(key_at(x)) * Row4<D>::kG, static_cast<uint32_t>(rows_at(x)) * (4 * Row4<D>::kG));
   };
   const uint8_t *kcp = nullptr, *vcp = nullptr;
   const uint32_t *kpp = nullptr, *vpp = nullptr;
@@ -242,11 +238,11 @@ chord_wide_kernel(ChordArgs a, KV4Args kv) {
              static_cast<uint32_t>(min(i, rows - 1) * a.q_st) * ES, h);
     }
   }
-  auto load_k = [&](int t) {  // (past the last tile: an empty buffer, zeros)
-    if constexpr (MODE == k4Bit) k4.load(code_buf(kcp, t), pair_buf(kpp, t), i);
-    else k.load(tile_buf(kp, a.k_st, t), koff, h);
+  auto load_k = [&](int x) {  // (past the last tile: an empty buffer, zeros)
+    if constexpr (MODE == k4Bit) k4.load(code_buf(kcp, x), pair_buf(kpp, x), i);
+    else k.load(tile_buf(kp, a.k_st, x), koff, h);
   };
-  if (w < ntiles) load_k(tile_at(w));
+  if (w < ntiles) load_k(w);
 
   const float mul = a.ssmax[head] * (MODE == kCausal ? a.log_n[b * a.ln_sb + int64_t(min(my_q, a.L - 1)) * a.ln_st]
                                                      : log_n_at(a, b, min(my_q, a.L - 1), q_start));
@@ -265,14 +261,14 @@ chord_wide_kernel(ChordArgs a, KV4Args kv) {
   for (int t = 0; t < VD; ++t) o[t] = f32x16{};
 
   for (int x = w; x < ntiles; x += NW) {
-    const int t = tile_at(x), n0 = 32 * t;
+    const int n0 = key_at(x);
     std::conditional_t<MODE == k4Bit, Piece4<D, VD>, Piece<T, VD>> v[16];
     if constexpr (MODE == k4Bit) {
-      const buf_t vcb = code_buf(vcp, t), vpb = pair_buf(vpp, t);
+      const buf_t vcb = code_buf(vcp, x), vpb = pair_buf(vpp, x);
 #pragma unroll
       for (int r = 0; r < 16; ++r) v[r].load(vcb, vpb, 8 * (r >> 2) + 4 * h + (r & 3), VD * (D < 32 ? i & (D - 1) : i));
     } else {
-      const buf_t vb = tile_buf(vp, a.v_st, t);
+      const buf_t vb = tile_buf(vp, a.v_st, x);
 #pragma unroll
       for (int r = 0; r < 16; ++r) v[r].load(vb, voff + static_cast<uint32_t>(8 * (r >> 2) + (r & 3)) * vrow);
     }
@@ -285,23 +281,17 @@ chord_wide_kernel(ChordArgs a, KV4Args kv) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) bias[r] = winr[8 * (r >> 2) + (r & 3)];
     __builtin_amdgcn_sched_barrier(0);
-    load_k(tile_at(x + NW));  // (past the last tile: an empty buffer, zeros)
+    load_k(x + NW);  // (past the last tile: an empty buffer, zeros)
     __builtin_amdgcn_sched_barrier(0);
     // the diagonal and the last tiles, and with a window those that not every query of the block sees whole
     const bool masked = n0 + 31 > q_start + q0 || n0 + 32 > kv_end ||
                         (MODE != kCausal && n0 <= q_start + q0 + 31 - a.window && n0 + 32 > a.sinks);
+    uint32_t seen = 0u;
+    if (MODE != kCausal && masked) seen = seen_keys(min(q_max - n0, walk.rows(x) - 1), q_abs - a.window - n0, a.sinks - n0) >> (4 * h);
     auto keep = [&](int r) {
       const int key = n0 + 8 * (r >> 2) + 4 * h + (r & 3);
-      return key <= q_abs && key < kv_end && (MODE == kCausal || key > q_abs - a.window || key < a.sinks);
+      return MODE == kCausal ? key <= q_abs && key < kv_end : (seen & (1u << (8 * (r >> 2) + (r & 3)))) != 0u;
     };
-    // rows that no query of the block sees may hold anything (0 * NaN in the products below)
-    if (MODE != kCausal && n0 < walk.lo && n0 + 32 > a.sinks) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int key = n0 + 8 * (r >> 2) + 4 * h + (r & 3);
-        if (key < walk.lo && key >= a.sinks) v[r].clear();
-      }
-    }
     // a logit plus `off`: the fp32 form adds the large terms first, so with off = -max they cancel
     // before the small result is rounded
     auto logit = [&](int r, float off) {

@@ -128,8 +128,8 @@ __global__ void __launch_bounds__(128 * PARTS) __attribute__((amdgpu_waves_per_e
   const float gka = (a.ssmax[head0 + bh] < 0.f ? -1.f : 1.f) / (a.scale != 0.f ? fabsf(a.scale) : 1.f);
   const buf_t dbuf = make_buf(a.dist, TAB ? static_cast<uint32_t>(a.H) * static_cast<uint32_t>(a.dist_n) * 8u : 0u);
   const uint32_t dhead = static_cast<uint32_t>(head0 + bh) * static_cast<uint32_t>(a.dist_n);
-  auto eval = [&](int t, int d) {  // for tile t
-    const bool ok = d <= 0 && (d > -a.window || t * kT < a.sinks);
+  auto eval = [&](int n0, int d) {  // for the tile from key n0 on
+    const bool ok = d <= 0 && (d > -a.window || n0 < a.sinks);
     float bias;
     if constexpr (TAB) {  // (a masked distance may lie past the table: entry 0 is read instead)
       bias = -gal * __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
@@ -153,25 +153,16 @@ __global__ void __launch_bounds__(128 * PARTS) __attribute__((amdgpu_waves_per_e
   const int krow = htid >> 3, vpair = htid & 15, vseg = htid >> 4;
   const uint32_t koff = static_cast<uint32_t>((krow * a.k_st + (htid & 7) * 8) * 2), koff2 = koff + static_cast<uint32_t>(32 * a.k_st);
   const uint32_t voff = static_cast<uint32_t>((2 * vpair * a.v_st + 8 * vseg) * 2), voff2 = voff + static_cast<uint32_t>(2 * a.v_st);
-  auto load_tile = [&](int t) {  // rows from kv_end on read zeros
-    const int rows = min(kT, kv_end - t * kT);
-    const buf_t kr = make_buf(kp + int64_t(t) * kT * a.k_st, rows > 0 ? static_cast<uint32_t>(((rows - 1) * a.k_st + kBD) * 2) : 0u);
-    const buf_t vr = make_buf(vp + int64_t(t) * kT * a.v_st, rows > 0 ? static_cast<uint32_t>(((rows - 1) * a.v_st + kBD) * 2) : 0u);
+  auto load_tile = [&](int x) {  // (rows past the tile's own read zeros)
+    const int n0 = walk.start(x), rows = walk.rows(x);
+    const buf_t kr = make_buf(kp + int64_t(n0) * a.k_st, rows > 0 ? static_cast<uint32_t>(((rows - 1) * a.k_st + kBD) * 2) : 0u);
+    const buf_t vr = make_buf(vp + int64_t(n0) * a.v_st, rows > 0 ? static_cast<uint32_t>(((rows - 1) * a.v_st + kBD) * 2) : 0u);
     kst[0] = buf_ld16(kr, koff);
     kst[1] = buf_ld16(kr, koff2);
     vst[0] = buf_ld16(vr, voff);
     vst[1] = buf_ld16(vr, voff2);
   };
-  auto store_tile = [&](int t, int buf) {
-    const int n0 = t * kT;
-    if (n0 < walk.lo && n0 + kT > a.sinks) {  // rows that no query of the block sees may hold anything
-      auto dead = [&](int row) { return n0 + row < walk.lo && n0 + row >= a.sinks; };
-      const uint4 z{0u, 0u, 0u, 0u};
-      if (dead(krow)) kst[0] = z;
-      if (dead(krow + 16)) kst[1] = z;
-      if (dead(2 * vpair)) vst[0] = z;
-      if (dead(2 * vpair + 1)) vst[1] = z;
-    }
+  auto store_tile = [&](int buf) {
     bf16_t *kd = sK(buf) + krow * kRowK + (htid & 7) * 8;
     *reinterpret_cast<uint4 *>(kd) = kst[0];
     *reinterpret_cast<uint4 *>(kd + 16 * kRowK) = kst[1];
@@ -187,20 +178,19 @@ __global__ void __launch_bounds__(128 * PARTS) __attribute__((amdgpu_waves_per_e
   float m_run = -INFINITY, l_run = 0.f;  // per column (m: acc units; l: this lane's share)
   f32x16 oacc[2] = {f32x16{}, f32x16{}};  // O^T rows d = 32 dt + 8 (r / 4) + 4 hh + r % 4, column lc
 
-  load_tile(walk.tile(t_first));
-  store_tile(walk.tile(t_first), 0);
-  float bnew = eval(walk.tile(t_first), walk.tile(t_first) * kT + d0);
-  store_bias(bnew, eval(walk.tile(t_first), walk.tile(t_first) * kT + d0 - kT));
-  load_tile(walk.tile(t_first + 1));
+  load_tile(t_first);
+  store_tile(0);
+  float bnew = eval(walk.start(t_first), walk.start(t_first) + d0);
+  store_bias(bnew, eval(walk.start(t_first), walk.start(t_first) + d0 - kT));
+  load_tile(t_first + 1);
   __syncthreads();
 
   for (int i = 0; i < nsteps; ++i) {
-    const int t = walk.tile(t_first + i), n0 = t * kT, buf = i & 1;
-    const int tn = walk.tile(t_first + i + 1);
+    const int n0 = walk.start(t_first + i), nn = walk.start(t_first + i + 1), buf = i & 1;
     // the next tile's new distances ahead of this tile's work
     float bold = bnew;
-    bnew = eval(tn, tn * kT + d0);
-    if (tn != t + 1 || n0 < a.sinks) bold = eval(tn, tn * kT + d0 - kT);
+    bnew = eval(nn, nn + d0);
+    if (nn != n0 + kT || n0 < a.sinks) bold = eval(nn, nn + d0 - kT);
     if (i < t_count && n0 < wave_kv_end && (n0 + kT - 1 > q_start + q0 - a.window || n0 < a.sinks)) {
       f32x16 acc;
 #pragma unroll
@@ -214,13 +204,10 @@ __global__ void __launch_bounds__(128 * PARTS) __attribute__((amdgpu_waves_per_e
       }
       // by key: tiles of first tokens at the window's edge, and the end of the keys
       if ((n0 < a.sinks && n0 + kT > a.sinks && n0 <= q_start + q_last - a.window) || n0 + kT > Skv) {
-        // (kk from Skv on, or outside the window without being a first token)
-        const int e = Skv - n0 - 4 * hh, lo = q_start + my_q - a.window - n0 - 4 * hh, first = a.sinks - n0 - 4 * hh;
+        const uint32_t seen =
+            seen_keys(walk.rows(t_first + i) - 1, q_start + my_q - a.window - n0, a.sinks - n0) >> (4 * hh);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int kk = 8 * (r >> 2) + (r & 3);
-          acc[r] = (kk < e) & ((kk > lo) | (kk < first)) ? acc[r] : -INFINITY;
-        }
+        for (int r = 0; r < 16; ++r) acc[r] = seen & (1u << (8 * (r >> 2) + (r & 3))) ? acc[r] : -INFINITY;
       }
       float mx = acc[0];
 #pragma unroll
@@ -267,8 +254,8 @@ __global__ void __launch_bounds__(128 * PARTS) __attribute__((amdgpu_waves_per_e
     // the next tile's bias rows (this wave's own; its reads above come first) and rows into LDS (the
     // other buffer, last read before the previous barrier), the tile after into flight
     store_bias(bnew, bold);
-    store_tile(tn, buf ^ 1);
-    load_tile(walk.tile(t_first + i + 2));
+    store_tile(buf ^ 1);
+    load_tile(t_first + i + 2);
     __syncthreads();
   }
 
