@@ -785,7 +785,8 @@ __device__ __forceinline__ void rms_norm16(uint4 &u0, uint4 &u1, const uint4 w0,
   u1 = uint4{o1[0], o1[1], o1[2], o1[3]};
 }
 
-template <bool STEP>
+// WIN: under a window (a.window, a.sinks): the splits share the 32-key tiles of first tokens and windows.
+template <bool STEP, bool WIN>
 __global__ void __launch_bounds__(256) chord_decode_mfma_kernel(ChordArgs a, StepArgs sa) {
   // wave index in an SGPR: the key loop below is then scalar (MFMAs must not sit
   // under a lane-mask branch, as they ignore EXEC)
@@ -833,6 +834,8 @@ __global__ void __launch_bounds__(256) chord_decode_mfma_kernel(ChordArgs a, Ste
   const int i_last = min(a.L - 1, (qc * kMfmaRows + kMfmaRows - 1) / group);
   const int k_lo = split * per;
   const int k_hi = min(min(kv_len, k_lo + per), q_start + i_last + 1);
+  const KeyWalk<32> walk(WIN ? q_start : 0, WIN ? min(kv_len, q_start + a.L) : 0, WIN ? a.window : 1, WIN ? a.sinks : 0);
+  const int x_per = (walk.count + a.splits - 1) / a.splits;  // tiles of a split (WIN)
 
   const bf16_t *kp = static_cast<const bf16_t *>(a.k) + b * a.k_sb + kvh * a.k_sh;
   const bf16_t *vp = static_cast<const bf16_t *>(a.v) + b * a.v_sb + kvh * a.v_sh;
@@ -858,6 +861,16 @@ __global__ void __launch_bounds__(256) chord_decode_mfma_kernel(ChordArgs a, Ste
     const int r = 8 * i + (lane >> 3);
     kdo[i] = static_cast<uint32_t>((r * a.k_st + 8 * ((lane & 7) ^ (r & 7))) * 2);
   }
+  auto load_tile = [&](int x, Stage &st) {  // WIN: tile x of the walk (rows past its own read zeros)
+    const int n0 = walk.start(x), rows = walk.rows(x);
+    const buf_t kt = make_buf(kp + int64_t(n0) * a.k_st, rows > 0 ? static_cast<uint32_t>(((rows - 1) * a.k_st + kD) * 2) : 0u);
+    const buf_t vt = make_buf(vp + int64_t(n0) * a.v_st, rows > 0 ? static_cast<uint32_t>(((rows - 1) * a.v_st + kD) * 2) : 0u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) buf_ld16_lds<2>(kt, myK + 8 * i * 64, kdo[i], 0);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      st.v[r] = buf_ld16_nt(vt, static_cast<uint32_t>(((8 * r + (lane >> 3)) * a.v_st + 8 * (lane & 7)) * 2));
+  };
   auto load_stage = [&](int n0, Stage &st) {
     const uint32_t ks = static_cast<uint32_t>(n0 * a.k_st * 2);
 #pragma unroll
@@ -880,7 +893,9 @@ __global__ void __launch_bounds__(256) chord_decode_mfma_kernel(ChordArgs a, Ste
     if (w == 0) {
       const int is_v = lane >> 5, t = (lane >> 3) & 3, piece = lane & 7;
       const int pos = q_start + t;
-      const bool mine = t < a.L && pos >= k_lo && pos < k_lo + per && pos < a.S;
+      // (a new position is never before the window's start)
+      const bool mine = t < a.L && pos < a.S &&
+                        (WIN ? (walk.ns + (pos - walk.lo) / 32) / max(x_per, 1) == split : pos >= k_lo && pos < k_lo + per);
       const bf16_t *src = sa.proj + b * sa.p_sb + int64_t(min(t, a.L - 1)) * sa.p_st + (is_v ? sa.v_off : sa.k_off) +
                           kvh * kD + 8 * piece;
       const uint4 u = *reinterpret_cast<const uint4 *>(src);
@@ -919,10 +934,18 @@ __global__ void __launch_bounds__(256) chord_decode_mfma_kernel(ChordArgs a, Ste
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
   }
 
-  int n0 = k_lo + w * 32;
+  // position of the loop: the step's first key, or (WIN) its tile
+  int at = WIN ? split * x_per + w : k_lo + w * 32;
+  const int at_end = WIN ? min(walk.count, (split + 1) * x_per) : k_hi, at_step = WIN ? 4 : 4 * 32;
+  auto load_at = [&](int x, Stage &st) {
+    if constexpr (WIN) load_tile(x, st);
+    else load_stage(x, st);
+  };
   Stage cur;
-  if (n0 < k_hi) load_stage(n0, cur);
-  for (; n0 < k_hi; n0 += 4 * 32) {
+  if (at < at_end) load_at(at, cur);
+  for (; at < at_end; at += at_step) {
+    const int n0 = WIN ? walk.start(at) : at;
+    const uint32_t seen = WIN ? seen_keys(min(qabs - n0, walk.rows(at) - 1), qabs - a.window - n0, a.sinks - n0) >> (4 * g) : 0u;
     // this step's K rows have landed in LDS (and its V rows in registers): operands out,
     // then the buffer takes the next step's rows
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -934,7 +957,7 @@ __global__ void __launch_bounds__(256) chord_decode_mfma_kernel(ChordArgs a, Ste
         kop[t][pc] = *reinterpret_cast<const uint4 *>(myK + (16 * t + c16) * 64 + 8 * ((2 * g + pc) ^ (c16 & 7)));
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     Stage nxt;
-    load_stage(n0 + 4 * 32, nxt);
+    load_at(at + at_step, nxt);
     __builtin_amdgcn_sched_barrier(0);
     // V rows of this step into the wave's LDS tile (row-major, padded rows)
 #pragma unroll
@@ -950,7 +973,7 @@ __global__ void __launch_bounds__(256) chord_decode_mfma_kernel(ChordArgs a, Ste
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int key = n0 + 16 * t + 4 * g + i;
-        const bool ok = key < k_hi && key <= qabs;
+        const bool ok = WIN ? (seen & (1u << (16 * t + i))) != 0u : key < k_hi && key <= qabs;
         const float bt = ggd_bias(static_cast<float>(key - qabs), g_alpha, g_beta, g_mu, a.eps);
         sc[t][i] = ok ? fmaf(sacc[i], c_qk, c_b * bt) : -INFINITY;
       }
@@ -1165,6 +1188,23 @@ static int decode_splits(int B, int Hkv, int S) {
   return std::max(1, std::min(want, 32));
 }
 
+// Splits of a windowed decode: about three workgroups per CU, and a tile for each of their waves.
+int chord_window_splits(int B, int Hkv, int L, int S, int window, int sinks) {
+  const int64_t keys = std::min<int64_t>(S, std::min<int64_t>(window, S) + L + std::min(sinks, S) + 2 * 32);
+  const int64_t base = std::max<int64_t>(1, int64_t(B) * Hkv), tiles = (keys + 31) / 32;
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(3 * device_cu_count() + base - 1) / base, (tiles + 3) / 4, 32})));
+}
+
+bool chord_window_decode_serves(int H, int Hkv, int L, int D, int dtype) {
+  return dtype == MOTIF_BF16 && D == kD && (H / Hkv) * static_cast<int64_t>(L) <= kMfmaRows;
+}
+
+int launch_chord_window_decode(const ChordArgs &a, hipStream_t s) {
+  chord_decode_mfma_kernel<false, true><<<dim3(a.splits, a.Hkv, a.B), dim3(256), 0, s>>>(a, StepArgs{});
+  if (const int rc = check_launch("chord_decode_mfma_kernel"); rc || !a.part) return rc;
+  return launch_chord_merge(a, MOTIF_BF16, kD, s);
+}
+
 template <typename T, int D>
 static void launch_decode_d(const ChordArgs &a, int R, const float *tab, int tab_n, hipStream_t s) {
   const dim3 grid(a.splits, a.Hkv, a.B * a.nqc), block(256);
@@ -1350,7 +1390,7 @@ extern "C" int motif_chord_fwd(
       if (rc) return rc;
     }
     if (!mfma) return launch_vector_dt(dtype, a, R, D, tab, tn, s);
-    chord_decode_mfma_kernel<false><<<dim3(a.splits, Hkv, B * a.nqc), dim3(256), 0, s>>>(a, StepArgs{});
+    chord_decode_mfma_kernel<false, false><<<dim3(a.splits, Hkv, B * a.nqc), dim3(256), 0, s>>>(a, StepArgs{});
     rc = check_launch("chord_decode_kernel");
     if (rc || a.splits == 1) return rc;
     chord_merge_kernel<bf16_t><<<dim3(rows, Hkv, B), dim3(64), 0, s>>>(a);
@@ -1457,7 +1497,7 @@ int motif::chord_decode_run(
     return launch_vector_dt(dtype, a, R, D, tab, tn, s);  // its merge advances the cursor
   }
   a.nqc = (rows + kMfmaRows - 1) / kMfmaRows;
-  chord_decode_mfma_kernel<false><<<dim3(splits, Hkv, B * a.nqc), dim3(256), 0, s>>>(a, StepArgs{});
+  chord_decode_mfma_kernel<false, false><<<dim3(splits, Hkv, B * a.nqc), dim3(256), 0, s>>>(a, StepArgs{});
   if ((rc = check_launch("chord_decode_kernel"))) return rc;
   chord_merge_kernel<bf16_t><<<dim3(rows, Hkv, B), dim3(64), 0, s>>>(a);
   return check_launch("chord_merge_kernel");
@@ -1495,7 +1535,12 @@ extern "C" size_t motif_chord_decode_step_workspace_bytes(int B, int H, int Hkv,
   return motif::step_ws_bytes(B, H, Hkv, L, motif::decode_splits(B, Hkv, capacity));
 }
 
-extern "C" int motif_chord_decode_step(
+namespace motif {
+
+constexpr int kNoWindow = 0;
+
+// The body of motif_chord_decode_step (window kNoWindow) and motif_chord_window_step.
+static int chord_decode_step_run(
     const void *proj, int64_t p_sb, int64_t p_st, int q_off, int k_off, int v_off,
     const void *q_norm_weight, const void *k_norm_weight, float norm_eps,
     void *k_cache, int64_t k_sb, int64_t k_sh, int64_t k_st,
@@ -1504,9 +1549,8 @@ extern "C" int motif_chord_decode_step(
     const float *alpha, const float *beta, const float *mu, const float *ssmax,
     const float *log_table, int log_table_len,
     void *out, int64_t o_sb, int64_t o_sh, int64_t o_st,
-    int B, int H, int Hkv, int L, int D, float scale, float eps,
+    int B, int H, int Hkv, int L, int D, float scale, float eps, int window, int sinks,
     void *workspace, size_t workspace_bytes, void *stream) {
-  using namespace motif;
   if (B < 0 || H <= 0 || Hkv <= 0 || L < 0 || H % Hkv)
     return set_error(MOTIF_ERR_INVALID, "chord_decode_step: bad size");
   if (D != kD || (H / Hkv) * L > kMfmaRows)
@@ -1523,7 +1567,8 @@ extern "C" int motif_chord_decode_step(
         reinterpret_cast<uintptr_t>(k_norm_weight) | reinterpret_cast<uintptr_t>(k_cache) |
         reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(out)) & 15) != 0)
     return set_error(MOTIF_ERR_UNSUPPORTED, "chord_decode_step: rows must be 16-byte aligned");
-  const int splits = decode_splits(B, Hkv, capacity);
+  const int splits = window != kNoWindow ? chord_window_splits(B, Hkv, L, capacity, window, sinks)
+                                         : decode_splits(B, Hkv, capacity);
   const size_t need = step_ws_bytes(B, H, Hkv, L, splits);
   if (!workspace || workspace_bytes < need)
     return set_error(MOTIF_ERR_INVALID, "chord_decode_step: workspace too small (need " + std::to_string(need) + " bytes)");
@@ -1543,6 +1588,7 @@ extern "C" int motif_chord_decode_step(
   a.splits = splits;
   a.nqc = 1;
   a.len_dev = length_dev; a.log_tab = log_table;
+  a.window = window; a.sinks = sinks;
   StepArgs sa;
   sa.proj = static_cast<const bf16_t *>(proj); sa.p_sb = p_sb; sa.p_st = p_st;
   sa.q_off = q_off; sa.k_off = k_off; sa.v_off = v_off;
@@ -1550,6 +1596,52 @@ extern "C" int motif_chord_decode_step(
   sa.neps = norm_eps;
   sa.cnt = reinterpret_cast<int *>(static_cast<char *>(workspace) + (need - (static_cast<size_t>(B) * Hkv + 1) * sizeof(int)));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  chord_decode_mfma_kernel<true><<<dim3(splits, Hkv, B), dim3(256), 0, s>>>(a, sa);
+  if (window != kNoWindow) chord_decode_mfma_kernel<true, true><<<dim3(splits, Hkv, B), dim3(256), 0, s>>>(a, sa);
+  else chord_decode_mfma_kernel<true, false><<<dim3(splits, Hkv, B), dim3(256), 0, s>>>(a, sa);
   return check_launch("chord_decode_step");
+}
+
+}  // namespace motif
+
+extern "C" int motif_chord_decode_step(
+    const void *proj, int64_t p_sb, int64_t p_st, int q_off, int k_off, int v_off,
+    const void *q_norm_weight, const void *k_norm_weight, float norm_eps,
+    void *k_cache, int64_t k_sb, int64_t k_sh, int64_t k_st,
+    void *v_cache, int64_t v_sb, int64_t v_sh, int64_t v_st,
+    int *length_dev, int capacity,
+    const float *alpha, const float *beta, const float *mu, const float *ssmax,
+    const float *log_table, int log_table_len,
+    void *out, int64_t o_sb, int64_t o_sh, int64_t o_st,
+    int B, int H, int Hkv, int L, int D, float scale, float eps,
+    void *workspace, size_t workspace_bytes, void *stream) {
+  return motif::chord_decode_step_run(proj, p_sb, p_st, q_off, k_off, v_off, q_norm_weight, k_norm_weight, norm_eps, k_cache,
+                                      k_sb, k_sh, k_st, v_cache, v_sb, v_sh, v_st, length_dev, capacity, alpha, beta, mu,
+                                      ssmax, log_table, log_table_len, out, o_sb, o_sh, o_st, B, H, Hkv, L, D, scale, eps,
+                                      motif::kNoWindow, 0, workspace, workspace_bytes, stream);
+}
+
+extern "C" size_t motif_chord_window_step_workspace_bytes(int B, int H, int Hkv, int L, int capacity, int window, int sinks) {
+  if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || L <= 0 || capacity < L || window < 1 || sinks < 0) return 0;
+  return motif::step_ws_bytes(B, H, Hkv, L, motif::chord_window_splits(B, Hkv, L, capacity, window, sinks));
+}
+
+extern "C" int motif_chord_window_step(
+    const void *proj, int64_t p_sb, int64_t p_st, int q_off, int k_off, int v_off,
+    const void *q_norm_weight, const void *k_norm_weight, float norm_eps,
+    void *k_cache, int64_t k_sb, int64_t k_sh, int64_t k_st,
+    void *v_cache, int64_t v_sb, int64_t v_sh, int64_t v_st,
+    int *length_dev, int capacity,
+    const float *alpha, const float *beta, const float *mu, const float *ssmax,
+    const float *log_table, int log_table_len,
+    void *out, int64_t o_sb, int64_t o_sh, int64_t o_st,
+    int B, int H, int Hkv, int L, int D, float scale, float eps,
+    int window, int sinks, void *workspace, size_t workspace_bytes, void *stream) {
+  using namespace motif;
+  if (window < 1 || sinks < 0) return set_error(MOTIF_ERR_INVALID, "chord_window_step: need window >= 1 and sinks >= 0");
+  if (capacity >= kMaxWindow || k_st < 0 || v_st < 0 || k_st >= (int64_t(1) << 24) || v_st >= (int64_t(1) << 24))
+    return set_error(MOTIF_ERR_UNSUPPORTED, "chord_window_step: cache too long or its row strides out of range");
+  return chord_decode_step_run(proj, p_sb, p_st, q_off, k_off, v_off, q_norm_weight, k_norm_weight, norm_eps, k_cache, k_sb,
+                               k_sh, k_st, v_cache, v_sb, v_sh, v_st, length_dev, capacity, alpha, beta, mu, ssmax, log_table,
+                               log_table_len, out, o_sb, o_sh, o_st, B, H, Hkv, L, D, scale, eps,
+                               std::min(window, kMaxWindow), std::min(sinks, kMaxWindow), workspace, workspace_bytes, stream);
 }

@@ -172,9 +172,8 @@ template <int D, int N> struct Piece4 {
   }
 };
 
-template <typename T, int D, int NW, int MODE>
-__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4)))
-chord_wide_kernel(ChordArgs a, KV4Args kv) {
+template <typename T, int D, int NW, int MODE, int EU>  // EU: waves per SIMD
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(EU, EU))) chord_wide_kernel(ChordArgs a, KV4Args kv) {
   constexpr int VD = D >= 32 ? D / 32 : 1;  // output tiles, and features of a V piece
   // the scores' operand type: a 4-bit cache's values are fp32
   using KT = std::conditional_t<MODE == k4Bit, float, T>;
@@ -281,7 +280,9 @@ chord_wide_kernel(ChordArgs a, KV4Args kv) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) bias[r] = winr[8 * (r >> 2) + (r & 3)];
     __builtin_amdgcn_sched_barrier(0);
-    load_k(x + NW);  // (past the last tile: an empty buffer, zeros)
+    // (fp32 keys under a window, whose masks need the registers, come in with the output's product)
+    constexpr bool kLateK = MODE != kCausal && KS == 4;
+    if constexpr (!kLateK) load_k(x + NW);  // (past the last tile: an empty buffer, zeros)
     __builtin_amdgcn_sched_barrier(0);
     // the diagonal and the last tiles, and with a window those that not every query of the block sees whole
     const bool masked = n0 + 31 > q_start + q0 || n0 + 32 > kv_end ||
@@ -333,6 +334,11 @@ chord_wide_kernel(ChordArgs a, KV4Args kv) {
       ps[r & 3] += s[r];
     }
     l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+    if constexpr (kLateK) {
+      __builtin_amdgcn_sched_barrier(0);
+      load_k(x + NW);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     if constexpr (ES == 4) {  // four fresh chains per tile, as for the scores
 #pragma unroll
       for (int t2 = 0; t2 < VD; ++t2) {
@@ -402,24 +408,37 @@ chord_wide_kernel(ChordArgs a, KV4Args kv) {
 // *len_dev += L behind the launch that read it
 __global__ void chord_advance_kernel(int *len_dev, int L, int capacity) { *len_dev = min(*len_dev + L, capacity); }
 
-template <typename T, int D, int NW, int MODE>
+template <typename T, int D, int NW, int MODE, int EU>
 int launch_wide(const ChordArgs &a, const KV4Args &kv, hipStream_t s) {
   constexpr int smem = (2 * 64 * NW + NW * 16 * 64) * static_cast<int>(sizeof(float));
   const dim3 grid(a.H, (a.L + 31) / 32, a.B), block(64 * NW);
-  chord_wide_kernel<T, D, NW, MODE><<<grid, block, smem, s>>>(a, kv);
+  chord_wide_kernel<T, D, NW, MODE, EU><<<grid, block, smem, s>>>(a, kv);
   if (const int rc = check_launch("chord_wide_kernel"); rc || MODE == kCausal || !a.len_dev) return rc;
   chord_advance_kernel<<<dim3(1), dim3(1), 0, s>>>(a.len_dev, a.L, a.S);
   return check_launch("chord_advance_kernel");
 }
 
+// A window's blocks are short and many: where they pass one per CU, four waves each let two blocks
+// share a CU (2 x 517 fp32 queries over 1023 keys, 408 blocks, windows of 128 / 259 / 1023: eight waves
+// 37 / 49 / 74 us, four KFOUR); where they do not, eight waves shorten the chain.
+template <typename T, int D, int MODE>
+int launch_wide_n(const ChordArgs &a, const KV4Args &kv, hipStream_t s) {
+  if constexpr (MODE != kCausal) {
+    if (static_cast<int64_t>(a.H) * ((a.L + 31) / 32) * a.B > chord_cu_count()) return launch_wide<T, D, 4, MODE, 2>(a, kv, s);
+  }
+  return launch_wide<T, D, 8, MODE, 2>(a, kv, s);
+}
+
 template <typename T, int MODE>
 int launch_wide_t(const ChordArgs &a, const KV4Args &kv, int D, hipStream_t s) {
   switch (D) {
-    case 16: return launch_wide<T, 16, 8, MODE>(a, kv, s);
-    case 32: return launch_wide<T, 32, 8, MODE>(a, kv, s);
-    case 64: return launch_wide<T, 64, 8, MODE>(a, kv, s);
-    // (fp32 rows of 128 features leave no registers for a second wave per SIMD)
-    default: return launch_wide<T, 128, sizeof(T) == 4 || MODE == k4Bit ? 4 : 8, MODE>(a, kv, s);
+    case 16: return launch_wide_n<T, 16, MODE>(a, kv, s);
+    case 32: return launch_wide_n<T, 32, MODE>(a, kv, s);
+    case 64: return launch_wide_n<T, 64, MODE>(a, kv, s);
+    default:
+      // (fp32 rows of 128 features leave no registers for a second wave per SIMD)
+      if constexpr (sizeof(T) == 4 || MODE == k4Bit) return launch_wide<T, 128, 4, MODE, 1>(a, kv, s);
+      else return launch_wide_n<T, 128, MODE>(a, kv, s);
   }
 }
 

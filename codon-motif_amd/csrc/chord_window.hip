@@ -421,8 +421,17 @@ extern "C" int motif_chord_window_fwd(
   int rc = fill(c, a);
   if (rc || B == 0 || L == 0) return rc;
   if ((rc = fill_rows(c, a, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st))) return rc;
-  (void)workspace; (void)workspace_bytes;
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (chord_window_decode_serves(H, Hkv, L, D, dtype) && !lse) {
+    a.splits = chord_window_splits(B, Hkv, L, S, window, sinks);
+    if (a.splits > 1 || length_dev) {  // (the merge advances the cursor)
+      const size_t need = motif_chord_window_workspace_bytes(B, H, Hkv, L, S, D, window, sinks, dtype);
+      if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 3))
+        return set_error(MOTIF_ERR_INVALID, "chord_window_fwd: workspace too small (need " + std::to_string(need) + " bytes) or not aligned");
+      a.part = static_cast<float *>(workspace);
+    }
+    return launch_chord_window_decode(a, st);
+  }
   if (distances && distances_len < distance_count(L, q_start, window, sinks))
     return set_error(MOTIF_ERR_INVALID, "chord_window_fwd: distance table too short");
   a.dist = reinterpret_cast<const float2 *>(distances);
@@ -449,8 +458,10 @@ extern "C" int motif_chord_distances(const float *beta, const float *mu, int H, 
 
 extern "C" size_t motif_chord_window_workspace_bytes(int B, int H, int Hkv, int L, int S, int D, int window, int sinks,
                                                      int dtype) {
-  (void)B; (void)H; (void)Hkv; (void)L; (void)S; (void)D; (void)window; (void)sinks; (void)dtype;
-  return 0;
+  if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || L <= 0 || S <= 0 || window < 1 || sinks < 0 ||
+      !chord_window_decode_serves(H, Hkv, L, D, dtype))
+    return 0;
+  return static_cast<size_t>(B) * H * L * chord_window_splits(B, Hkv, L, S, window, sinks) * (D + 2) * sizeof(float);
 }
 
 extern "C" size_t motif_chord_kv4_workspace_bytes(int B, int H, int Hkv, int L, int S, int D, int window, int sinks,

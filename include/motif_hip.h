@@ -499,6 +499,23 @@ int motif_chord_window_fwd(
     void *workspace, size_t workspace_bytes, int dtype, void *stream);
 
 /*
+ * motif_chord_decode_step under a window: the same arguments, conditions and arithmetic, with
+ * motif_chord_window_fwd's keys (the rows that q and the new keys see are the same as there).
+ */
+size_t motif_chord_window_step_workspace_bytes(int B, int H, int Hkv, int L, int capacity, int window, int sinks);
+int motif_chord_window_step(
+    const void *proj, int64_t p_sb, int64_t p_st, int q_off, int k_off, int v_off,
+    const void *q_norm_weight, const void *k_norm_weight, float norm_eps,
+    void *k_cache, int64_t k_sb, int64_t k_sh, int64_t k_st,
+    void *v_cache, int64_t v_sb, int64_t v_sh, int64_t v_st,
+    int *length_dev, int capacity,
+    const float *alpha, const float *beta, const float *mu, const float *ssmax,
+    const float *log_table, int log_table_len,
+    void *out, int64_t o_sb, int64_t o_sh, int64_t o_st,
+    int B, int H, int Hkv, int L, int D, float scale, float eps,
+    int window, int sinks, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
  * Table of the bias's distances for motif_chord_window_fwd / _bwd: n = motif_chord_distances_len(..)
  * entries per head (3 * H * n floats, 8-byte aligned) in 64-bit arithmetic, with
  * x_d = |-d - mu_h| + eps: out[h][d] = {x_d^beta, x_d^beta log2 x_d} for d = 0 .. n - 1, then
