@@ -730,6 +730,7 @@ __global__ void __launch_bounds__(256) chord_decode_kernel(ChordArgs a, const fl
 // this kernel needs no bias table.  The next step's K / V loads are issued before the
 // current step's arithmetic.
 constexpr int kMfmaRows = 16;
+constexpr int kDecodeWaves = 16;  // of an unsplit windowed call
 constexpr int kVRow = 72;  // LDS V row stride (bf16): 144 bytes, conflict-free gathers
 
 // The whole decode step of a Chord layer in one launch (motif_chord_decode_step): q, k
@@ -786,8 +787,9 @@ __device__ __forceinline__ void rms_norm16(uint4 &u0, uint4 &u1, const uint4 w0,
 }
 
 // WIN: under a window (a.window, a.sinks): the splits share the 32-key tiles of first tokens and windows.
-template <bool STEP, bool WIN>
-__global__ void __launch_bounds__(256) chord_decode_mfma_kernel(ChordArgs a, StepArgs sa) {
+// NW: waves of a workgroup (a windowed call that is not split takes kDecodeWaves).
+template <bool STEP, bool WIN, int NW = 4>
+__global__ void __launch_bounds__(64 * NW) chord_decode_mfma_kernel(ChordArgs a, StepArgs sa) {
   // wave index in an SGPR: the key loop below is then scalar (MFMAs must not sit
   // under a lane-mask branch, as they ignore EXEC)
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -843,11 +845,11 @@ __global__ void __launch_bounds__(256) chord_decode_mfma_kernel(ChordArgs a, Ste
   const buf_t kbuf = make_buf(kp, k_hi > 0 ? static_cast<uint32_t>(((k_hi - 1) * a.k_st + kD) * 2) : 0u);
   const buf_t vbuf = make_buf(vp, k_hi > 0 ? static_cast<uint32_t>(((k_hi - 1) * a.v_st + kD) * 2) : 0u);
 
-  __shared__ __attribute__((aligned(16))) bf16_t sV[4][32 * kVRow];
+  __shared__ __attribute__((aligned(16))) bf16_t sV[NW][32 * kVRow];
   // per wave: the step's 32 K rows (128 bytes each, 16-byte chunks XOR-swizzled by row),
   // filled by buffer-to-LDS loads of whole rows, 8 rows per instruction (the operand
   // layout would read 16 rows x 64 bytes per instruction: half of each line)
-  __shared__ __attribute__((aligned(16))) bf16_t sKs[4][32 * 64];
+  __shared__ __attribute__((aligned(16))) bf16_t sKs[NW][32 * 64];
   bf16_t *myV = sV[w], *myK = sKs[w];
 
   struct Stage {
@@ -936,7 +938,7 @@ __global__ void __launch_bounds__(256) chord_decode_mfma_kernel(ChordArgs a, Ste
 
   // position of the loop: the step's first key, or (WIN) its tile
   int at = WIN ? split * x_per + w : k_lo + w * 32;
-  const int at_end = WIN ? min(walk.count, (split + 1) * x_per) : k_hi, at_step = WIN ? 4 : 4 * 32;
+  const int at_end = WIN ? min(walk.count, (split + 1) * x_per) : k_hi, at_step = WIN ? NW : 4 * 32;
   auto load_at = [&](int x, Stage &st) {
     if constexpr (WIN) load_tile(x, st);
     else load_stage(x, st);
@@ -1030,27 +1032,31 @@ __global__ void __launch_bounds__(256) chord_decode_mfma_kernel(ChordArgs a, Ste
   lsum += __shfl_xor(lsum, 16, 64);
   lsum += __shfl_xor(lsum, 32, 64);
 
-  // merge the 4 waves through LDS (reusing the V tiles' space is not needed: small)
-  __shared__ float sm[4][kMfmaRows], sl[4][kMfmaRows], so[4][kMfmaRows][kD + 1];
+  // merge the waves through LDS (more than 4: over the V tiles, which the LDS would not hold beside them)
+  __shared__ float sm[NW][kMfmaRows], sl[NW][kMfmaRows];
+  __shared__ float so4[NW == 4 ? 4 : 1][kMfmaRows][kD + 1];
+  static_assert(NW == 4 || sizeof(float) * kMfmaRows * (kD + 1) <= sizeof(sV[0]), "a wave's output fits its V tile");
+  if constexpr (NW != 4) __syncthreads();  // (every wave's V tile is read)
+  auto so = [&](int ww) { return NW == 4 ? so4[ww] : reinterpret_cast<float (*)[kD + 1]>(sV[ww]); };
   if (g == 0) { sm[w][c16] = m; sl[w][c16] = lsum; }
 #pragma unroll
   for (int ft = 0; ft < 4; ++ft)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) so[w][c16][16 * ft + 4 * g + i] = o[ft][i];
+    for (int i = 0; i < 4; ++i) so(w)[c16][16 * ft + 4 * g + i] = o[ft][i];
   __syncthreads();
-  for (int e = tid; e < kMfmaRows * kD; e += 256) {
+  for (int e = tid; e < kMfmaRows * kD; e += 64 * NW) {
     const int r = e / kD, d = e % kD;
     const int grr = qc * kMfmaRows + r;
     if (grr >= total_rows) continue;
     float M = -INFINITY;
 #pragma unroll
-    for (int ww = 0; ww < 4; ++ww) M = fmaxf(M, sm[ww][r]);
+    for (int ww = 0; ww < NW; ++ww) M = fmaxf(M, sm[ww][r]);
     const float Mu = M == -INFINITY ? 0.f : M;
     float ov = 0.f, Ls = 0.f;
 #pragma unroll
-    for (int ww = 0; ww < 4; ++ww) {
+    for (int ww = 0; ww < NW; ++ww) {
       const float f = fast_exp2(sm[ww][r] - Mu);
-      ov += so[ww][r][d] * f;
+      ov += so(ww)[r][d] * f;
       Ls += sl[ww][r] * f;
     }
     if (!a.part) {
@@ -1188,8 +1194,20 @@ static int decode_splits(int B, int Hkv, int S) {
   return std::max(1, std::min(want, 32));
 }
 
-// Splits of a windowed decode: about three workgroups per CU, and a tile for each of their waves.
+// Shares of a windowed decode's tiles, 1: one workgroup of 16 waves per kv head and nothing to merge.
+// Measured, us, 4 query heads per kv head, one token, unsplit / 4 / 8 shares (and their merge): 3 kv heads
+// (one sequence), a window of 1024 keys 9.8 / 9.7 / 10.7, 2048 14.6 / 13.0 / 12.1, 4096 25.3 / 19.5 / 15.9; 48
+// 2048 16.0 / 15.3 / 16.0, 4096 26.5 / 21.6 / 20.0; 96 2048 19.3 / 17.5 / 20.9, 4096 32.7 / 25.3 / 28.5; 192
+// (64 sequences) 1024 13.7 / 17.7 / 26.5, 4096 37.4 / 41.3 / 48.0.
 int chord_window_splits(int B, int Hkv, int L, int S, int window, int sinks) {
+  const int64_t keys = std::min<int64_t>(S, std::min<int64_t>(window, S) + L + std::min(sinks, S) + 2 * 32);
+  const int64_t heads = int64_t(B) * Hkv, tiles = (keys + 31) / 32;
+  if (tiles <= 48 || heads >= 160) return 1;
+  return heads >= 80 ? 4 : 8;
+}
+// The one-launch step's: its four-wave workgroups merge themselves (about three of them per CU, a tile for
+// each of their waves).
+static int window_step_splits(int B, int Hkv, int L, int S, int window, int sinks) {
   const int64_t keys = std::min<int64_t>(S, std::min<int64_t>(window, S) + L + std::min(sinks, S) + 2 * 32);
   const int64_t base = std::max<int64_t>(1, int64_t(B) * Hkv), tiles = (keys + 31) / 32;
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(3 * device_cu_count() + base - 1) / base, (tiles + 3) / 4, 32})));
@@ -1200,9 +1218,10 @@ bool chord_window_decode_serves(int H, int Hkv, int L, int D, int dtype) {
 }
 
 int launch_chord_window_decode(const ChordArgs &a, hipStream_t s) {
-  chord_decode_mfma_kernel<false, true><<<dim3(a.splits, a.Hkv, a.B), dim3(256), 0, s>>>(a, StepArgs{});
-  if (const int rc = check_launch("chord_decode_mfma_kernel"); rc || !a.part) return rc;
-  return launch_chord_merge(a, MOTIF_BF16, kD, s);
+  if (a.part) chord_decode_mfma_kernel<false, true><<<dim3(a.splits, a.Hkv, a.B), dim3(256), 0, s>>>(a, StepArgs{});
+  else chord_decode_mfma_kernel<false, true, kDecodeWaves><<<dim3(1, a.Hkv, a.B), dim3(64 * kDecodeWaves), 0, s>>>(a, StepArgs{});
+  if (const int rc = check_launch("chord_decode_mfma_kernel")) return rc;
+  return a.part ? launch_chord_merge(a, MOTIF_BF16, kD, s) : launch_chord_advance(a, s);
 }
 
 template <typename T, int D>
@@ -1567,7 +1586,7 @@ static int chord_decode_step_run(
         reinterpret_cast<uintptr_t>(k_norm_weight) | reinterpret_cast<uintptr_t>(k_cache) |
         reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(out)) & 15) != 0)
     return set_error(MOTIF_ERR_UNSUPPORTED, "chord_decode_step: rows must be 16-byte aligned");
-  const int splits = window != kNoWindow ? chord_window_splits(B, Hkv, L, capacity, window, sinks)
+  const int splits = window != kNoWindow ? window_step_splits(B, Hkv, L, capacity, window, sinks)
                                          : decode_splits(B, Hkv, capacity);
   const size_t need = step_ws_bytes(B, H, Hkv, L, splits);
   if (!workspace || workspace_bytes < need)
@@ -1622,7 +1641,7 @@ extern "C" int motif_chord_decode_step(
 
 extern "C" size_t motif_chord_window_step_workspace_bytes(int B, int H, int Hkv, int L, int capacity, int window, int sinks) {
   if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || L <= 0 || capacity < L || window < 1 || sinks < 0) return 0;
-  return motif::step_ws_bytes(B, H, Hkv, L, motif::chord_window_splits(B, Hkv, L, capacity, window, sinks));
+  return motif::step_ws_bytes(B, H, Hkv, L, motif::window_step_splits(B, Hkv, L, capacity, window, sinks));
 }
 
 extern "C" int motif_chord_window_step(

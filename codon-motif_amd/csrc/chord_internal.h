@@ -115,19 +115,20 @@ int launch_chord_wide(const ChordArgs &a, int dtype, int D, hipStream_t s);
 int launch_chord_wide_window(const ChordArgs &a, int dtype, int D, hipStream_t s);
 int launch_chord_wide_kv4(const ChordArgs &a, const KV4Args &kv, int dtype, int D, hipStream_t s);
 
-// Few rows of bf16 at head dim 64 under a window ((H / Hkv) L <= 16), a.splits shares of the tiles:
-// partials and a merge where a.part is set (with the cursor always), else straight to out.
+// Few rows of bf16 at head dim 64 under a window ((H / Hkv) L <= 16): a.splits shares of the tiles, their
+// partials (a.part) and a merge, or unsplit straight to out; the cursor, if any, advances.
 bool chord_window_decode_serves(int H, int Hkv, int L, int D, int dtype);
 int chord_window_splits(int B, int Hkv, int L, int S, int window, int sinks);
 int launch_chord_window_decode(const ChordArgs &a, hipStream_t s);
 
-// Few rows over a 4-bit cache (chord_kv4.hip; (H / Hkv) L <= 16, bf16 or fp16, head dim 64), a.splits
-// key ranges: partials and a merge where a.part is set (with the cursor always), else straight to out.
+// The same over a 4-bit cache (chord_kv4.hip; bf16 or fp16).
 bool chord_kv4_serves(int H, int Hkv, int L, int D, int dtype);
 int chord_kv4_splits(int B, int Hkv, int L, int S, int window, int sinks);
 int launch_chord_kv4(const ChordArgs &a, const KV4Args &kv, int dtype, hipStream_t s);
 // The merge of split partials (and the cursor's advance).
 int launch_chord_merge(const ChordArgs &a, int dtype, int D, hipStream_t s);
+// The cursor's advance alone (nothing without a cursor).
+int launch_chord_advance(const ChordArgs &a, hipStream_t s);
 int chord_cu_count();
 
 // Chord decode over a device cursor, shared by the C-ABI entry points that take

@@ -61,8 +61,8 @@ __device__ __forceinline__ float sum_g(float x) {
   return x + __shfl_xor(x, 16, 64);
 }
 
-template <typename T, int U>
-__global__ void __launch_bounds__(256) chord_kv4_kernel(ChordArgs a, KV4Args kv) {
+template <typename T, int U, int NW>  // NW: waves of a workgroup
+__global__ void __launch_bounds__(64 * NW) chord_kv4_kernel(ChordArgs a, KV4Args kv) {
   constexpr int RC = 16 / U, TPL = 4 / U, NK = 4 * TPL;  // rows, tiles and keys of a lane
   constexpr bool kBf = sizeof(T) == 2 && __is_same(T, bf16_t);
   constexpr int kHalves = kBf ? 1 : 2;  // fp16 weights as two bf16 (17 bits; fp16's range would not hold p scale)
@@ -119,8 +119,8 @@ __global__ void __launch_bounds__(256) chord_kv4_kernel(ChordArgs a, KV4Args kv)
 
   // per wave: codes of 64 keys and values (2 KB each) and their pairs (512 bytes each, written as 1 KB)
   constexpr int kWave = 2 * 2048 + 2 * 1024;
-  constexpr int kMerge = 4 * 16 * (kD + 1) * 4 + 4 * 16 * 4 * 4;
-  __shared__ __attribute__((aligned(16))) uint8_t smem[4 * kWave > kMerge ? 4 * kWave : kMerge];
+  constexpr int kMerge = NW * 16 * (kD + 1) * 4 + NW * 16 * 4 * 4;
+  __shared__ __attribute__((aligned(16))) uint8_t smem[NW * kWave > kMerge ? NW * kWave : kMerge];
   uint8_t *sk = smem + w * kWave, *sv = sk + 2048, *skp = sv + 2048, *svp = skp + 1024;
   const uint8_t *kc = kv.kc + b * kv.kc_sb + kvh * kv.kc_sh, *vc = kv.vc + b * kv.vc_sb + kvh * kv.vc_sh;
   const uint32_t *kp = kv.kp + b * kv.kp_sb + kvh * kv.kp_sh, *vp = kv.vp + b * kv.vp_sb + kvh * kv.vp_sh;
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(256) chord_kv4_kernel(ChordArgs a, KV4Args kv)
 
   int x = split * per + w;
   if (x < x_end) stage(x);
-  for (; x < x_end; x += 4) {
+  for (; x < x_end; x += NW) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this step's rows are in LDS
     uint32_t kw[4][2];
     i32x2 vw[4];
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(256) chord_kv4_kernel(ChordArgs a, KV4Args kv)
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and out of it again
     const int n0 = walk.start(x);
-    if (x + 4 < x_end) stage(x + 4);
+    if (x + NW < x_end) stage(x + NW);
     __builtin_amdgcn_sched_barrier(0);
 
     f32x4 acc[TPL][2];
@@ -303,23 +303,23 @@ __global__ void __launch_bounds__(256) chord_kv4_kernel(ChordArgs a, KV4Args kv)
   ob[0] = sum_g(ob[0]);
   ob[1] = sum_g(ob[1]);
   __syncthreads();  // every wave's staged rows are read
-  float *so = reinterpret_cast<float *>(smem), *sm = so + 4 * 16 * (kD + 1);  // [wave][column][feature], [wave][column][m, l, ..]
+  float *so = reinterpret_cast<float *>(smem), *sm = so + NW * 16 * (kD + 1);  // [wave][column][feature], [wave][column][m, l, ..]
   if (g == 0) *reinterpret_cast<f32x4 *>(sm + 4 * (16 * w + c16)) = f32x4{m, l, ob[0], ob[1]};
 #pragma unroll
   for (int ft = 0; ft < 4; ++ft)
 #pragma unroll
     for (int i = 0; i < 4; ++i) so[(16 * w + c16) * (kD + 1) + 16 * ft + 4 * g + i] = o[ft][i];
   __syncthreads();
-  for (int e = tid; e < RC * kD; e += 256) {
+  for (int e = tid; e < RC * kD; e += 64 * NW) {
     const int rr = e / kD, d = e % kD;
     if (rr >= rows) continue;
     float M = -INFINITY;
 #pragma unroll
-    for (int c = 0; c < 4 * U; ++c) M = fmaxf(M, sm[4 * (16 * (c / U) + (c % U) * RC + rr)]);
+    for (int c = 0; c < NW * U; ++c) M = fmaxf(M, sm[4 * (16 * (c / U) + (c % U) * RC + rr)]);
     const float Mu = M == -INFINITY ? 0.f : M;
     float ov = 0.f, Ls = 0.f;
 #pragma unroll
-    for (int c = 0; c < 4 * U; ++c) {
+    for (int c = 0; c < NW * U; ++c) {
       const int col = 16 * (c / U) + (c % U) * RC + rr;
       const float f = fast_exp2(sm[4 * col] - Mu);
       ov = fmaf(so[col * (kD + 1) + d] + sm[4 * col + 2 + d / 32], f, ov);
@@ -336,13 +336,22 @@ __global__ void __launch_bounds__(256) chord_kv4_kernel(ChordArgs a, KV4Args kv)
   }
 }
 
+// waves of an unsplit call: what the registers let a CU hold
+constexpr int waves_of(int U) { return U == 1 ? 8 : 12; }
+
+template <typename T, int U>
+int launch_u(const ChordArgs &a, const KV4Args &kv, hipStream_t s) {
+  const dim3 grid(a.splits, a.Hkv, a.B);
+  if (a.part) chord_kv4_kernel<T, U, 4><<<grid, dim3(256), 0, s>>>(a, kv);
+  else chord_kv4_kernel<T, U, waves_of(U)><<<grid, dim3(64 * waves_of(U)), 0, s>>>(a, kv);
+  return check_launch("chord_kv4_kernel");
+}
+
 template <typename T>
 int launch_t(const ChordArgs &a, const KV4Args &kv, int rows, hipStream_t s) {
-  const dim3 grid(a.splits, a.Hkv, a.B), block(256);
-  if (rows <= 4) chord_kv4_kernel<T, 4><<<grid, block, 0, s>>>(a, kv);
-  else if (rows <= 8) chord_kv4_kernel<T, 2><<<grid, block, 0, s>>>(a, kv);
-  else chord_kv4_kernel<T, 1><<<grid, block, 0, s>>>(a, kv);
-  return check_launch("chord_kv4_kernel");
+  if (rows <= 4) return launch_u<T, 4>(a, kv, s);
+  if (rows <= 8) return launch_u<T, 2>(a, kv, s);
+  return launch_u<T, 1>(a, kv, s);
 }
 
 }  // namespace
@@ -351,18 +360,25 @@ bool chord_kv4_serves(int H, int Hkv, int L, int D, int dtype) {
   return D == kD && (dtype == MOTIF_BF16 || dtype == MOTIF_F16) && (H / Hkv) * static_cast<int64_t>(L) <= 16;
 }
 
+// Key ranges of a call, 1: one workgroup of up to 12 waves per kv head and nothing to merge.  Measured, us,
+// 4 query heads per kv head, one token, unsplit / 4 / 8 ranges (and their merge): 3 kv heads (one sequence)
+// over 1000 keys 9.4 / 8.7 / 8.9, 2000 12.2 / 10.2 / 10.6, 4097 19.4 / 13.7 / 12.8, 8000 31.5 / 17.6 / 14.3;
+// 48 (16 sequences) 4097 19.9 / 14.7 / 16.0, 8000 31.7 / 19.0 / 18.8; 96 4097 20.1 / 17.8 / 18.5, 8000
+// 32.6 / 24.3 / 23.1; 192 (64 sequences) 2000 13.4 / 15.3 / 21.7, 4097 21.4 / 22.2 / 29.1, 8000 34.4 /
+// 30.8 / 38.7.  (Up to 1280 keys a second launch would cost the host more than it saves the device.)
 int chord_kv4_splits(int B, int Hkv, int L, int S, int window, int sinks) {
   const int64_t keys = std::min<int64_t>(S, std::min<int64_t>(window, S) + L + std::min(sinks, S) + 2 * kStep);
-  const int steps = static_cast<int>((keys + kStep - 1) / kStep);
-  // about four workgroups per CU, and a step for each of their waves
-  const int want = static_cast<int>((4 * static_cast<int64_t>(chord_cu_count()) + int64_t(B) * Hkv - 1) / (int64_t(B) * Hkv));
-  return std::max(1, std::min({want, (steps + 3) / 4, 32}));
+  const int64_t steps = (keys + kStep - 1) / kStep, heads = int64_t(B) * Hkv;
+  if (steps <= 20) return 1;
+  if (heads >= 160) return steps > 96 ? 4 : 1;
+  return steps > 96 || (heads < 32 && steps > 48) ? 8 : 4;
 }
 
 int launch_chord_kv4(const ChordArgs &a, const KV4Args &kv, int dtype, hipStream_t s) {
   const int rows = a.L * (a.H / a.Hkv);
   const int rc = dtype == MOTIF_BF16 ? launch_t<bf16_t>(a, kv, rows, s) : launch_t<f16_t>(a, kv, rows, s);
-  return rc || !a.part ? rc : launch_chord_merge(a, dtype, kD, s);
+  if (rc) return rc;
+  return a.part ? launch_chord_merge(a, dtype, kD, s) : launch_chord_advance(a, s);
 }
 
 }  // namespace motif

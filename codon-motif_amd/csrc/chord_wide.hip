@@ -413,14 +413,13 @@ int launch_wide(const ChordArgs &a, const KV4Args &kv, hipStream_t s) {
   constexpr int smem = (2 * 64 * NW + NW * 16 * 64) * static_cast<int>(sizeof(float));
   const dim3 grid(a.H, (a.L + 31) / 32, a.B), block(64 * NW);
   chord_wide_kernel<T, D, NW, MODE, EU><<<grid, block, smem, s>>>(a, kv);
-  if (const int rc = check_launch("chord_wide_kernel"); rc || MODE == kCausal || !a.len_dev) return rc;
-  chord_advance_kernel<<<dim3(1), dim3(1), 0, s>>>(a.len_dev, a.L, a.S);
-  return check_launch("chord_advance_kernel");
+  const int rc = check_launch("chord_wide_kernel");
+  return rc || MODE == kCausal ? rc : launch_chord_advance(a, s);
 }
 
 // A window's blocks are short and many: where they pass one per CU, four waves each let two blocks
 // share a CU (2 x 517 fp32 queries over 1023 keys, 408 blocks, windows of 128 / 259 / 1023: eight waves
-// 37 / 49 / 74 us, four KFOUR); where they do not, eight waves shorten the chain.
+// 37 / 49 / 74 us, four 27 / 37 / 67); where they do not, eight waves shorten the chain.
 template <typename T, int D, int MODE>
 int launch_wide_n(const ChordArgs &a, const KV4Args &kv, hipStream_t s) {
   if constexpr (MODE != kCausal) {
@@ -458,6 +457,11 @@ bool chord_wide_serves(const ChordArgs &a) {
          int64_t(a.q_start) + a.L < (int64_t(1) << 30);
 }
 
+int launch_chord_advance(const ChordArgs &a, hipStream_t s) {
+  if (!a.len_dev) return MOTIF_OK;
+  chord_advance_kernel<<<dim3(1), dim3(1), 0, s>>>(a.len_dev, a.L, a.S);
+  return check_launch("chord_advance_kernel");
+}
 int launch_chord_wide(const ChordArgs &a, int dtype, int D, hipStream_t s) {
   return launch_wide_m<kCausal>(a, KV4Args{}, dtype, D, s);
 }

@@ -424,7 +424,7 @@ extern "C" int motif_chord_window_fwd(
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (chord_window_decode_serves(H, Hkv, L, D, dtype) && !lse) {
     a.splits = chord_window_splits(B, Hkv, L, S, window, sinks);
-    if (a.splits > 1 || length_dev) {  // (the merge advances the cursor)
+    if (a.splits > 1) {
       const size_t need = motif_chord_window_workspace_bytes(B, H, Hkv, L, S, D, window, sinks, dtype);
       if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 3))
         return set_error(MOTIF_ERR_INVALID, "chord_window_fwd: workspace too small (need " + std::to_string(need) + " bytes) or not aligned");
@@ -461,7 +461,8 @@ extern "C" size_t motif_chord_window_workspace_bytes(int B, int H, int Hkv, int 
   if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || L <= 0 || S <= 0 || window < 1 || sinks < 0 ||
       !chord_window_decode_serves(H, Hkv, L, D, dtype))
     return 0;
-  return static_cast<size_t>(B) * H * L * chord_window_splits(B, Hkv, L, S, window, sinks) * (D + 2) * sizeof(float);
+  const int sp = chord_window_splits(B, Hkv, L, S, window, sinks);
+  return sp > 1 ? static_cast<size_t>(B) * H * L * sp * (D + 2) * sizeof(float) : 0;
 }
 
 extern "C" size_t motif_chord_kv4_workspace_bytes(int B, int H, int Hkv, int L, int S, int D, int window, int sinks,
@@ -469,7 +470,8 @@ extern "C" size_t motif_chord_kv4_workspace_bytes(int B, int H, int Hkv, int L, 
   if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || L <= 0 || S <= 0 || window < 1 || sinks < 0 ||
       !chord_kv4_serves(H, Hkv, L, D, dtype))
     return 0;
-  return static_cast<size_t>(B) * H * L * chord_kv4_splits(B, Hkv, L, S, window, sinks) * (D + 2) * sizeof(float);
+  const int sp = chord_kv4_splits(B, Hkv, L, S, window, sinks);
+  return sp > 1 ? static_cast<size_t>(B) * H * L * sp * (D + 2) * sizeof(float) : 0;
 }
 
 extern "C" int motif_chord_kv4_fwd(
@@ -494,7 +496,7 @@ extern "C" int motif_chord_kv4_fwd(
   // more rows, fp32 and other head dims: the fp32-accumulating flash kernel, which expands the codes
   if (!chord_kv4_serves(H, Hkv, L, D, dtype)) return launch_chord_wide_kv4(a, kv, dtype, D, st);
   a.splits = chord_kv4_splits(B, Hkv, L, S, window, sinks);
-  if (a.splits > 1 || length_dev) {  // (the merge advances the cursor)
+  if (a.splits > 1) {
     const size_t need = motif_chord_kv4_workspace_bytes(B, H, Hkv, L, S, D, window, sinks, dtype);
     if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 3))
       return set_error(MOTIF_ERR_INVALID, "chord_kv4_fwd: workspace too small (need " + std::to_string(need) + " bytes) or not aligned");
