@@ -24,13 +24,15 @@ import torch
 import torch.nn as nn
 
 from motif.block.attention.base import AttentionOutput, BasicAttention
-from motif.model.cache import KVLayerCache, StaticKVLayerCache, expand_kv_heads
+from motif.model.cache import KV4LayerCache, KVLayerCache, StaticKVLayerCache, expand_kv_heads
 from motif.ops import RMSNorm, apply_chord_attention, apply_chord_attention_varlen
 from motif.ops.packed import PackedSeqs
 from motif.ops import _lib
 from motif.ops.autograd_path import wants_grad
-from motif.ops.chord_attention import (HEAD_DIMS, chord_decode_cursor, chord_decode_step, chord_decode_step_serves,
-                                       chord_decode_step_workspace, chord_decode_workspace, serves_head_dim)
+from motif.ops.chord_attention import (HEAD_DIMS, check_window, chord_decode_cursor, chord_decode_step,
+                                       chord_decode_step_serves, chord_decode_step_workspace, chord_decode_workspace,
+                                       chord_window_workspace, serves_head_dim)
+from motif.ops.kv4 import chord_decode_kv4_cursor, chord_decode_kv4_workspace, kv4_append
 from motif.ops.epilogue import mul_sigmoid, usable
 from motif.ops.linear_rows import cat_weights, linear_rows, project, rows_eligible
 
@@ -81,8 +83,10 @@ def _f32(t: torch.Tensor) -> torch.Tensor:
 class ChordAttention(BasicAttention):
     '''Softmax attention with the per-head gated geometric-decay (GGD) bias.'''
 
-    def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: Optional[int] = None, **kwargs):
+    def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: Optional[int] = None,
+                 window: Optional[int] = None, sinks: int = 0, **kwargs):
         super().__init__(hidden_size=hidden_size, num_heads=num_heads, num_kv_heads=num_kv_heads)
+        self.window, self.sinks = check_window(window, sinks)
         self.q_proj = nn.Linear(hidden_size, hidden_size, bias=False)
         self.k_proj = nn.Linear(hidden_size, self.kv_dim, bias=False)
         self.v_proj = nn.Linear(hidden_size, self.kv_dim, bias=False)
@@ -153,7 +157,7 @@ class ChordAttention(BasicAttention):
             return False
         if self.q_norm.weight is None or self.k_norm.weight is None or self.q_norm.eps != self.k_norm.eps:
             return False
-        if cache is not None and (cache.wide or type(cache) not in (KVLayerCache, StaticKVLayerCache)):
+        if cache is not None and (cache.wide or type(cache) not in (KVLayerCache, StaticKVLayerCache, KV4LayerCache)):
             return False
         return not wants_grad(x, self)
 
@@ -163,7 +167,7 @@ class ChordAttention(BasicAttention):
         return (isinstance(cache, StaticKVLayerCache) and cache.capacity > 0 and not cache.wide
                 and self.head_dim in HEAD_DIMS
                 and q_start == cache.length and cache.length + L <= cache.capacity
-                and cache.k.dtype == x.dtype and self.num_kv_queries * L <= _DECODE_ROWS
+                and cache.row_dtype == x.dtype and self.num_kv_queries * L <= _DECODE_ROWS
                 and self._prep_fusable(x, cache))
 
     # ------------------------------------------------------------------ inputs
@@ -193,10 +197,12 @@ class ChordAttention(BasicAttention):
             proj = self._fused_proj(hidden_states)
             hs, kd = self.hidden_size, self.kv_dim
             q = torch.empty(B, self.num_heads, L, self.head_dim, dtype=proj.dtype, device=proj.device)
-            if cache is None:
+            if cache is None or isinstance(cache, KV4LayerCache):
                 k = torch.empty(B, self.num_kv_heads, L, self.head_dim, dtype=proj.dtype, device=proj.device)
                 v = torch.empty_like(k)
                 self._prep(proj, q, k, v, None, 0, L)
+                if cache is not None:
+                    k, v = cache.update(k, v)
             else:
                 ks, vs, first = cache.append_slots(L, q.new_empty(B, self.num_kv_heads, 0, self.head_dim))
                 length_dev = cache.length_dev if isinstance(cache, StaticKVLayerCache) else None
@@ -312,7 +318,7 @@ class ChordAttention(BasicAttention):
             out = apply_chord_attention(q, k, v, alpha, beta, mu, ssmax,
                                         log_n if log_n.dim() == 2 else log_n.expand(B, L),
                                         q_start=int(q_start), softmax_scale=self.head_dim ** -0.5, eps=GGD_EPS,
-                                        out=self._heads_out(q))
+                                        out=self._heads_out(q), window=self.window, sinks=self.sinks)
             return self._merge_heads(out), g, cache
         return self._materialised(q, k, v, g, q_start, log_n, attention_mask, output_attentions, cache)
 
@@ -347,32 +353,50 @@ class ChordAttention(BasicAttention):
         '''The cursor step from the projected tokens proj [B, L, q|k|v|g]: (merged
         attention output [B, L, hidden], gate pre-activation [B, L, hidden]).'''
         B, L = proj.shape[0], proj.shape[1]
-        ks, vs = cache._slab
         if cache.__dict__.get('log_table') is None or cache.log_table.numel() < cache.capacity:
             cache.log_table = LogPositions.get(cache.capacity, proj.device)  # held: a graph keeps its address
         alpha, beta, mu, ssmax = self.ggd_params()
-        if FUSED_STEP and chord_decode_step_serves(proj, self.num_heads, self.num_kv_heads, self.head_dim):
+        if isinstance(cache, KV4LayerCache):
+            out = self._kv4_step(proj, cache, alpha, beta, mu, ssmax)
+        elif FUSED_STEP and chord_decode_step_serves(proj, self.num_heads, self.num_kv_heads, self.head_dim):
             # norms, append, attention, merge and cursor advance in one launch
-            if cache.step_workspace is None:
-                cache.step_workspace = chord_decode_step_workspace(B, self.num_heads, self.num_kv_heads, L,
-                                                                   cache.capacity, proj.device)
+            work = cache.workspace(('step', L, self.window, self.sinks), lambda: chord_decode_step_workspace(
+                B, self.num_heads, self.num_kv_heads, L, cache.capacity, proj.device, self.window, self.sinks))
+            ks, vs = cache._slab
             dt = proj.dtype
             hs, kd = self.hidden_size, self.kv_dim
             out = chord_decode_step(proj, (0, hs, hs + kd), self.q_norm.weight.to(dt).contiguous(),
                                     self.k_norm.weight.to(dt).contiguous(), self.q_norm.eps, ks, vs, cache.length_dev,
                                     alpha, beta, mu, ssmax, cache.log_table, self.num_heads, self.head_dim ** -0.5,
-                                    GGD_EPS, cache.step_workspace)
+                                    GGD_EPS, work, self.window, self.sinks)
         else:
+            ks, vs = cache._slab
             q = torch.empty(B, self.num_heads, L, self.head_dim, dtype=proj.dtype, device=proj.device)
             self._prep(proj, q, ks, vs, cache.length_dev, -1, cache.capacity)
-            if cache.decode_workspace is None:
-                cache.decode_workspace = chord_decode_workspace(B, self.num_heads, self.num_kv_heads, L, cache.capacity,
-                                                                self.head_dim, proj.dtype, proj.device)
+            sizes = (B, self.num_heads, self.num_kv_heads, L, cache.capacity, self.head_dim, proj.dtype, proj.device)
+            work = cache.workspace(('decode', L, self.window, self.sinks), lambda: chord_decode_workspace(
+                *sizes) if self.window is None else chord_window_workspace(*sizes, self.window, self.sinks))
             out = chord_decode_cursor(q, ks, vs, cache.length_dev, alpha, beta, mu, ssmax, cache.log_table,
-                                      self.head_dim ** -0.5, GGD_EPS, workspace=cache.decode_workspace)
+                                      self.head_dim ** -0.5, GGD_EPS, workspace=work,
+                                      window=self.window, sinks=self.sinks)
         cache.length += L
         cache.cursor_steps = getattr(cache, 'cursor_steps', 0) + 1
         return self._merge_heads(out), proj[..., self.hidden_size + 2 * self.kv_dim:]
+
+    def _kv4_step(self, proj, cache: KV4LayerCache, alpha, beta, mu, ssmax):
+        '''The attention of a cursor step over a 4-bit cache: norms, the rows into the cache at
+        the device cursor, attention and the cursor's advance.'''
+        B, L = proj.shape[0], proj.shape[1]
+        q = torch.empty(B, self.num_heads, L, self.head_dim, dtype=proj.dtype, device=proj.device)
+        k = torch.empty(B, self.num_kv_heads, L, self.head_dim, dtype=proj.dtype, device=proj.device)
+        v = torch.empty_like(k)
+        self._prep(proj, q, k, v, None, 0, L)
+        kv4_append(cache.slab, k, v, cache.length_dev)
+        work = cache.workspace(('kv4', L, self.window, self.sinks), lambda: chord_decode_kv4_workspace(
+            B, self.num_heads, self.num_kv_heads, L, cache.capacity, self.head_dim, proj.dtype, proj.device, self.window,
+            self.sinks))
+        return chord_decode_kv4_cursor(q, cache.slab, cache.length_dev, alpha, beta, mu, ssmax, cache.log_table,
+                                       self.head_dim ** -0.5, GGD_EPS, self.window, self.sinks, work)
 
     def forward_varlen(self, hidden_states: torch.Tensor, cu_seqlens) -> AttentionOutput:
         '''Packed sequences (B == 1; new): each sequence attends causally within itself
@@ -389,7 +413,8 @@ class ChordAttention(BasicAttention):
         log_n = table[ps.positions()][None]
         alpha, beta, mu, ssmax = self.ggd_params()
         out = apply_chord_attention_varlen(q, k, v, alpha, beta, mu, ssmax, log_n, ps,
-                                           softmax_scale=self.head_dim ** -0.5, eps=GGD_EPS, out=self._heads_out(q))
+                                           softmax_scale=self.head_dim ** -0.5, eps=GGD_EPS, out=self._heads_out(q),
+                                           window=self.window, sinks=self.sinks)
         return AttentionOutput(output=self._gated_output(self._merge_heads(out), g), payload={'k': k, 'v': v})
 
     def _materialised(self, q, k, v, g, q_start, log_n, attention_mask, output_attentions, cache):
@@ -412,7 +437,10 @@ class ChordAttention(BasicAttention):
         ln = log_n.view(1, 1, L, 1) if log_n.dim() == 1 else log_n.view(B, 1, L, 1)
         logits = (scores.to(fdt) + bias[None]) * (ssmax.view(1, H, 1, 1).to(fdt) * ln.to(fdt))
         logits = logits.clamp_min(torch.finfo(fdt).min / 4)
-        logits = logits.masked_fill(k_pos[None, :] > q_pos[:, None], float('-inf'))
+        hidden = k_pos[None, :] > q_pos[:, None]
+        if self.window is not None:
+            hidden = hidden | ((k_pos[None, :] <= q_pos[:, None] - self.window) & (k_pos[None, :] >= self.sinks))
+        logits = logits.masked_fill(hidden, float('-inf'))
         if attention_mask is not None:
             if attention_mask.dtype == torch.bool:
                 keep = attention_mask

@@ -36,7 +36,7 @@ class Decoder(nn.Module):
         self.attn_norm = RMSNorm(config.model_dim)
         if self.attn_type == 'chord':
             self.attn = ChordAttention(hidden_size=config.model_dim, num_heads=config.num_heads,
-                                       num_kv_heads=config.num_kv_heads)
+                                       num_kv_heads=config.num_kv_heads, window=config.window, sinks=config.sinks)
         else:
             self.attn = GatedDeltaAttention(hidden_size=config.model_dim, num_heads=config.num_heads,
                                             head_k_dim=config.head_k_dim, expand_v=2.0, chunk_size=64,

@@ -6,7 +6,7 @@ KVLayerCache, FunctionalKVLayerCache, GatedDeltaAttentionLayerCache,
 AttnResCache, DecoderBlockCache, ModelCache and build_cache.
 
 Design.  A key / value cache is a slab `[B, heads, capacity, D]` plus a cursor
-(the number of valid positions).  The three key / value classes differ only in
+(the number of valid positions).  The key / value classes differ only in
 how the slab gets room for new positions:
 
   * KVLayerCache            grows: the capacity doubles, in whole 256-position
@@ -17,7 +17,8 @@ how the slab gets room for new positions:
                             kept in a device int32 (`length_dev`), the value the
                             Chord decode kernels read and advance, so a decode
                             step captured once as a hipGraph can be replayed token
-                            after token without host involvement.
+                            after token without host involvement;
+  * KV4LayerCache           the same, its rows held in 4 bits (motif/ops/kv4.py).
 
 `append_slots(n)` hands the slab and the first free position to a writer (the
 fused Chord input kernel writes new keys / values straight into the cache);
@@ -36,6 +37,7 @@ from typing import Iterator, List, Optional, Sequence, Tuple
 import torch
 
 from motif.ops.epilogue import MAX_CHAIN, residual_fold
+from motif.ops.kv4 import KV4Slab, kv4_alloc, kv4_append, kv4_read
 
 PAGE = 256  # positions per allocation unit of a growing key / value slab
 
@@ -236,16 +238,32 @@ class StaticKVLayerCache(KVLayerCache):
     def __init__(self, num_heads: Optional[int] = None):
         super().__init__(num_heads)
         self.length_dev: Optional[torch.Tensor] = None
-        self.decode_workspace: Optional[torch.Tensor] = None
-        self.step_workspace: Optional[torch.Tensor] = None  # the fused decode step's (zeroed once)
+        self._workspaces: dict = {}
+
+    def workspace(self, key: tuple, make) -> Optional[torch.Tensor]:
+        '''The decode kernels' scratch for steps of this kind (`make()` on its first use): one
+        per key = (kind, tokens a step, ...), since a size is laid out for its own steps, and all
+        of them kept, since a captured step holds its address.'''
+        if key not in self._workspaces:
+            self._workspaces[key] = make()
+        return self._workspaces[key]
+
+    @property
+    def step_workspace(self) -> Optional[torch.Tensor]:
+        '''The one-launch decode step's scratch (zeroed once) used first, None before.'''
+        return next((w for key, w in self._workspaces.items() if key[0] == 'step'), None)
+
+    @property
+    def row_dtype(self) -> Optional[torch.dtype]:
+        '''The dtype of the rows the layer reads and writes.'''
+        return None if self._slab is None else self._slab[0].dtype
 
     def allocate(self, batch, kv_heads, capacity, head_dim, device, dtype):
         shape = (batch, kv_heads, capacity, head_dim)
         self._slab = (torch.zeros(shape, device=device, dtype=dtype), torch.zeros(shape, device=device, dtype=dtype))
         self.length = 0
         self.length_dev = torch.zeros(1, dtype=torch.int32, device=device)
-        self.decode_workspace = None
-        self.step_workspace = None
+        self._workspaces = {}
         return self
 
     def _room(self, like, n):
@@ -285,6 +303,83 @@ class StaticKVLayerCache(KVLayerCache):
         if self._slab is not None:
             self._slab = tuple(t.to(device=device, dtype=dtype) for t in self._slab)
             self.length_dev = self.length_dev.to(device=device)
+            self._workspaces = {}
+        return self
+
+
+class KV4LayerCache(StaticKVLayerCache):
+    '''Fixed-capacity key / value cache in 4 bits (new): 40 bytes a row at head dim 64 where
+    bf16 takes 128.  `slab` is a motif.ops.kv4.KV4Slab; `k` / `v` are new tensors of the
+    values that the cached rows stand for, in the dtype given to `allocate`.
+
+    `update` writes the new rows in 4 bits and returns every cached position: the rows
+    as given when nothing was cached before (a prompt attends to itself unrounded), the
+    values as they are held otherwise.  Decode steps on the kernel path read the 4-bit rows
+    themselves, the newest included.
+    '''
+
+    def __init__(self, num_heads: Optional[int] = None):
+        if num_heads is not None:
+            raise ValueError('KV4LayerCache stores grouped heads only')
+        super().__init__()
+        self._dtype: Optional[torch.dtype] = None
+
+    def allocate(self, batch, kv_heads, capacity, head_dim, device, dtype):
+        self._slab = kv4_alloc(batch, kv_heads, capacity, head_dim, device)
+        self._dtype = dtype
+        self.length = 0
+        self.length_dev = torch.zeros(1, dtype=torch.int32, device=device)
+        self._workspaces = {}
+        return self
+
+    @property
+    def slab(self) -> Optional[KV4Slab]:
+        return self._slab
+
+    @property
+    def row_dtype(self) -> Optional[torch.dtype]:
+        return self._dtype
+
+    @property
+    def k(self) -> Optional[torch.Tensor]:
+        return None if self._slab is None else kv4_read(self._slab, 0, self.length, self._dtype)[0]
+
+    @property
+    def v(self) -> Optional[torch.Tensor]:
+        return None if self._slab is None else kv4_read(self._slab, 0, self.length, self._dtype)[1]
+
+    def adopt(self, k, v):
+        raise TypeError('KV4LayerCache holds its rows in 4 bits; use fill() or update()')
+
+    def append_slots(self, n, like):
+        raise TypeError('KV4LayerCache has no rows to write into; use update()')
+
+    def update(self, k_new, v_new, dim: int = 2):
+        if dim != 2:
+            k, v = self.update(k_new.movedim(dim, 2), v_new.movedim(dim, 2), 2)
+            return k.movedim(2, dim), v.movedim(2, dim)
+        n, first = k_new.shape[2], self.length
+        self._room(k_new, n)
+        k_new, v_new = k_new.detach(), v_new.detach()
+        kv4_append(self._slab, k_new, v_new, first)
+        self.length += n
+        self.length_dev.fill_(self.length)
+        return (k_new, v_new) if first == 0 else kv4_read(self._slab, 0, self.length, k_new.dtype)
+
+    def fill(self, k: torch.Tensor, v: torch.Tensor) -> None:
+        n = k.shape[2]
+        self._room(k, n - self.length)
+        kv4_append(self._slab, k.detach(), v.detach(), 0)
+        self.length = n
+        self.length_dev.fill_(n)
+
+    def to(self, device=None, dtype=None):
+        '''Moves the slab; `dtype` is that of the values read back.'''
+        if self._slab is not None:
+            self._slab = KV4Slab(*(t.to(device=device) for t in self._slab))
+            self.length_dev = self.length_dev.to(device=device)
+            self._dtype = dtype or self._dtype
+            self._workspaces = {}
         return self
 
 
@@ -524,18 +619,21 @@ class ModelCache:
         return cls([DecoderBlockCache() for _ in range(num_blocks)])
 
     @classmethod
-    def for_decode(cls, model, batch: int, capacity: int, device, dtype) -> 'ModelCache':
+    def for_decode(cls, model, batch: int, capacity: int, device, dtype, kv_bits: int = 16) -> 'ModelCache':
         '''Fixed-capacity cache of `model` for graph-captured decoding (new): a
-        StaticKVLayerCache of `capacity` positions per Chord layer, an in-place
-        GatedDelta cache with zero state and tails per GatedDelta layer.'''
+        StaticKVLayerCache of `capacity` positions per Chord layer, or with kv_bits=4 a
+        KV4LayerCache (kv_bits=16: rows in `dtype`), an in-place GatedDelta cache with
+        zero state and tails per GatedDelta layer.'''
+        if kv_bits not in (4, 16):
+            raise ValueError(f'kv_bits must be 16 (rows in dtype) or 4, got {kv_bits!r}')
+        kv_type = KV4LayerCache if kv_bits == 4 else StaticKVLayerCache
         blocks = []
         for block in model.blocks:
             layers = []
             for decoder in block.features:
                 attn = decoder.attn
                 if issubclass(decoder.cache_type, KVLayerCache):
-                    layers.append(StaticKVLayerCache().allocate(batch, attn.num_kv_heads, capacity, attn.head_dim,
-                                                                device, dtype))
+                    layers.append(kv_type().allocate(batch, attn.num_kv_heads, capacity, attn.head_dim, device, dtype))
                 else:
                     chans = (attn.num_heads * attn.dk, attn.num_heads * attn.dk, attn.num_heads * attn.dv)
                     layers.append(GatedDeltaAttentionLayerCache().allocate(

@@ -80,8 +80,12 @@ def looks_like_safetensors(path: str) -> bool:
 
 
 def config_to_dict(config: MotifChordConfig) -> Dict[str, Any]:
-    '''Plain JSON-compatible fields (tuples as lists).'''
-    return {k: list(v) if isinstance(v, tuple) else v for k, v in asdict(config).items()}
+    '''Plain JSON-compatible fields (tuples as lists); the window's only where there is one, so
+    that a model without it is written with the reference's fields.'''
+    d = {k: list(v) if isinstance(v, tuple) else v for k, v in asdict(config).items()}
+    if d['window'] is None:
+        del d['window'], d['sinks']
+    return d
 
 
 def config_from_mapping(spec: Dict[str, Any]) -> MotifChordConfig:

@@ -1,5 +1,6 @@
 '''Model hyper-parameters; same fields and defaults as the reference's
-motif/model/config.py:5-39.'''
+motif/model/config.py:5-39, and (new) the Chord layers' sliding window: a query sees the
+keys less than `window` positions back (None: all of them) and the first `sinks` tokens.'''
 from dataclasses import dataclass
 from typing import Literal, Optional, Tuple
 
@@ -14,3 +15,5 @@ class MotifChordConfig:
     tied_weight: bool = True
     block: Tuple[Literal['chord', 'gdn'], ...] = ('gdn', 'gdn', 'gdn', 'chord')
     block_n: int = 4
+    window: Optional[int] = None
+    sinks: int = 0

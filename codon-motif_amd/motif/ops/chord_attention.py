@@ -525,15 +525,19 @@ def chord_decode_step_serves(proj, H, Hkv, D) -> bool:
             and _lib.available())
 
 
-def chord_decode_step_workspace(B, H, Hkv, L, capacity, device) -> torch.Tensor:
+def chord_decode_step_workspace(B, H, Hkv, L, capacity, device, window=None, sinks=0) -> torch.Tensor:
     '''A zeroed workspace for chord_decode_step at these sizes (its arrival counters must
     start at zero; every call leaves them zero).'''
-    n = int(_lib.lib().motif_chord_decode_step_workspace_bytes(B, H, Hkv, L, capacity))
+    window, sinks = check_window(window, sinks)
+    if window is None:
+        n = int(_lib.lib().motif_chord_decode_step_workspace_bytes(B, H, Hkv, L, capacity))
+    else:
+        n = int(_lib.lib().motif_chord_window_step_workspace_bytes(B, H, Hkv, L, capacity, window, sinks))
     return torch.zeros(max(n, 1), dtype=torch.uint8, device=device)
 
 
 def chord_decode_step(proj, offsets, q_norm_weight, k_norm_weight, norm_eps, k_cache, v_cache, length_dev, alpha,
-                      beta, mu, ssmax, log_table, num_heads, softmax_scale, eps, workspace):
+                      beta, mu, ssmax, log_table, num_heads, softmax_scale, eps, workspace, window=None, sinks=0):
     '''A Chord decode step at the device cursor in one launch (new; the reference's
     motif/block/attention/chord_attn.py:255-265 q / k norms and v, the cache append
     motif/model/cache.py:170-215 and the decode call of apply_chord_attention): from the
@@ -541,18 +545,22 @@ def chord_decode_step(proj, offsets, q_norm_weight, k_norm_weight, norm_eps, k_c
     normalised keys and the values at length_dev, attends over length_dev + L keys with
     q_start = length_dev and log_n = log_table[q_start + i], advances length_dev by L.
     Returns out [B, H, L, 64], the same bits as chord_qkv_prep followed by
-    chord_decode_cursor.'''
+    chord_decode_cursor.  `window` / `sinks` limit what a query sees, as for
+    apply_chord_attention (the sums then run over other splits than chord_decode_cursor's).'''
+    window, sinks = check_window(window, sinks)
     B, L = proj.shape[0], proj.shape[1]
     Hkv, cap, D = k_cache.shape[1], k_cache.shape[2], k_cache.shape[3]
     out = torch.empty(B, num_heads, L, D, dtype=proj.dtype, device=proj.device)
-    rc = _lib.lib().motif_chord_decode_step(
+    lib = _lib.lib()
+    fn, limits = (lib.motif_chord_decode_step, ()) if window is None else (lib.motif_chord_window_step, (window, sinks))
+    rc = fn(
         proj.data_ptr(), proj.stride(0), proj.stride(1), *[int(o) for o in offsets],
         q_norm_weight.data_ptr(), k_norm_weight.data_ptr(), float(norm_eps),
         *_lib.t4(k_cache), *_lib.t4(v_cache), length_dev.data_ptr(), cap,
         alpha.data_ptr(), beta.data_ptr(), mu.data_ptr(), ssmax.data_ptr(), log_table.data_ptr(), log_table.numel(),
-        *_lib.t4(out), B, num_heads, Hkv, L, D, float(softmax_scale), float(eps),
+        *_lib.t4(out), B, num_heads, Hkv, L, D, float(softmax_scale), float(eps), *limits,
         workspace.data_ptr(), workspace.numel(), _lib.stream_ptr(proj.device))
-    _lib.check(rc, 'motif_chord_decode_step')
+    _lib.check(rc, 'motif_chord_decode_step' if window is None else 'motif_chord_window_step')
     return out
 
 
