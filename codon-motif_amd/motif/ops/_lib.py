@@ -205,7 +205,7 @@ def stream_ptr(device) -> int:
 def on_device(device):
     '''A context in which `device` is the current one (launches go to the current device;
     switching costs a few us, so only where it is another).'''
-    if device.index is None or device.index == torch.cuda.current_device():
+    if device.index is None or device.index == torch._C._cuda_getDevice():
         return _HERE
     return torch.cuda.device(device)
 

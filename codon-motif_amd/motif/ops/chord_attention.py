@@ -30,6 +30,7 @@ from .autograd_path import chord_attention_torch, chord_attention_varlen_torch, 
 
 HEAD_DIM = 64                  # the model's head dim: bf16 runs on the MFMA kernels
 HEAD_DIMS = (16, 32, 64, 128)  # head dims the kernels serve
+_DTYPES = frozenset((torch.float16, torch.bfloat16, torch.float32))
 NO_WINDOW = 2 ** 31 - 1        # window argument of the kernels that always take one
 
 
@@ -125,26 +126,26 @@ class ChordWindowFunction(torch.autograd.Function):
         q, k, v = _rows4(q)[0], _rows4(k)[0], _rows4(v)[0]
         B, H, L, D = q.shape
         dev = q.device
-        out = torch.empty((B, L, H, D), dtype=q.dtype, device=dev).transpose(1, 2)
-        lse = torch.empty((B, H, L), dtype=torch.float32, device=dev)
+        out = q.new_empty((B, L, H, D)).transpose(1, 2)
         lib = _lib.lib()
         n = lib.motif_chord_distances_len(L, q_start, window, sinks)
-        distances = torch.empty(3 * H * n, dtype=torch.float32, device=dev)
+        rows = -(-B * H * L // 4) * 4
+        stats = log_n.new_empty(rows + 3 * H * n)  # the rows' log-sum-exp, then the distance table
+        lse, distances = stats.data_ptr(), (stats.data_ptr() + 4 * rows, n)
         with _lib.on_device(dev):
-            rc = lib.motif_chord_distances(beta.data_ptr(), mu.data_ptr(), H, n, eps, distances.data_ptr(),
-                                           _lib.stream_ptr(dev))
+            rc = lib.motif_chord_distances(beta.data_ptr(), mu.data_ptr(), H, n, eps, distances[0], _lib.stream_ptr(dev))
         if rc:
             _lib.check(rc, 'motif_chord_distances')
         _launch_window(q, k, v, (alpha, beta, mu, ssmax), log_n, q_start, scale, eps, window, sinks, out, lse,
                        distances=distances)
-        ctx.save_for_backward(q, k, v, out, lse, alpha, beta, mu, ssmax, log_n, distances)
-        ctx.args = q_start, scale, eps, window, sinks
+        ctx.save_for_backward(q, k, v, out, alpha, beta, mu, ssmax, log_n, stats)
+        ctx.args = q_start, scale, eps, window, sinks, rows, n
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        q, k, v, out, lse, alpha, beta, mu, ssmax, log_n, distances = ctx.saved_tensors
-        q_start, scale, eps, window, sinks = ctx.args
+        q, k, v, out, alpha, beta, mu, ssmax, log_n, stats = ctx.saved_tensors
+        q_start, scale, eps, window, sinks, rows, n = ctx.args
         needs = ctx.needs_input_grad
         B, H, L, D = q.shape
         Hkv, S = k.shape[1], k.shape[2]
@@ -152,24 +153,22 @@ class ChordWindowFunction(torch.autograd.Function):
         # (the kernels read dout's own rows, expanded ones too)
         dout = _aligned(dout if dout.stride(-1) == 1 else dout.contiguous())
         # gradients in storage of their own (an expanded input's would share elements)
-        dq = torch.empty((B, L, H, D), dtype=q.dtype, device=dev).transpose(1, 2)
-        dk = torch.empty((B, Hkv, S, D), dtype=q.dtype, device=dev)
-        dv = torch.empty((B, Hkv, S, D), dtype=q.dtype, device=dev)
-        d_params = torch.empty((4, H), dtype=torch.float32, device=dev)
+        dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
+        d_params = log_n.new_empty((4, H))
         ws = torch.empty(_window_bwd_workspace_bytes(B, H, Hkv, L, S, q_start, window, sinks), dtype=torch.uint8, device=dev)
         with _lib.on_device(dev):
             rc = _lib.lib().motif_chord_window_bwd(
                 q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3],
                 out.data_ptr(), *out.stride()[:3], dout.data_ptr(), *dout.stride()[:3],
-                lse.data_ptr(), alpha.data_ptr(), beta.data_ptr(), mu.data_ptr(), ssmax.data_ptr(),
+                stats.data_ptr(), alpha.data_ptr(), beta.data_ptr(), mu.data_ptr(), ssmax.data_ptr(),
                 log_n.data_ptr(), *log_n.stride(), dq.data_ptr(), *dq.stride()[:3], dk.data_ptr(), *dk.stride()[:3],
                 dv.data_ptr(), *dv.stride()[:3], d_params.data_ptr(), B, H, Hkv, L, S, D, q_start, scale, eps,
-                window, sinks, 1 if needs[5] else 0, distances.data_ptr(), distances.numel() // (3 * H), ws.data_ptr(),
-                ws.numel(), _lib.MOTIF_BF16, _lib.stream_ptr(dev))
+                window, sinks, 1 if needs[5] else 0, stats.data_ptr() + 4 * rows, n, ws.data_ptr(), ws.numel(),
+                _lib.MOTIF_BF16, _lib.stream_ptr(dev))
         if rc:
             _lib.check(rc, 'motif_chord_window_bwd')
         return (dq if needs[0] else None, dk if needs[1] else None, dv if needs[2] else None,
-                *(d_params[i] if needs[3 + i] else None for i in range(4)), None, None, None, None, None, None)
+                *(g if need else None for g, need in zip(d_params.unbind(0), needs[3:7])), None, None, None, None, None, None)
 
 
 @functools.lru_cache(maxsize=256)
@@ -232,6 +231,31 @@ def _check_params(alpha, beta, mu, ssmax, num_heads):
             raise ValueError(f'{name} must be contiguous')
 
 
+def _check_call(q, k, v, params, log_n):
+    '''_check_tensors and _check_params of a windowed call, and that its tensors share a device:
+    asked for at once, and one by one (for the message) only where something is off.'''
+    at, dt, shape, ks = q.get_device(), q.dtype, q.shape, k.shape
+    if at >= 0 and len(shape) == 4 and len(ks) == 4 and dt in _DTYPES:
+        B, H, L, D = shape
+        Hkv = ks[1]
+        if k.dtype == dt and v.dtype == dt and ks == v.shape and ks[0] == B and ks[3] == D and D >= 16 \
+                and Hkv and H % Hkv == 0 and k.get_device() == at and v.get_device() == at \
+                and q.stride()[3] == 1 and k.stride()[3] == 1 and v.stride()[3] == 1 \
+                and log_n.get_device() == at and log_n.dtype == torch.float32 and log_n.shape == (B, L) \
+                and log_n.stride()[1] == 1:
+            for t in params:
+                if t.get_device() != at or t.dtype != torch.float32 or t.shape != (H,) or not t.is_contiguous():
+                    break
+            else:
+                return B, H, L, D, Hkv, ks[2]
+    sizes = _check_tensors(q, k, v, log_n)
+    _check_params(*params, sizes[1])
+    for t in (k, v, log_n, *params):
+        if t.device != q.device:
+            raise ValueError(f'the tensors of a call must live on one device, got {q.device} and {t.device}')
+    return sizes
+
+
 def _aligned(t):
     '''Rows must start on 16-byte boundaries for the vector loads.  (A copy where they do not:
     contiguous() returns a contiguous tensor as it is, whatever its address.)'''
@@ -255,7 +279,7 @@ def _check_out(out, shape, dtype, device):
 def _out_for(out, q):
     '''The kernel's destination: the caller's `out` (checked) or a new [B, H, L, D].'''
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
     return _check_out(out, q.shape, q.dtype, q.device)
 
 
@@ -305,7 +329,8 @@ def _launch(q, k, v, alpha, beta, mu, ssmax, log_n, q_start, scale, eps, out, ls
 def _launch_window(q, k, v, params, log_n, q_start, scale, eps, window, sinks, out, lse=None, length_dev=None,
                    log_table=None, workspace=None, distances=None):
     '''motif_chord_window_fwd into `out`: host positions (log_n), or the device cursor over a
-    fixed-capacity cache (length_dev and log_table; the launch advances it).'''
+    fixed-capacity cache (length_dev and log_table; the launch advances it).  `lse` is a pointer,
+    `distances` a (pointer, distances) pair.'''
     B, H, L, D = q.shape
     Hkv, S = k.shape[1], k.shape[2]
     if D not in HEAD_DIMS:  # zero-padded to the next size, as in _launch
@@ -333,10 +358,9 @@ def _launch_window(q, k, v, params, log_n, q_start, scale, eps, window, sinks, o
         rc = _lib.lib().motif_chord_window_fwd(
             *q4, *k4, *v4, alpha.data_ptr(), beta.data_ptr(), mu.data_ptr(), ssmax.data_ptr(), *ln,
             None if log_table is None else log_table.data_ptr(), 0 if log_table is None else log_table.numel(),
-            out.data_ptr(), *out.stride()[:3], None if lse is None else lse.data_ptr(),
+            out.data_ptr(), *out.stride()[:3], lse,
             None if length_dev is None else length_dev.data_ptr(), B, H, Hkv, L, S, D, q_start, scale, eps,
-            window, sinks, None if distances is None else distances.data_ptr(),
-            0 if distances is None else distances.numel() // (3 * H),
+            window, sinks, *(distances or (None, 0)),
             None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel(), code,
             _lib.stream_ptr(q.device))
     if rc:
@@ -412,8 +436,7 @@ def apply_chord_attention(
         if q_start is not None and int(q_start) < 0:
             raise ValueError(f'q_start must not be negative, got {q_start}')
         if window is not None and _window_grad_kernels_serve(q, k, v, alpha, beta, mu, ssmax, log_n):
-            _check_tensors(q, k, v, log_n)
-            _check_params(alpha, beta, mu, ssmax, q.shape[1])
+            _check_call(q, k, v, (alpha, beta, mu, ssmax), log_n)
             scale = q.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale)
             qs = k.shape[2] - q.shape[2] if q_start is None else int(q_start)
             if qs < 0:
@@ -430,8 +453,11 @@ def apply_chord_attention(
         return res if out is None else _check_out(out, res.shape, res.dtype, res.device).copy_(res)
     if not _lib.available():
         raise RuntimeError('there is no usable HIP backend in the current environment')
-    B, H, L, D, Hkv, S = _check_tensors(q, k, v, log_n)
-    _check_params(alpha, beta, mu, ssmax, H)
+    if window is None:
+        B, H, L, D, Hkv, S = _check_tensors(q, k, v, log_n)
+        _check_params(alpha, beta, mu, ssmax, H)
+    else:
+        B, H, L, D, Hkv, S = _check_call(q, k, v, (alpha, beta, mu, ssmax), log_n)
     if softmax_scale is None:
         softmax_scale = D ** -0.5
     if q_start is None:
@@ -482,8 +508,11 @@ def apply_chord_attention_varlen(q, k, v, alpha, beta, mu, ssmax, log_n, cu_seql
         return res if out is None else _check_out(out, res.shape, res.dtype, res.device).copy_(res)
     if not _lib.available():
         raise RuntimeError('there is no usable HIP backend in the current environment')
-    B, H, L, D, Hkv, S = _check_tensors(q, k, v, log_n)
-    _check_params(alpha, beta, mu, ssmax, H)
+    if window is None:
+        B, H, L, D, Hkv, S = _check_tensors(q, k, v, log_n)
+        _check_params(alpha, beta, mu, ssmax, H)
+    else:
+        B, H, L, D, Hkv, S = _check_call(q, k, v, (alpha, beta, mu, ssmax), log_n)
     if B != 1 or S != L:
         raise ValueError('apply_chord_attention_varlen: needs B == 1 and packed q / k of equal length')
     ps = PackedSeqs.of(cu_seqlens, L, q.device)
@@ -594,6 +623,15 @@ def chord_decode_cursor(q, k_cache, v_cache, length_dev, alpha, beta, mu, ssmax,
             raise ValueError('chord_decode_cursor: a window and library_scratch do not go together')
         if L > cap:
             raise ValueError('chord_decode_cursor: more queries than the capacity')
+        _check_params(alpha, beta, mu, ssmax, H)
+        if k_cache.shape != v_cache.shape or k_cache.shape[0] != B or k_cache.shape[3] != D or H % Hkv \
+                or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype or not log_table.is_contiguous() \
+                or log_n is not None and (log_n.shape != (B, L) or log_n.dtype != torch.float32):
+            raise ValueError(f'chord_decode_cursor: q {tuple(q.shape)} does not fit the caches {tuple(k_cache.shape)} and '
+                             f'{tuple(v_cache.shape)}, their dtype, log_n or log_table')
+        for t in (k_cache, v_cache, log_table, alpha, beta, mu, ssmax):
+            if t.get_device() != q.get_device():
+                raise ValueError('chord_decode_cursor: the tensors of a call must live on one device')
         if out.numel() == 0:
             return out
         return _launch_window(q, k_cache, v_cache, (alpha, beta, mu, ssmax), log_n, 0, float(softmax_scale), float(eps),

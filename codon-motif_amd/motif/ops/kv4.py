@@ -21,7 +21,7 @@ import torch
 
 from . import _lib
 from .autograd_path import wants_grad
-from .chord_attention import HEAD_DIMS, NO_WINDOW, _check_params, _out_for, _rows4, check_window
+from .chord_attention import _DTYPES, HEAD_DIMS, NO_WINDOW, _check_params, _out_for, _rows4, check_window
 
 GROUP = 32  # features that share a (scale, base) pair
 
@@ -67,10 +67,10 @@ def _check_slab(slab: KV4Slab, what: str):
     if vc.shape != shape or kp.shape != pshape or vp.shape != pshape \
             or kp.dtype != torch.bfloat16 or vp.dtype != torch.bfloat16:
         raise ValueError(f'{what}: codes of keys and values must have one shape, params must be bfloat16 {pshape}')
-    dev = kc.device
-    if dev.type != 'cuda':
+    at = kc.get_device()
+    if at < 0:
         raise ValueError(f'{what}: the cache must live on CUDA')
-    if kp.device != dev or vc.device != dev or vp.device != dev:
+    if kp.get_device() != at or vc.get_device() != at or vp.get_device() != at:
         raise ValueError(f'{what}: the cache tensors must live on one device')
     args = []
     for c, p in ((kc, kp), (vc, vp)):
@@ -131,7 +131,7 @@ def kv4_read(slab: KV4Slab, start: int, n: int, dtype: torch.dtype = torch.bfloa
     code = _lib.chord_dtype_code(dtype)
     _need_backend()
     k = torch.empty(B, Hkv, n, D, dtype=dtype, device=slab.k_codes.device)
-    v = torch.empty(B, Hkv, n, D, dtype=dtype, device=slab.k_codes.device)
+    v = torch.empty_like(k)
     if k.numel():
         s0, s1, s2, _ = k.stride()
         with _lib.on_device(k.device):
@@ -144,16 +144,17 @@ def kv4_read(slab: KV4Slab, start: int, n: int, dtype: torch.dtype = torch.bfloa
 
 def _check_query(q, slab, params, what):
     (B, Hkv, cap, D), args = _check_slab(slab, what)
-    shape, dev = q.shape, q.device
+    shape, at = q.shape, q.get_device()
     if len(shape) != 4 or shape[0] != B or shape[3] != D or shape[1] % Hkv:
         raise ValueError(f'{what}: q {tuple(shape)} does not fit a cache of {B} rows, {Hkv} kv heads of {D}')
-    if q.dtype not in (torch.float16, torch.bfloat16, torch.float32) or q.stride(3) != 1:
+    if q.dtype not in _DTYPES or q.stride()[3] != 1:
         raise ValueError(f'{what}: q must be fp16 / bf16 / fp32 and contiguous along the last dimension')
-    if dev != slab[0].device:
+    if at != slab[0].get_device():
         raise ValueError(f'{what}: q and the cache must live on one device')
     _check_params(*params, shape[1])
-    if any(t.device != dev for t in params):
-        raise ValueError(f'{what}: the head parameters must live on q\'s device')
+    for t in params:
+        if t.get_device() != at:
+            raise ValueError(f'{what}: the head parameters must live on q\'s device')
     return B, shape[1], Hkv, shape[2], D, cap, args
 
 
@@ -242,7 +243,7 @@ def chord_decode_kv4_cursor(q, slab: KV4Slab, length_dev, alpha, beta, mu, ssmax
     if L > cap:
         raise ValueError('chord_decode_kv4_cursor: more queries than the capacity')
     _need_backend()
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = _out_for(None, q)
     if out.numel() == 0:
         return out
     return _launch_kv4(q, args, Hkv, params, None, log_table, length_dev, cap, 0,
