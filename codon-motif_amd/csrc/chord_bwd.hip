@@ -214,7 +214,6 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
   const float lam = a.log_n[b * a.ln_sb + int64_t(qr) * a.ln_st];
   const float sig = a.ssmax[h], al = a.alpha[h], be = a.beta[h], mu = a.mu[h];
   const float s = a.scale, c = sig * lam, cl = c * kLog2e, cs = c * s;
-  const float cls = cl * s, cla = -cl * al;
   if (!WIN && chunk == 0 && qv && hh == 0) a.rows[ri] = float4{lse2, delta, cl, cs};
   const int q_abs = a.q_start + my_q;
   const int wave_kv_end = a.q_start + min(a.L, q0 + 32);  // keys this wave sees: < wave_kv_end
@@ -232,8 +231,10 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
   dqacc[0] = f32x16{};
   dqacc[1] = f32x16{};
   float sa = 0.f, sb = 0.f, sm = 0.f, ss = 0.f;
-  // WIN: sums of P (dP - Delta), P x, P S and P K, see below
-  float rho = 0.f, psum = 0.f, ea = 0.f, eb = 0.f, em = 0.f, es = 0.f;
+  // WIN: a row's sums of P and g = P (dP - Delta), and of both times r, x^beta, x^beta log2 x and mu's
+  // factor, see below
+  struct RowSums { float p, g, gs, ga, gb, gm, ps, pa, pb, pm; };
+  RowSums sum = {};
   f32x16 pkacc[2];
   pkacc[0] = pkacc[1] = f32x16{};
 
@@ -293,6 +294,7 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
       float dz[16], pr[WIN ? 16 : 1];
       auto body = [&](auto masked) {
         uint32_t seen = 0u;  // WIN: the tile's keys that this query sees
+        RowSums t;
         if constexpr (WIN && decltype(masked)::value)
           seen = qv ? seen_keys(min(k_max - n0, walk.rows(kt) - 1), q_abs - a.window - n0, a.sinks - n0) >> (4 * hh) : 0u;
 #pragma unroll
@@ -300,26 +302,26 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
           const int kk = 8 * (r >> 2) + 4 * hh + (r & 3);
           const DistV wv = sW[w][kk - lc + 31];
           if constexpr (WIN) {
-            // log2e c r = cls S + cla x^beta; the sums of g r, g b and g b ln x follow from those of g S,
-            // g x^beta and g x^beta log2 x
-            // (the two large terms that cancel first: what is left is of the bias's size)
-            float p = fast_exp2(fmaf(cla, wv.x, fmaf(cls, sacc[r], -lse2)));
+            const float rr = fmaf(-al, wv.x, s * sacc[r]);
+            float p = fast_exp2(fmaf(cl, rr, -lse2));
             if constexpr (decltype(masked)::value) p = seen & (1u << (8 * (r >> 2) + (r & 3))) ? p : 0.f;
             const float g = p * (pacc[r] - delta);
-            psum += p;
-            rho += g;
-            ss = fmaf(g, sacc[r], ss);
-            sa = fmaf(g, wv.x, sa);
-            sb = fmaf(g, wv.y, sb);
-            es = fmaf(p, sacc[r], es);
-            ea = fmaf(p, wv.x, ea);
-            eb = fmaf(p, wv.y, eb);
+            // a tile's sums on their own, then onto the row's: half the terms to round with
+            auto add = [r](float &x, float f, float y) { x = r ? fmaf(f, y, x) : f * y; };
+            t.p = r ? t.p + p : p;
+            t.g = r ? t.g + g : g;
+            add(t.gs, g, rr);
+            add(t.ga, g, wv.x);
+            add(t.gb, g, wv.y);
+            add(t.ps, p, rr);
+            add(t.pa, p, wv.x);
+            add(t.pb, p, wv.y);
             if constexpr (MU) {
-              sm = fmaf(g, wv.z, sm);
-              em = fmaf(p, wv.z, em);
+              add(t.gm, g, wv.z);
+              add(t.pm, p, wv.z);
             }
             pr[r] = p;
-            dz[r] = g * cs;
+            dz[r] = g;  // (c s goes onto the sum)
           } else {
             const float rr = fmaf(s, sacc[r], wv.x);
             float p = fast_exp2(fmaf(cl, rr, -lse2));
@@ -331,6 +333,12 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
             sm = fmaf(g, wv.w, sm);
             dz[r] = g * cs;  // (rounded to bf16 with its factor, as the dK / dV kernel rounds it)
           }
+        }
+        if constexpr (WIN) {
+          sum.p += t.p, sum.g += t.g;
+          sum.gs += t.gs, sum.ga += t.ga, sum.gb += t.gb;
+          sum.ps += t.ps, sum.pa += t.pa, sum.pb += t.pb;
+          if constexpr (MU) sum.gm += t.gm, sum.pm += t.pm;
         }
       };
       // every key of the tile at or before every query of the wave (and in its window), all queries valid
@@ -357,24 +365,22 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
   // right by rho times that of P x, and the second kernel is given Delta + rho.  The weights' own sum
   // takes the log-sum-exp's fp32 rounding (1e-6 of a weight) out of the parameter sums.  (2 x 2048
   // tokens, a window of 512, against 64 bits: dq and dk 4.6e-3 off without, 2.4e-3 with; alpha's
-  // gradient 1e-2 and 1e-6.)
+  // gradient 1e-2 and 1e-6.  Summed by tiles of r itself, ssmax's is 0.6e-6 off; one long sum of S and one
+  // of x^beta, put together at the end, were 2.5e-6 off.)
   if constexpr (WIN) {
     auto both = [](float x) {  // over the two lane halves
       const auto s32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
       return __uint_as_float(s32[0]) + __uint_as_float(s32[1]);
     };
-    const float ps = both(psum), inv = ps > 0.f ? 1.f / ps : 0.f, r = both(rho) * inv;
-    sa = fmaf(-r, ea, sa) * inv;
-    sb = fmaf(-r, eb, sb) * inv;
-    ss = fmaf(-r, es, ss) * inv;
-    ss = fmaf(s, ss, -al * sa);             // r = s S + b, b = -alpha x^beta
-    sa = -sa;                               // d b / d alpha
-    sb = sb * (-al * 0.6931471805599453f);  // d b / d beta = b ln x
-    if constexpr (MU) sm = fmaf(-r, em, sm) * inv * (al * be);
+    const float ps = both(sum.p), inv = ps > 0.f ? 1.f / ps : 0.f, r = both(sum.g) * inv;
+    ss = fmaf(-r, sum.ps, sum.gs) * inv;                                    // r = s S + b, b = -alpha x^beta
+    sa = -fmaf(-r, sum.pa, sum.ga) * inv;                                   // d b / d alpha
+    sb = fmaf(-r, sum.pb, sum.gb) * inv * (-al * 0.6931471805599453f);      // d b / d beta = b ln x
+    if constexpr (MU) sm = fmaf(-r, sum.pm, sum.gm) * inv * (al * be);
 #pragma unroll
     for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) dqacc[dt][i] = fmaf(-r * cs, pkacc[dt][i], dqacc[dt][i]);
+      for (int i = 0; i < 16; ++i) dqacc[dt][i] = cs * fmaf(-r, pkacc[dt][i], dqacc[dt][i]);
     if (qv && hh == 0) a.rows[ri] = float4{lse2, delta + r, cl, cs};
   }
 
