@@ -412,8 +412,8 @@ extern "C" int motif_chord_window_fwd(
     const float *log_n, int64_t ln_sb, int64_t ln_st, const float *log_table, int log_table_len,
     void *out, int64_t o_sb, int64_t o_sh, int64_t o_st, float *lse,
     int *length_dev, int B, int H, int Hkv, int L, int S, int D, int q_start, float scale, float eps,
-    int window, int sinks, const float *distances, int distances_len, void *workspace, size_t workspace_bytes, int dtype,
-    void *stream) {
+    int window, int sinks, const float *distances, int distances_len, const int32_t *cu_seqlens, int nseq, int max_seqlen,
+    void *workspace, size_t workspace_bytes, int dtype, void *stream) {
   const Call c{"chord_window_fwd", q, q_sb, q_sh, q_st, alpha, beta, mu, ssmax, log_n, ln_sb, ln_st, log_table,
                log_table_len, out, o_sb, o_sh, o_st, lse, length_dev, B, H, Hkv, L, S, D, q_start, scale, eps,
                window, sinks, dtype};
@@ -422,6 +422,14 @@ extern "C" int motif_chord_window_fwd(
   if (rc || B == 0 || L == 0) return rc;
   if ((rc = fill_rows(c, a, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st))) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (cu_seqlens) {
+    if (B != 1 || S != L || q_start || nseq < 0 || nseq > 65535 || max_seqlen < 0 || max_seqlen > L)
+      return set_error(MOTIF_ERR_INVALID, "chord_window_fwd: packed sequences need B == 1, S == L, q_start 0 and sizes within L");
+    if (dtype != MOTIF_BF16 || D != kBD || length_dev || lse || distances || !log_n || max_seqlen > 65535 * 16)
+      return set_error(MOTIF_ERR_UNSUPPORTED, "chord_window_fwd: packed sequences need bf16, head_dim 64 and host positions");
+    a.cu = cu_seqlens;
+    return nseq && max_seqlen ? launch_window(a, nseq, max_seqlen, st) : MOTIF_OK;
+  }
   if (chord_window_decode_serves(H, Hkv, L, D, dtype) && !lse) {
     a.splits = chord_window_splits(B, Hkv, L, S, window, sinks);
     if (a.splits > 1) {

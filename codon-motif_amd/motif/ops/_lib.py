@@ -88,7 +88,7 @@ _SIGNATURES = {
     'motif_chord_window_workspace_bytes': ([_I32] * 9, _SZ),
     'motif_chord_window_fwd': (
         _T4 * 3 + [_P] * 4 + [_P, _I64, _I64, _P, _I32] + _T4 + [_P, _P] + [_I32] * 7 + [_F32, _F32]
-        + [_I32, _I32, _P, _I32, _P, _SZ, _I32, _P], _I32),
+        + [_I32, _I32, _P, _I32, _P, _I32, _I32, _P, _SZ, _I32, _P], _I32),
     'motif_chord_distances_len': ([_I32] * 4, _I32),
     'motif_chord_distances': ([_P, _P, _I32, _I32, _F32, _P, _P], _I32),
     'motif_chord_window_bwd_workspace_bytes': ([_I32] * 8, _SZ),

@@ -327,10 +327,11 @@ def _launch(q, k, v, alpha, beta, mu, ssmax, log_n, q_start, scale, eps, out, ls
 
 
 def _launch_window(q, k, v, params, log_n, q_start, scale, eps, window, sinks, out, lse=None, length_dev=None,
-                   log_table=None, workspace=None, distances=None):
+                   log_table=None, workspace=None, distances=None, packed=(None, 0, 0)):
     '''motif_chord_window_fwd into `out`: host positions (log_n), or the device cursor over a
     fixed-capacity cache (length_dev and log_table; the launch advances it).  `lse` is a pointer,
-    `distances` a (pointer, distances) pair.'''
+    `distances` a (pointer, distances) pair, `packed` the boundaries' pointer, the sequences and the
+    longest one's length.'''
     B, H, L, D = q.shape
     Hkv, S = k.shape[1], k.shape[2]
     if D not in HEAD_DIMS:  # zero-padded to the next size, as in _launch
@@ -360,7 +361,7 @@ def _launch_window(q, k, v, params, log_n, q_start, scale, eps, window, sinks, o
             None if log_table is None else log_table.data_ptr(), 0 if log_table is None else log_table.numel(),
             out.data_ptr(), *out.stride()[:3], lse,
             None if length_dev is None else length_dev.data_ptr(), B, H, Hkv, L, S, D, q_start, scale, eps,
-            window, sinks, *(distances or (None, 0)),
+            window, sinks, *(distances or (None, 0)), *packed,
             None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel(), code,
             _lib.stream_ptr(q.device))
     if rc:
@@ -410,7 +411,7 @@ def apply_chord_attention(
     Args:
         q: [B, H, L, D];  k, v: [B, H_kv, S, D] (fp16, bf16 or fp32; 16 <= D <= 128).
         alpha, beta, mu, ssmax: [H] fp32 contiguous.
-        log_n: [B, L] fp32.
+        log_n: [B, L] fp32, not negative (the logarithm of a count).
         q_start: absolute position of the first query; defaults to S - L.
         softmax_scale: defaults to D ** -0.5.
         eps: GGD epsilon.
@@ -522,7 +523,11 @@ def apply_chord_attention_varlen(q, k, v, alpha, beta, mu, ssmax, log_n, cu_seql
     if L == 0:
         return out
     if window is not None:
-        for a, b in ps.bounds():
+        if q.dtype == torch.bfloat16 and D == HEAD_DIM and ps.nseq <= 65535:
+            cu = ps.cu if ps.cu.device == q.device else ps.cu.to(q.device)
+            return _launch_window(q, k, v, (alpha, beta, mu, ssmax), log_n, 0, float(softmax_scale), float(eps), window,
+                                  sinks, out, packed=(cu.data_ptr(), ps.nseq, ps.max_len))
+        for a, b in ps.bounds():  # other types and head dims, sequence by sequence
             if b > a:
                 _launch_window(q[:, :, a:b], k[:, :, a:b], v[:, :, a:b], (alpha, beta, mu, ssmax), log_n[:, a:b], 0,
                                float(softmax_scale), float(eps), window, sinks, out[:, :, a:b])

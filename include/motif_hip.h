@@ -484,6 +484,9 @@ int motif_chord_qkv_prep(const void *proj, int64_t p_sb, int64_t p_st, int q_off
  *   (the argument must be 0), and the launch advances *length_dev by L.
  *   distances: NULL (the bias is evaluated in fp32), or motif_chord_distances' table, which a
  *   forward whose gradients follow is given so that both use the same weights.
+ *   cu_seqlens: NULL, or packed sequences (bf16, D 64, host positions): B == 1, S == L,
+ *   cu_seqlens[nseq + 1] (device, non-decreasing, 0 to L), the longest sequence max_seqlen;
+ *   each is causal from position 0 on its own, log_n is given and read at the packed row.
  *   workspace: motif_chord_window_workspace_bytes(...) bytes (may be 0), 16-byte aligned.
  */
 size_t motif_chord_window_workspace_bytes(int B, int H, int Hkv, int L, int S, int D, int window, int sinks, int dtype);
@@ -496,6 +499,7 @@ int motif_chord_window_fwd(
     void *out, int64_t o_sb, int64_t o_sh, int64_t o_st, float *lse,
     int *length_dev, int B, int H, int Hkv, int L, int S, int D, int q_start, float scale, float eps,
     int window, int sinks, const float *distances, int distances_len,
+    const int32_t *cu_seqlens, int nseq, int max_seqlen,
     void *workspace, size_t workspace_bytes, int dtype, void *stream);
 
 /*

@@ -108,7 +108,50 @@ def test_packed_equals_sequences_apart(dtype):
     for a, b in zip(cu[:-1].tolist(), cu[1:].tolist()):
         if b > a:
             one = apply_chord_attention(*(t[:, :, a:b] for t in args[:3]), *args[3:7], args[7][:, a:b], window=40, sinks=2)
-            assert torch.equal(got[:, :, a:b], one)
+            if dtype == F16 or b - a > 8:  # (short bf16 sequences on their own are decodes)
+                assert torch.equal(got[:, :, a:b], one)
+            check_attention(got[:, :, a:b].cpu(), *(t[:, :, a:b] for t in (q, k, v)), par, log_n[:, a:b], 0, 40, 2, what=str((a, b)))
+
+
+@pytest.mark.parametrize('H,Hkv', [(2, 2), (4, 2), (8, 2)])
+@torch.no_grad()
+def test_packed_sequences_see_themselves_only(H, Hkv):
+    from motif.ops import apply_chord_attention_varlen
+    from motif.ops.packed import PackedSeqs
+    lens = [3, 17, 1, 0, 200, 64, 129, 2, 0]
+    T = sum(lens)
+    q, k, v, par = inputs(1, H, Hkv, T, T, 64, BF, seed=H)
+    log_n = torch.cat([log_n_of(1, n, 0) for n in lens], 1)
+    ps = PackedSeqs(torch.tensor([0, *torch.tensor(lens).cumsum(0).tolist()]))  # (boundaries on the host)
+    run = lambda k, v: apply_chord_attention_varlen(*(t.to(DEV) for t in (q, k, v, *par, log_n)), ps, window=30, sinks=2)
+    got = run(k, v)
+    for a, b in ps.bounds():
+        if b > a:
+            check_attention(got[:, :, a:b].cpu(), *(t[:, :, a:b] for t in (q, k, v)), par, log_n[:, a:b], 0, 30, 2)
+    for a, b in ps.bounds():  # rows of one sequence are nothing to the others
+        if b > a:
+            k2, v2 = k.clone(), v.clone()
+            k2[:, :, a:b] = v2[:, :, a:b] = float('nan')
+            other = run(k2, v2)
+            assert torch.equal(other[:, :, :a], got[:, :, :a]) and torch.equal(other[:, :, b:], got[:, :, b:])
+
+
+@torch.no_grad()
+def test_packed_call_replays():
+    from motif.ops import apply_chord_attention_varlen
+    from motif.ops.packed import PackedSeqs
+    ps = PackedSeqs(torch.tensor([0, 40, 41, 170]), 170, torch.device(DEV, 0))
+    q, k, v, par = (inputs(1, 4, 2, 170, 170, 64, BF, seed=1))
+    args = [t.to(DEV) for t in (q, k, v, *par, log_n_of(1, 170, 0))]
+    want = apply_chord_attention_varlen(*args, ps, window=30, sinks=2)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = apply_chord_attention_varlen(*args, ps, window=30, sinks=2)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        assert torch.equal(got, want)
+        want = apply_chord_attention_varlen(*args, ps, window=30, sinks=2)
 
 
 @pytest.mark.parametrize('dtype,D,L', [(BF, 64, 1), (BF, 64, 2), (F16, 64, 1), (F32, 128, 1), (BF, 32, 3)])
