@@ -1205,12 +1205,16 @@ int chord_window_splits(int B, int Hkv, int L, int S, int window, int sinks) {
   if (tiles <= 48 || heads >= 160) return 1;
   return heads >= 80 ? 4 : 8;
 }
-// The one-launch step's: its four-wave workgroups merge themselves (about three of them per CU, a tile for
-// each of their waves).
+// The one-launch step's, whose four-wave workgroups merge themselves: three for every two CUs, a tile for
+// each of their waves, and no more than 12 (the last to arrive reads them all).  Measured, us, as above,
+// 1 / 2 / 4 / 8 / 12 / 32 shares: 3 kv heads, a window of 1024 keys 16.9 / 12.9 / 11.1 / 10.8 / 10.1 / 10.0, 4096
+// 42.9 / 27.5 / 19.9 / 15.2 / 13.2 / 18.7; 48 1024 18.4 / 15.1 / 12.7 / 13.1 / 12.5 / 12.5, 4096 51.9 / 32.7 / 21.9 /
+// 18.6 / 19.6 / 41.5; 96 1024 19.4 / 15.6 / 14.1 / 16.7 / 19.1, 4096 53.5 / 33.7 / 25.6 / 27.7 / 34.9; 192 1024
+// 21.0 / 17.5 / 18.4 / 30.0, 4096 56.7 / 39.6 / 41.5 / 50.2.
 static int window_step_splits(int B, int Hkv, int L, int S, int window, int sinks) {
   const int64_t keys = std::min<int64_t>(S, std::min<int64_t>(window, S) + L + std::min(sinks, S) + 2 * 32);
   const int64_t base = std::max<int64_t>(1, int64_t(B) * Hkv), tiles = (keys + 31) / 32;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(3 * device_cu_count() + base - 1) / base, (tiles + 3) / 4, 32})));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(3 * device_cu_count() / 2 + base - 1) / base, (tiles + 3) / 4, 12})));
 }
 
 bool chord_window_decode_serves(int H, int Hkv, int L, int D, int dtype) {

@@ -36,6 +36,14 @@
 // tokens: dQ 73 -> 57 us, dK / dV 72 -> 62, reductions 26 (three launches) -> 14 (one).  Whole
 // backward, back to back: that size 165 -> 131 us, 4096 tokens (3 kv heads) 282 -> 193, 1024 tokens
 // 71 -> 45, 16 x 512 tokens 125 -> 88.
+//
+// Under a window (WIN) both loops walk only the tiles that a block's windows and first tokens reach, and
+// every block has about the same work, so nothing is cut but the queries that see a block's first tokens
+// from behind its windows (plan_bwd_window).  The distances' powers come from a 64-bit table: in
+// registers they took 20 instructions a score where 12 are left, and were the parameter gradients'
+// largest error.  2 x 2048 tokens, 12 heads, window 512: dQ 44 us, dK / dV 39, reduction 4, table 3;
+// 4001 tokens, 3 kv heads, window 1000: 70, 63, 10, 3.  Bound as above; with 384 workgroups on 256 CUs
+// those with two set the time (30 us of work for dQ spread evenly).
 #include <algorithm>
 #include <string>
 #include <type_traits>

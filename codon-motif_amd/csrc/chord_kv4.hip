@@ -7,15 +7,21 @@
 // (bf16; a mask and an or per pair, exact, and 128 times the other operand's sum is taken out in
 // fp32) or n (fp16), the key's scale is applied to the score product, the value's to the weight.
 //
-// A workgroup is four waves over one kv head's rows and a range of the keys; a wave step is 64 keys
-// (5 KB), staged by buffer-to-LDS loads one step ahead, so a wave's loads fly while it computes.
+// A workgroup is four waves over one kv head's rows and a range of the keys, or up to twelve over all of
+// them (chord_kv4_splits); a wave step is 64 keys (5 KB), staged by buffer-to-LDS loads one step ahead, so a wave's loads fly while it computes.
 // Key 16 g + 4 t + i of a step is row 4 g + i of score tile t, which leaves lane group g its own 16
 // keys; ds_read_b64_tr_b4 gives a lane one feature of those 16 keys, the operand of O^T += V^T P^T.
 // The MFMA has 16 columns, the rows of a step are few: U = 16 / rows copies of the query rows sit in
 // the columns, copy u with zeros but for the tiles t of its own, so one accumulator holds the scores
 // of U tiles and every lane's softmax work is on scores of its own (4 a step at U = 4, where columns
 // of padding would make it 16).  The weights enter the second product masked the same way, and
-// the copies' outputs are added with the waves'.
+// the copies' outputs are added with the waves'.  The weights are rounded to bf16 with the value's scale
+// (fp16: to two bf16, 17 bits, as fp16's range would not hold the product).
+// Bound by VALU issue (codes to operands 112 of some 420 instructions a step, the bias's logarithm and
+// exponential and the softmax's at a quarter of the rate; the vector unit issues in 73% of the busy
+// cycles): 64 sequences of 4097 keys, 12 heads on 3, 63 MB of cache in 21 us (3.0 TB/s); the bf16 rows
+// of the same cache are 201 MB, 40 us.  One sequence of 300 keys 8 us; 32 x 2 fp16 rows, window 4000 of 8190
+// keys, 18.5 us and a merge of 4.  Without the matrix instructions (chord_wide_kernel) 592 us.
 #include <algorithm>
 #include <string>
 

@@ -26,6 +26,12 @@
 // us (and of the vector kernel that served these shapes, with its bias table's launch): fp32 1023
 // tokens 34.5 (151), 4096 tokens 325 (1355), 3 tokens over 4096 82 (101); fp16 1023 tokens 22 (148);
 // bf16 D = 128 1000 tokens 36 (381).  Error against 64 bits, fp32: 3.7e-7 (4.1e-7).
+//
+// Under a window, and over a 4-bit cache (its values expanded to fp32 in registers: code * scale + base),
+// the same loop over the tiles of the first tokens and of the block's windows: the general forms of every
+// type, head dim and query count, beside the bf16 and fp16 kernels at head dim 64 (chord_window.hip,
+// chord_kv4.hip and the windowed decode of chord.hip).  2 x 517 fp32 queries over 1023 keys, window 259:
+// 29 us, the matrix pipe busy 27% of the time (408 short blocks, three tiles a wave: each wave's chain).
 #include <algorithm>
 #include <type_traits>
 

@@ -14,7 +14,15 @@
 // (two heads) or 63 distances meet in a tile, 32 of them new, so each lane evaluates one per tile
 // (-inf where the distance is masked) into its wave's LDS row, and the score accumulators start from
 // it.  Tiles with first tokens are masked by key instead.  The row sums take P before its rounding to
-// bf16, so that the log-sum-exp the backward rebuilds P from is exact to fp32.
+// bf16, so that the log-sum-exp the backward rebuilds P from is exact to fp32; P and Q K^T's operands are
+// the bf16 that the matrix instructions take (P's rounding, 2^-9 in the mean of a weight, is the
+// output's own).
+// Bound by VALU issue: a score takes some ten instructions and an exponential at a quarter of the rate,
+// four times its matrix instructions' time (8192 tokens, window 2048: the vector unit issues in 67% of
+// the busy cycles, the matrix unit in 22%), which puts the floor of this form at 2.5 times the
+// products'.  12 heads on 3 kv heads: 4096 tokens, window 1024 32 us (350 TFLOP/s of visible pairs; a
+// large library product 1190), 8192 and 2048 97 us (470); as chord_wide_kernel 113 and 349.  16 packed
+// sequences of 115 to 528 tokens 16 us in one launch (one by one 301).
 #include <algorithm>
 #include <string>
 

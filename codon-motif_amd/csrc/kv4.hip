@@ -9,10 +9,13 @@
 // keeps every input's range, and its rounding of base and scale (2^-9 of them) is small beside half a
 // step (1 / 30 of the range).  The quotient is an IEEE division, so that a value exactly between two
 // codes goes to the even one on every machine.  A group that holds an infinity or a NaN gets a NaN
-// scale: its values read back NaN, no other group's do.
+// scale: its values read back NaN, no other group's do.  So does one whose max - min passes fp32's
+// largest number.
 //
 // A lane takes 8 features (16 bytes of a 16-bit row, one 4-byte word of codes), a group 4 lanes (2 at
-// head dim 16): minimum and maximum by lane exchanges, no LDS.  Bound by the rows' bytes.
+// head dim 16): minimum and maximum by lane exchanges, no LDS.  Bound by the rows' bytes where there are
+// many, by the launch below some thousands: 192 rows 3.4 us to write and 2.8 to read, 24576 rows (8.3 MB
+// either way) 5.9 and 4.8 us, of which 2.5 are a launch's own.
 #include "capi_internal.h"
 #include "chord_internal.h"
 #include "common.h"

@@ -7,7 +7,8 @@ How a call is served:
   * decode over a StaticKVLayerCache (the graph-captured step): one projection
     GEMM, one kernel for the q / k RMSNorms and the append at the device cursor,
     the device-cursor attention kernel (which also advances the cursor), the gated
-    output projection -- no host value enters the launch sequence;
+    output projection -- no host value enters the launch sequence (over a
+    KV4LayerCache the rows are written in 4 bits and read as held);
   * other inference calls on bf16 / fp32 ROCm tensors with head_dim 64: the HIP
     kernels with host positions (apply_chord_attention);
   * calls that need gradients: the differentiable torch form (inside
@@ -16,6 +17,7 @@ How a call is served:
     (`embedding_start` as a tensor) or a shape the kernels do not serve (fp16,
     head_dim != 64): the explicit materialised-bias computation below, the
     reference's rule for leaving its kernel (chord_attn.py:295-298).
+`window` and `sinks` (new; MotifChordConfig's) limit what a query sees on every route.
 '''
 import warnings
 from typing import Optional, Union
@@ -81,7 +83,8 @@ def _f32(t: torch.Tensor) -> torch.Tensor:
 
 
 class ChordAttention(BasicAttention):
-    '''Softmax attention with the per-head gated geometric-decay (GGD) bias.'''
+    '''Softmax attention with the per-head gated geometric-decay (GGD) bias; with a `window`, over
+    the keys less than that many positions back and the first `sinks` tokens.'''
 
     def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: Optional[int] = None,
                  window: Optional[int] = None, sinks: int = 0, **kwargs):

@@ -17,6 +17,13 @@ forward kernel with its log-sum-exp, then the backward kernels (motif_chord_bwd:
 dv and the four per-head parameter gradients, the reference's custom backward
 :1348-1554).  Other gradient calls take the differentiable torch forms
 (motif/ops/autograd_path.py).
+
+Under a window (new: `window` / `sinks`, forward, packed, cursor and one-launch step; gradients
+through `ChordWindowFunction`) a query sees the keys less than `window` positions back and the
+first `sinks` tokens.  The kernels walk only the tiles that a block's windows and first tokens
+reach: bf16 at head dim 64 on kernels of its own for prefill, for decode (at most 16 query rows
+per kv head) and for the backward, every other type and head dim on the fp32-accumulating
+flash kernel.  `motif.ops.kv4` has the attention over a 4-bit cache.
 '''
 import functools
 import numbers

@@ -93,7 +93,8 @@ def kv4_append(slab: KV4Slab, k: torch.Tensor, v: torch.Tensor, start) -> None:
     '''Write the rows k, v [B, Hkv, n, D] (fp16, bf16 or fp32, any strides) at positions
     [start, start + n) of the slab.  `start` is an int, or a device int32 tensor of one
     entry that the kernel reads (for a captured step; rows past the capacity are then
-    dropped).  A group of features that holds an infinity or a NaN reads back as NaN.'''
+    dropped).  A group of features that holds an infinity or a NaN, or whose
+    range passes fp32's largest number, reads back as NaN.'''
     if wants_grad(k, v):
         raise RuntimeError('kv4_append is forward-only: detach the rows or call it under no_grad')
     (B, Hkv, cap, D), args = _check_slab(slab, 'kv4_append')

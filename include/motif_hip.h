@@ -2,7 +2,8 @@
  * motif_hip.h - C ABI of the MI355X (gfx950) kernels for Motif Chord's
  * sequence-mixing hot path: the Gated DeltaNet (GDN) delta rule (token
  * recurrence and chunked prefill), its short causal conv front end, and Chord
- * GGD-biased softmax attention (prefill and split-K decode).
+ * GGD-biased softmax attention (prefill and split-K decode; under a sliding window, and
+ * over a key / value cache held in 4 bits).
  *
  * Conventions
  *  - Every entry point is `extern "C"`, takes raw device pointers, element
@@ -13,7 +14,7 @@
  *  - Return value: MOTIF_OK (0) or a motif_status code; `motif_last_error()`
  *    returns a message for the last failure on the calling thread.
  *  - dtype codes: MOTIF_F32 = 0, MOTIF_BF16 = 1, MOTIF_F16 = 2 (fp16: the Chord attention
- *    entries only).
+ *    and 4-bit cache entries only).
  *  - Recurrent state is always fp32, row-major [.., dk, dv], contiguous.
  */
 #ifndef MOTIF_HIP_H
