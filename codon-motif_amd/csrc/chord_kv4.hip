@@ -15,13 +15,12 @@
 // the columns, copy u with zeros but for the tiles t of its own, so one accumulator holds the scores
 // of U tiles and every lane's softmax work is on scores of its own (4 a step at U = 4, where columns
 // of padding would make it 16).  The weights enter the second product masked the same way, and
-// the copies' outputs are added with the waves'.  The weights are rounded to bf16 with the value's scale
+// the copies' outputs are added in the wave, the waves' through LDS.  The weights are rounded to bf16 with the value's scale
 // (fp16: to two bf16, 17 bits, as fp16's range would not hold the product).
-// Bound by VALU issue (codes to operands 112 of some 420 instructions a step, the bias's logarithm and
-// exponential and the softmax's at a quarter of the rate; the vector unit issues in 73% of the busy
-// cycles): 64 sequences of 4097 keys, 12 heads on 3, 63 MB of cache in 21 us (3.0 TB/s); the bf16 rows
-// of the same cache are 201 MB, 40 us.  One sequence of 300 keys 8 us; 32 x 2 fp16 rows, window 4000 of 8190
-// keys, 18.5 us and a merge of 4.  Without the matrix instructions (chord_wide_kernel) 592 us.
+// Bound by VALU issue (codes to operands 112 of some 280 instructions a step, the bias's logarithm and
+// exponential and the softmax's at a quarter of the rate): 64 sequences of 4097 keys, 12 heads on 3, 63 MB
+// of cache in 18.8 us (3.3 TB/s); the bf16 rows of the same cache are 201 MB, 40 us.  One sequence of 300
+// keys 6.5 us; 32 x 2 fp16 rows, window 4000 of 8190 keys, 19.7 us with the merge.  Without the matrix instructions (chord_wide_kernel) 592 us.
 #include <algorithm>
 #include <string>
 
@@ -43,15 +42,22 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pk2bf(float x0, float x1) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2v){x0, x1}, bf16x2v));
 }
-// 8 codes to an MFMA operand: pairs (n0, n4), (n1, n5), (n2, n6), (n3, n7), bf16 128 + n
-__device__ __forceinline__ uint4 codes_bf16(uint32_t w) {
-  constexpr uint32_t m = 0x000f000fu, b = 0x43004300u;
+// The mask of a pair of codes, in a register: as a constant it and the bits or'ed in are two literals, which
+// take two instructions where v_and_or_b32 takes one (64 of 340 vector instructions of a step).
+__device__ __forceinline__ uint32_t pair_mask() {
+  uint32_t m = 0x000f000fu;
+  asm("" : "+v"(m));
+  return m;
+}
+// 8 codes to an MFMA operand: pairs (n0, n4), (n1, n5), (n2, n6), (n3, n7), bf16 128 + n (m: pair_mask())
+__device__ __forceinline__ uint4 codes_bf16(uint32_t w, uint32_t m) {
+  constexpr uint32_t b = 0x43004300u;
   return uint4{(w & m) | b, ((w >> 4) & m) | b, ((w >> 8) & m) | b, ((w >> 12) & m) | b};
 }
 // the same as fp16 n (1024 + n less 1024)
-__device__ __forceinline__ uint4 codes_f16(uint32_t w) {
-  auto one = [](uint32_t x) {
-    const f16x2 v = __builtin_bit_cast(f16x2, (x & 0x000f000fu) | 0x64006400u) - f16x2{1024, 1024};
+__device__ __forceinline__ uint4 codes_f16(uint32_t w, uint32_t m) {
+  auto one = [m](uint32_t x) {
+    const f16x2 v = __builtin_bit_cast(f16x2, (x & m) | 0x64006400u) - f16x2{1024, 1024};
     return __builtin_bit_cast(uint32_t, v);
   };
   return uint4{one(w), one(w >> 4), one(w >> 8), one(w >> 12)};
@@ -65,6 +71,19 @@ __device__ __forceinline__ float max_g(float x) {  // over the four lane groups 
 __device__ __forceinline__ float sum_g(float x) {
   x += __shfl_xor(x, 32, 64);
   return x + __shfl_xor(x, 16, 64);
+}
+
+// over the U columns c % (16 / U) of 16 lanes
+template <int N> __device__ __forceinline__ float row_ror(float x) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x120 + N, 0xf, 0xf, false));
+}
+template <int U> __device__ __forceinline__ float sum_copies(float x) {
+  x += row_ror<8>(x);
+  return U == 4 ? x + row_ror<4>(x) : x;
+}
+template <int U> __device__ __forceinline__ float max_copies(float x) {
+  x = fmaxf(x, row_ror<8>(x));
+  return U == 4 ? fmaxf(x, row_ror<4>(x)) : x;
 }
 
 template <typename T, int U, int NW>  // NW: waves of a workgroup
@@ -125,7 +144,7 @@ __global__ void __launch_bounds__(64 * NW) chord_kv4_kernel(ChordArgs a, KV4Args
 
   // per wave: codes of 64 keys and values (2 KB each) and their pairs (512 bytes each, written as 1 KB)
   constexpr int kWave = 2 * 2048 + 2 * 1024;
-  constexpr int kMerge = NW * 16 * (kD + 1) * 4 + NW * 16 * 4 * 4;
+  constexpr int kRow = kD + 4, kMerge = NW * RC * (kRow + 4) * 4;
   __shared__ __attribute__((aligned(16))) uint8_t smem[NW * kWave > kMerge ? NW * kWave : kMerge];
   uint8_t *sk = smem + w * kWave, *sv = sk + 2048, *skp = sv + 2048, *svp = skp + 1024;
   const uint8_t *kc = kv.kc + b * kv.kc_sb + kvh * kv.kc_sh, *vc = kv.vc + b * kv.vc_sb + kvh * kv.vc_sh;
@@ -162,6 +181,7 @@ __global__ void __launch_bounds__(64 * NW) chord_kv4_kernel(ChordArgs a, KV4Args
     return __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) i32x2 *)p);
   };
 
+  const uint32_t nib = pair_mask();
   float m = -INFINITY, l = 0.f, ob[2] = {0.f, 0.f};
   f32x4 o[4];
 #pragma unroll
@@ -205,10 +225,10 @@ __global__ void __launch_bounds__(64 * NW) chord_kv4_kernel(ChordArgs a, KV4Args
 #pragma unroll
         for (int v = 0; v < U; ++v) {
           if constexpr (kBf)
-            acc[tt][p] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, codes_bf16(kw[v * TPL + tt][p])),
+            acc[tt][p] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, codes_bf16(kw[v * TPL + tt][p], nib)),
                                                                  __builtin_bit_cast(bf16x8, qm[v][p]), acc[tt][p], 0, 0, 0);
           else
-            acc[tt][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, codes_f16(kw[v * TPL + tt][p])),
+            acc[tt][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, codes_f16(kw[v * TPL + tt][p], nib)),
                                                                 __builtin_bit_cast(f16x8, qm[v][p]), acc[tt][p], 0, 0, 0);
         }
       }
@@ -260,7 +280,7 @@ __global__ void __launch_bounds__(64 * NW) chord_kv4_kernel(ChordArgs a, KV4Args
 #pragma unroll
     for (int ft = 0; ft < 4; ++ft)
 #pragma unroll
-      for (int t2 = 0; t2 < 2; ++t2) vA[ft][t2] = codes_bf16(static_cast<uint32_t>(t2 ? vw[ft].y : vw[ft].x));
+      for (int t2 = 0; t2 < 2; ++t2) vA[ft][t2] = codes_bf16(static_cast<uint32_t>(t2 ? vw[ft].y : vw[ft].x), nib);
 #pragma unroll
     for (int gr = 0; gr < 2; ++gr) {
       float ps[NK];
@@ -308,28 +328,39 @@ __global__ void __launch_bounds__(64 * NW) chord_kv4_kernel(ChordArgs a, KV4Args
   l = sum_g(l);
   ob[0] = sum_g(ob[0]);
   ob[1] = sum_g(ob[1]);
+  if constexpr (U > 1) {  // the copies of a row, columns RC apart, to one
+    const float M = max_copies<U>(m), f = m == -INFINITY ? 0.f : fast_exp2(m - M);
+    l = sum_copies<U>(l * f);
+    ob[0] = sum_copies<U>(ob[0] * f);
+    ob[1] = sum_copies<U>(ob[1] * f);
+#pragma unroll
+    for (int ft = 0; ft < 4; ++ft)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[ft][i] = sum_copies<U>(o[ft][i] * f);
+    m = M;
+  }
   __syncthreads();  // every wave's staged rows are read
-  float *so = reinterpret_cast<float *>(smem), *sm = so + NW * 16 * (kD + 1);  // [wave][column][feature], [wave][column][m, l, ..]
-  if (g == 0) *reinterpret_cast<f32x4 *>(sm + 4 * (16 * w + c16)) = f32x4{m, l, ob[0], ob[1]};
+  float *so = reinterpret_cast<float *>(smem), *sm = so + NW * RC * kRow;  // [wave][row][feature], [wave][row][m, l, ..]
+  if (u == 0) {
+    if (g == 0) *reinterpret_cast<f32x4 *>(sm + 4 * (RC * w + r)) = f32x4{m, l, ob[0], ob[1]};
 #pragma unroll
-  for (int ft = 0; ft < 4; ++ft)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) so[(16 * w + c16) * (kD + 1) + 16 * ft + 4 * g + i] = o[ft][i];
+    for (int ft = 0; ft < 4; ++ft) *reinterpret_cast<f32x4 *>(so + (RC * w + r) * kRow + 16 * ft + 4 * g) = o[ft];
+  }
   __syncthreads();
   for (int e = tid; e < RC * kD; e += 64 * NW) {
     const int rr = e / kD, d = e % kD;
     if (rr >= rows) continue;
     float M = -INFINITY;
 #pragma unroll
-    for (int c = 0; c < NW * U; ++c) M = fmaxf(M, sm[4 * (16 * (c / U) + (c % U) * RC + rr)]);
+    for (int c = 0; c < NW; ++c) M = fmaxf(M, sm[4 * (RC * c + rr)]);
     const float Mu = M == -INFINITY ? 0.f : M;
     float ov = 0.f, Ls = 0.f;
 #pragma unroll
-    for (int c = 0; c < NW * U; ++c) {
-      const int col = 16 * (c / U) + (c % U) * RC + rr;
-      const float f = fast_exp2(sm[4 * col] - Mu);
-      ov = fmaf(so[col * (kD + 1) + d] + sm[4 * col + 2 + d / 32], f, ov);
-      Ls = fmaf(sm[4 * col + 1], f, Ls);
+    for (int c = 0; c < NW; ++c) {
+      const f32x4 st4 = *reinterpret_cast<const f32x4 *>(sm + 4 * (RC * c + rr));
+      const float f = fast_exp2(st4[0] - Mu);
+      ov = fmaf(so[(RC * c + rr) * kRow + d] + (d < 32 ? st4[2] : st4[3]), f, ov);
+      Ls = fmaf(st4[1], f, Ls);
     }
     if (a.part) {
       float *pp = a.part + (((static_cast<size_t>(b) * a.Hkv + kvh) * a.splits + split) * rows + rr) * (kD + 2);
@@ -366,8 +397,8 @@ bool chord_kv4_serves(int H, int Hkv, int L, int D, int dtype) {
   return D == kD && (dtype == MOTIF_BF16 || dtype == MOTIF_F16) && (H / Hkv) * static_cast<int64_t>(L) <= 16;
 }
 
-// Key ranges of a call, 1: one workgroup of up to 12 waves per kv head and nothing to merge.  Measured, us,
-// 4 query heads per kv head, one token, unsplit / 4 / 8 ranges (and their merge): 3 kv heads (one sequence)
+// Key ranges of a call, 1: one workgroup of up to 12 waves per kv head and nothing to merge.  Measured (a
+// tenth more than they take now), us, 4 query heads per kv head, one token, unsplit / 4 / 8 ranges (and their merge): 3 kv heads (one sequence)
 // over 1000 keys 9.4 / 8.7 / 8.9, 2000 12.2 / 10.2 / 10.6, 4097 19.4 / 13.7 / 12.8, 8000 31.5 / 17.6 / 14.3;
 // 48 (16 sequences) 4097 19.9 / 14.7 / 16.0, 8000 31.7 / 19.0 / 18.8; 96 4097 20.1 / 17.8 / 18.5, 8000
 // 32.6 / 24.3 / 23.1; 192 (64 sequences) 2000 13.4 / 15.3 / 21.7, 4097 21.4 / 22.2 / 29.1, 8000 34.4 /
