@@ -59,6 +59,36 @@ const char *kv4_check(const KV4Args &kv, int D);  // what is wrong with a cache'
 __device__ __forceinline__ float kv4_scale(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float kv4_base(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
+// A lane's N features of a row, LPG lanes to a group: their codes (4 bits each from the lowest on) and the
+// group's pair.  Every lane of the group calls it.
+template <int N, int LPG> __device__ __forceinline__ uint32_t kv4_codes(const float (&x)[N], uint32_t &pair) {
+  float lo = x[0], hi = x[0], bad = x[0] * 0.f;
+#pragma unroll
+  for (int e = 1; e < N; ++e) {
+    lo = fminf(lo, x[e]);
+    hi = fmaxf(hi, x[e]);
+    bad = fmaf(x[e], 0.f, bad);  // NaN once any feature is not finite
+  }
+#pragma unroll
+  for (int off = 1; off < LPG; off <<= 1) {
+    lo = fminf(lo, __shfl_xor(lo, off, 64));
+    hi = fmaxf(hi, __shfl_xor(hi, off, 64));
+    bad += __shfl_xor(bad, off, 64);
+  }
+  const bf16_t sb = f32_to_bf16((hi - lo) * (1.f / 15.f) + bad), bb = f32_to_bf16(lo);
+  const float scale = bf16_to_f32(sb), base = bf16_to_f32(bb);
+  pair = sb | (static_cast<uint32_t>(bb) << 16);
+  uint32_t w = 0;
+  if (scale > 0.f && scale < INFINITY) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float c = fminf(fmaxf(rintf(__fdiv_rn(x[e] - base, scale)), 0.f), 15.f);
+      w |= static_cast<uint32_t>(c) << (4 * e);
+    }
+  }
+  return w;
+}
+
 // The tiles of TS keys that queries at positions [first, ..], whose last key is end - 1, meet under a
 // window: those of the first tokens, then those from the lowest key in a window on.  No tile holds a
 // row that none of these queries sees (first tokens end at `se`, windows start at `lo`): what lies

@@ -87,34 +87,13 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(RowsArgs a) {
   float x[8];
   load8(src + 8 * sub, x);
   const int pos = (a.len_dev ? *a.len_dev : a.pos) + t;
-  float lo = x[0], hi = x[0], bad = x[0] * 0.f;
-#pragma unroll
-  for (int e = 1; e < 8; ++e) {
-    lo = fminf(lo, x[e]);
-    hi = fmaxf(hi, x[e]);
-    bad = fmaf(x[e], 0.f, bad);  // NaN once any feature is not finite
-  }
-#pragma unroll
-  for (int off = 1; off < LPG; off <<= 1) {
-    lo = fminf(lo, __shfl_xor(lo, off, 64));
-    hi = fmaxf(hi, __shfl_xor(hi, off, 64));
-    bad += __shfl_xor(bad, off, 64);
-  }
+  uint32_t pair;
+  const uint32_t w = kv4_codes<8, LPG>(x, pair);
   if (!valid || pos < 0 || pos >= a.capacity) return;  // (never outside the slab)
-  const bf16_t sb = f32_to_bf16((hi - lo) * (1.f / 15.f) + bad), bb = f32_to_bf16(lo);
-  const float scale = bf16_to_f32(sb), base = bf16_to_f32(bb);
-  uint32_t w = 0;
-  if (scale > 0.f && scale < INFINITY) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float c = fminf(fmaxf(rintf(__fdiv_rn(x[e] - base, scale)), 0.f), 15.f);
-      w |= static_cast<uint32_t>(c) << (4 * e);
-    }
-  }
   uint8_t *codes = const_cast<uint8_t *>(is_v ? a.kv.vc + b * a.kv.vc_sb + h * a.kv.vc_sh : a.kv.kc + b * a.kv.kc_sb + h * a.kv.kc_sh);
   uint32_t *pairs = const_cast<uint32_t *>(is_v ? a.kv.vp + b * a.kv.vp_sb + h * a.kv.vp_sh : a.kv.kp + b * a.kv.kp_sb + h * a.kv.kp_sh);
   *reinterpret_cast<uint32_t *>(codes + int64_t(pos) * (D / 2) + 4 * sub) = w;
-  if (sub % LPG == 0) pairs[int64_t(pos) * G + sub / LPG] = sb | (static_cast<uint32_t>(bb) << 16);
+  if (sub % LPG == 0) pairs[int64_t(pos) * G + sub / LPG] = pair;
 }
 
 template <typename T, int D>

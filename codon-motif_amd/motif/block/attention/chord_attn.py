@@ -34,7 +34,7 @@ from motif.ops.autograd_path import wants_grad
 from motif.ops.chord_attention import (HEAD_DIMS, check_window, chord_decode_cursor, chord_decode_step,
                                        chord_decode_step_serves, chord_decode_step_workspace, chord_decode_workspace,
                                        chord_window_workspace, serves_head_dim)
-from motif.ops.kv4 import chord_decode_kv4_cursor, chord_decode_kv4_workspace, kv4_append
+from motif.ops.kv4 import chord_decode_kv4_cursor, chord_decode_kv4_workspace, chord_kv4_prep
 from motif.ops.epilogue import mul_sigmoid, usable
 from motif.ops.linear_rows import cat_weights, linear_rows, project, rows_eligible
 
@@ -390,11 +390,10 @@ class ChordAttention(BasicAttention):
         '''The attention of a cursor step over a 4-bit cache: norms, the rows into the cache at
         the device cursor, attention and the cursor's advance.'''
         B, L = proj.shape[0], proj.shape[1]
-        q = torch.empty(B, self.num_heads, L, self.head_dim, dtype=proj.dtype, device=proj.device)
-        k = torch.empty(B, self.num_kv_heads, L, self.head_dim, dtype=proj.dtype, device=proj.device)
-        v = torch.empty_like(k)
-        self._prep(proj, q, k, v, None, 0, L)
-        kv4_append(cache.slab, k, v, cache.length_dev)
+        hs, dt = self.hidden_size, proj.dtype
+        q = chord_kv4_prep(proj, (0, hs, hs + self.kv_dim), self.q_norm.weight.to(dt).contiguous(),
+                           self.k_norm.weight.to(dt).contiguous(), self.q_norm.eps, cache.slab, cache.length_dev,
+                           self.num_heads)
         work = cache.workspace(('kv4', L, self.window, self.sinks), lambda: chord_decode_kv4_workspace(
             B, self.num_heads, self.num_kv_heads, L, cache.capacity, self.head_dim, proj.dtype, proj.device, self.window,
             self.sinks))

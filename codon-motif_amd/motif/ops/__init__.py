@@ -8,8 +8,8 @@ from . import _lib
 from .rms_norm import RMSNorm, GatedRMSNorm
 from .swiglu import SwiGLU
 from .chord_attention import apply_chord_attention, apply_chord_attention_varlen
-from .kv4 import (KV4Slab, chord_attention_kv4, chord_decode_kv4_cursor, chord_decode_kv4_workspace, kv4_alloc,
-                  kv4_append, kv4_read)
+from .kv4 import (KV4Slab, chord_attention_kv4, chord_decode_kv4_cursor, chord_decode_kv4_workspace, chord_kv4_prep,
+                  kv4_alloc, kv4_append, kv4_read)
 from .gated_deltanet import (
     recurrent_gated_delta_rule,
     chunk_gated_delta_rule,
@@ -30,7 +30,7 @@ __all__ = [
     'RMSNorm', 'GatedRMSNorm', 'SwiGLU',
     'apply_chord_attention', 'apply_chord_attention_varlen',
     'KV4Slab', 'kv4_alloc', 'kv4_append', 'kv4_read', 'chord_attention_kv4', 'chord_decode_kv4_cursor',
-    'chord_decode_kv4_workspace',
+    'chord_decode_kv4_workspace', 'chord_kv4_prep',
     'recurrent_gated_delta_rule', 'chunk_gated_delta_rule',
     'chunk_gated_delta_rule_triton', 'chunk_gated_delta_rule_varlen', 'chunk_gated_delta_rule_gated_norm',
     'gdn_prefill_fused',

@@ -95,6 +95,8 @@ _SIGNATURES = {
     'motif_chord_window_bwd': (
         _T4 * 5 + [_P] * 5 + [_P, _I64, _I64] + _T4 * 3 + [_P] + [_I32] * 7 + [_F32, _F32]
         + [_I32, _I32, _I32, _P, _I32, _P, _SZ, _I32, _P], _I32),
+    'motif_chord_kv4_prep': (
+        [_P, _I64, _I64, _I32, _I32, _I32, _P, _P, _F32] + _T4 + [_P, _I64, _I64] * 4 + [_P] + [_I32] * 7 + [_P], _I32),
     'motif_kv4_append': (_T4 * 2 + [_P, _I64, _I64] * 4 + [_P] + [_I32] * 7 + [_P], _I32),
     'motif_kv4_read': ([_P, _I64, _I64] * 4 + _T4 * 2 + [_I32] * 7 + [_P], _I32),
     'motif_chord_kv4_workspace_bytes': ([_I32] * 9, _SZ),

@@ -9,7 +9,8 @@ For every (batch row, kv head, position), keys and values alike, a `KV4Slab` hol
           min(32, D) features; a feature's value is code * scale + base.
 
 `kv4_append` writes rows (base = bf16(min), scale = bf16((max - min) / 15), the code
-nearest to (x - base) / scale, ties to even), `kv4_read` gives the values back, and
+nearest to (x - base) / scale, ties to even), `kv4_read` gives the values back,
+`chord_kv4_prep` writes a decode step's rows straight from its projections, and
 `chord_attention_kv4` / `chord_decode_kv4_cursor` attend over the cache without
 expanding it in memory: 40 bytes a row at head dim 64 where bf16 takes 128.  All of them
 are forward-only: calls that would need a gradient raise.
@@ -141,6 +142,42 @@ def kv4_read(slab: KV4Slab, start: int, n: int, dtype: torch.dtype = torch.bfloa
         if rc:
             _lib.check(rc, 'motif_kv4_read')
     return k, v
+
+
+def chord_kv4_prep(proj: torch.Tensor, offsets, q_norm_weight: torch.Tensor, k_norm_weight: torch.Tensor, norm_eps: float,
+                   slab: KV4Slab, length_dev: torch.Tensor, num_heads: int) -> torch.Tensor:
+    '''The input side of a Chord decode step over a 4-bit cache in one launch: from the fused
+    projection rows proj [B, L, ncols] (bf16 or fp32; q, k, v from column offsets[i]), q [B, H, L, D]
+    normalised, and the normalised keys and the values written in 4 bits at positions length_dev ..
+    (a device int32, read and not advanced; rows past the capacity are dropped).  The same bits as the
+    norms followed by kv4_append.'''
+    (B, Hkv, cap, D), args = _check_slab(slab, 'chord_kv4_prep')
+    if wants_grad(proj, q_norm_weight, k_norm_weight):
+        raise RuntimeError('chord_kv4_prep is forward-only: call it under no_grad')
+    if proj.dim() != 3 or proj.shape[0] != B or proj.stride(-1) != 1 or proj.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f'chord_kv4_prep: proj must be bf16 or fp32 [{B}, L, columns], got {tuple(proj.shape)} {proj.dtype}')
+    offsets = [int(o) for o in offsets]
+    if num_heads < 1 or num_heads % Hkv or len(offsets) != 3 or min(offsets) < 0 \
+            or max(offsets[0] + num_heads * D, max(offsets[1:]) + Hkv * D) > proj.shape[2]:
+        raise ValueError(f'chord_kv4_prep: {num_heads} heads of {D} over {Hkv} kv heads do not fit the columns {offsets}')
+    for t in (q_norm_weight, k_norm_weight):
+        if t.shape != (D,) or t.dtype != proj.dtype or not t.is_contiguous() or t.device != proj.device:
+            raise ValueError(f'chord_kv4_prep: norm weights must be contiguous [{D}] in proj\'s dtype and on its device')
+    if slab.k_codes.device != proj.device:
+        raise ValueError('chord_kv4_prep: proj and the cache must live on one device')
+    if length_dev.dtype != torch.int32 or length_dev.device != proj.device or length_dev.numel() != 1:
+        raise ValueError('chord_kv4_prep: length_dev must be one int32 on proj\'s device')
+    _need_backend()
+    q = torch.empty(B, num_heads, proj.shape[1], D, dtype=proj.dtype, device=proj.device)
+    if q.numel() == 0:
+        return q
+    with _lib.on_device(proj.device):
+        rc = _lib.lib().motif_chord_kv4_prep(
+            proj.data_ptr(), proj.stride(0), proj.stride(1), *offsets, q_norm_weight.data_ptr(), k_norm_weight.data_ptr(),
+            float(norm_eps), *_lib.t4(q), *args, length_dev.data_ptr(), cap, B, proj.shape[1], num_heads, Hkv, D,
+            _lib.dtype_code(proj.dtype), _lib.stream_ptr(proj.device))
+    _lib.check(rc, 'motif_chord_kv4_prep')
+    return q
 
 
 def _check_query(q, slab, params, what):

@@ -460,7 +460,7 @@ int motif_chord_decode_step(
  *   pos < 0:  the position is read from the device cursor *length_dev (left as is:
  *             motif_chord_decode advances it); cache rows at or past `capacity` are
  *             not written.
- * All row starts 16-byte aligned; D * sizeof(T) in {64, 128, 256, 512} bytes.
+ * All row starts 16-byte aligned; D * sizeof(T) in {32 (bf16), 64, 128, 256, 512} bytes.
  */
 int motif_chord_qkv_prep(const void *proj, int64_t p_sb, int64_t p_st, int q_off, int k_off, int v_off,
                          const void *q_norm_weight, const void *k_norm_weight, float eps,
@@ -578,6 +578,20 @@ int motif_kv4_read(const void *k_codes, int64_t kc_sb, int64_t kc_sh, const void
                    const void *v_codes, int64_t vc_sb, int64_t vc_sh, const void *v_params, int64_t vp_sb, int64_t vp_sh,
                    void *k, int64_t k_sb, int64_t k_sh, int64_t k_st, void *v, int64_t v_sb, int64_t v_sh, int64_t v_st,
                    int position, int capacity, int B, int n, int Hkv, int D, int dtype, void *stream);
+
+/*
+ * motif_chord_qkv_prep for a 4-bit cache at the device cursor: q as there, the normalised keys and
+ * the values (rounded to the dtype, bf16 or fp32) into the cache's rows *position_dev + t (read, not
+ * advanced; rows at or past `capacity` are dropped): the bits of motif_chord_qkv_prep into
+ * plain tensors followed by motif_kv4_append.
+ */
+int motif_chord_kv4_prep(const void *proj, int64_t p_sb, int64_t p_st, int q_off, int k_off, int v_off,
+                         const void *q_norm_weight, const void *k_norm_weight, float eps,
+                         void *q, int64_t q_sb, int64_t q_sh, int64_t q_st,
+                         void *k_codes, int64_t kc_sb, int64_t kc_sh, void *k_params, int64_t kp_sb, int64_t kp_sh,
+                         void *v_codes, int64_t vc_sb, int64_t vc_sh, void *v_params, int64_t vp_sb, int64_t vp_sh,
+                         const int *position_dev, int capacity, int B, int L, int H, int Hkv, int D, int dtype,
+                         void *stream);
 
 /*
  * Chord attention over a 4-bit cache: motif_chord_window_fwd's formula and arguments with the

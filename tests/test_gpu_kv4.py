@@ -271,3 +271,71 @@ def test_captured_steps_replay(dtype):
     assert int(cur) == int(cur_e) == 40
     for a, b in zip(slab, eager):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('dtype,D', [(BF, 16), (BF, 32), (BF, 64), (BF, 128), (F32, 16), (F32, 32), (F32, 64), (F32, 128)])
+@pytest.mark.parametrize('B,L,H,Hkv,start', [(1, 1, 4, 1, 0), (3, 2, 6, 3, 17), (2, 5, 2, 2, 29)])
+@torch.no_grad()
+def test_prep_equals_norms_then_append(dtype, D, B, L, H, Hkv, start):
+    '''The bits of the input kernel into plain rows followed by kv4_append; the last size's rows 32 .. pass
+    the capacity and are dropped.'''
+    from motif.block.attention.chord_attn import ChordAttention
+    from motif.ops import chord_kv4_prep, kv4_alloc, kv4_append
+    cap = 32
+    layer = ChordAttention(hidden_size=H * D, num_heads=H, num_kv_heads=Hkv).to(DEV, dtype)
+    g = torch.Generator().manual_seed(D + B)
+    layer.q_norm.weight.copy_(1 + 0.2 * torch.randn(D, generator=g))
+    layer.k_norm.weight.copy_(1 + 0.2 * torch.randn(D, generator=g))
+    wide = torch.randn(B, L, (2 * H + 2 * Hkv) * D + 16, generator=g).to(DEV, dtype)
+    wide[0, 0, H * D + 3] = float('inf') if B == 3 else 4.0
+    proj = wide[..., :-16]
+    ld = torch.tensor([start], dtype=torch.int32, device=DEV)
+    slab, want = kv4_alloc(B, Hkv, cap, D, DEV), kv4_alloc(B, Hkv, cap, D, DEV)
+    q = chord_kv4_prep(proj, (0, H * D, (H + Hkv) * D), layer.q_norm.weight, layer.k_norm.weight, layer.q_norm.eps,
+                       slab, ld, H)
+    qw = torch.empty_like(q)
+    k, v = (torch.empty(B, Hkv, L, D, dtype=dtype, device=DEV) for _ in range(2))
+    layer._prep(proj, qw, k, v, None, 0, L)
+    kv4_append(want, k, v, ld)
+    assert torch.equal(q, qw) and int(ld) == start
+    for a, b in zip(slab, want):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@torch.no_grad()
+def test_layer_of_head_dim_16_decodes():
+    from motif.block.attention.chord_attn import ChordAttention
+    from motif.model.cache import KV4LayerCache, StaticKVLayerCache
+    torch.manual_seed(0)
+    layer = ChordAttention(hidden_size=64, num_heads=4, num_kv_heads=2).to(DEV, BF).eval()
+    x = torch.randn(2, 20, 64, generator=torch.Generator().manual_seed(1)).to(DEV, BF)
+    for kind in (StaticKVLayerCache, KV4LayerCache):
+        cache = kind().allocate(2, 2, 32, 16, DEV, BF)
+        first = layer(x[:, :16], past_key_value=cache).output
+        steps = [layer(x[:, i:i + 1], past_key_value=cache).output for i in range(16, 20)]
+        assert int(cache.length_dev) == cache.length == 20
+        whole = layer(x).output
+        assert (first - whole[:, :16]).abs().max() < 2e-2
+        if kind is StaticKVLayerCache:
+            assert (torch.cat(steps, 1) - whole[:, 16:]).abs().max() < 2e-2
+
+
+@torch.no_grad()
+def test_prep_refusals():
+    from motif.ops import chord_kv4_prep, kv4_alloc
+    slab = kv4_alloc(2, 2, 16, 64, DEV)
+    proj, w = torch.zeros(2, 1, 512, dtype=BF, device=DEV), torch.ones(64, dtype=BF, device=DEV)
+    ld = torch.zeros(1, dtype=torch.int32, device=DEV)
+    ok = dict(proj=proj, offsets=(0, 256, 384), q_norm_weight=w, k_norm_weight=w, norm_eps=1e-5, slab=slab, length_dev=ld,
+              num_heads=4)
+    assert chord_kv4_prep(**ok).shape == (2, 4, 1, 64)
+    for bad in (dict(proj=proj[:1]), dict(proj=proj.half()), dict(proj=proj[0]), dict(offsets=(0, 256, 448)),
+                dict(offsets=(0, 256)), dict(offsets=(-64, 256, 384)), dict(num_heads=3), dict(num_heads=10),
+                dict(q_norm_weight=w[:32]), dict(k_norm_weight=w.float()), dict(length_dev=ld.long()),
+                dict(length_dev=ld.cpu()), dict(length_dev=torch.zeros(2, dtype=torch.int32, device=DEV)),
+                dict(proj=proj.transpose(0, 2).contiguous().transpose(0, 2))):
+        with pytest.raises(ValueError, match='chord_kv4_prep'):
+            chord_kv4_prep(**{**ok, **bad})
+    odd = torch.zeros(2, 1, 516, dtype=BF, device=DEV)[..., 1:513]
+    with pytest.raises(NotImplementedError, match='aligned'):
+        chord_kv4_prep(**{**ok, 'proj': odd})

@@ -84,3 +84,10 @@ def test_gradients_are_refused():
     p = torch.zeros(4)
     with pytest.raises(RuntimeError, match='forward-only'):
         chord_attention_kv4(torch.zeros(1, 4, 1, 64, requires_grad=True), s, p, p, p, p, torch.zeros(1, 1), 4)
+
+
+def test_prep_into_a_slab_refuses_on_the_host():
+    from motif.ops import chord_kv4_prep
+    s, w = _cpu_slab(), torch.ones(64)
+    with pytest.raises(ValueError, match='CUDA'):
+        chord_kv4_prep(torch.zeros(1, 1, 512), (0, 256, 384), w, w, 1e-5, s, torch.zeros(1, dtype=torch.int32), 4)
