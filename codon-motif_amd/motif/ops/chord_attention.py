@@ -151,6 +151,8 @@ class ChordWindowFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout):
+        if torch.is_grad_enabled():  # (create_graph: what the kernels give carries no graph)
+            raise RuntimeError('windowed Chord attention has no second derivatives')
         q, k, v, out, alpha, beta, mu, ssmax, log_n, stats = ctx.saved_tensors
         q_start, scale, eps, window, sinks, rows, n = ctx.args
         needs = ctx.needs_input_grad
@@ -449,6 +451,8 @@ def apply_chord_attention(
             qs = k.shape[2] - q.shape[2] if q_start is None else int(q_start)
             if qs < 0:
                 raise ValueError(f'q_start must not be negative, got {qs}')
+            if sinks >= k.shape[2]:  # every key is a first token: no window (whose backward holds less)
+                window, sinks = NO_WINDOW, 0
             res = ChordWindowFunction.apply(q, k, v, alpha, beta, mu, ssmax, log_n, qs, scale, float(eps), window, sinks)
         elif window is not None:
             res = chord_attention_torch(q, k, v, alpha, beta, mu, ssmax, log_n, q_start, softmax_scale, eps, window, sinks)

@@ -234,3 +234,34 @@ def test_captured_and_on_another_stream():
                 dst.copy_(src)
             graph.replay()
             assert torch.equal(got, apply_chord_attention(*args, window=window, sinks=sinks))
+
+
+@pytest.mark.parametrize('dtype', [BF, F16, F32], ids=['bf16', 'fp16', 'fp32'])
+@pytest.mark.parametrize('L', [1, 3, 90])
+@pytest.mark.parametrize('scale', [0.125, -0.125, 0.0])
+@torch.no_grad()
+def test_parameters_at_their_edges(dtype, L, scale):
+    '''Heads with ssmax zero and negative, alpha zero and negative, beta zero and negative, mu on a key, and
+    scales of either sign and zero.'''
+    H, Hkv, S, window, sinks = 8, 2, 140, 45, 3
+    q, k, v, par = inputs(2, H, Hkv, L, S, 64, dtype, seed=L)
+    al, be, mu, ss = (t.clone() for t in par)
+    ss[0], ss[1], ss[7] = 0.0, -ss[1], -ss[7]
+    al[2], al[3] = 0.0, -al[3]
+    be[4], be[5] = 0.0, -0.3
+    mu[6], mu[7] = 0.0, -7.0
+    par = (al, be, mu, ss)
+    log_n = log_n_of(2, L, S - L)
+    got = _run(q, k, v, par, log_n, window=window, sinks=sinks, softmax_scale=scale)
+    check_attention(got, q, k, v, par, log_n, S - L, window, sinks, scale=scale)
+
+
+@pytest.mark.parametrize('B', [1, 40])
+@torch.no_grad()
+def test_split_decode_of_rows_that_see_nothing(B):
+    '''A window that ends past the keys, long enough to be split over workgroups: zeros.'''
+    q, k, v, par = inputs(B, 4, 2, 2, 2000, 64, BF, seed=2)
+    log_n = log_n_of(B, 2, 5000)
+    assert not _run(q, k, v, par, log_n, q_start=5000, window=2000).any()
+    got = _run(q, k, v, par, log_n, q_start=5000, window=2000, sinks=2)
+    check_attention(got, q, k, v, par, log_n, 5000, 2000, 2)

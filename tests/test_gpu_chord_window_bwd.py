@@ -239,3 +239,38 @@ def test_training_step_in_a_graph():
         for a, b in zip(got, want):
             assert torch.equal(a, b)
 
+
+
+def test_parameters_at_their_edges():
+    '''Heads with ssmax zero and negative, alpha zero and negative, beta zero and negative, mu on a key.'''
+    H, Hkv, L, window, sinks = 8, 4, 150, 45, 3
+    q, k, v, par = inputs(1, H, Hkv, L, L, 64, BF, seed=6)
+    al, be, mu, ss = (t.clone() for t in par)
+    ss[0], ss[1] = 0.0, -ss[1]
+    al[2], al[3] = 0.0, -al[3]
+    be[4], be[5] = 0.0, -0.3
+    mu[6], mu[7] = 0.0, -7.0
+    par = (al, be, mu, ss)
+    log_n = log_n_of(1, L, 0)
+    do = torch.randn(1, H, L, 64, generator=gen(1)).to(BF)
+    _, got = _grads(q, k, v, par, log_n, do, 0, window, sinks)
+    want, lims = formula64(q, k, v, par, log_n, do, 0, window, sinks)
+    for n, a, b, lim in zip(('dq', 'dk', 'dv', 'dalpha', 'dbeta', 'dmu', 'dssmax'), got, want, lims):
+        assert ((a.cpu().double() - b).abs() <= lim).all(), n
+
+
+def test_every_token_a_first_token():
+    q, k, v, par = inputs(1, 4, 2, 200, 200, 64, BF, seed=3)
+    log_n, do = log_n_of(1, 200, 0), torch.randn(1, 4, 200, 64, generator=gen(2)).to(BF)
+    o, a = _grads(q, k, v, par, log_n, do, 0, 10, 200)
+    o2, b = _grads(q, k, v, par, log_n, do, 0, 1000, 0)
+    assert torch.equal(o, o2) and all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_second_derivatives_are_refused():
+    q, k, v, par = inputs(1, 2, 1, 20, 20, 64, BF, seed=3)
+    from motif.ops import apply_chord_attention
+    q = q.to(DEV).requires_grad_()
+    o = apply_chord_attention(q, *(t.to(DEV) for t in (k, v, *par, log_n_of(1, 20, 0))), window=5)
+    with pytest.raises(RuntimeError, match='second derivatives'):
+        torch.autograd.grad(o.float().sum(), q, create_graph=True)
