@@ -99,14 +99,17 @@ __global__ void __launch_bounds__(128 * PARTS) __attribute__((amdgpu_waves_per_e
   const bf16_t *kp = static_cast<const bf16_t *>(a.k) + batch * a.k_sb + kvh * a.k_sh + int64_t(tok0) * a.k_st;
   const bf16_t *vp = static_cast<const bf16_t *>(a.v) + batch * a.v_sb + kvh * a.v_sh + int64_t(tok0) * a.v_st;
 
-  // logit = a_row acc with acc = rho q.k + kappa GGD, rho = sign(ssmax scale) (0 when scale is 0), kappa =
-  // sign(ssmax) / |scale| (sign(ssmax) when scale is 0), a_row = |ssmax log_n scale| (|ssmax log_n|);
-  // p = exp2(A (acc - m)), A = log2e a_row > 0 so that a masked key's -inf stays one
+  // logit = a_row acc with acc = rho q.k + kappa GGD, rho = sign(ssmax log_n scale) (0 when scale is 0), kappa =
+  // sign(ssmax log_n) / |scale| (sign(ssmax log_n) when scale is 0), a_row = |ssmax log_n scale| (|ssmax log_n|);
+  // p = exp2(A (acc - m)), A = log2e a_row > 0 so that a masked key's -inf stays one.  (The bias rows,
+  // which the wave's queries share, hold sign(ssmax) only: see `neg`.)
   const float ssm = a.ssmax[head], sg = ssm < 0.f ? -1.f : 1.f;
-  const float rho = a.scale > 0.f ? sg : a.scale < 0.f ? -sg : 0.f;
   const float lnv = a.log_n ? a.log_n[batch * a.ln_sb + int64_t(tok0 + min(my_q, Lq - 1)) * a.ln_st]
                             : a.log_tab[q_start + min(my_q, Lq - 1)];
-  const float A = q_valid ? fmaxf(fabsf(ssm) * (a.scale != 0.f ? fabsf(a.scale) : 1.f) * lnv * kLog2e, 1e-30f) : 1.f;
+  const bool neg = q_valid && lnv < 0.f;
+  const uint64_t any_neg = __ballot(neg);
+  const float sgr = neg ? -sg : sg, rho = a.scale > 0.f ? sgr : a.scale < 0.f ? -sgr : 0.f;
+  const float A = q_valid ? fmaxf(fabsf(ssm) * (a.scale != 0.f ? fabsf(a.scale) : 1.f) * fabsf(lnv) * kLog2e, 1e-30f) : 1.f;
 
   bf16x8 qreg[4];  // rho Q^T, the B operand: features 16 ds + 8 hh .. of this lane's row
   {
@@ -205,6 +208,10 @@ __global__ void __launch_bounds__(128 * PARTS) __attribute__((amdgpu_waves_per_e
       for (int q4 = 0; q4 < 4; ++q4)
 #pragma unroll
         for (int p4 = 0; p4 < 4; ++p4) acc[4 * q4 + p4] = bwr[8 * q4 + p4];
+      if (any_neg) {  // (a factor log_n below 0, no logarithm of a count: the bias's sign turned, masked keys kept so)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[r] = neg && acc[r] != -INFINITY ? -acc[r] : acc[r];
+      }
 #pragma unroll
       for (int ds = 0; ds < 4; ++ds) {
         const bf16x8 kop = *reinterpret_cast<const bf16x8 *>(sK(buf) + lc * kRowK + 16 * ds + 8 * hh);

@@ -420,7 +420,8 @@ def apply_chord_attention(
     Args:
         q: [B, H, L, D];  k, v: [B, H_kv, S, D] (fp16, bf16 or fp32; 16 <= D <= 128).
         alpha, beta, mu, ssmax: [H] fp32 contiguous.
-        log_n: [B, L] fp32, not negative (the logarithm of a count).
+        log_n: [B, L] fp32 (a logarithm of a count; bf16 prefills without a window take a
+            negative one as 0).
         q_start: absolute position of the first query; defaults to S - L.
         softmax_scale: defaults to D ** -0.5.
         eps: GGD epsilon.

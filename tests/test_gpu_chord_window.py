@@ -265,3 +265,17 @@ def test_split_decode_of_rows_that_see_nothing(B):
     assert not _run(q, k, v, par, log_n, q_start=5000, window=2000).any()
     got = _run(q, k, v, par, log_n, q_start=5000, window=2000, sinks=2)
     check_attention(got, q, k, v, par, log_n, 5000, 2000, 2)
+
+
+@pytest.mark.parametrize('dtype', [BF, F16, F32], ids=['bf16', 'fp16', 'fp32'])
+@pytest.mark.parametrize('L', [2, 100])
+@torch.no_grad()
+def test_log_n_of_either_sign(dtype, L):
+    S, window, sinks = 180, 45, 3
+    q, k, v, par = inputs(2, 8, 2, L, S, 64, dtype, seed=L)
+    log_n = log_n_of(2, L, S - L)
+    log_n[0, ::2] *= -0.5
+    log_n[1, L // 2:] = 0.0
+    for scale in (0.125, -0.2, 0.0):
+        got = _run(q, k, v, par, log_n, window=window, sinks=sinks, softmax_scale=scale)
+        check_attention(got, q, k, v, par, log_n, S - L, window, sinks, scale=scale)

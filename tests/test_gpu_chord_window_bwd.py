@@ -274,3 +274,15 @@ def test_second_derivatives_are_refused():
     o = apply_chord_attention(q, *(t.to(DEV) for t in (k, v, *par, log_n_of(1, 20, 0))), window=5)
     with pytest.raises(RuntimeError, match='second derivatives'):
         torch.autograd.grad(o.float().sum(), q, create_graph=True)
+
+
+def test_log_n_of_either_sign():
+    q, k, v, par = inputs(1, 4, 2, 140, 140, 64, BF, seed=8)
+    log_n = log_n_of(1, 140, 0)
+    log_n[0, ::3] *= -0.5
+    log_n[0, 100:] = 0.0
+    do = torch.randn(1, 4, 140, 64, generator=gen(2)).to(BF)
+    _, got = _grads(q, k, v, par, log_n, do, 0, 40, 2)
+    want, lims = formula64(q, k, v, par, log_n, do, 0, 40, 2)
+    for n, a, b, lim in zip(('dq', 'dk', 'dv', 'dalpha', 'dbeta', 'dmu', 'dssmax'), got, want, lims):
+        assert ((a.cpu().double() - b).abs() <= lim).all(), n
