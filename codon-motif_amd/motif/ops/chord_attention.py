@@ -133,9 +133,9 @@ class ChordWindowFunction(torch.autograd.Function):
         q, k, v = _rows4(q)[0], _rows4(k)[0], _rows4(v)[0]
         B, H, L, D = q.shape
         dev = q.device
-        out = q.new_empty((B, L, H, D)).transpose(1, 2)
+        out = torch.empty_like(q)  # (laid out as q is: heads beside each other where a projection made it)
         lib = _lib.lib()
-        n = lib.motif_chord_distances_len(L, q_start, window, sinks)
+        n = _distances_len(L, q_start, window, sinks)
         rows = -(-B * H * L // 4) * 4
         stats = log_n.new_empty(rows + 3 * H * n)  # the rows' log-sum-exp, then the distance table
         lse, distances = stats.data_ptr(), (stats.data_ptr() + 4 * rows, n)
@@ -164,7 +164,7 @@ class ChordWindowFunction(torch.autograd.Function):
         # gradients in storage of their own (an expanded input's would share elements)
         dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
         d_params = log_n.new_empty((4, H))
-        ws = torch.empty(_window_bwd_workspace_bytes(B, H, Hkv, L, S, q_start, window, sinks), dtype=torch.uint8, device=dev)
+        ws = log_n.new_empty(_window_bwd_workspace_bytes(B, H, Hkv, L, S, q_start, window, sinks) + 3 >> 2)
         with _lib.on_device(dev):
             rc = _lib.lib().motif_chord_window_bwd(
                 q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3],
@@ -172,12 +172,17 @@ class ChordWindowFunction(torch.autograd.Function):
                 stats.data_ptr(), alpha.data_ptr(), beta.data_ptr(), mu.data_ptr(), ssmax.data_ptr(),
                 log_n.data_ptr(), *log_n.stride(), dq.data_ptr(), *dq.stride()[:3], dk.data_ptr(), *dk.stride()[:3],
                 dv.data_ptr(), *dv.stride()[:3], d_params.data_ptr(), B, H, Hkv, L, S, D, q_start, scale, eps,
-                window, sinks, 1 if needs[5] else 0, stats.data_ptr() + 4 * rows, n, ws.data_ptr(), ws.numel(),
+                window, sinks, 1 if needs[5] else 0, stats.data_ptr() + 4 * rows, n, ws.data_ptr(), 4 * ws.numel(),
                 _lib.MOTIF_BF16, _lib.stream_ptr(dev))
         if rc:
             _lib.check(rc, 'motif_chord_window_bwd')
         return (dq if needs[0] else None, dk if needs[1] else None, dv if needs[2] else None,
                 *(g if need else None for g, need in zip(d_params.unbind(0), needs[3:7])), None, None, None, None, None, None)
+
+
+@functools.lru_cache(maxsize=256)
+def _distances_len(*sizes) -> int:
+    return int(_lib.lib().motif_chord_distances_len(*sizes))
 
 
 @functools.lru_cache(maxsize=256)
@@ -599,13 +604,14 @@ def chord_decode_step(proj, offsets, q_norm_weight, k_norm_weight, norm_eps, k_c
     out = torch.empty(B, num_heads, L, D, dtype=proj.dtype, device=proj.device)
     lib = _lib.lib()
     fn, limits = (lib.motif_chord_decode_step, ()) if window is None else (lib.motif_chord_window_step, (window, sinks))
-    rc = fn(
-        proj.data_ptr(), proj.stride(0), proj.stride(1), *[int(o) for o in offsets],
-        q_norm_weight.data_ptr(), k_norm_weight.data_ptr(), float(norm_eps),
-        *_lib.t4(k_cache), *_lib.t4(v_cache), length_dev.data_ptr(), cap,
-        alpha.data_ptr(), beta.data_ptr(), mu.data_ptr(), ssmax.data_ptr(), log_table.data_ptr(), log_table.numel(),
-        *_lib.t4(out), B, num_heads, Hkv, L, D, float(softmax_scale), float(eps), *limits,
-        workspace.data_ptr(), workspace.numel(), _lib.stream_ptr(proj.device))
+    with _lib.on_device(proj.device):
+        rc = fn(
+            proj.data_ptr(), proj.stride(0), proj.stride(1), *[int(o) for o in offsets],
+            q_norm_weight.data_ptr(), k_norm_weight.data_ptr(), float(norm_eps),
+            *_lib.t4(k_cache), *_lib.t4(v_cache), length_dev.data_ptr(), cap,
+            alpha.data_ptr(), beta.data_ptr(), mu.data_ptr(), ssmax.data_ptr(), log_table.data_ptr(), log_table.numel(),
+            *_lib.t4(out), B, num_heads, Hkv, L, D, float(softmax_scale), float(eps), *limits,
+            workspace.data_ptr(), workspace.numel(), _lib.stream_ptr(proj.device))
     _lib.check(rc, 'motif_chord_decode_step' if window is None else 'motif_chord_window_step')
     return out
 

@@ -238,3 +238,29 @@ def test_model_trains_with_a_window():
     b = torch.cat([grads[1][n].flatten() for n in sorted(grads[0])])
     # two decoders deep, each bf16 tensor rounded to 2^-9 in the mean: a few per cent of the whole gradient
     assert float((a - b).norm() / b.norm()) < 0.1
+
+
+@pytest.mark.parametrize('B,L,length,window,sinks', [(1, 1, 4200, 4000, 4), (2, 3, 2047, 1500, 40), (20, 2, 1200, 1000, 0),
+                                                     (64, 1, 700, 600, 3), (1, 4, 60, 1, 0), (1, 1, 0, 5, 2)])
+@torch.no_grad()
+def test_one_launch_step_of_many_shares(B, L, length, window, sinks):
+    '''From one to twelve workgroups a kv head: the rows and the cursor of the several launches, their output
+    within bf16 rounding; three steps over one scratch, whose counters each leaves at zero.'''
+    from motif.model.cache import StaticKVLayerCache
+    from motif.block.attention import chord_attn
+    layer = _layer(BF, window=window, sinks=sinks)
+    rows = torch.randn(2, B, 2, length, 64, generator=gen(B), dtype=F32).to(DEV, BF)
+    x = _x(B, 3 * L, BF)
+    outs, slabs = [], []
+    for fused in (True, False):
+        chord_attn.FUSED_STEP = fused
+        try:
+            cache = StaticKVLayerCache().allocate(B, 2, length + 3 * L, 64, DEV, BF)
+            cache.fill(rows[0], rows[1])
+            outs.append(torch.cat([layer(x[:, L * i:L * i + L], past_key_value=cache).output for i in range(3)], 1))
+        finally:
+            chord_attn.FUSED_STEP = True
+        assert cache.length == int(cache.length_dev) == length + 3 * L
+        slabs.append(cache._slab)
+    assert all(torch.equal(a, b) for a, b in zip(*slabs))
+    assert_bf16_close(outs[0], outs[1])
