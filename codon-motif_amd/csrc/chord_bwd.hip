@@ -42,8 +42,9 @@
 // from behind its windows (plan_bwd_window).  The distances' powers come from a 64-bit table: in
 // registers they took 20 instructions a score where 12 are left, and were the parameter gradients'
 // largest error.  2 x 2048 tokens, 12 heads, window 512: dQ 44 us, dK / dV 39, reduction 4, table 3;
-// 4001 tokens, 3 kv heads, window 1000: 70, 63, 10, 3.  Bound as above; with 384 workgroups on 256 CUs
-// those with two set the time (30 us of work for dQ spread evenly).
+// 4001 tokens, 3 kv heads, window 1000: 69, 63, 9, 3.  At these lengths no unit is busy half of the time
+// (4001 tokens: VALU 48% and 30% of the busy cycles, LDS 25% and 36%, MFMA 20%): 1.5 workgroups per CU,
+// a wave or two per SIMD, each a chain of reads, products, exponentials and a barrier a tile.
 #include <algorithm>
 #include <string>
 #include <type_traits>
