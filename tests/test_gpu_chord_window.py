@@ -4,7 +4,8 @@ inside, beside and past the window), strides, rows that no query sees, the curso
 import pytest
 import torch
 
-from window_ref import attention64, check_attention, inputs, log_n_of
+from support import gen
+from window_ref import attention64, check_attention, inputs, log_n_of, over_rows64
 
 pytestmark = pytest.mark.gpu
 
@@ -279,3 +280,24 @@ def test_log_n_of_either_sign(dtype, L):
     for scale in (0.125, -0.2, 0.0):
         got = _run(q, k, v, par, log_n, window=window, sinks=sinks, softmax_scale=scale)
         check_attention(got, q, k, v, par, log_n, S - L, window, sinks, scale=scale)
+
+
+@pytest.mark.parametrize('dtype', [BF, F32], ids=['bf16', 'fp32'])
+@torch.no_grad()
+def test_long_context_far_rows_of_a_prefill(dtype):
+    '''The same for many queries: rows past 2^31 bytes from the start of the keys, and more than 2^24 back.'''
+    S, L, window, sinks = 2 ** 25, 70, 300, 5
+    g = gen(4)
+    k = torch.zeros(1, 1, S, 64, dtype=dtype, device=DEV)  # 4.3 GB (bf16), and as much for the values
+    v = torch.zeros(1, 1, S, 64, dtype=dtype, device=DEV)
+    rows = list(range(sinks)) + list(range(S - L - window, S))
+    idx = torch.tensor(rows, device=DEV)
+    for t in (k, v):
+        t[:, :, idx] = torch.randn(1, 1, len(rows), 64, generator=g).to(dtype).to(DEV)
+    q, _, _, par = inputs(1, 2, 1, L, 1, 64, dtype, seed=1)
+    log_n = log_n_of(1, L, S - L)
+    got = _run(q, k, v, par, log_n, window=window, sinks=sinks).cpu().double()
+    want, mean = over_rows64(q, rows, k[:, :, idx], v[:, :, idx], par, log_n, S - L, window, sinks)
+    # logits to 2^7, a weight to 2^-15 of itself by fp32's steps; bf16: P's and the output's rounding besides
+    lim = 2.0 ** -14 * mean + ((2.0 ** -8 * mean + 2.0 ** -8 * want.abs()) if dtype == BF else 0)
+    assert ((got - want).abs() <= lim).all()

@@ -5,7 +5,8 @@ import pytest
 import torch
 
 from support import gen
-from window_ref import (check_attention, code_sizes64, inputs, log_n_of, quantise64, random_slab, slab_values64, values64)
+from window_ref import (check_attention, code_sizes64, inputs, log_n_of, over_rows64, quantise64, random_slab, slab_values64,
+                        values64)
 
 pytestmark = pytest.mark.gpu
 
@@ -339,3 +340,30 @@ def test_prep_refusals():
     odd = torch.zeros(2, 1, 516, dtype=BF, device=DEV)[..., 1:513]
     with pytest.raises(NotImplementedError, match='aligned'):
         chord_kv4_prep(**{**ok, 'proj': odd})
+
+
+@pytest.mark.parametrize('dtype,L', [(BF, 1), (F16, 2), (BF, 70), (F32, 1)])
+@torch.no_grad()
+def test_long_cache_far_rows(dtype, L):
+    '''Codes past 2^31 bytes from the start of the cache: written, read back and attended to.'''
+    from motif.ops import chord_attention_kv4, kv4_alloc, kv4_append, kv4_read
+    S, window, sinks = 70_000_000, 200, 3
+    slab = kv4_alloc(1, 1, S, 64, DEV)  # 5.6 GB
+    n = window + L
+    far = [torch.randn(1, 1, n, 64, generator=gen(5 + i)).to(dtype).to(DEV) for i in range(2)]
+    near = [torch.randn(1, 1, sinks, 64, generator=gen(7 + i)).to(dtype).to(DEV) for i in range(2)]
+    kv4_append(slab, *far, S - n)
+    kv4_append(slab, *near, torch.zeros(1, dtype=torch.int32, device=DEV))
+    small = kv4_alloc(1, 1, n + sinks, 64, DEV)
+    kv4_append(small, *(torch.cat([a, b], 2) for a, b in zip(near, far)), 0)
+    for a, b in zip(kv4_read(slab, S - n, n, F32), kv4_read(small, sinks, n, F32)):
+        assert torch.equal(a, b)
+    q, _, _, par = inputs(1, 4, 1, L, 1, 64, dtype, seed=1)
+    log_n = log_n_of(1, L, S - L)
+    got = chord_attention_kv4(q.to(DEV), slab, *(t.to(DEV) for t in par), log_n.to(DEV), S, window=window, sinks=sinks)
+    k, v = slab_values64(small)
+    rows = list(range(sinks)) + list(range(S - n, S))
+    want, mean = over_rows64(q, rows, k, v, par, log_n, S - L, window, sinks)
+    # logits to 2^7 in fp32; 16-bit types: their weights' rounding (times codes to 15 steps) and the output's
+    h = {BF: 2.0 ** -8, F16: 2.0 ** -11, F32: 0.0}[dtype]
+    assert ((got.cpu().double() - want).abs() <= (2.0 ** -13 + 3 * h) * mean + h * want.abs()).all()

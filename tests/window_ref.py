@@ -133,3 +133,18 @@ def random_slab(B, Hkv, cap, D, device, seed=0):
         code = code.to(torch.uint8)
         ts += [code[..., 0::2] | (code[..., 1::2] << 4), torch.stack([scale, base], -1)]
     return KV4Slab(*[t.contiguous().to(device) for t in ts])
+
+
+def over_rows64(q, rows, k, v, par, log_n, q_start, window, sinks, eps=1e-5):
+    '''(out, the same of |v|) in float64 where only the keys at positions `rows` (given as k, v) count.'''
+    H, L, D = q.shape[1:]
+    al, be, mu, ss = (t.double().view(H, 1, 1) for t in par)
+    pos = torch.tensor(rows, dtype=torch.float64)
+    G = H // k.shape[1]
+    k, v = (t.cpu().double().repeat_interleave(G, 1) for t in (k, v))
+    i = (q_start + torch.arange(L))[:, None].double()
+    d = pos[None] - i
+    z = (q.double() @ k.transpose(-1, -2) * D ** -0.5 - al * ((d - mu).abs() + eps) ** be) * (ss * log_n.double()[:, None, :, None])
+    z = z.masked_fill(~((d <= 0) & ((d > -window) | (pos < sinks)[None])), float('-inf'))
+    p = torch.softmax(z, -1)
+    return p @ v, p @ v.abs()
