@@ -190,16 +190,22 @@ def _window_bwd_workspace_bytes(*sizes) -> int:
     return int(_lib.lib().motif_chord_window_bwd_workspace_bytes(*sizes))
 
 
-def _window_grad_kernels_serve(q, k, v, alpha, beta, mu, ssmax, log_n):
-    '''As _grad_kernels_serve, for a window (any q_start >= 0; something to differentiate).'''
-    if not (q.is_cuda and q.dtype == torch.bfloat16 and k.dtype == q.dtype and v.dtype == q.dtype
-            and q.dim() == 4 and k.dim() == 4 and q.shape[-1] == HEAD_DIM and k.shape == v.shape
-            and k.shape[-1] == HEAD_DIM and q.shape[0] == k.shape[0] and q.shape[1] % max(k.shape[1], 1) == 0
-            and q.numel() and k.numel() and _lib.available()):
+def _window_grad_kernels_serve(q, k, v, params, log_n):
+    '''As _grad_kernels_serve, for a window (any q_start >= 0; something to differentiate); a call that
+    they serve but for a stride or a device is refused here.'''
+    if q.dtype != torch.bfloat16 or log_n.requires_grad or not _lib.available():
         return False
-    if log_n.requires_grad or any(t.dtype != torch.float32 or t.dim() != 1 for t in (alpha, beta, mu, ssmax)):
-        return False
-    return log_n.dtype == torch.float32 and log_n.shape == (q.shape[0], q.shape[2])
+    sizes = _fits(q, k, v, params, log_n)
+    if sizes is None:
+        if not (q.is_cuda and k.dtype == q.dtype and v.dtype == q.dtype and q.dim() == 4 and k.dim() == 4
+                and q.shape[-1] == HEAD_DIM and k.shape == v.shape and k.shape[-1] == HEAD_DIM
+                and q.shape[0] == k.shape[0] and q.shape[1] % max(k.shape[1], 1) == 0
+                and log_n.dtype == torch.float32 and log_n.shape == (q.shape[0], q.shape[2])) \
+                or any(t.dtype != torch.float32 or t.dim() != 1 for t in params):
+            return False
+        sizes = _check_call(q, k, v, params, log_n)
+    B, H, L, D, Hkv, S = sizes
+    return D == HEAD_DIM and B > 0 and L > 0 and S > 0
 
 
 def _check_tensors(q, k, v, log_n):
@@ -245,23 +251,30 @@ def _check_params(alpha, beta, mu, ssmax, num_heads):
             raise ValueError(f'{name} must be contiguous')
 
 
-def _check_call(q, k, v, params, log_n):
-    '''_check_tensors and _check_params of a windowed call, and that its tensors share a device:
-    asked for at once, and one by one (for the message) only where something is off.'''
+def _fits(q, k, v, params, log_n):
+    '''(B, H, L, D, Hkv, S) where a windowed call's tensors pass _check_tensors and _check_params and share
+    a device, asked for at once; None where something is off.'''
     at, dt, shape, ks = q.get_device(), q.dtype, q.shape, k.shape
-    if at >= 0 and len(shape) == 4 and len(ks) == 4 and dt in _DTYPES:
-        B, H, L, D = shape
-        Hkv = ks[1]
-        if k.dtype == dt and v.dtype == dt and ks == v.shape and ks[0] == B and ks[3] == D and D >= 16 \
-                and Hkv and H % Hkv == 0 and k.get_device() == at and v.get_device() == at \
-                and q.stride()[3] == 1 and k.stride()[3] == 1 and v.stride()[3] == 1 \
-                and log_n.get_device() == at and log_n.dtype == torch.float32 and log_n.shape == (B, L) \
-                and log_n.stride()[1] == 1:
-            for t in params:
-                if t.get_device() != at or t.dtype != torch.float32 or t.shape != (H,) or not t.is_contiguous():
-                    break
-            else:
-                return B, H, L, D, Hkv, ks[2]
+    if at < 0 or len(shape) != 4 or len(ks) != 4 or dt not in _DTYPES:
+        return None
+    B, H, L, D = shape
+    Hkv = ks[1]
+    if k.dtype != dt or v.dtype != dt or ks != v.shape or ks[0] != B or ks[3] != D or D < 16 or not Hkv or H % Hkv \
+            or k.get_device() != at or v.get_device() != at \
+            or q.stride()[3] != 1 or k.stride()[3] != 1 or v.stride()[3] != 1 \
+            or log_n.get_device() != at or log_n.dtype != torch.float32 or log_n.shape != (B, L) or log_n.stride()[1] != 1:
+        return None
+    for t in params:
+        if t.get_device() != at or t.dtype != torch.float32 or t.shape != (H,) or not t.is_contiguous():
+            return None
+    return B, H, L, D, Hkv, ks[2]
+
+
+def _check_call(q, k, v, params, log_n):
+    '''_fits, or what is off, one by one.'''
+    sizes = _fits(q, k, v, params, log_n)
+    if sizes is not None:
+        return sizes
     sizes = _check_tensors(q, k, v, log_n)
     _check_params(*params, sizes[1])
     for t in (k, v, log_n, *params):
@@ -451,8 +464,7 @@ def apply_chord_attention(
     if wants_grad(q, k, v, alpha, beta, mu, ssmax, log_n):
         if q_start is not None and int(q_start) < 0:
             raise ValueError(f'q_start must not be negative, got {q_start}')
-        if window is not None and _window_grad_kernels_serve(q, k, v, alpha, beta, mu, ssmax, log_n):
-            _check_call(q, k, v, (alpha, beta, mu, ssmax), log_n)
+        if window is not None and _window_grad_kernels_serve(q, k, v, (alpha, beta, mu, ssmax), log_n):
             scale = q.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale)
             qs = k.shape[2] - q.shape[2] if q_start is None else int(q_start)
             if qs < 0:
