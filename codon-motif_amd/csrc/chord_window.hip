@@ -36,14 +36,20 @@ namespace {
 
 constexpr int kBD = 64;    // head dim
 constexpr int kT = 32;     // keys per tile
-constexpr int kRowK = 72;  // padded LDS row of 64 bf16: row-per-lane 16-byte reads without bank conflicts
-constexpr int kRowV = 40;  // padded LDS row of a V^T tile (32 keys)
 
 __device__ __forceinline__ f32x16 mma32(const bf16x8 &a, const bf16x8 &b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
-// Position of key k (0..31) in a V^T row: the eight keys a lane half holds of each 16-key group together
-__device__ __forceinline__ int vperm(int k) { return (k & ~15) | ((k & 4) << 1) | ((k & 8) >> 1) | (k & 3); }
+// A tile in LDS is its 32 rows of eight 16-byte pieces, piece c of row r at c ^ piece_swap(r): 16-byte reads of
+// one piece of eight rows and of four pieces of two rows, and transpose reads of 16 features of four rows,
+// all meet every bank alike.
+__device__ __forceinline__ int piece_swap(int r) { return ((r & 1) << 2) | ((r >> 1) & 3); }
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+// Lane l: feature l % 32 of keys 4 (l / 32) .. + 3, from the address of 4 features of key 4 (l / 32) + l % 16 / 4
+// (16 (l / 16 % 2) + 4 (l % 4) on)
+__device__ __forceinline__ uint2 ld_transposed(const bf16_t *p) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p));
+}
 typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
 typedef float f32x2v __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pk2bf(float x0, float x1) {
@@ -123,12 +129,12 @@ __global__ void __launch_bounds__(128 * PARTS) __attribute__((amdgpu_waves_per_e
     }
   }
 
-  constexpr int kTileK = kT * kRowK, kTileV = kBD * kRowV;
-  constexpr int kStage = PARTS * 2 * (kTileK + kTileV), kMerge = (PARTS - 1) * 2 * 32 * 64 * 2;  // in bf16 elements
+  constexpr int kTile = kT * kBD;
+  constexpr int kStage = PARTS * 2 * 2 * kTile, kMerge = (PARTS - 1) * 2 * 32 * 64 * 2;  // in bf16 elements
   __shared__ __attribute__((aligned(16))) bf16_t sKV[kStage > kMerge ? kStage : kMerge];
   __shared__ float sB[2 * PARTS][RH * kWin > 128 ? RH * kWin : 128];
-  auto sK = [&](int buf) { return sKV + (part * 2 + buf) * (kTileK + kTileV); };
-  auto sV = [&](int buf) { return sKV + (part * 2 + buf) * (kTileK + kTileV) + kTileK; };
+  auto sK = [&](int buf) { return sKV + (part * 2 + buf) * 2 * kTile; };
+  auto sV = [&](int buf) { return sKV + (part * 2 + buf) * 2 * kTile + kTile; };
 
   // Bias rows: entry j of a head is distance key - q_abs = n0 - q_start - q0 - (RQ - 1) + j.  Lane l
   // (head l / 32 of two) holds entry RQ - 1 + l % 32 of its tile in `bnew`; the first RQ - 1 entries are
@@ -159,32 +165,33 @@ __global__ void __launch_bounds__(128 * PARTS) __attribute__((amdgpu_waves_per_e
   // this lane's entries for keys 8 q4 + 4 hh + (0..3): j = 8 q4 + p + 4 hh - cq + RQ - 1
   const float *bwr = &sB[wv][(lc / RQ) * kWin] + 4 * hh - cq + RQ - 1;
 
-  // Staging by the part's 128 threads: K rows htid / 8 and + 16; V rows 2 (htid % 16) and + 1 (8 features)
+  // Staging by the part's 128 threads: row htid / 4, pieces htid % 4 and + 4
   uint4 kst[2], vst[2];
-  const int krow = htid >> 3, vpair = htid & 15, vseg = htid >> 4;
-  const uint32_t koff = static_cast<uint32_t>((krow * a.k_st + (htid & 7) * 8) * 2), koff2 = koff + static_cast<uint32_t>(32 * a.k_st);
-  const uint32_t voff = static_cast<uint32_t>((2 * vpair * a.v_st + 8 * vseg) * 2), voff2 = voff + static_cast<uint32_t>(2 * a.v_st);
+  const int srow = htid >> 2;
+  const uint32_t koff = static_cast<uint32_t>((srow * a.k_st + (htid & 3) * 8) * 2);
+  const uint32_t voff = static_cast<uint32_t>((srow * a.v_st + (htid & 3) * 8) * 2);
+  const int sto = srow * kBD + 8 * ((htid & 3) ^ piece_swap(srow));
   auto load_tile = [&](int x) {  // (rows past the tile's own read zeros)
     const int n0 = walk.start(x), rows = walk.rows(x);
     const buf_t kr = make_buf(kp + int64_t(n0) * a.k_st, rows > 0 ? static_cast<uint32_t>(((rows - 1) * a.k_st + kBD) * 2) : 0u);
     const buf_t vr = make_buf(vp + int64_t(n0) * a.v_st, rows > 0 ? static_cast<uint32_t>(((rows - 1) * a.v_st + kBD) * 2) : 0u);
     kst[0] = buf_ld16(kr, koff);
-    kst[1] = buf_ld16(kr, koff2);
+    kst[1] = buf_ld16(kr, koff + 64u);
     vst[0] = buf_ld16(vr, voff);
-    vst[1] = buf_ld16(vr, voff2);
+    vst[1] = buf_ld16(vr, voff + 64u);
   };
   auto store_tile = [&](int buf) {
-    bf16_t *kd = sK(buf) + krow * kRowK + (htid & 7) * 8;
-    *reinterpret_cast<uint4 *>(kd) = kst[0];
-    *reinterpret_cast<uint4 *>(kd + 16 * kRowK) = kst[1];
-    const uint32_t v0[4] = {vst[0].x, vst[0].y, vst[0].z, vst[0].w}, v1[4] = {vst[1].x, vst[1].y, vst[1].z, vst[1].w};
-    bf16_t *vd = sV(buf) + 8 * vseg * kRowV + vperm(2 * vpair);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      *reinterpret_cast<uint32_t *>(vd + (2 * i) * kRowV) = (v0[i] & 0xffffu) | (v1[i] << 16);
-      *reinterpret_cast<uint32_t *>(vd + (2 * i + 1) * kRowV) = (v0[i] >> 16) | (v1[i] & 0xffff0000u);
-    }
+    bf16_t *kd = sK(buf), *vd = sV(buf);
+    *reinterpret_cast<uint4 *>(kd + sto) = kst[0];
+    *reinterpret_cast<uint4 *>(kd + (sto ^ 32)) = kst[1];
+    *reinterpret_cast<uint4 *>(vd + sto) = vst[0];
+    *reinterpret_cast<uint4 *>(vd + (sto ^ 32)) = vst[1];
   };
+  // this lane's reads: K row lc, pieces 2 ds + hh; V^T, keys 4 hh + lane % 16 / 4 (+ 8, + 16), features
+  // 16 (lane / 16 % 2) + 4 (lane % 4) (+ 32) on
+  const int ko = lc * kBD + 8 * (hh ^ piece_swap(lc));
+  const int vrow = 4 * hh + ((lane & 15) >> 2), vpiece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  const int vo = vrow * kBD + 8 * (vpiece ^ piece_swap(vrow)) + 4 * (lane & 1);
 
   float m_run = -INFINITY, l_run = 0.f;  // per column (m: acc units; l: this lane's share)
   f32x16 oacc[2] = {f32x16{}, f32x16{}};  // O^T rows d = 32 dt + 8 (r / 4) + 4 hh + r % 4, column lc
@@ -214,7 +221,7 @@ __global__ void __launch_bounds__(128 * PARTS) __attribute__((amdgpu_waves_per_e
       }
 #pragma unroll
       for (int ds = 0; ds < 4; ++ds) {
-        const bf16x8 kop = *reinterpret_cast<const bf16x8 *>(sK(buf) + lc * kRowK + 16 * ds + 8 * hh);
+        const bf16x8 kop = *reinterpret_cast<const bf16x8 *>(sK(buf) + (ko ^ (16 * ds)));
         acc = mma32(kop, qreg[ds], acc);
       }
       // by key: tiles of first tokens at the window's edge, and the end of the keys
@@ -261,8 +268,9 @@ __global__ void __launch_bounds__(128 * PARTS) __attribute__((amdgpu_waves_per_e
         const bf16x8 pb = __builtin_bit_cast(bf16x8, uint4{pw[0], pw[1], pw[2], pw[3]});
 #pragma unroll
         for (int dt = 0; dt < 2; ++dt) {
-          const bf16x8 va = *reinterpret_cast<const bf16x8 *>(sV(buf) + (32 * dt + lc) * kRowV + 16 * hk + 8 * hh);
-          oacc[dt] = mma32(va, pb, oacc[dt]);
+          const bf16_t *vp = sV(buf) + (vo ^ (32 * dt)) + 16 * hk * kBD;
+          const uint2 v0 = ld_transposed(vp), v1 = ld_transposed(vp + 8 * kBD);
+          oacc[dt] = mma32(__builtin_bit_cast(bf16x8, uint4{v0.x, v0.y, v1.x, v1.y}), pb, oacc[dt]);
         }
       }
     }
