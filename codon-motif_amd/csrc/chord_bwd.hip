@@ -59,8 +59,6 @@ namespace {
 
 constexpr int kBD = 64;    // head dim
 constexpr int kT = 32;     // keys (dQ kernel) or queries (dK / dV kernel) per tile
-constexpr int kRowP = 72;  // padded LDS row of 64 bf16 (144 B)
-constexpr int kTRow = 40;  // padded LDS row of a transposed 32-element tile (80 B)
 constexpr int kBlk = 128;  // queries (dQ kernel) or keys (dK / dV kernel) per workgroup
 
 struct ChordBwdArgs {
@@ -109,10 +107,6 @@ __host__ __device__ inline int kv_window_end(int kb, int L, int q_start, int win
 __device__ __forceinline__ f32x16 mma32(const bf16x8 &a, const bf16x8 &b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
-// Position of element e (0..31) in a transposed tile row: accumulator lane half h holds
-// elements 8a + 4h + (0..3) of each 16-element group, stored together at 8h + 4a.
-__device__ __forceinline__ int tperm(int e) { return (e & ~15) | ((e & 4) << 1) | ((e & 8) >> 1) | (e & 3); }
-
 typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
 typedef float f32x2v __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pk2bf(float x0, float x1) {
@@ -123,7 +117,7 @@ __device__ __forceinline__ bf16x8 pack8(const float *x) {
 }
 __device__ __forceinline__ uint4 ld16(const bf16_t *p) { return *reinterpret_cast<const uint4 *>(p); }
 
-// Tile staging by 128 threads t: rows 2 (t & 15) and + 1, 8-element segment t >> 4 of a
+// Tile staging by 128 threads t: row t >> 2, 8-element pieces t & 3 and + 4 of a
 // 32-row x 64 tile of [rows][64] bf16 rows, through a range-checked buffer that starts at the
 // tile's first row (uniform) and ends at row `nrows` of the matrix: rows past it read 0 with no
 // branch, and a tile costs two loads and its base.  The loads go to registers one tile ahead of the
@@ -137,39 +131,46 @@ struct StageSrc {
   const bf16_t *base;
   int64_t st;
   int nrows;
-  uint32_t off, off1;  // this thread's two row segments
+  uint32_t off;  // this thread's first piece
   __device__ __forceinline__ StageSrc(const bf16_t *p, int64_t s, int n, int t)
-      : base(p), st(s), nrows(n), off(static_cast<uint32_t>((2 * (t & 15) * s + 8 * (t >> 4)) * 2)),
-        off1(off + static_cast<uint32_t>(2 * s)) {}
+      : base(p), st(s), nrows(n), off(static_cast<uint32_t>(((t >> 2) * s + 8 * (t & 3)) * 2)) {}
   __device__ __forceinline__ Stage2 load(int row0) const { return load(row0, min(kT, nrows - row0)); }
   __device__ __forceinline__ Stage2 load(int row0, int rows) const {
     if constexpr (ANY) {
-      const int r0 = 2 * (threadIdx.x & 15);
-      const bf16_t *p = base + (row0 + r0) * st + 8 * ((threadIdx.x & 127) >> 4);
+      const int r = (threadIdx.x & 127) >> 2;
+      const bf16_t *p = base + (row0 + r) * st + 8 * (threadIdx.x & 3);
       const uint4 z = {0u, 0u, 0u, 0u};
-      return {r0 < rows ? ld16(p) : z, r0 + 1 < rows ? ld16(p + st) : z};
+      return {r < rows ? ld16(p) : z, r < rows ? ld16(p + 32) : z};
     }
     const buf_t buf = make_buf(base + int64_t(row0) * st, rows > 0 ? static_cast<uint32_t>(((rows - 1) * st + kBD) * 2) : 0u);
-    return {buf_ld16(buf, off), buf_ld16(buf, off1)};
+    return {buf_ld16(buf, off), buf_ld16(buf, off + 64u)};
   }
 };
-// The rows (padded) into `rows`, and, when `tr` is set, the transposed tile [64][32]
-// (elements in tperm order) into `tr`.
-__device__ __forceinline__ void stage_store(const Stage2 &g, int t, bf16_t *rows, bf16_t *tr) {
-  const int pr = t & 15, seg = t >> 4;
-  const int r0 = 2 * pr, r1 = 2 * pr + 1;
-  *reinterpret_cast<uint4 *>(rows + r0 * kRowP + 8 * seg) = g.a;
-  *reinterpret_cast<uint4 *>(rows + r1 * kRowP + 8 * seg) = g.b;
-  if (tr) {
-    const uint32_t aw[4] = {g.a.x, g.a.y, g.a.z, g.a.w}, bw[4] = {g.b.x, g.b.y, g.b.z, g.b.w};
-    const int col = tperm(r0);  // r0 even: r1 sits right after it
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      *reinterpret_cast<uint32_t *>(tr + (8 * seg + 2 * i) * kTRow + col) = (aw[i] & 0xffffu) | (bw[i] << 16);
-      *reinterpret_cast<uint32_t *>(tr + (8 * seg + 2 * i + 1) * kTRow + col) = (aw[i] >> 16) | (bw[i] & 0xffff0000u);
-    }
-  }
+// The pieces into the tile's rows.
+__device__ __forceinline__ void stage_store(const Stage2 &g, int t, bf16_t *rows) {
+  const int o = (t >> 2) * kBD + 8 * ((t & 3) ^ piece_swap(t >> 2));
+  *reinterpret_cast<uint4 *>(rows + o) = g.a;
+  *reinterpret_cast<uint4 *>(rows + (o ^ 32)) = g.b;
 }
+// This lane's reads of a tile: row lane % 32, features 16 ds + 8 (lane / 32) .. + 7 (a product over
+// features), and feature 32 dt + lane % 32 of rows 16 ks + 4 (lane / 32) .. + 3 and + 8 .. + 11 (over rows,
+// in the order in which the accumulators hold them).
+struct TileReads {
+  int ro, to;
+  __device__ __forceinline__ explicit TileReads(int lane) {
+    const int lc = lane & 31, hh = lane >> 5, r = 4 * hh + ((lane & 15) >> 2);
+    ro = lc * kBD + 8 * (hh ^ piece_swap(lc));
+    to = r * kBD + 8 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ piece_swap(r)) + 4 * (lane & 1);
+  }
+  __device__ __forceinline__ bf16x8 row(const bf16_t *tile, int ds) const {
+    return *reinterpret_cast<const bf16x8 *>(tile + (ro ^ (16 * ds)));
+  }
+  __device__ __forceinline__ bf16x8 col(const bf16_t *tile, int dt, int ks) const {
+    const bf16_t *p = tile + (to ^ (32 * dt)) + 16 * ks * kBD;
+    const uint2 a = ld_transposed(p), b = ld_transposed(p + 8 * kBD);
+    return __builtin_bit_cast(bf16x8, uint4{a.x, a.y, b.x, b.y});
+  }
+};
 
 // ------------------------------------------------------------------ dQ (+ Delta, parameter sums)
 // WIN: with a window; MU: mu's gradient too (the layer's is frozen; it costs a window kernel 2 of 13
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
   const int q0 = qb * kBlk + 32 * w;
   const int my_q = q0 + lc;
   const bool qv = my_q < a.L;
-  // waves 0, 1 stage K (rows and K^T), 2, 3 V (rows); the first tile's loads go ahead of the rest
+  // waves 0, 1 stage K, 2, 3 V; the first tile's loads go ahead of the rest
   const bool kside = w < 2;
   const StageSrc<ANY> src(kside ? a.k + b * a.k_sb + kvh * a.k_sh : a.v + b * a.v_sb + kvh * a.v_sh, kside ? a.k_st : a.v_st,
                      kv_end, tid & 127);
@@ -228,9 +229,8 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
   const int wave_kv_end = a.q_start + min(a.L, q0 + 32);  // keys this wave sees: < wave_kv_end
   const int k_max = WIN ? min(q_abs, a.S - 1) : q_abs;    // this query's last key
 
-  __shared__ __attribute__((aligned(16))) bf16_t sK[2][kT * kRowP];    // K rows of the tile
-  __shared__ __attribute__((aligned(16))) bf16_t sV[2][kT * kRowP];    // V rows
-  __shared__ __attribute__((aligned(16))) bf16_t sKT[2][kBD * kTRow];  // K^T, keys in tperm order
+  __shared__ __attribute__((aligned(16))) bf16_t sK[2][kT * kBD], sV[2][kT * kBD];  // the tile's rows
+  const TileReads rd(lane);
   // per wave and distance: {b, d/d alpha, d/d beta, d/d mu}; WIN: {x^beta, x^beta log2 x, d x^beta / d x sign}
   using DistV = std::conditional_t<WIN && !MU, float2, float4>;
   __shared__ DistV sW[4][64];
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
   f32x16 pkacc[2];
   pkacc[0] = pkacc[1] = f32x16{};
 
-  auto store_kv = [&](const Stage2 &g, int buf) { stage_store(g, tid & 127, kside ? sK[buf] : sV[buf], kside ? sKT[buf] : nullptr); };
+  auto store_kv = [&](const Stage2 &g, int buf) { stage_store(g, tid & 127, kside ? sK[buf] : sV[buf]); };
   // WIN: this lane's entry of tile x's window, d = key - q_abs = key_at(x) - q_start - q0 - 31 + lane, loaded a
   // tile ahead (outside the table, where no query of the wave sees a key: zeros)
   const buf_t dbuf = make_buf(WIN ? a.dist + static_cast<size_t>(h) * a.dist_n : nullptr, WIN ? a.dist_n * 8u : 0u);
@@ -295,10 +295,8 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
       f32x16 sacc = {}, pacc = {};
 #pragma unroll
       for (int ds = 0; ds < 4; ++ds) {
-        const bf16x8 ko = *reinterpret_cast<const bf16x8 *>(sK[buf] + lc * kRowP + 16 * ds + 8 * hh);
-        const bf16x8 vo = *reinterpret_cast<const bf16x8 *>(sV[buf] + lc * kRowP + 16 * ds + 8 * hh);
-        sacc = mma32(ko, qreg[ds], sacc);
-        pacc = mma32(vo, dreg[ds], pacc);
+        sacc = mma32(rd.row(sK[buf], ds), qreg[ds], sacc);
+        pacc = mma32(rd.row(sV[buf], ds), dreg[ds], pacc);
       }
       float dz[16], pr[WIN ? 16 : 1];
       auto body = [&](auto masked) {
@@ -360,7 +358,7 @@ __global__ void __launch_bounds__(256) chord_bwd_dq_kernel(ChordBwdArgs a) {
         const bf16x8 zb = pack8(dz + 8 * ks);
 #pragma unroll
         for (int dt = 0; dt < 2; ++dt) {
-          const bf16x8 kto = *reinterpret_cast<const bf16x8 *>(sKT[buf] + (32 * dt + lc) * kTRow + 16 * ks + 8 * hh);
+          const bf16x8 kto = rd.col(sK[buf], dt, ks);
           dqacc[dt] = mma32(kto, zb, dqacc[dt]);
           if constexpr (WIN) pkacc[dt] = mma32(kto, pack8(pr + 8 * ks), pkacc[dt]);
         }
@@ -454,8 +452,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int k0w = kb * kBlk + 32 * w;
   const int my_k = k0w + lc;
   const bool kvld = my_k < a.S;
-  // waves 0, 1 stage Q, 2, 3 dO (rows and transposed); threads 0-31 the row values; the first
-  // tile's loads go ahead of the rest
+  // waves 0, 1 stage Q, 2, 3 dO; threads 0-31 the row values; the first tile's loads go ahead of the rest
   const bool qside = w < 2;
   const size_t rbase = (static_cast<size_t>(b) * a.H + h) * a.L;
   const StageSrc<ANY> src(qside ? a.q + b * a.q_sb + h * a.q_sh : a.dout + b * a.d_sb + h * a.d_sh, qside ? a.q_st : a.d_st, a.L,
@@ -477,10 +474,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     vreg[ds] = __builtin_bit_cast(bf16x8, ld16(vrow + 16 * ds + 8 * hh));
   }
 
-  __shared__ __attribute__((aligned(16))) bf16_t sQ[2][kT * kRowP];    // Q rows of the query tile
-  __shared__ __attribute__((aligned(16))) bf16_t sD[2][kT * kRowP];    // dO rows
-  __shared__ __attribute__((aligned(16))) bf16_t sQT[2][kBD * kTRow];  // Q^T, queries in tperm order
-  __shared__ __attribute__((aligned(16))) bf16_t sDT[2][kBD * kTRow];  // dO^T
+  __shared__ __attribute__((aligned(16))) bf16_t sQ[2][kT * kBD], sD[2][kT * kBD];  // Q and dO rows of the query tile
+  const TileReads rd(lane);
   __shared__ float4 sRow[2][kT];  // per query: {lse2, Delta, c log2 e, c s}
   __shared__ float sW[4][64];     // per wave: the bias window
 
@@ -489,7 +484,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   const float s = a.scale;
   const float sig = a.ssmax[h], al = a.alpha[h], be = a.beta[h], mu = a.mu[h];
   auto store_q = [&](const Stage2 &g, const float4 &rv, int buf) {
-    stage_store(g, tid & 127, qside ? sQ[buf] : sD[buf], qside ? sQT[buf] : sDT[buf]);
+    stage_store(g, tid & 127, qside ? sQ[buf] : sD[buf]);
     if (tid < kT) sRow[buf][tid] = rv;
   };
   // WIN: this lane's entry of the window of query tile qt, distance k0w - q_start - 32 qt - 31 + lane
@@ -533,10 +528,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       f32x16 sacc = {}, pacc = {};
 #pragma unroll
       for (int ds = 0; ds < 4; ++ds) {
-        const bf16x8 qo = *reinterpret_cast<const bf16x8 *>(sQ[buf] + lc * kRowP + 16 * ds + 8 * hh);
-        const bf16x8 dov = *reinterpret_cast<const bf16x8 *>(sD[buf] + lc * kRowP + 16 * ds + 8 * hh);
-        sacc = mma32(qo, kreg[ds], sacc);
-        pacc = mma32(dov, vreg[ds], pacc);
+        sacc = mma32(rd.row(sQ[buf], ds), kreg[ds], sacc);
+        pacc = mma32(rd.row(sD[buf], ds), vreg[ds], pacc);
       }
       float pv[16], dz[16];
       // the tile's queries that see this lane's key: q_lo .. q_lo + q_n - 1 (one compare per element)
@@ -567,10 +560,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
         const bf16x8 pb = pack8(pv + 8 * ks), zb = pack8(dz + 8 * ks);
 #pragma unroll
         for (int dt = 0; dt < 2; ++dt) {
-          const bf16x8 dto = *reinterpret_cast<const bf16x8 *>(sDT[buf] + (32 * dt + lc) * kTRow + 16 * ks + 8 * hh);
-          const bf16x8 qto = *reinterpret_cast<const bf16x8 *>(sQT[buf] + (32 * dt + lc) * kTRow + 16 * ks + 8 * hh);
-          dvacc[dt] = mma32(dto, pb, dvacc[dt]);
-          dkacc[dt] = mma32(qto, zb, dkacc[dt]);
+          dvacc[dt] = mma32(rd.col(sD[buf], dt, ks), pb, dvacc[dt]);
+          dkacc[dt] = mma32(rd.col(sQ[buf], dt, ks), zb, dkacc[dt]);
         }
       }
     }

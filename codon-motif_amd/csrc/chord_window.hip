@@ -40,16 +40,6 @@ constexpr int kT = 32;     // keys per tile
 __device__ __forceinline__ f32x16 mma32(const bf16x8 &a, const bf16x8 &b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
-// A tile in LDS is its 32 rows of eight 16-byte pieces, piece c of row r at c ^ piece_swap(r): 16-byte reads of
-// one piece of eight rows and of four pieces of two rows, and transpose reads of 16 features of four rows,
-// all meet every bank alike.
-__device__ __forceinline__ int piece_swap(int r) { return ((r & 1) << 2) | ((r >> 1) & 3); }
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-// Lane l: feature l % 32 of keys 4 (l / 32) .. + 3, from the address of 4 features of key 4 (l / 32) + l % 16 / 4
-// (16 (l / 16 % 2) + 4 (l % 4) on)
-__device__ __forceinline__ uint2 ld_transposed(const bf16_t *p) {
-  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p));
-}
 typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
 typedef float f32x2v __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pk2bf(float x0, float x1) {
