@@ -1009,18 +1009,12 @@ __global__ void __launch_bounds__(64 * NW) chord_decode_mfma_kernel(ChordArgs a,
       u.w = pb[6] | (static_cast<uint32_t>(pb[7]) << 16);
       pB = __builtin_bit_cast(bf16x8, u);
     }
-    // O^T += V^T P^T per 16-feature tile
+    // O^T += V^T P^T per 16-feature tile: feature 16 ft + c16 of keys 4 g .. + 3 and 16 + 4 g .. + 3
 #pragma unroll
     for (int ft = 0; ft < 4; ++ft) {
-      const int e = 16 * ft + c16;
-      uint32_t wv[4];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const bf16_t *col = myV + (16 * h + 4 * g) * kVRow + e;
-        wv[2 * h] = col[0] | (static_cast<uint32_t>(col[kVRow]) << 16);
-        wv[2 * h + 1] = col[2 * kVRow] | (static_cast<uint32_t>(col[3 * kVRow]) << 16);
-      }
-      const bf16x8 vA = __builtin_bit_cast(bf16x8, uint4{wv[0], wv[1], wv[2], wv[3]});
+      const bf16_t *vp = myV + (4 * g + (c16 >> 2)) * kVRow + 16 * ft + 4 * (c16 & 3);
+      const uint2 v0 = ld_transposed(vp), v1 = ld_transposed(vp + 16 * kVRow);
+      const bf16x8 vA = __builtin_bit_cast(bf16x8, uint4{v0.x, v0.y, v1.x, v1.y});
       o[ft] *= resc;
       o[ft] = mma16(vA, pB, o[ft]);
     }
