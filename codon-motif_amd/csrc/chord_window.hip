@@ -5,7 +5,7 @@
 //
 // chord_window_kernel: flash attention whose key loop visits the tiles that hold first tokens and
 // those that the block's windows reach, and no others.  With a window every query block has the same
-// work, so the workgroups are small and even: PARTS parts of two waves, a part taking its run of the
+// work, so the workgroups are small and even: PARTS (two or four) parts of two waves, a part taking its run of the
 // 32-key tiles.  A wave owns 32 score columns (16 queries of two heads that share a kv head, or 32 of
 // one head): S^T = K Q^T on v_mfma_f32_32x32x16_bf16, lane l column l % 32, register r of lane half h
 // key 8 (r / 4) + 4 h + r % 4; P^T enters O^T += V^T P^T from the same registers, V^T stored in LDS in
@@ -325,11 +325,22 @@ __global__ void __launch_bounds__(128 * PARTS) __attribute__((amdgpu_waves_per_e
   }
 }
 
+// Key parts of a workgroup: four where the blocks are at most three for every two CUs and a block's tiles at
+// least 12, so that the parts shorten its chain by more than they cost to join.  Measured, us, 12 heads,
+// two parts / four: 3 kv heads, 512 tokens (96 blocks), a window of 512 11.7 / 10.1; 1024 (192) 256 9.3 / 9.2,
+// 1024 19.1 / 15.2; 1500 (282) 600 16.2 / 14.9; 2048 (384) 256 11.6 / 12.6, 1024 24.1 / 21.5; 3000 (564) 1024
+// 27.9 / 27.7; 4096 (768) 1024 32.1 / 34.9; 300 (57) 128 7.2 / 7.7; 12 kv heads, 1024 (192) 512 12.9 / 11.1, 2048
+// (384) 512 17.2 / 16.1.  One part: 8192 tokens, 1024 63.5 (two: 56.7), 2 x 2048 25.3 (20.8).
 template <int HPW>
 int launch_window_h(const ChordArgs &a, int nseq, int max_len, hipStream_t s) {
   constexpr int kQ = HPW == 4 ? 16 : HPW == 2 ? 32 : 64;
   const dim3 grid(a.H / HPW, (max_len + kQ - 1) / kQ, nseq);
-  (a.dist ? chord_window_kernel<HPW, 2, true> : chord_window_kernel<HPW, 2, false>)<<<grid, dim3(256), 0, s>>>(a);
+  const int64_t blocks = int64_t(grid.x) * grid.y * grid.z;
+  const int keys = std::min(a.cu ? max_len : std::min(a.S, a.q_start + a.L), a.window + kQ + std::min(a.sinks, kMaxWindow / 2));
+  if (2 * blocks <= 3 * chord_cu_count() && keys >= 12 * kT)
+    (a.dist ? chord_window_kernel<HPW, 4, true> : chord_window_kernel<HPW, 4, false>)<<<grid, dim3(512), 0, s>>>(a);
+  else
+    (a.dist ? chord_window_kernel<HPW, 2, true> : chord_window_kernel<HPW, 2, false>)<<<grid, dim3(256), 0, s>>>(a);
   return check_launch("chord_window_kernel");
 }
 

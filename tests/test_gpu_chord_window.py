@@ -40,6 +40,11 @@ SHAPES = [
     (1, 4, 2, 150, 150, 0, 128, 40, 2),
     (1, 4, 2, 60, 150, 90, 24, 40, 2),     # head dims between the kernels'
     (1, 2, 2, 3, 90, 87, 80, 17, 5),
+    (1, 4, 2, 500, 500, 0, 64, 450, 3),    # long windows of few blocks
+    (2, 4, 1, 130, 700, 570, 64, 400, 20),
+    (1, 3, 3, 433, 600, 167, 64, 600, 0),
+    (1, 4, 4, 60, 500, 480, 64, 900, 1),   # queries past the keys
+    (1, 8, 2, 90, 450, 700, 64, 380, 0),   # the last of them see nothing
 ]
 
 

@@ -76,6 +76,8 @@ SHAPES = [
     (1, 4, 2, 40, 16, 100, 16, 2),
     (1, 4, 2, 1, 300, 299, 100, 4),
     (2, 2, 2, 3, 500, 300, 100, 4),      # keys behind the last query
+    (1, 4, 2, 480, 480, 0, 420, 2),      # a long window of few blocks
+    (2, 2, 1, 100, 620, 520, 500, 0),
 ]
 
 
