@@ -41,9 +41,9 @@
 // every block has about the same work, so nothing is cut but the queries that see a block's first tokens
 // from behind its windows (plan_bwd_window).  The distances' powers come from a 64-bit table: in
 // registers they took 20 instructions a score where 12 are left, and were the parameter gradients'
-// largest error.  2 x 2048 tokens, 12 heads, window 512: dQ 44 us, dK / dV 39, reduction 4, table 3;
-// 4001 tokens, 3 kv heads, window 1000: 69, 63, 9, 3.  At these lengths no unit is busy half of the time
-// (4001 tokens: VALU 48% and 30% of the busy cycles, LDS 25% and 36%, MFMA 20%): 1.5 workgroups per CU,
+// largest error.  2 x 2048 tokens, 12 heads, window 512: dQ 43 us, dK / dV 37, reduction 4, table 3;
+// 4001 tokens, 3 kv heads, window 1000: 68, 60, 10, 3.  At these lengths no unit is busy half of the time
+// (4001 tokens: VALU 49% and 31% of the busy cycles, LDS 26% and 35%, MFMA 20%): 1.5 workgroups per CU,
 // a wave or two per SIMD, each a chain of reads, products, exponentials and a barrier a tile.
 #include <algorithm>
 #include <string>
@@ -117,7 +117,7 @@ __device__ __forceinline__ bf16x8 pack8(const float *x) {
 }
 __device__ __forceinline__ uint4 ld16(const bf16_t *p) { return *reinterpret_cast<const uint4 *>(p); }
 
-// Tile staging by 128 threads t: row t >> 2, 8-element pieces t & 3 and + 4 of a
+// Tile staging by 128 threads t: row stage_row(t), 8-element pieces t & 3 and + 4 of a
 // 32-row x 64 tile of [rows][64] bf16 rows, through a range-checked buffer that starts at the
 // tile's first row (uniform) and ends at row `nrows` of the matrix: rows past it read 0 with no
 // branch, and a tile costs two loads and its base.  The loads go to registers one tile ahead of the
@@ -133,11 +133,11 @@ struct StageSrc {
   int nrows;
   uint32_t off;  // this thread's first piece
   __device__ __forceinline__ StageSrc(const bf16_t *p, int64_t s, int n, int t)
-      : base(p), st(s), nrows(n), off(static_cast<uint32_t>(((t >> 2) * s + 8 * (t & 3)) * 2)) {}
+      : base(p), st(s), nrows(n), off(static_cast<uint32_t>((stage_row(t) * s + 8 * (t & 3)) * 2)) {}
   __device__ __forceinline__ Stage2 load(int row0) const { return load(row0, min(kT, nrows - row0)); }
   __device__ __forceinline__ Stage2 load(int row0, int rows) const {
     if constexpr (ANY) {
-      const int r = (threadIdx.x & 127) >> 2;
+      const int r = stage_row(threadIdx.x & 127);
       const bf16_t *p = base + (row0 + r) * st + 8 * (threadIdx.x & 3);
       const uint4 z = {0u, 0u, 0u, 0u};
       return {r < rows ? ld16(p) : z, r < rows ? ld16(p + 32) : z};
@@ -148,7 +148,7 @@ struct StageSrc {
 };
 // The pieces into the tile's rows.
 __device__ __forceinline__ void stage_store(const Stage2 &g, int t, bf16_t *rows) {
-  const int o = (t >> 2) * kBD + 8 * ((t & 3) ^ piece_swap(t >> 2));
+  const int r = stage_row(t), o = r * kBD + 8 * ((t & 3) ^ piece_swap(r));
   *reinterpret_cast<uint4 *>(rows + o) = g.a;
   *reinterpret_cast<uint4 *>(rows + (o ^ 32)) = g.b;
 }

@@ -110,10 +110,14 @@ template <int TS> struct KeyWalk {
   }
 };
 
-// A tile of 64 features in LDS (the windowed prefill's and the backward's) is 32 rows of eight 16-byte pieces, piece c of row r at c ^ piece_swap(r): 16-byte reads of
-// one piece of eight rows and of four pieces of two rows, and transpose reads of 16 features of four rows,
-// all meet every bank alike.
-__device__ __forceinline__ int piece_swap(int r) { return ((r & 1) << 2) | ((r >> 1) & 3); }
+// A tile of 64 features in LDS (the windowed prefill's and the backward's) is 32 rows of eight 16-byte pieces,
+// piece c of row r at c ^ piece_swap(r): 16-byte reads of one piece of eight rows, transpose reads of 16
+// features of four rows, and stores of four pieces of two rows in stage_row's order meet the banks alike.
+// (Rows stored in their own order collide: 8.7M conflict cycles at 8192 tokens where 2.8M are left; so did the
+// transpose reads with the swap's bits the other way round, 5.7M.)
+__device__ __forceinline__ int piece_swap(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
+// The row that thread t of 128 stores pieces t % 4 and + 4 of
+__device__ __forceinline__ int stage_row(int t) { const int r = t >> 2; return (r & ~3) | ((r & 1) << 1) | ((r >> 1) & 1); }
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 // Lane l: feature l % 32 of keys 4 (l / 32) .. + 3, from the address of 4 features of key 4 (l / 32) + l % 16 / 4
 // (16 (l / 16 % 2) + 4 (l % 4) on)

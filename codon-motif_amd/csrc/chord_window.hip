@@ -8,8 +8,8 @@
 // work, so the workgroups are small and even: PARTS (two or four) parts of two waves, a part taking its run of the
 // 32-key tiles.  A wave owns 32 score columns (16 queries of two heads that share a kv head, or 32 of
 // one head): S^T = K Q^T on v_mfma_f32_32x32x16_bf16, lane l column l % 32, register r of lane half h
-// key 8 (r / 4) + 4 h + r % 4; P^T enters O^T += V^T P^T from the same registers, V^T stored in LDS in
-// that key order.  K / V tiles are double buffered in LDS, one barrier a tile, the tile after next in
+// key 8 (r / 4) + 4 h + r % 4; P^T enters O^T += V^T P^T from the same registers, V transposed in that
+// key order as it is read from LDS.  K / V tiles are double buffered in LDS, one barrier a tile, the tile after next in
 // registers.  The distance bias, the diagonal and the window's edge are one value per distance: 47
 // (two heads) or 63 distances meet in a tile, 32 of them new, so each lane evaluates one per tile
 // (-inf where the distance is masked) into its wave's LDS row, and the score accumulators start from
@@ -18,9 +18,9 @@
 // the bf16 that the matrix instructions take (P's rounding, 2^-9 in the mean of a weight, is the
 // output's own).
 // Bound by VALU issue: a score takes some ten instructions and an exponential at a quarter of the rate,
-// four times its matrix instructions' time (8192 tokens, window 2048: the vector unit issues in 67% of
-// the busy cycles, the matrix unit in 22%), which puts the floor of this form at 2.5 times the
-// products'.  12 heads on 3 kv heads: 4096 tokens, window 1024 32 us (350 TFLOP/s of visible pairs; a
+// three times its matrix instructions' time (8192 tokens, window 2048: the vector unit issues in 64% of
+// the busy cycles, LDS is read or written in 43%, the matrix unit works in 23%), which puts the floor of
+// this form at 2.5 times the products'.  12 heads on 3 kv heads: 4096 tokens, window 1024 32 us (350 TFLOP/s of visible pairs; a
 // large library product 1190), 8192 and 2048 97 us (470); as chord_wide_kernel 113 and 349.  16 packed
 // sequences of 115 to 528 tokens 16 us in one launch (one by one 301).
 #include <algorithm>
@@ -155,9 +155,9 @@ __global__ void __launch_bounds__(128 * PARTS) __attribute__((amdgpu_waves_per_e
   // this lane's entries for keys 8 q4 + 4 hh + (0..3): j = 8 q4 + p + 4 hh - cq + RQ - 1
   const float *bwr = &sB[wv][(lc / RQ) * kWin] + 4 * hh - cq + RQ - 1;
 
-  // Staging by the part's 128 threads: row htid / 4, pieces htid % 4 and + 4
+  // Staging by the part's 128 threads: row stage_row(htid), pieces htid % 4 and + 4
   uint4 kst[2], vst[2];
-  const int srow = htid >> 2;
+  const int srow = stage_row(htid);
   const uint32_t koff = static_cast<uint32_t>((srow * a.k_st + (htid & 3) * 8) * 2);
   const uint32_t voff = static_cast<uint32_t>((srow * a.v_st + (htid & 3) * 8) * 2);
   const int sto = srow * kBD + 8 * ((htid & 3) ^ piece_swap(srow));
