@@ -722,16 +722,16 @@ __global__ void __launch_bounds__(256) chord_decode_kernel(ChordArgs a, const fl
 //   same features).  The accumulator gives lane l the scores of row l % 16 for keys
 //   4 g + i, so the softmax statistics of a row live in the 4 lanes l % 16 + 16 g.
 //   O^T += V^T P^T -- B = P^T straight from the scores (slots 0..3: tile 0 keys 4 g + i,
-//   slots 4..7: tile 1 keys 16 + 4 g + i), A = V^T with the same key slots, gathered
-//   from the wave's V tile in LDS (V rows are loaded with 16-byte coalesced reads and
-//   written row-major).  O^T's accumulator gives lane l features 16 ft + 4 g + i of
+//   slots 4..7: tile 1 keys 16 + 4 g + i), A = V^T with the same key slots, transposed
+//   as it is read from the wave's V tile in LDS (V rows are loaded with 16-byte coalesced
+//   reads and written row-major).  O^T's accumulator gives lane l features 16 ft + 4 g + i of
 //   row l % 16, so no cross-lane sum is needed for O.
 // The GGD bias of each (row, key) is evaluated in registers (one exp2 / log2 pair), so
 // this kernel needs no bias table.  The next step's K / V loads are issued before the
 // current step's arithmetic.
 constexpr int kMfmaRows = 16;
 constexpr int kDecodeWaves = 16;  // of an unsplit windowed call
-constexpr int kVRow = 72;  // LDS V row stride (bf16): 144 bytes, conflict-free gathers
+constexpr int kVRow = 72;  // LDS V row stride (bf16): 144 bytes, conflict-free transpose reads
 
 // The whole decode step of a Chord layer in one launch (motif_chord_decode_step): q, k
 // and v come from the layer's projection rows, q and k RMSNormed here exactly as
