@@ -243,10 +243,19 @@ class StaticKVLayerCache(KVLayerCache):
     def workspace(self, key: tuple, make) -> Optional[torch.Tensor]:
         '''The decode kernels' scratch for steps of this kind (`make()` on its first use): one
         per key = (kind, tokens a step, ...), since a size is laid out for its own steps, and all
-        of them kept, since a captured step holds its address.'''
+        of them kept, since a captured step holds its address.  (One that a capture makes is the
+        graph's alone: its zeros are written as the graph runs.)'''
         if key not in self._workspaces:
-            self._workspaces[key] = make()
+            made = make()
+            if made is not None and made.is_cuda and torch.cuda.is_current_stream_capturing():
+                return made
+            self._workspaces[key] = made
         return self._workspaces[key]
+
+    @property
+    def decode_workspace(self) -> Optional[torch.Tensor]:
+        '''The decode kernel's scratch used first, None before.'''
+        return next((w for key, w in self._workspaces.items() if key[0] == 'decode'), None)
 
     @property
     def step_workspace(self) -> Optional[torch.Tensor]:

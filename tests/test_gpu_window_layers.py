@@ -264,3 +264,36 @@ def test_one_launch_step_of_many_shares(B, L, length, window, sinks):
         slabs.append(cache._slab)
     assert all(torch.equal(a, b) for a, b in zip(*slabs))
     assert_bf16_close(outs[0], outs[1])
+
+
+@pytest.mark.parametrize('kind', ['rows', 'window', 'kv4'])
+@torch.no_grad()
+def test_a_step_of_another_length_captured_first(kind):
+    '''A two-token step whose first run is a capture, after one-token steps: its replays, and eager steps
+    of both lengths among them, equal eager steps throughout.'''
+    from motif.model.cache import KV4LayerCache, StaticKVLayerCache
+    layer = _layer(BF, **(dict(window=700, sinks=2) if kind == 'window' else {}))
+    x = _x(2, 1420, BF)
+    caches = [(KV4LayerCache if kind == 'kv4' else StaticKVLayerCache)().allocate(2, 2, 1500, 64, DEV, BF) for _ in range(2)]
+    step = lambda cache, t: layer(t, past_key_value=cache).output
+    for cache in caches:
+        step(cache, x[:, :1400])
+        step(cache, x[:, 1400:1401])
+    buf, graph = x[:, :2].clone(), torch.cuda.CUDAGraph()
+    length = caches[0].length
+    with torch.cuda.graph(graph):
+        got = step(caches[0], buf)
+    caches[0].length = length
+    at = 1401
+    for n in (2, 2, 1, 2, -2, 1, 2):  # (-2: an eager step of two)
+        part = x[:, at:at + abs(n)]
+        if n == 2:
+            buf.copy_(part)
+            graph.replay()
+            caches[0].advance(2)
+            a = got
+        else:
+            a = step(caches[0], part)
+        assert torch.equal(a, step(caches[1], part)), at
+        at += abs(n)
+    assert int(caches[0].length_dev) == int(caches[1].length_dev) == caches[0].length == at

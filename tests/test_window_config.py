@@ -105,3 +105,9 @@ def test_kv4_cache_on_the_host():
     assert all(type(c) is KV4LayerCache for c in made.layer_caches())
     plain = ModelCache.for_decode(model, 1, 8, 'cpu', torch.float32)
     assert not any(isinstance(c, KV4LayerCache) for c in plain.layer_caches())
+    static = plain.layer_caches()
+    for c in static:
+        assert c.step_workspace is None and c.decode_workspace is None
+        made = c.workspace(('decode', 1, None, 0), lambda: torch.zeros(3))
+        assert c.decode_workspace is made and c.workspace(('decode', 1, None, 0), lambda: None) is made
+        assert c.workspace(('decode', 2, None, 0), lambda: torch.zeros(4)).numel() == 4 and c.step_workspace is None
