@@ -31,7 +31,7 @@
 // the same loop over the tiles of the first tokens and of the block's windows: the general forms of every
 // type, head dim and query count, beside the bf16 and fp16 kernels at head dim 64 (chord_window.hip,
 // chord_kv4.hip and the windowed decode of chord.hip).  2 x 517 fp32 queries over 1023 keys, window 259:
-// 29 us, the matrix pipe busy 27% of the time (408 short blocks, three tiles a wave: each wave's chain).
+// 25 us, the matrix pipe busy a third of the time (408 short blocks, five tiles a wave: each wave's chain).
 #include <algorithm>
 #include <type_traits>
 
@@ -424,10 +424,22 @@ int launch_wide(const ChordArgs &a, const KV4Args &kv, hipStream_t s) {
 }
 
 // A window's blocks are short and many: where they pass one per CU, four waves each let two blocks
-// share a CU (2 x 517 fp32 queries over 1023 keys, 408 blocks, windows of 128 / 259 / 1023: eight waves
-// 37 / 49 / 74 us, four 27 / 37 / 67); where they do not, eight waves shorten the chain.
+// share a CU (2 x 517 fp32 queries over 1023 keys, 408 blocks, windows of 128 / 259 / 1023, before keys came
+// in late: eight waves 37 / 49 / 74 us, four 27 / 37 / 67); where they do not, eight waves shorten the chain.
+// fp32 at head dim 64, which two waves per SIMD leave short of registers (88 bytes a lane are spilled), takes one
+// wave per SIMD where the chain is at most 24 tiles, and half as many waves.  Measured, us, 12 heads on 3, 517
+// queries over 1023 keys, as above / one per SIMD: two sequences, windows of 259 / 600 / 1023 29.7 / 24.9, 45.6 / 40.8,
+// 59.2 / 60.4; one sequence 259 / 1023 19.5 / 16.5, 32.0 / 33.2; 64 tokens 10.3 / 8.3; 1024 under 1024 45.3 / 60.1.
+// (fp16 2 x 517, 259: 14.8 / 15.4; fp32 at head dim 32 13.6 / 15.0.)
 template <typename T, int D, int MODE>
 int launch_wide_n(const ChordArgs &a, const KV4Args &kv, hipStream_t s) {
+  if constexpr (MODE == kWindow && sizeof(T) == 4 && D == 64) {
+    const int keys = std::min(a.len_dev ? a.S : std::min(a.S, a.q_start + a.L), a.window + 31 + std::min(a.sinks, kMaxWindow / 2));
+    if (keys <= 24 * 32) {
+      if (static_cast<int64_t>(a.H) * ((a.L + 31) / 32) * a.B > chord_cu_count()) return launch_wide<T, D, 2, MODE, 1>(a, kv, s);
+      return launch_wide<T, D, 4, MODE, 1>(a, kv, s);
+    }
+  }
   if constexpr (MODE != kCausal) {
     if (static_cast<int64_t>(a.H) * ((a.L + 31) / 32) * a.B > chord_cu_count()) return launch_wide<T, D, 4, MODE, 2>(a, kv, s);
   }

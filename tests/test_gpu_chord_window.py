@@ -45,6 +45,9 @@ SHAPES = [
     (1, 3, 3, 433, 600, 167, 64, 600, 0),
     (1, 4, 4, 60, 500, 480, 64, 900, 1),   # queries past the keys
     (1, 8, 2, 90, 450, 700, 64, 380, 0),   # the last of them see nothing
+    (3, 12, 3, 250, 250, 0, 64, 70, 2),    # more blocks than CUs
+    (3, 12, 3, 250, 1100, 850, 64, 1000, 2),
+    (1, 2, 1, 40, 1000, 960, 64, 900, 0),  # one short block under a long window
 ]
 
 
