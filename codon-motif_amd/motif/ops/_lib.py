@@ -157,6 +157,8 @@ def available() -> bool:
 
 def lib():
     '''The loaded library; raises RuntimeError when it cannot be loaded.'''
+    if _lib is not None:
+        return _lib
     _load()
     if _lib is None:
         raise RuntimeError(
@@ -180,11 +182,13 @@ def check(rc: int, what: str):
     raise RuntimeError(f'{what}: {msg}')
 
 
+_CHORD_CODES = {torch.float32: MOTIF_F32, torch.bfloat16: MOTIF_BF16, torch.float16: MOTIF_F16}
+
+
 def chord_dtype_code(dt: torch.dtype) -> int:
     '''dtype code of the Chord attention entries, which also take fp16.'''
-    if dt == torch.float16:
-        return MOTIF_F16
-    return dtype_code(dt)
+    code = _CHORD_CODES.get(dt)
+    return dtype_code(dt) if code is None else code
 
 
 def dtype_code(dt: torch.dtype) -> int:
