@@ -890,45 +890,48 @@ __global__ void __launch_bounds__(64 * NW) chord_decode_mfma_kernel(ChordArgs a,
   if constexpr (STEP) {
     // The new positions [q_start, q_start + L) this split holds: wave 0 appends their key
     // (RMSNormed, chord_prep_kernel's order: an fma chain per lane, then the 8-lane
-    // butterfly) and value rows, lane = 32 (value?) + 8 t + piece, before any load of
-    // this workgroup reads them; no other workgroup reads these positions.
+    // butterfly) and value rows, four positions at a time, lane = 32 (value?) + 8 (t % 4) + piece,
+    // before any load of this workgroup reads them; no other workgroup reads these positions.
     if (w == 0) {
-      const int is_v = lane >> 5, t = (lane >> 3) & 3, piece = lane & 7;
-      const int pos = q_start + t;
-      // (a new position is never before the window's start)
-      const bool mine = t < a.L && pos < a.S &&
-                        (WIN ? (walk.ns + (pos - walk.lo) / 32) / max(x_per, 1) == split : pos >= k_lo && pos < k_lo + per);
-      const bf16_t *src = sa.proj + b * sa.p_sb + int64_t(min(t, a.L - 1)) * sa.p_st + (is_v ? sa.v_off : sa.k_off) +
-                          kvh * kD + 8 * piece;
-      const uint4 u = *reinterpret_cast<const uint4 *>(src);
+      const int is_v = lane >> 5, piece = lane & 7;
       const uint4 wr = *reinterpret_cast<const uint4 *>(sa.kw + 8 * piece);
-      float x[8], wk[8];
-      const uint32_t ua[4] = {u.x, u.y, u.z, u.w}, wa[4] = {wr.x, wr.y, wr.z, wr.w};
+      for (int t0 = 0; t0 < a.L; t0 += 4) {
+        const int t = t0 + ((lane >> 3) & 3);
+        const int pos = q_start + t;
+        // (a new position is never before the window's start)
+        const bool mine = t < a.L && pos < a.S &&
+                          (WIN ? (walk.ns + (pos - walk.lo) / 32) / max(x_per, 1) == split : pos >= k_lo && pos < k_lo + per);
+        const bf16_t *src = sa.proj + b * sa.p_sb + int64_t(min(t, a.L - 1)) * sa.p_st + (is_v ? sa.v_off : sa.k_off) +
+                            kvh * kD + 8 * piece;
+        const uint4 u = *reinterpret_cast<const uint4 *>(src);
+        float x[8], wk[8];
+        const uint32_t ua[4] = {u.x, u.y, u.z, u.w}, wa[4] = {wr.x, wr.y, wr.z, wr.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[2 * i] = __uint_as_float(ua[i] << 16); x[2 * i + 1] = __uint_as_float(ua[i] & 0xffff0000u);
-        wk[2 * i] = __uint_as_float(wa[i] << 16); wk[2 * i + 1] = __uint_as_float(wa[i] & 0xffff0000u);
-      }
-      float ss = 0.f;
+        for (int i = 0; i < 4; ++i) {
+          x[2 * i] = __uint_as_float(ua[i] << 16); x[2 * i + 1] = __uint_as_float(ua[i] & 0xffff0000u);
+          wk[2 * i] = __uint_as_float(wa[i] << 16); wk[2 * i + 1] = __uint_as_float(wa[i] & 0xffff0000u);
+        }
+        float ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
 #pragma unroll
-      for (int off = 1; off < 8; off <<= 1) ss += __shfl_xor(ss, off, 64);
-      uint4 o = u;
-      if (!is_v) {
-        const float rs = rsqrtf(ss / kD + sa.neps);
-        uint32_t ow[4];
+        for (int off = 1; off < 8; off <<= 1) ss += __shfl_xor(ss, off, 64);
+        uint4 o = u;
+        if (!is_v) {
+          const float rs = rsqrtf(ss / kD + sa.neps);
+          uint32_t ow[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          ow[i] = static_cast<uint32_t>(f32_to_bf16(bf16_to_f32(f32_to_bf16(x[2 * i] * rs)) * wk[2 * i])) |
-                  (static_cast<uint32_t>(f32_to_bf16(bf16_to_f32(f32_to_bf16(x[2 * i + 1] * rs)) * wk[2 * i + 1]))
-                   << 16);
-        o = uint4{ow[0], ow[1], ow[2], ow[3]};
-      }
-      if (mine) {
-        bf16_t *dst = is_v ? static_cast<bf16_t *>(const_cast<void *>(a.v)) + b * a.v_sb + kvh * a.v_sh + int64_t(pos) * a.v_st
-                           : static_cast<bf16_t *>(const_cast<void *>(a.k)) + b * a.k_sb + kvh * a.k_sh + int64_t(pos) * a.k_st;
-        *reinterpret_cast<uint4 *>(dst + 8 * piece) = o;
+          for (int i = 0; i < 4; ++i)
+            ow[i] = static_cast<uint32_t>(f32_to_bf16(bf16_to_f32(f32_to_bf16(x[2 * i] * rs)) * wk[2 * i])) |
+                    (static_cast<uint32_t>(f32_to_bf16(bf16_to_f32(f32_to_bf16(x[2 * i + 1] * rs)) * wk[2 * i + 1]))
+                     << 16);
+          o = uint4{ow[0], ow[1], ow[2], ow[3]};
+        }
+        if (mine) {
+          bf16_t *dst = is_v ? static_cast<bf16_t *>(const_cast<void *>(a.v)) + b * a.v_sb + kvh * a.v_sh + int64_t(pos) * a.v_st
+                             : static_cast<bf16_t *>(const_cast<void *>(a.k)) + b * a.k_sb + kvh * a.k_sh + int64_t(pos) * a.k_st;
+          *reinterpret_cast<uint4 *>(dst + 8 * piece) = o;
+        }
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
