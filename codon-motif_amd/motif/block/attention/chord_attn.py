@@ -451,7 +451,11 @@ class ChordAttention(BasicAttention):
                 logits = logits.masked_fill(~keep, float('-inf'))
             else:
                 logits = logits + attention_mask
-        weights = torch.softmax(logits, dim=-1)
+        if self.window is None:
+            weights = torch.softmax(logits, dim=-1)
+        else:  # a row that sees no key (a mask may hide its whole window) gives zeros, as on the kernels
+            empty = (logits == float('-inf')).all(-1, keepdim=True)
+            weights = torch.softmax(logits.masked_fill(empty, 0.), dim=-1).masked_fill(empty, 0.)
         out = self._merge_heads(torch.matmul(weights.to(vf.dtype), vf))
         out = self.o_proj(out) * torch.sigmoid(g)
         payload = None
