@@ -59,15 +59,19 @@ const char *kv4_check(const KV4Args &kv, int D);  // what is wrong with a cache'
 __device__ __forceinline__ float kv4_scale(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float kv4_base(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
+constexpr float kBf16Max = 0x1.fep+127f;
 // A lane's N features of a row, LPG lanes to a group: their codes (4 bits each from the lowest on) and the
-// group's pair.  Every lane of the group calls it.
-template <int N, int LPG> __device__ __forceinline__ uint32_t kv4_codes(const float (&x)[N], uint32_t &pair) {
-  float lo = x[0], hi = x[0], bad = x[0] * 0.f;
+// group's pair.  Every lane of the group calls it.  Features past bf16's largest number M (fp32 ones only)
+// count as M: with every |x| <= M = (1 - 2^-8) fp32's largest, neither the base's rounding nor 15 times
+// the scale's (2^-8 of them) takes a value past fp32's range.
+template <int N, int LPG> __device__ __forceinline__ uint32_t kv4_codes(float (&x)[N], uint32_t &pair) {
+  float lo = INFINITY, hi = -INFINITY, bad = 0.f;
 #pragma unroll
-  for (int e = 1; e < N; ++e) {
+  for (int e = 0; e < N; ++e) {
+    bad = fmaf(x[e], 0.f, bad);  // NaN once any feature is not finite
+    x[e] = __builtin_amdgcn_fmed3f(x[e], -kBf16Max, kBf16Max);
     lo = fminf(lo, x[e]);
     hi = fmaxf(hi, x[e]);
-    bad = fmaf(x[e], 0.f, bad);  // NaN once any feature is not finite
   }
 #pragma unroll
   for (int off = 1; off < LPG; off <<= 1) {

@@ -6,7 +6,7 @@
 //   base = bf16(min x), scale = bf16((max x - min x) / 15), code = rint((x - base) / scale) in 0 .. 15,
 //   value = code * scale + base.
 // Both ends of the range are held (a code for either), so features with an offset lose nothing; bf16
-// keeps every input's range, and its rounding of base and scale (2^-9 of them) is small beside half a
+// keeps the inputs' range (fp32 features past bf16's largest number, 3.3895e38, count as that), and its rounding of base and scale (2^-9 of them) is small beside half a
 // step (1 / 30 of the range).  The quotient is an IEEE division, so that a value exactly between two
 // codes goes to the even one on every machine.  A group that holds an infinity or a NaN gets a NaN
 // scale: its values read back NaN, no other group's do.  So does one whose max - min passes fp32's

@@ -95,7 +95,8 @@ def kv4_append(slab: KV4Slab, k: torch.Tensor, v: torch.Tensor, start) -> None:
     [start, start + n) of the slab.  `start` is an int, or a device int32 tensor of one
     entry that the kernel reads (for a captured step; rows past the capacity are then
     dropped).  A group of features that holds an infinity or a NaN, or whose
-    range passes fp32's largest number, reads back as NaN.'''
+    range passes fp32's largest number, reads back as NaN; fp32 features past bf16's
+    largest (3.3895e38) count as that.'''
     if wants_grad(k, v):
         raise RuntimeError('kv4_append is forward-only: detach the rows or call it under no_grad')
     (B, Hkv, cap, D), args = _check_slab(slab, 'kv4_append')
