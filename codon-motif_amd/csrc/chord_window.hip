@@ -49,14 +49,17 @@ __device__ __forceinline__ uint32_t pk2bf(float x0, float x1) {
 // x^beta and its derivatives' factors at distances d = 0, -1, .. of a head, x = |d - mu| + eps:
 // dist[h][-d] = {x^beta, x^beta log2 x}, dmu[h][-d] = x^(beta - 1) sign(d - mu).  In 64 bits and rounded
 // once: through fp32 log2 and exp2 the power is 3e-7 off, which the scaled logits turn into 1e-5 of a
-// weight, and the parameter gradients are small differences of sums over weights.
+// weight, and the parameter gradients are small differences of sums over weights.  At distance x = 0 (eps 0, mu
+// a whole number) x^beta log2 x is taken as 0, its limit beside a beta
+// above 0, and x^0 as 1.
 __global__ void __launch_bounds__(256) chord_distance_kernel(const float *beta, const float *mu, float eps, float2 *dist,
                                                              float *dmu, int n) {
   const int h = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
-  const double e = -static_cast<double>(i) - mu[h], x = fabs(e) + eps, l = log2(x), p = exp2(beta[h] * l);
+  const double e = -static_cast<double>(i) - mu[h], x = fabs(e) + eps, l = log2(x);
+  const double p = beta[h] == 0.f ? 1. : exp2(beta[h] * l);
   const size_t o = static_cast<size_t>(h) * n + i;
-  dist[o] = float2{static_cast<float>(p), static_cast<float>(p * l)};
+  dist[o] = float2{static_cast<float>(p), x == 0. && beta[h] >= 0.f ? 0.f : static_cast<float>(p * l)};
   dmu[o] = e == 0. ? 0.f : static_cast<float>(e > 0. ? p / x : -p / x);
 }
 
