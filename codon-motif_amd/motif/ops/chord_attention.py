@@ -645,8 +645,14 @@ def chord_decode_cursor(q, k_cache, v_cache, length_dev, alpha, beta, mu, ssmax,
     window, sinks = check_window(window, sinks)
     B, H, L, D = q.shape
     Hkv, cap = k_cache.shape[1], k_cache.shape[2]
-    if length_dev.dtype != torch.int32 or length_dev.device != q.device:
+    if length_dev.dtype != torch.int32 or length_dev.device != q.device or not length_dev.numel():
         raise ValueError('chord_decode_cursor: length_dev must be a device int32 tensor')
+    if k_cache.stride(-1) != 1 or v_cache.stride(-1) != 1:
+        raise ValueError('chord_decode_cursor: the caches must have unit feature stride')
+    if log_n is not None and (log_n.shape != (B, L) or log_n.dtype != torch.float32 or log_n.device != q.device):
+        raise ValueError(f'chord_decode_cursor: log_n must be fp32 {(B, L)} on q\'s device')
+    if workspace is not None and workspace.device != q.device:
+        raise ValueError('chord_decode_cursor: workspace must live on q\'s device')
     if log_table.dtype != torch.float32 or log_table.numel() < cap:
         raise ValueError('chord_decode_cursor: log_table must be fp32 with at least `capacity` entries')
     if softmax_scale is None:
@@ -660,10 +666,9 @@ def chord_decode_cursor(q, k_cache, v_cache, length_dev, alpha, beta, mu, ssmax,
             raise ValueError('chord_decode_cursor: more queries than the capacity')
         _check_params(alpha, beta, mu, ssmax, H)
         if k_cache.shape != v_cache.shape or k_cache.shape[0] != B or k_cache.shape[3] != D or H % Hkv \
-                or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype or not log_table.is_contiguous() \
-                or log_n is not None and (log_n.shape != (B, L) or log_n.dtype != torch.float32):
+                or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype or not log_table.is_contiguous():
             raise ValueError(f'chord_decode_cursor: q {tuple(q.shape)} does not fit the caches {tuple(k_cache.shape)} and '
-                             f'{tuple(v_cache.shape)}, their dtype, log_n or log_table')
+                             f'{tuple(v_cache.shape)}, their dtype or log_table')
         for t in (k_cache, v_cache, log_table, alpha, beta, mu, ssmax):
             if t.get_device() != q.get_device():
                 raise ValueError('chord_decode_cursor: the tensors of a call must live on one device')
