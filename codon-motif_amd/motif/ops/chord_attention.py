@@ -599,6 +599,70 @@ def chord_decode_step_workspace(B, H, Hkv, L, capacity, device, window=None, sin
     return torch.zeros(max(n, 1), dtype=torch.uint8, device=device)
 
 
+def _step_fits(proj, offsets, norms, caches, length_dev, params, log_table, H, workspace):
+    '''Whether chord_decode_step's tensors pass _check_step, asked for at once.'''
+    at, bf, f32 = proj.get_device(), torch.bfloat16, torch.float32
+    shape, (k, v) = proj.shape, caches
+    ks = k.shape
+    if at < 0 or len(shape) != 3 or len(ks) != 4 or ks != v.shape or len(offsets) != 3:
+        return False
+    B, Hkv, cap, D = ks
+    oq, ok, ov = offsets
+    if D != HEAD_DIM or shape[0] != B or H < 1 or not Hkv or H % Hkv or H // Hkv * shape[1] > 16 \
+            or oq < 0 or ok < 0 or ov < 0 or oq + H * D > shape[2] or (ok if ok > ov else ov) + Hkv * D > shape[2] \
+            or proj.dtype != bf or k.dtype != bf or v.dtype != bf \
+            or proj.stride(2) != 1 or k.stride(3) != 1 or v.stride(3) != 1 \
+            or k.get_device() != at or v.get_device() != at \
+            or length_dev.get_device() != at or length_dev.dtype != torch.int32 or not length_dev.numel() \
+            or log_table.get_device() != at or log_table.dtype != f32 or log_table.numel() < cap \
+            or not log_table.is_contiguous() \
+            or workspace.get_device() != at or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        return False
+    for t in params:
+        if t.get_device() != at or t.dtype != f32 or t.dim() != 1 or t.numel() != H or not t.is_contiguous():
+            return False
+    for t in norms:
+        if t.get_device() != at or t.dtype != bf or t.dim() != 1 or t.numel() != D or not t.is_contiguous():
+            return False
+    return True
+
+
+def _check_step(proj, offsets, norms, caches, length_dev, params, log_table, H, workspace):
+    '''ValueError where chord_decode_step's tensors are not what motif_chord_decode_step reads behind
+    their pointers.'''
+    what, (k, v) = 'chord_decode_step', caches
+    shape, ks = proj.shape, k.shape
+    if len(ks) != 4 or ks != v.shape or ks[3] != HEAD_DIM or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 \
+            or k.stride()[3] != 1 or v.stride()[3] != 1:
+        raise ValueError(f'{what}: the caches must be bf16 [B, Hkv, capacity, {HEAD_DIM}] of unit feature stride, got '
+                         f'{tuple(ks)} {k.dtype} and {tuple(v.shape)} {v.dtype}')
+    B, Hkv, cap, D = ks
+    if len(shape) != 3 or shape[0] != B or proj.dtype != torch.bfloat16 or proj.stride()[2] != 1:
+        raise ValueError(f'{what}: proj must be bf16 [{B}, L, columns] of unit column stride, got {tuple(shape)} {proj.dtype}')
+    if H < 1 or not Hkv or H % Hkv:
+        raise ValueError(f'{what}: {H} query heads do not share {Hkv} kv heads')
+    if (H // Hkv) * shape[1] > 16:
+        raise ValueError(f'{what}: {shape[1]} tokens of {H // Hkv} query heads a kv head pass 16 query rows')
+    if len(offsets) != 3 or min(offsets) < 0 or max(offsets[0] + H * D, max(offsets[1:]) + Hkv * D) > shape[2]:
+        raise ValueError(f'{what}: {H} heads of {D} over {Hkv} kv heads do not fit the columns {offsets} of {shape[2]}')
+    if any(t.shape != (D,) or t.dtype != torch.bfloat16 or not t.is_contiguous() for t in norms):
+        raise ValueError(f'{what}: norm weights must be contiguous bf16 [{D}]')
+    if length_dev.dtype != torch.int32 or not length_dev.numel():
+        raise ValueError(f'{what}: length_dev must be a device int32 tensor')
+    if any(t.shape != (H,) or t.dtype != torch.float32 or not t.is_contiguous() for t in params):
+        raise ValueError(f'{what}: the head parameters must be contiguous fp32 [{H}]')
+    if log_table.dtype != torch.float32 or log_table.numel() < cap or not log_table.is_contiguous():
+        raise ValueError(f'{what}: log_table must be contiguous fp32 with at least `capacity` entries')
+    if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise ValueError(f'{what}: workspace must be chord_decode_step_workspace\'s')
+    dev = proj.device
+    for t in (*norms, k, v, length_dev, *params, log_table, workspace):
+        if t.device != dev:
+            raise ValueError(f'{what}: the tensors of a call must live on one device, got {dev} and {t.device}')
+    if not proj.is_cuda:
+        raise ValueError(f'{what}: proj must live on CUDA')
+
+
 def chord_decode_step(proj, offsets, q_norm_weight, k_norm_weight, norm_eps, k_cache, v_cache, length_dev, alpha,
                       beta, mu, ssmax, log_table, num_heads, softmax_scale, eps, workspace, window=None, sinks=0):
     '''A Chord decode step at the device cursor in one launch (new; the reference's
@@ -611,6 +675,11 @@ def chord_decode_step(proj, offsets, q_norm_weight, k_norm_weight, norm_eps, k_c
     chord_decode_cursor.  `window` / `sinks` limit what a query sees, as for
     apply_chord_attention (the sums then run over other splits than chord_decode_cursor's).'''
     window, sinks = check_window(window, sinks)
+    offsets = [int(o) for o in offsets]
+    args = (proj, offsets, (q_norm_weight, k_norm_weight), (k_cache, v_cache), length_dev, (alpha, beta, mu, ssmax),
+            log_table, num_heads, workspace)
+    if not _step_fits(*args):
+        _check_step(*args)
     B, L = proj.shape[0], proj.shape[1]
     Hkv, cap, D = k_cache.shape[1], k_cache.shape[2], k_cache.shape[3]
     out = torch.empty(B, num_heads, L, D, dtype=proj.dtype, device=proj.device)
@@ -618,7 +687,7 @@ def chord_decode_step(proj, offsets, q_norm_weight, k_norm_weight, norm_eps, k_c
     fn, limits = (lib.motif_chord_decode_step, ()) if window is None else (lib.motif_chord_window_step, (window, sinks))
     with _lib.on_device(proj.device):
         rc = fn(
-            proj.data_ptr(), proj.stride(0), proj.stride(1), *[int(o) for o in offsets],
+            proj.data_ptr(), proj.stride(0), proj.stride(1), *offsets,
             q_norm_weight.data_ptr(), k_norm_weight.data_ptr(), float(norm_eps),
             *_lib.t4(k_cache), *_lib.t4(v_cache), length_dev.data_ptr(), cap,
             alpha.data_ptr(), beta.data_ptr(), mu.data_ptr(), ssmax.data_ptr(), log_table.data_ptr(), log_table.numel(),
