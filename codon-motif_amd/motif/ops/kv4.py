@@ -28,7 +28,8 @@ GROUP = 32  # features that share a (scale, base) pair
 
 
 class KV4Slab(NamedTuple):
-    '''The four tensors of a 4-bit cache (positions back to back, any batch / head strides).'''
+    '''The four tensors of a 4-bit cache (positions back to back, any batch / head strides; one whose
+    batch rows or heads share memory, an expanded one, is for reading only).'''
     k_codes: torch.Tensor
     k_params: torch.Tensor
     v_codes: torch.Tensor
@@ -53,7 +54,7 @@ def kv4_alloc(batch: int, kv_heads: int, capacity: int, head_dim: int, device) -
     return KV4Slab(z(codes, torch.uint8), z(params, torch.bfloat16), z(codes, torch.uint8), z(params, torch.bfloat16))
 
 
-def _check_slab(slab: KV4Slab, what: str):
+def _check_slab(slab: KV4Slab, what: str, writes: bool = False):
     '''((B, Hkv, capacity, D), the entry points' arguments), or ValueError.'''
     kc, kp, vc, vp = slab
     shape = kc.shape
@@ -68,11 +69,6 @@ def _check_slab(slab: KV4Slab, what: str):
     if vc.shape != shape or kp.shape != pshape or vp.shape != pshape \
             or kp.dtype != torch.bfloat16 or vp.dtype != torch.bfloat16:
         raise ValueError(f'{what}: codes of keys and values must have one shape, params must be bfloat16 {pshape}')
-    at = kc.get_device()
-    if at < 0:
-        raise ValueError(f'{what}: the cache must live on CUDA')
-    if kp.get_device() != at or vc.get_device() != at or vp.get_device() != at:
-        raise ValueError(f'{what}: the cache tensors must live on one device')
     args = []
     for c, p in ((kc, kp), (vc, vp)):
         cs, ps, cp, pp = c.stride(), p.stride(), c.data_ptr(), p.data_ptr()
@@ -81,7 +77,14 @@ def _check_slab(slab: KV4Slab, what: str):
                 raise ValueError(f'{what}: rows of codes must lie back to back on 4-byte boundaries')
             if ps[4] != 1 or (G > 1 and ps[3] != 2) or (cap > 1 and ps[2] != 2 * G) or pp & 3 or (ps[0] | ps[1]) & 1:
                 raise ValueError(f'{what}: rows of params must lie back to back on 4-byte boundaries')
+        if writes and (B > 1 and not (cs[0] and ps[0]) or Hkv > 1 and not (cs[1] and ps[1])):
+            raise ValueError(f'{what}: the rows or heads of the cache share memory')
         args += (cp, cs[0], cs[1], pp, ps[0] >> 1, ps[1] >> 1)
+    at = kc.get_device()
+    if at < 0:
+        raise ValueError(f'{what}: the cache must live on CUDA')
+    if kp.get_device() != at or vc.get_device() != at or vp.get_device() != at:
+        raise ValueError(f'{what}: the cache tensors must live on one device')
     return (B, Hkv, cap, D), args
 
 
@@ -99,7 +102,7 @@ def kv4_append(slab: KV4Slab, k: torch.Tensor, v: torch.Tensor, start) -> None:
     largest (3.3895e38) count as that.'''
     if wants_grad(k, v):
         raise RuntimeError('kv4_append is forward-only: detach the rows or call it under no_grad')
-    (B, Hkv, cap, D), args = _check_slab(slab, 'kv4_append')
+    (B, Hkv, cap, D), args = _check_slab(slab, 'kv4_append', writes=True)
     if k.shape != v.shape or k.dim() != 4 or k.shape[:2] != (B, Hkv) or k.shape[3] != D:
         raise ValueError(f'kv4_append: k / v must be [{B}, {Hkv}, n, {D}], got {tuple(k.shape)} and {tuple(v.shape)}')
     if k.dtype != v.dtype or k.device != slab.k_codes.device or v.device != k.device:
@@ -152,7 +155,7 @@ def chord_kv4_prep(proj: torch.Tensor, offsets, q_norm_weight: torch.Tensor, k_n
     normalised, and the normalised keys and the values written in 4 bits at positions length_dev ..
     (a device int32, read and not advanced; rows past the capacity are dropped).  The same bits as the
     norms followed by kv4_append.'''
-    (B, Hkv, cap, D), args = _check_slab(slab, 'chord_kv4_prep')
+    (B, Hkv, cap, D), args = _check_slab(slab, 'chord_kv4_prep', writes=True)
     if wants_grad(proj, q_norm_weight, k_norm_weight):
         raise RuntimeError('chord_kv4_prep is forward-only: call it under no_grad')
     if proj.dim() != 3 or proj.shape[0] != B or proj.stride(-1) != 1 or proj.dtype not in (torch.bfloat16, torch.float32):
