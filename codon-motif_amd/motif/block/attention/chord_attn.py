@@ -394,7 +394,7 @@ class ChordAttention(BasicAttention):
         q = chord_kv4_prep(proj, (0, hs, hs + self.kv_dim), self.q_norm.weight.to(dt).contiguous(),
                            self.k_norm.weight.to(dt).contiguous(), self.q_norm.eps, cache.slab, cache.length_dev,
                            self.num_heads)
-        work = cache.workspace(('kv4', L, self.window, self.sinks), lambda: chord_decode_kv4_workspace(
+        work = cache.workspace(('kv4', L, dt, self.window, self.sinks), lambda: chord_decode_kv4_workspace(
             B, self.num_heads, self.num_kv_heads, L, cache.capacity, self.head_dim, proj.dtype, proj.device, self.window,
             self.sinks))
         return chord_decode_kv4_cursor(q, cache.slab, cache.length_dev, alpha, beta, mu, ssmax, cache.log_table,

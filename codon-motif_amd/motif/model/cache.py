@@ -310,10 +310,17 @@ class StaticKVLayerCache(KVLayerCache):
 
     def to(self, device=None, dtype=None):
         if self._slab is not None:
-            self._slab = tuple(t.to(device=device, dtype=dtype) for t in self._slab)
-            self.length_dev = self.length_dev.to(device=device)
-            self._workspaces = {}
+            self._place(tuple(t.to(device=device, dtype=dtype) for t in self._slab), self.length_dev.to(device=device))
         return self
+
+    def _place(self, slab, length_dev) -> None:
+        '''Take these for the slab and the cursor; what belongs to the old ones (scratch, the log
+        table) is dropped where they are others, and kept where nothing moved (a captured step may
+        hold all of it).'''
+        if any(a is not b for a, b in zip((*slab, length_dev), (*self._slab, self.length_dev))):
+            self._workspaces = {}
+            self.__dict__.pop('log_table', None)
+        self._slab, self.length_dev = slab, length_dev
 
 
 class KV4LayerCache(StaticKVLayerCache):
@@ -385,10 +392,8 @@ class KV4LayerCache(StaticKVLayerCache):
     def to(self, device=None, dtype=None):
         '''Moves the slab; `dtype` is that of the values read back.'''
         if self._slab is not None:
-            self._slab = KV4Slab(*(t.to(device=device) for t in self._slab))
-            self.length_dev = self.length_dev.to(device=device)
+            self._place(KV4Slab(*(t.to(device=device) for t in self._slab)), self.length_dev.to(device=device))
             self._dtype = dtype or self._dtype
-            self._workspaces = {}
         return self
 
 
