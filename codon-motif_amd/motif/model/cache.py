@@ -245,6 +245,8 @@ class StaticKVLayerCache(KVLayerCache):
         per key = (kind, tokens a step, ...), since a size is laid out for its own steps, and all
         of them kept, since a captured step holds its address.  (One that a capture makes is the
         graph's alone: its zeros are written as the graph runs.)'''
+        if key not in self._workspaces and (key[0],) in self._workspaces:  # the caller's own, for the first to ask
+            self._workspaces[key] = self._workspaces.pop((key[0],))
         if key not in self._workspaces:
             made = make()
             if made is not None and made.is_cuda and torch.cuda.is_current_stream_capturing():
@@ -252,15 +254,32 @@ class StaticKVLayerCache(KVLayerCache):
             self._workspaces[key] = made
         return self._workspaces[key]
 
+    def _scratch(self, kind: str) -> Optional[torch.Tensor]:
+        return next((w for key, w in self._workspaces.items() if key[0] == kind), None)
+
+    def _set_scratch(self, kind: str, value: Optional[torch.Tensor]) -> None:
+        self._workspaces = {key: w for key, w in self._workspaces.items() if key[0] != kind}
+        if value is not None:
+            self._workspaces[(kind,)] = value
+
     @property
     def decode_workspace(self) -> Optional[torch.Tensor]:
-        '''The decode kernel's scratch used first, None before.'''
-        return next((w for key, w in self._workspaces.items() if key[0] == 'decode'), None)
+        '''The decode kernel's scratch used first, None before.  Set: the next step's (None: a new one).'''
+        return self._scratch('decode')
+
+    @decode_workspace.setter
+    def decode_workspace(self, value: Optional[torch.Tensor]) -> None:
+        self._set_scratch('decode', value)
 
     @property
     def step_workspace(self) -> Optional[torch.Tensor]:
-        '''The one-launch decode step's scratch (zeroed once) used first, None before.'''
-        return next((w for key, w in self._workspaces.items() if key[0] == 'step'), None)
+        '''The one-launch decode step's scratch (zeroed once) used first, None before.  Set: the next
+        step's (None: a new one).'''
+        return self._scratch('step')
+
+    @step_workspace.setter
+    def step_workspace(self, value: Optional[torch.Tensor]) -> None:
+        self._set_scratch('step', value)
 
     @property
     def row_dtype(self) -> Optional[torch.dtype]:
