@@ -795,8 +795,12 @@ static WinBwdPlan plan_bwd_window(int B, int H, int Hkv, int L, int S, int q_sta
   int most = 0;  // query tiles behind a window that see first tokens
   for (int kb = 0; kb < p.nsb; ++kb)
     most = std::max(most, qt_end - std::max(kv_window_end(kb, L, q_start, window), kv_first_tile(kb, q_start)));
-  // chunks about as long as a window's loop, at most 16 of them
-  p.csink = std::max({8, (window + kBlk) / kT, (most + 15) / 16});
+  // chunks about as long as a window's loop, at most 16 of them and no more than make 2048 workgroups, eight per
+  // CU: each is a copy of the blocks' fp32 partials (at 8192 tokens, 12 heads, every second of them a first
+  // token, 16 are 403 MB, 5 are 126)
+  const int64_t blocks = static_cast<int64_t>(p.nsb) * H * B;
+  const int cap = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(16, 2048 / std::max<int64_t>(1, blocks))));
+  p.csink = std::max({8, (window + kBlk) / kT, (most + cap - 1) / cap});
   p.nsc = (most + p.csink - 1) / p.csink;
   p.kv_direct = H == Hkv;
   p.prows = p.kv_direct ? p.nsb * kBlk : S;
