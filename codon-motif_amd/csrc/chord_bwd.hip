@@ -45,7 +45,10 @@
 // largest error.  2 x 2048 tokens, 12 heads, window 512: dQ 43 us, dK / dV 37, reduction 4, table 3;
 // 4001 tokens, 3 kv heads, window 1000: 68, 60, 10, 3.  At these lengths no unit is busy half of the time
 // (4001 tokens: VALU 49% and 31% of the busy cycles, LDS 26% and 35%, MFMA 20%): 1.5 workgroups per CU,
-// a wave or two per SIMD, each a chain of reads, products, exponentials and a barrier a tile.
+// a wave or two per SIMD, each a chain of reads, products, exponentials and a barrier a tile.  P and P (dP -
+// Delta) are rounded to bf16 where they enter the products for dQ, dK and dV, as in the causal kernels, since
+// the matrix instructions' fp32 form would take 16 times as long (2.4e-3 off against 64 bits, where rounding the
+// gradients alone gives 1.7e-3); the parameter sums take them in fp32.
 #include <algorithm>
 #include <string>
 #include <type_traits>

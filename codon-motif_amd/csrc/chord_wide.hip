@@ -31,7 +31,8 @@
 // the same loop over the tiles of the first tokens and of the block's windows: the general forms of every
 // type, head dim and query count, beside the bf16 and fp16 kernels at head dim 64 (chord_window.hip,
 // chord_kv4.hip and the windowed decode of chord.hip).  2 x 517 fp32 queries over 1023 keys, window 259:
-// 25 us, the matrix pipe busy a third of the time (408 short blocks, five tiles a wave: each wave's chain).
+// 24 us, the matrix pipe busy 38% of the CUs' busy cycles and the vector unit 33% (408 short blocks of two
+// waves, five tiles a wave: each wave's chain).
 #include <algorithm>
 #include <type_traits>
 

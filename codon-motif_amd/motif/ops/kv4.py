@@ -129,7 +129,8 @@ def kv4_append(slab: KV4Slab, k: torch.Tensor, v: torch.Tensor, start) -> None:
 
 def kv4_read(slab: KV4Slab, start: int, n: int, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     '''The values of positions [start, start + n) as (k, v), new [B, Hkv, n, D] tensors of
-    `dtype` (fp16, bf16 or fp32; the fp32 value rounded once).'''
+    `dtype` (fp16, bf16 or fp32; the fp32 value rounded once, in fp16 held at +-65504 where
+    rounding would give an infinity).'''
     (B, Hkv, cap, D), args = _check_slab(slab, 'kv4_read')
     start, n = int(start), int(n)
     if start < 0 or n < 0 or start + n > cap:

@@ -524,7 +524,7 @@ int motif_chord_window_step(
  * Table of the bias's distances for motif_chord_window_fwd / _bwd: n = motif_chord_distances_len(..)
  * entries per head (3 * H * n floats, 8-byte aligned) in 64-bit arithmetic, with
  * x_d = |-d - mu_h| + eps: out[h][d] = {x_d^beta, x_d^beta log2 x_d} for d = 0 .. n - 1, then
- * x_d^(beta - 1) sign(-d - mu_h).
+ * x_d^(beta - 1) sign(-d - mu_h).  Where x_d is 0: {0, 0} for beta > 0, {1, 0} for beta 0.
  */
 int motif_chord_distances_len(int L, int q_start, int window, int sinks);
 int motif_chord_distances(const float *beta, const float *mu, int H, int n, float eps, float *out, void *stream);
@@ -565,8 +565,11 @@ int motif_chord_window_bwd(
  * motif_kv4_append writes n rows of k / v [B,Hkv,n,D] (fp32, fp16 or bf16, 16-byte aligned rows)
  * at `position`, or at *position_dev (read, not advanced; rows at or past `capacity` are dropped):
  *   base = bf16(min), scale = bf16((max - min) / 15), code = rint((x - base) / scale) held to
- *   0 .. 15, over each group; a group with an infinity or a NaN reads back NaN.
- * motif_kv4_read gives the values of n rows from `position` on as k / v [B,Hkv,n,D].
+ *   0 .. 15, over each group; a group with an infinity or a NaN reads back NaN, features past
+ *   bf16's largest number (3.3895e38, fp32 rows only) count as that.  No two (batch row, kv head)
+ *   pairs may share memory.
+ * motif_kv4_read gives the values of n rows from `position` on as k / v [B,Hkv,n,D], the fp32 value
+ * rounded once (fp16 rows: values past 65504 are held there).
  */
 int motif_kv4_append(const void *k, int64_t k_sb, int64_t k_sh, int64_t k_st,
                      const void *v, int64_t v_sb, int64_t v_sh, int64_t v_st,
