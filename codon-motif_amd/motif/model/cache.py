@@ -291,7 +291,7 @@ class StaticKVLayerCache(KVLayerCache):
         self._slab = (torch.zeros(shape, device=device, dtype=dtype), torch.zeros(shape, device=device, dtype=dtype))
         self.length = 0
         self.length_dev = torch.zeros(1, dtype=torch.int32, device=device)
-        self._workspaces = {}
+        self._forget()
         return self
 
     def _room(self, like, n):
@@ -337,9 +337,12 @@ class StaticKVLayerCache(KVLayerCache):
         table) is dropped where they are others, and kept where nothing moved (a captured step may
         hold all of it).'''
         if any(a is not b for a, b in zip((*slab, length_dev), (*self._slab, self.length_dev))):
-            self._workspaces = {}
-            self.__dict__.pop('log_table', None)
+            self._forget()
         self._slab, self.length_dev = slab, length_dev
+
+    def _forget(self) -> None:
+        self._workspaces = {}
+        self.__dict__.pop('log_table', None)
 
 
 class KV4LayerCache(StaticKVLayerCache):
@@ -364,7 +367,7 @@ class KV4LayerCache(StaticKVLayerCache):
         self._dtype = dtype
         self.length = 0
         self.length_dev = torch.zeros(1, dtype=torch.int32, device=device)
-        self._workspaces = {}
+        self._forget()
         return self
 
     @property
