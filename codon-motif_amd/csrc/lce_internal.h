@@ -1,0 +1,156 @@
+// Softmax cross entropy straight from hidden states X [N, d] and the vocabulary's rows W [V, d]
+// (linear_ce.hip: the entries and the row kernels; lce_general.hip: fp32 matrix products for every
+// type, size and alignment; lce_bf16.hip: bf16 on the matrix instructions).
+//
+// With z_iv = x_i . w_v, s_i the gradient of row i's loss and t_i its label:
+//   loss_i = log sum_v e^{z_iv} - z_{i t_i}
+//   P_iv   = s_i (e^{z_iv} / sum_u e^{z_iu} - [v = t_i]),  dX = P W,  dW = P^T X
+// The forward keeps one number per row (the base-2 log-sum-exp); the backward forms P again in
+// pieces of the vocabulary and multiplies each piece on both sides.  Rows without a label are
+// taken out first: every product runs over the `count` rows that have one, in their order.
+#pragma once
+
+#include "capi_internal.h"
+#include "common.h"
+
+namespace motif {
+
+struct LceArgs {
+  const void *x;       // [count, ldx]: the labelled rows
+  const void *w;       // [V, d], row stride ldw
+  int64_t ldx, ldw;
+  int N, d, V;
+  const int *row;      // [N] original row of labelled row i
+  const int *label;    // [N] its label (-1: outside the vocabulary; loss and gradient are NaN)
+  const int *pos;      // [N] labelled position of original row r, or -1
+  const int *count;    // labelled rows
+  float *part_m, *part_s;  // [nparts, N] maxima (times log2 e) and sums of a vocabulary part
+  float *at_label;     // [N] z at the label
+  float *lse;          // [N] base-2 log-sum-exp of z log2 e
+  const float *dloss;  // gradient of the loss(es)
+  int64_t dl_st;       // 0: one for all rows
+  int mean;            // divided by count
+  void *p;             // P of a vocabulary piece (layout: the kernels' own)
+  int v0, vc, vn;      // the piece: first vocabulary row, rows laid out, rows of the vocabulary in it
+  float *dx_part;      // [dx_splits, n_pad, d] fp32
+  int64_t n_pad;
+  int dx_splits, first;  // first: the first piece (nothing to add to)
+  void *dw;            // [V, d]
+};
+
+// A wave's accumulators of 32 x 32 products with the vocabulary (or P's rows) on the left: register
+// i of lane l is row 8 (i / 4) + 4 (l / 32) + i % 4, column l % 32.
+__device__ __forceinline__ int acc_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
+
+// log-sum-exp pairs (m, s) = (max, sum 2^{z - m}); an empty pair is (-inf, 0)
+__device__ __forceinline__ void lse_merge(float &m, float &s, float m2, float s2) {
+  const float top = fmaxf(m, m2);
+  const float ref = top == -INFINITY ? 0.f : top;
+  s = s * fast_exp2(m - ref) + s2 * fast_exp2(m2 - ref);
+  m = top;
+}
+
+// Forward: the pair of a wave's MB x 32 vocabulary rows from v0 for each of its NB x 32 tokens from t0,
+// into part `part`, and z at the labels among them.
+template <int MB, int NB>
+__device__ __forceinline__ void lce_row_stats(const LceArgs &a, f32x16 (&acc)[MB][NB], int v0, int t0, int count, int part) {
+  const int l = threadIdx.x & 63, h = l >> 5;
+  if (v0 + 32 * MB > a.V) {
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (v0 + 32 * mb + acc_row(i, h) >= a.V)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) acc[mb][nb][i] = -INFINITY;
+  }
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int t = t0 + 32 * nb + (l & 31);
+    const bool live = t < count;
+    const int rel = live ? a.label[t] - v0 : -1;
+    if (live && rel >= 0 && rel < 32 * MB && ((rel >> 2) & 1) == h && a.label[t] >= 0) {
+      float z = 0.f;
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (rel == 32 * mb + acc_row(i, h)) z = acc[mb][nb][i];
+      a.at_label[t] = z;
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) m = fmaxf(m, acc[mb][nb][i]);
+    m *= kLog2e;
+    const float ref = m == -INFINITY ? 0.f : m;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i & 3] += fast_exp2(fmaf(acc[mb][nb][i], kLog2e, -ref));
+    float sum = (s[0] + s[1]) + (s[2] + s[3]);
+    lse_merge(m, sum, __shfl_xor(m, 32, 64), __shfl_xor(sum, 32, 64));
+    if (live && h == 0) {
+      a.part_m[int64_t(part) * a.N + t] = m;
+      a.part_s[int64_t(part) * a.N + t] = sum;
+    }
+  }
+}
+
+// The gradient of labelled row t's loss (NaN for a label outside the vocabulary)
+__device__ __forceinline__ float lce_row_scale(const LceArgs &a, int t, int count) {
+  float s = a.dloss[a.dl_st ? int64_t(a.row[t]) * a.dl_st : 0];
+  if (a.mean) s /= static_cast<float>(count);
+  return a.label[t] < 0 ? __builtin_nanf("") : s;
+}
+
+// Backward: P over the same accumulators, in place; 0 behind the last labelled row and the vocabulary.
+template <int MB, int NB>
+__device__ __forceinline__ void lce_row_grads(const LceArgs &a, f32x16 (&acc)[MB][NB], int v0, int t0, int count) {
+  const int l = threadIdx.x & 63, h = l >> 5;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int t = t0 + 32 * nb + (l & 31);
+    const bool live = t < count;
+    const float lse = live ? a.lse[t] : 0.f, scale = live ? lce_row_scale(a, t, count) : 0.f;
+    const int rel = live ? a.label[t] - v0 : -1;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[mb][nb][i] = fast_exp2(fmaf(acc[mb][nb][i], kLog2e, -lse));
+    if (rel >= 0 && rel < 32 * MB && ((rel >> 2) & 1) == h) {
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (rel == 32 * mb + acc_row(i, h)) acc[mb][nb][i] -= 1.f;
+    }
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float p = acc[mb][nb][i] * scale;
+        acc[mb][nb][i] = live ? p : 0.f;  // (a row of infinities in W times no row is no number)
+      }
+  }
+  if (v0 + 32 * MB > a.V) {
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (v0 + 32 * mb + acc_row(i, h) >= a.V)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) acc[mb][nb][i] = 0.f;
+  }
+}
+
+// lce_general.hip: the products on fp32 matrix instructions, any alignment (P is fp32 [N, vc])
+int lce_general_parts(int V);
+int launch_lce_general_stats(const LceArgs &a, int dtype, hipStream_t s);
+int launch_lce_general_grads(const LceArgs &a, int dtype, hipStream_t s);  // P of the piece
+int launch_lce_general_dx(const LceArgs &a, int dtype, hipStream_t s);
+int launch_lce_general_dw(const LceArgs &a, int dtype, hipStream_t s);
+
+}  // namespace motif

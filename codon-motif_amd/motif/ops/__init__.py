@@ -22,6 +22,9 @@ from .short_conv import short_conv_silu, short_conv_silu_multi, short_conv_silu_
 from .attn_res import apply_block_attn_res, attn_res_read, attn_res_read_norms
 from .gdn_decode import gdn_decode_fused
 from .linear_rows import cat_weights, linear_rows, project, rows_eligible
+from .linear_ce import linear_cross_entropy
+from .norm import layer_norm_rows, rms_norm_rows
+from .dropout import dropout_add
 
 HAS_TRITON = _lib.available()
 HAS_HIP = HAS_TRITON
@@ -37,5 +40,6 @@ __all__ = [
     'short_conv_silu', 'short_conv_silu_multi', 'short_conv_silu_varlen',
     'apply_block_attn_res', 'attn_res_read', 'attn_res_read_norms', 'gdn_decode_fused',
     'cat_weights', 'linear_rows', 'project', 'rows_eligible',
+    'linear_cross_entropy', 'rms_norm_rows', 'layer_norm_rows', 'dropout_add',
     'HAS_TRITON', 'HAS_HIP',
 ]

@@ -18,6 +18,8 @@ MOTIF_F16 = 2
 
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int
+_U32 = ctypes.c_uint32
+_U64 = ctypes.c_uint64
 _P = ctypes.c_void_p
 _F32 = ctypes.c_float
 _SZ = ctypes.c_size_t
@@ -122,6 +124,17 @@ _SIGNATURES = {
     'motif_chord_bwd': (
         _T4 * 5 + [_P] * 5 + [_P, _I64, _I64] + _T4 * 3 + [_P] + [_I32] * 7 + [_F32, _F32]
         + [_P, _SZ, _I32, _P], _I32),
+    'motif_linear_ce_rows_bytes': ([_I32] * 3, _SZ),
+    'motif_linear_ce_workspace_bytes': ([_I32] * 5, _SZ),
+    'motif_linear_ce_fwd': (
+        [_P, _I64, _P, _I64, _P, _I64, _I64] + [_I32] * 4 + [_P, _P, _P, _P, _SZ, _I32, _P], _I32),
+    'motif_linear_ce_bwd': (
+        [_P, _P, _I64, _P, _P, _I64] + [_I32] * 4 + [_P, _P, _P, _SZ, _I32, _P], _I32),
+    'motif_row_norm_bwd_workspace_bytes': ([_I32] * 3, _SZ),
+    'motif_row_norm_fwd': ([_P, _I64, _P, _P, _P, _I64, _P, _P, _I32, _I32, _F32, _I32, _I32, _P], _I32),
+    'motif_row_norm_bwd': (
+        [_P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _P, _P] + [_I32] * 3 + [_P, _SZ, _I32, _P], _I32),
+    'motif_dropout_add': ([_P, _P, _P, _I64, _U32, _F32, _U64, _P, _I32, _P], _I32),
 }
 
 EXPORTED = tuple(_SIGNATURES)

@@ -1,0 +1,115 @@
+'''Softmax cross entropy straight from hidden states, the logits never stored
+(csrc/linear_ce.hip; the reference forms the logits and calls F.cross_entropy on them,
+motif/model/motif.py:600-628).
+'''
+import torch
+
+from . import _lib
+from .autograd_path import wants_grad
+
+_REDUCTIONS = {'none': 0, 'sum': 1, 'mean': 2}
+
+
+class LinearCEFunction(torch.autograd.Function):
+    '''motif_linear_ce_fwd / motif_linear_ce_bwd: gradients for x [N, d] and weight [V, d].
+
+    What is kept for the backward: the labelled rows of x (a copy), the weight and 16 bytes a
+    row.  The backward's scratch is P in pieces of the vocabulary (256 MB, or 4096 vocabulary
+    rows where that is more) and the partial sums of x's gradient in fp32.'''
+
+    @staticmethod
+    def forward(ctx, x, weight, labels, ignore_index, reduction):
+        N, d = x.shape
+        V = weight.shape[0]
+        dev, code = x.device, _lib.dtype_code(x.dtype)
+        lib = _lib.lib()
+        rows = torch.empty(lib.motif_linear_ce_rows_bytes(N, d, code), dtype=torch.uint8, device=dev)
+        kept = torch.empty(4 * N + 1, dtype=torch.int32, device=dev)
+        loss = torch.empty((N,) if reduction == 0 else (), dtype=torch.float32, device=dev)
+        nbytes = lib.motif_linear_ce_workspace_bytes(N, d, V, code, 0)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        with _lib.on_device(dev):
+            rc = lib.motif_linear_ce_fwd(
+                x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), labels.data_ptr(), labels.stride(0),
+                ignore_index, N, d, V, reduction, rows.data_ptr(), kept.data_ptr(), loss.data_ptr(), ws.data_ptr(),
+                nbytes, code, _lib.stream_ptr(dev))
+        if rc:
+            _lib.check(rc, 'motif_linear_ce_fwd')
+        if ctx is not None:
+            ctx.save_for_backward(rows, weight, kept)
+            ctx.args = N, d, V, reduction
+        return loss
+
+    @staticmethod
+    def backward(ctx, dloss):
+        if torch.is_grad_enabled():  # (create_graph: what the kernels give carries no graph)
+            raise RuntimeError('linear_cross_entropy has no second derivatives')
+        rows, weight, kept = ctx.saved_tensors
+        N, d, V, reduction = ctx.args
+        dev, dt = weight.device, weight.dtype
+        code = _lib.dtype_code(dt)
+        dx = torch.empty((N, d), dtype=dt, device=dev) if ctx.needs_input_grad[0] else None
+        dw = torch.empty((V, d), dtype=dt, device=dev) if ctx.needs_input_grad[1] else None
+        lib = _lib.lib()
+        nbytes = lib.motif_linear_ce_workspace_bytes(N, d, V, code, 1)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        with _lib.on_device(dev):
+            rc = lib.motif_linear_ce_bwd(
+                rows.data_ptr(), weight.data_ptr(), weight.stride(0), kept.data_ptr(), dloss.data_ptr(),
+                dloss.stride(0) if reduction == 0 else 0, N, d, V, reduction, _lib.ptr(dx), _lib.ptr(dw),
+                ws.data_ptr(), nbytes, code, _lib.stream_ptr(dev))
+        if rc:
+            _lib.check(rc, 'motif_linear_ce_bwd')
+        return dx, dw, None, None, None
+
+
+def _row_major(t):
+    '''t, or a copy, with features beside each other and rows that do not overlap.'''
+    return t if t.stride(1) == 1 and (t.shape[0] < 2 or t.stride(0) >= t.shape[1]) else t.contiguous()
+
+
+def linear_cross_entropy(x, weight, labels, ignore_index=-100, reduction='mean'):
+    '''F.cross_entropy(F.linear(x, weight).float(), labels, ignore_index=, reduction=) without the
+    logits in memory: x [..., d] hidden states, weight [V, d] of the same dtype (bf16 or
+    fp32), labels [...] int64.  Returns fp32: a scalar, or one loss per label for 'none' (0
+    where ignored).  The mean is over the labels that count (NaN when none does).
+
+    Rows whose label is `ignore_index` are left out of every product: they get a zero
+    gradient and nothing that they hold reaches the loss.  A label outside [0, V) that is not
+    `ignore_index` gives NaN (loss and gradients).  Under autocast, x and weight are cast to its
+    dtype, as F.linear does.  Differentiable once in x and weight.'''
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"linear_cross_entropy: reduction must be 'none', 'sum' or 'mean', got {reduction!r}")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f'linear_cross_entropy: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match')
+    if labels.shape != x.shape[:-1]:
+        raise ValueError(f'linear_cross_entropy: labels {tuple(labels.shape)} for x {tuple(x.shape)}')
+    if labels.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f'linear_cross_entropy: labels must be int64, got {labels.dtype}')
+    if weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f'linear_cross_entropy: an empty weight {tuple(weight.shape)}')
+    if weight.device != x.device or labels.device != x.device:
+        raise ValueError(f'linear_cross_entropy: x on {x.device}, weight on {weight.device}, labels on {labels.device}')
+    if torch.is_autocast_enabled(x.device.type):
+        dt = torch.get_autocast_dtype(x.device.type)
+        x, weight = x.to(dt), weight.to(dt)
+    if x.dtype != weight.dtype:
+        raise ValueError(f'linear_cross_entropy: x is {x.dtype}, weight {weight.dtype}')
+    _lib.dtype_code(x.dtype)
+    N, d = labels.numel(), x.shape[-1]
+    if N >= 2 ** 28 or weight.shape[0] > 2 ** 30 or d > 2 ** 20:
+        raise ValueError(f'linear_cross_entropy: {N} rows of {d} features over {weight.shape[0]} are out of range')
+    if not x.is_cuda:
+        raise ValueError(f'linear_cross_entropy: x is on {x.device}, the kernels need a ROCm device')
+    if N == 0:  # (connected to the graph; the sum of nothing, and its mean)
+        zero = x.float().sum() + 0.0 * weight[:0].float().sum()
+        return {'none': zero.expand(labels.shape), 'sum': zero, 'mean': zero * float('nan')}[reduction]
+    red = _REDUCTIONS[reduction]
+    x2, lab = x.reshape(-1, d), labels.reshape(-1).to(torch.int64)
+    x2 = x2 if x2.stride(1) == 1 else x2.contiguous()
+    w = _row_major(weight)
+    if wants_grad(x2, w):
+        loss = LinearCEFunction.apply(x2, w, lab, int(ignore_index), red)
+    else:
+        loss = LinearCEFunction.forward(None, x2, w, lab, int(ignore_index), red)
+    return loss.view(labels.shape) if red == 0 else loss

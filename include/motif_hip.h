@@ -792,6 +792,56 @@ int motif_mul_sigmoid(const void *x, int64_t x_rs, const void *g, int64_t g_rs, 
                       int M, int N, int dtype, void *stream);
 
 /*
+ * Softmax cross entropy straight from hidden states x [N, d] and the vocabulary's rows w [V, d]
+ * (the reference computes the logits and then F.cross_entropy, motif/model/motif.py:600-628), the
+ * logits never stored: loss_i = log sum_v exp(x_i . w_v) - x_i . w_{t_i} in fp32.
+ *   x row stride x_rs, w row stride w_rs >= d, features beside each other; labels int64, stride
+ *   labels_st.  A row whose label is ignore_index has no loss and no gradient, whatever it holds; a
+ *   label outside [0, V) gives a loss and gradients of NaN.
+ *   reduction 0: loss [N] fp32 (0 where ignored); 1: the sum; 2: the mean over the labelled rows
+ *   (NaN when there are none).
+ *   rows (motif_linear_ce_rows_bytes bytes, 16-byte aligned) and kept (4 N + 1 words) are written for
+ *   the backward: the labelled rows beside each other, and which they are with their base-2
+ *   log-sum-exps.
+ * Backward: dloss fp32 ([N] at stride dloss_st for reduction 0, else one value); dx [N, d] and dw
+ * [V, d], contiguous, dtype's type, either may be NULL.  Workspaces 16-byte aligned, of
+ * motif_linear_ce_workspace_bytes(.., backward).  dtype: MOTIF_F32 or MOTIF_BF16.
+ */
+size_t motif_linear_ce_rows_bytes(int N, int d, int dtype);
+size_t motif_linear_ce_workspace_bytes(int N, int d, int V, int dtype, int backward);
+int motif_linear_ce_fwd(const void *x, int64_t x_rs, const void *w, int64_t w_rs, const int64_t *labels,
+                        int64_t labels_st, int64_t ignore_index, int N, int d, int V, int reduction, void *rows,
+                        int *kept, float *loss, void *workspace, size_t workspace_bytes, int dtype, void *stream);
+int motif_linear_ce_bwd(const void *rows, const void *w, int64_t w_rs, const int *kept, const float *dloss,
+                        int64_t dloss_st, int N, int d, int V, int reduction, void *dx, void *dw, void *workspace,
+                        size_t workspace_bytes, int dtype, void *stream);
+
+/*
+ * RMSNorm (layer 0) or LayerNorm (layer 1) of rows x [rows, D] (motif/ops/rms_norm.py:17-113 for the
+ * former), D at most 16384: y = (x - m) r w + b with r = 1 / sqrt(mean((x - m)^2) + eps), m = 0 for
+ * RMSNorm; w and b [D] of x's type or NULL (b: LayerNorm only).  rstd (and mean) [rows] fp32 are
+ * written for the backward unless NULL.  dtype: MOTIF_F32, MOTIF_BF16 or MOTIF_F16; row strides in
+ * elements, features beside each other.
+ * Backward: dx (or NULL), and dw, db [D] (or NULL) with a workspace of
+ * motif_row_norm_bwd_workspace_bytes, 16-byte aligned.
+ */
+size_t motif_row_norm_bwd_workspace_bytes(int rows, int D, int layer);
+int motif_row_norm_fwd(const void *x, int64_t x_rs, const void *w, const void *b, void *y, int64_t y_rs, float *rstd,
+                       float *mean, int rows, int D, float eps, int layer, int dtype, void *stream);
+int motif_row_norm_bwd(const void *dy, int64_t dy_rs, const void *x, int64_t x_rs, const void *w, const float *rstd,
+                       const float *mean, void *dx, int64_t dx_rs, void *dw, void *db, int rows, int D, int layer,
+                       void *workspace, size_t workspace_bytes, int dtype, void *stream);
+
+/*
+ * Dropout of a branch: y_e = residual_e + x_e * scale where word e mod 4 of Philox4x32-10 at counter
+ * (e / 4 as two words, 0, 0) under the 64-bit key is >= threshold, else residual_e (0 without a
+ * residual).  n contiguous elements; the key is *seed_dev, or `seed` when seed_dev is NULL.  The
+ * gradient for x is the same call on dy without a residual.
+ */
+int motif_dropout_add(const void *x, const void *residual, void *y, int64_t n, uint32_t threshold, float scale,
+                      uint64_t seed, const int64_t *seed_dev, int dtype, void *stream);
+
+/*
  * Measurement probes (no reference counterpart): the measured denominators of the
  * roofline fractions bench.py reports beside the published MI355X peaks.
  *   motif_probe_copy       dst = src over `bytes` (a multiple of 16): each byte read
