@@ -1,98 +1,120 @@
 // Cross entropy from hidden states on the fp32 matrix instructions (v_mfma_f32_32x32x2_f32): fp32
 // inputs, and bf16 ones whose rows the bf16 kernels cannot load 16 bytes at a time.  One product,
 // C = A B^T over k, in four uses: z = W X^T (row statistics, or P), dX = P W, dW = P^T X.  A
-// workgroup of four waves owns 128 x 128 of C (64 x 64 a wave) and stages 16 k of both sides in LDS
-// as fp32, k outermost, the next 16 in registers meanwhile; the matrix instruction (64 cycles for two
-// k) bounds it, so LDS reads of single words suffice.
+// workgroup of four waves owns 64 x 64 or 128 x 128 of C and stages 32 or 16 k of both sides in LDS
+// as fp32, k outermost, the next ones in registers meanwhile; the matrix instruction (64 cycles for two
+// k) bounds it, so LDS reads of single words suffice.  Sums run over 512 k at a time, which are then added (one
+// chain over a vocabulary of 5000 lost a bit of dX: 1.3e-6 off where this is 7e-7).
 #include "lce_internal.h"
+
+#include <algorithm>
 
 namespace motif {
 
 namespace {
 
-constexpr int TM = 128, BK = 16, LD = TM + 4;
+// Tiles of TM x TM, TM = 64 MB: one or two blocks of 32 a side for each of the four waves.
+template <int MB> struct Tile {
+  static constexpr int TM = 64 * MB, BK = 2048 / TM, LD = TM + 4, SIZE = BK * LD;
+};
+constexpr int kChain = 512;  // k summed after each other
 
-// 128 rows x 16 k of an operand: element (m, k) at p[m ld + k] (KIN) or p[k ld + m]; zero outside.
-template <typename T, bool KIN> struct Side {
+// TM rows x BK k of an operand: element (m, k) at p[m ld + k] (KIN) or p[k ld + m]; zero outside.
+template <int MB, typename T, bool KIN> struct Side {
+  using X = Tile<MB>;
   const T *p;
   int64_t ld;
   int m_max, k_max;  // elements from p on
   float r[8];
+  __device__ __forceinline__ static int m_of(int i) { return KIN ? threadIdx.x / X::BK + 256 / X::BK * i : threadIdx.x % X::TM; }
+  __device__ __forceinline__ static int k_of(int i) { return KIN ? threadIdx.x % X::BK : threadIdx.x / X::TM + 256 / X::TM * i; }
   __device__ __forceinline__ void load(int k0) {
-    const int t = threadIdx.x;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int m = KIN ? (t >> 4) + 16 * i : t & 127, k = k0 + (KIN ? t & 15 : (t >> 7) + 2 * i);
-      r[i] = m < m_max && k < k_max ? ld_(KIN ? int64_t(m) * ld + k : int64_t(k) * ld + m) : 0.f;
+      const int m = m_of(i), k = k0 + k_of(i);
+      r[i] = m < m_max && k < k_max ? motif::ld(p + (KIN ? int64_t(m) * ld + k : int64_t(k) * ld + m)) : 0.f;
     }
   }
-  __device__ __forceinline__ float ld_(int64_t e) const { return motif::ld(p + e); }
   __device__ __forceinline__ void store(float *s) const {
-    const int t = threadIdx.x;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      s[KIN ? (t & 15) * LD + (t >> 4) + 16 * i : ((t >> 7) + 2 * i) * LD + (t & 127)] = r[i];
+    for (int i = 0; i < 8; ++i) s[k_of(i) * X::LD + m_of(i)] = r[i];
   }
 };
 
-template <typename SA, typename SB>
-__device__ __forceinline__ void product(SA &A, SB &B, int K, float *sa, float *sb, f32x16 (&acc)[2][2]) {
+template <int MB, typename SA, typename SB>
+__device__ __forceinline__ void product(SA &A, SB &B, int kb, int ke, float *sa, float *sb, f32x16 (&sum)[MB][MB]) {
+  using X = Tile<MB>;
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6, h = l >> 5;
+  f32x16 acc[MB][MB];
 #pragma unroll
-  for (int mb = 0; mb < 2; ++mb)
+  for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-    for (int nb = 0; nb < 2; ++nb)
+    for (int nb = 0; nb < MB; ++nb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[mb][nb][i] = 0.f;
-  A.load(0);
-  B.load(0);
-  const float *pa = sa + 64 * (w & 1) + (l & 31), *pb = sb + 64 * (w >> 1) + (l & 31);
-  for (int k0 = 0; k0 < K; k0 += BK) {
+      for (int i = 0; i < 16; ++i) acc[mb][nb][i] = sum[mb][nb][i] = 0.f;
+  if (kb >= ke) return;
+  A.load(kb);
+  B.load(kb);
+  const float *pa = sa + 32 * MB * (w & 1) + (l & 31), *pb = sb + 32 * MB * (w >> 1) + (l & 31);
+  for (int k0 = kb; k0 < ke; k0 += X::BK) {
     __syncthreads();
     A.store(sa);
     B.store(sb);
     __syncthreads();
-    if (k0 + BK < K) {
-      A.load(k0 + BK);
-      B.load(k0 + BK);
+    if (k0 + X::BK < ke) {
+      A.load(k0 + X::BK);
+      B.load(k0 + X::BK);
     }
 #pragma unroll
-    for (int k = 0; k < BK; k += 2) {
-      const int o = (k + h) * LD;
-      const float a0 = pa[o], a1 = pa[o + 32], b0 = pb[o], b1 = pb[o + 32];
-      acc[0][0] = __builtin_amdgcn_mfma_f32_32x32x2f32(a0, b0, acc[0][0], 0, 0, 0);
-      acc[0][1] = __builtin_amdgcn_mfma_f32_32x32x2f32(a0, b1, acc[0][1], 0, 0, 0);
-      acc[1][0] = __builtin_amdgcn_mfma_f32_32x32x2f32(a1, b0, acc[1][0], 0, 0, 0);
-      acc[1][1] = __builtin_amdgcn_mfma_f32_32x32x2f32(a1, b1, acc[1][1], 0, 0, 0);
+    for (int k = 0; k < X::BK; k += 2) {
+      float fa[MB], fb[MB];
+#pragma unroll
+      for (int b = 0; b < MB; ++b) fa[b] = pa[(k + h) * X::LD + 32 * b], fb[b] = pb[(k + h) * X::LD + 32 * b];
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int nb = 0; nb < MB; ++nb)
+          acc[mb][nb] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[mb], fb[nb], acc[mb][nb], 0, 0, 0);
     }
+    if ((k0 - kb) % kChain == kChain - X::BK || k0 + X::BK >= ke)
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int nb = 0; nb < MB; ++nb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            sum[mb][nb][i] += acc[mb][nb][i];
+            acc[mb][nb][i] = 0.f;
+          }
   }
 }
 
-// z of 128 vocabulary rows and 128 tokens, then their statistics or P
-template <typename T, bool GRADS>
+// z of TM vocabulary rows and TM tokens, then their statistics or P
+template <int MB, typename T, bool GRADS>
 __global__ void __launch_bounds__(256) lce_general_z_kernel(LceArgs a) {
-  __shared__ float sa[BK * LD], sb[BK * LD];
+  using X = Tile<MB>;
+  __shared__ float sa[X::SIZE], sb[X::SIZE];
   const int count = __builtin_amdgcn_readfirstlane(*a.count);
-  const int t0 = blockIdx.y * TM, v0 = (GRADS ? a.v0 : 0) + blockIdx.x * TM;
+  const int t0 = blockIdx.y * X::TM, v0 = (GRADS ? a.v0 : 0) + blockIdx.x * X::TM;
   if (t0 >= count) return;
-  Side<T, true> A{static_cast<const T *>(a.w) + int64_t(v0) * a.ldw, a.ldw, a.V - v0, a.d};
-  Side<T, true> B{static_cast<const T *>(a.x) + int64_t(t0) * a.ldx, a.ldx, count - t0, a.d};
-  f32x16 acc[2][2];
-  product(A, B, a.d, sa, sb, acc);
+  Side<MB, T, true> A{static_cast<const T *>(a.w) + int64_t(v0) * a.ldw, a.ldw, a.V - v0, a.d};
+  Side<MB, T, true> B{static_cast<const T *>(a.x) + int64_t(t0) * a.ldx, a.ldx, count - t0, a.d};
+  f32x16 acc[MB][MB];
+  product<MB>(A, B, 0, a.d, sa, sb, acc);
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6, h = l >> 5;
-  const int vw = v0 + 64 * (w & 1), tw = t0 + 64 * (w >> 1);
+  const int vw = v0 + 32 * MB * (w & 1), tw = t0 + 32 * MB * (w >> 1);
   if (!GRADS) {
-    lce_row_stats<2, 2>(a, acc, vw, tw, count, 2 * blockIdx.x + (w & 1));
+    lce_row_stats<MB, MB>(a, acc, vw, tw, count, 2 * blockIdx.x + (w & 1));
     return;
   }
-  lce_row_grads<2, 2>(a, acc, vw, tw, count);
+  lce_row_grads<MB, MB>(a, acc, vw, tw, count);
   float *p = static_cast<float *>(a.p) + (vw - a.v0);
 #pragma unroll
-  for (int nb = 0; nb < 2; ++nb) {
+  for (int nb = 0; nb < MB; ++nb) {
     const int t = tw + 32 * nb + (l & 31);
     if (t >= count) continue;
 #pragma unroll
-    for (int mb = 0; mb < 2; ++mb)
+    for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
         const f32x4 v = {acc[mb][nb][i], acc[mb][nb][i + 1], acc[mb][nb][i + 2], acc[mb][nb][i + 3]};
@@ -101,28 +123,32 @@ __global__ void __launch_bounds__(256) lce_general_z_kernel(LceArgs a) {
   }
 }
 
-// dX [tokens, d] += P W over the piece
-template <typename T>
+// Share blockIdx.z of dX [tokens, d] += P W over the piece
+template <int MB, typename T>
 __global__ void __launch_bounds__(256) lce_general_dx_kernel(LceArgs a) {
-  __shared__ float sa[BK * LD], sb[BK * LD];
+  using X = Tile<MB>;
+  __shared__ float sa[X::SIZE], sb[X::SIZE];
   const int count = __builtin_amdgcn_readfirstlane(*a.count);
-  const int t0 = blockIdx.y * TM, c0 = blockIdx.x * TM;
+  const int t0 = blockIdx.y * X::TM, c0 = blockIdx.x * X::TM;
   if (t0 >= count) return;
-  Side<float, true> A{static_cast<const float *>(a.p) + int64_t(t0) * a.vc, a.vc, count - t0, a.vn};
-  Side<T, false> B{static_cast<const T *>(a.w) + int64_t(a.v0) * a.ldw + c0, a.ldw, a.d - c0, a.vn};
-  f32x16 acc[2][2];
-  product(A, B, a.vn, sa, sb, acc);
+  const int steps = (a.vn + X::BK - 1) / X::BK, per = (steps + a.dx_splits - 1) / a.dx_splits;
+  const int kb = min(a.vn, int(blockIdx.z) * per * X::BK), ke = min(a.vn, kb + per * X::BK);
+  Side<MB, float, true> A{static_cast<const float *>(a.p) + int64_t(t0) * a.vc, a.vc, count - t0, a.vn};
+  Side<MB, T, false> B{static_cast<const T *>(a.w) + int64_t(a.v0) * a.ldw + c0, a.ldw, a.d - c0, a.vn};
+  f32x16 acc[MB][MB];
+  product<MB>(A, B, kb, ke, sa, sb, acc);
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6, h = l >> 5;
+  float *out = a.dx_part + int64_t(blockIdx.z) * a.n_pad * a.d;
 #pragma unroll
-  for (int mb = 0; mb < 2; ++mb)
+  for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-    for (int nb = 0; nb < 2; ++nb) {
-      const int c = c0 + 64 * (w >> 1) + 32 * nb + (l & 31);
+    for (int nb = 0; nb < MB; ++nb) {
+      const int c = c0 + 32 * MB * (w >> 1) + 32 * nb + (l & 31);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int t = t0 + 64 * (w & 1) + 32 * mb + acc_row(i, h);
+        const int t = t0 + 32 * MB * (w & 1) + 32 * mb + acc_row(i, h);
         if (t < count && c < a.d) {
-          float *o = a.dx_part + int64_t(t) * a.d + c;
+          float *o = out + int64_t(t) * a.d + c;
           *o = a.first ? acc[mb][nb][i] : *o + acc[mb][nb][i];
         }
       }
@@ -130,41 +156,71 @@ __global__ void __launch_bounds__(256) lce_general_dx_kernel(LceArgs a) {
 }
 
 // dW rows of the piece = P^T X
-template <typename T>
+template <int MB, typename T>
 __global__ void __launch_bounds__(256) lce_general_dw_kernel(LceArgs a) {
-  __shared__ float sa[BK * LD], sb[BK * LD];
+  using X = Tile<MB>;
+  __shared__ float sa[X::SIZE], sb[X::SIZE];
   const int count = __builtin_amdgcn_readfirstlane(*a.count);
-  const int r0 = blockIdx.y * TM, c0 = blockIdx.x * TM;
-  Side<float, false> A{static_cast<const float *>(a.p) + r0, a.vc, a.vn - r0, count};
-  Side<T, false> B{static_cast<const T *>(a.x) + c0, a.ldx, a.d - c0, count};
-  f32x16 acc[2][2];
-  product(A, B, count, sa, sb, acc);
+  const int r0 = blockIdx.y * X::TM, c0 = blockIdx.x * X::TM;
+  Side<MB, float, false> A{static_cast<const float *>(a.p) + r0, a.vc, a.vn - r0, count};
+  Side<MB, T, false> B{static_cast<const T *>(a.x) + c0, a.ldx, a.d - c0, count};
+  f32x16 acc[MB][MB];
+  product<MB>(A, B, 0, count, sa, sb, acc);
+  const float f = lce_factor(a, count);
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6, h = l >> 5;
 #pragma unroll
-  for (int mb = 0; mb < 2; ++mb)
+  for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-    for (int nb = 0; nb < 2; ++nb) {
-      const int c = c0 + 64 * (w >> 1) + 32 * nb + (l & 31);
+    for (int nb = 0; nb < MB; ++nb) {
+      const int c = c0 + 32 * MB * (w >> 1) + 32 * nb + (l & 31);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int r = r0 + 64 * (w & 1) + 32 * mb + acc_row(i, h);
-        if (r < a.vn && c < a.d) st(static_cast<T *>(a.dw) + int64_t(a.v0 + r) * a.d + c, acc[mb][nb][i]);
+        const int r = r0 + 32 * MB * (w & 1) + 32 * mb + acc_row(i, h);
+        if (r < a.vn && c < a.d) st(static_cast<T *>(a.dw) + int64_t(a.v0 + r) * a.d + c, acc[mb][nb][i] * f);
       }
     }
 }
 
-dim3 tiles(int x, int y) { return dim3((x + TM - 1) / TM, (y + TM - 1) / TM); }
+// Tiles of 64 until tiles of 128 give two workgroups to every CU (301 rows, 256 features, 5003 words: the
+// three products 39, 40 and 597 us with 128, see the table's case for now).
+bool small(int x, int y, int z = 1) { return int64_t((x + 127) / 128) * ((y + 127) / 128) * z < 512; }
+template <int MB> dim3 tiles(int x, int y, int z = 1) {
+  return dim3((x + Tile<MB>::TM - 1) / Tile<MB>::TM, (y + Tile<MB>::TM - 1) / Tile<MB>::TM, z);
+}
 
 template <typename T> void z_launch(const LceArgs &a, bool grads, hipStream_t s) {
-  if (grads)
-    lce_general_z_kernel<T, true><<<tiles(a.vn, a.N), 256, 0, s>>>(a);
-  else
-    lce_general_z_kernel<T, false><<<tiles(a.V, a.N), 256, 0, s>>>(a);
+  if (grads) {
+    if (small(a.vn, a.N)) lce_general_z_kernel<1, T, true><<<tiles<1>(a.vn, a.N), 256, 0, s>>>(a);
+    else lce_general_z_kernel<2, T, true><<<tiles<2>(a.vn, a.N), 256, 0, s>>>(a);
+  } else {
+    if (small(a.V, a.N)) lce_general_z_kernel<1, T, false><<<tiles<1>(a.V, a.N), 256, 0, s>>>(a);
+    else lce_general_z_kernel<2, T, false><<<tiles<2>(a.V, a.N), 256, 0, s>>>(a);
+  }
+}
+
+template <typename T> void dx_launch(const LceArgs &a, hipStream_t s) {
+  if (small(a.d, a.N, a.dx_splits)) lce_general_dx_kernel<1, T><<<tiles<1>(a.d, a.N, a.dx_splits), 256, 0, s>>>(a);
+  else lce_general_dx_kernel<2, T><<<tiles<2>(a.d, a.N, a.dx_splits), 256, 0, s>>>(a);
+}
+
+template <typename T> void dw_launch(const LceArgs &a, hipStream_t s) {
+  if (small(a.d, a.vn)) lce_general_dw_kernel<1, T><<<tiles<1>(a.d, a.vn), 256, 0, s>>>(a);
+  else lce_general_dw_kernel<2, T><<<tiles<2>(a.d, a.vn), 256, 0, s>>>(a);
 }
 
 }  // namespace
 
-int lce_general_parts(int V) { return 2 * ((V + TM - 1) / TM); }
+int lce_general_parts(int V, int N) {
+  const int tm = small(V, N) ? 64 : 128;
+  return 2 * ((V + tm - 1) / tm);
+}
+
+// Shares of a piece's vocabulary rows: until 512 workgroups of 64 x 64, each with 128 rows at least
+int lce_general_dx_splits(int64_t N, int d, int V, int vc) {
+  const int64_t t = ((N + 63) / 64) * ((d + 63) / 64);
+  const int most = (std::min(V, vc) + 127) / 128;
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({512 / t, int64_t(most), int64_t(16)})));
+}
 
 int launch_lce_general_stats(const LceArgs &a, int dtype, hipStream_t s) {
   if (dtype == MOTIF_F32) z_launch<float>(a, false, s);
@@ -179,16 +235,14 @@ int launch_lce_general_grads(const LceArgs &a, int dtype, hipStream_t s) {
 }
 
 int launch_lce_general_dx(const LceArgs &a, int dtype, hipStream_t s) {
-  const dim3 g = tiles(a.d, a.N);
-  if (dtype == MOTIF_F32) lce_general_dx_kernel<float><<<g, 256, 0, s>>>(a);
-  else lce_general_dx_kernel<bf16_t><<<g, 256, 0, s>>>(a);
+  if (dtype == MOTIF_F32) dx_launch<float>(a, s);
+  else dx_launch<bf16_t>(a, s);
   return check_launch("lce_general_dx_kernel");
 }
 
 int launch_lce_general_dw(const LceArgs &a, int dtype, hipStream_t s) {
-  const dim3 g = tiles(a.d, a.vn);
-  if (dtype == MOTIF_F32) lce_general_dw_kernel<float><<<g, 256, 0, s>>>(a);
-  else lce_general_dw_kernel<bf16_t><<<g, 256, 0, s>>>(a);
+  if (dtype == MOTIF_F32) dw_launch<float>(a, s);
+  else dw_launch<bf16_t>(a, s);
   return check_launch("lce_general_dw_kernel");
 }
 

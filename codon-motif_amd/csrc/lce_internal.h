@@ -5,6 +5,8 @@
 // With z_iv = x_i . w_v, s_i the gradient of row i's loss and t_i its label:
 //   loss_i = log sum_v e^{z_iv} - z_{i t_i}
 //   P_iv   = s_i (e^{z_iv} / sum_u e^{z_iu} - [v = t_i]),  dX = P W,  dW = P^T X
+// Where all s_i are one number (sum, mean), it multiplies dX and dW instead: P rounded to bf16 with a
+// factor 1 / 15565 in it was off by the same quarter of a percent in every row.
 // The forward keeps one number per row (the base-2 log-sum-exp); the backward forms P again in
 // pieces of the vocabulary and multiplies each piece on both sides.  Rows without a label are
 // taken out first: every product runs over the `count` rows that have one, in their order.
@@ -29,7 +31,7 @@ struct LceArgs {
   float *lse;          // [N] base-2 log-sum-exp of z log2 e
   const float *dloss;  // gradient of the loss(es)
   int64_t dl_st;       // 0: one for all rows
-  int mean;            // divided by count
+  int reduction;       // 0: a gradient per row, 1: sum, 2: mean over count
   void *p;             // P of a vocabulary piece (layout: the kernels' own)
   int v0, vc, vn;      // the piece: first vocabulary row, rows laid out, rows of the vocabulary in it
   float *dx_part;      // [dx_splits, n_pad, d] fp32
@@ -99,11 +101,15 @@ __device__ __forceinline__ void lce_row_stats(const LceArgs &a, f32x16 (&acc)[MB
   }
 }
 
-// The gradient of labelled row t's loss (NaN for a label outside the vocabulary)
-__device__ __forceinline__ float lce_row_scale(const LceArgs &a, int t, int count) {
-  float s = a.dloss[a.dl_st ? int64_t(a.row[t]) * a.dl_st : 0];
-  if (a.mean) s /= static_cast<float>(count);
+// What P holds of the gradient of labelled row t's loss (NaN for a label outside the vocabulary)
+__device__ __forceinline__ float lce_row_scale(const LceArgs &a, int t) {
+  const float s = a.reduction ? 1.f : a.dloss[int64_t(a.row[t]) * a.dl_st];
   return a.label[t] < 0 ? __builtin_nanf("") : s;
+}
+// ... and what multiplies the products afterwards
+__device__ __forceinline__ float lce_factor(const LceArgs &a, int count) {
+  if (!a.reduction) return 1.f;
+  return a.reduction == 1 ? *a.dloss : count ? *a.dloss / static_cast<float>(count) : 0.f;
 }
 
 // Backward: P over the same accumulators, in place; 0 behind the last labelled row and the vocabulary.
@@ -114,7 +120,7 @@ __device__ __forceinline__ void lce_row_grads(const LceArgs &a, f32x16 (&acc)[MB
   for (int nb = 0; nb < NB; ++nb) {
     const int t = t0 + 32 * nb + (l & 31);
     const bool live = t < count;
-    const float lse = live ? a.lse[t] : 0.f, scale = live ? lce_row_scale(a, t, count) : 0.f;
+    const float lse = live ? a.lse[t] : 0.f, scale = live ? lce_row_scale(a, t) : 0.f;
     const int rel = live ? a.label[t] - v0 : -1;
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
@@ -147,10 +153,19 @@ __device__ __forceinline__ void lce_row_grads(const LceArgs &a, f32x16 (&acc)[MB
 }
 
 // lce_general.hip: the products on fp32 matrix instructions, any alignment (P is fp32 [N, vc])
-int lce_general_parts(int V);
+int lce_general_parts(int V, int N);
 int launch_lce_general_stats(const LceArgs &a, int dtype, hipStream_t s);
 int launch_lce_general_grads(const LceArgs &a, int dtype, hipStream_t s);  // P of the piece
+int lce_general_dx_splits(int64_t N, int d, int V, int vc);
 int launch_lce_general_dx(const LceArgs &a, int dtype, hipStream_t s);
 int launch_lce_general_dw(const LceArgs &a, int dtype, hipStream_t s);
+
+// lce_bf16.hip: bf16 whose vocabulary rows start on 16-byte boundaries (P is bf16 in blocks)
+bool lce_bf16_serves(const void *w, int64_t ldw, int d, int dtype);
+int lce_bf16_parts(int V);
+int lce_bf16_dx_splits(int64_t N, int d, int V, int vc);
+int launch_lce_bf16_stats(const LceArgs &a, hipStream_t s);
+int launch_lce_bf16_grads(const LceArgs &a, hipStream_t s);
+int launch_lce_bf16_products(const LceArgs &a, bool dx, bool dw, hipStream_t s);
 
 }  // namespace motif

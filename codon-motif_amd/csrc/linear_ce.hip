@@ -15,37 +15,65 @@ namespace motif {
 namespace {
 
 // ------------------------------------------------------------ which rows have a label
-// One workgroup: each thread counts and then places a run of labels (16384 labels: 8 us).
+// One workgroup, 16384 labels at a time: 16 a thread, all loaded before the first is looked at.
 __global__ void __launch_bounds__(1024) lce_plan_kernel(const int64_t *labels, int64_t st, int64_t ignore, int N, int V,
                                                         int *row, int *label, int *pos, int *count, float *loss_rows) {
-  __shared__ int wsum[16];
-  const int tid = threadIdx.x;
-  const int per = (N + 1023) / 1024;
-  const int64_t lo = min(int64_t(tid) * per, int64_t(N)), hi = min(lo + per, int64_t(N));
-  int n = 0;
-  for (int64_t r = lo; r < hi; ++r) n += labels[r * st] != ignore;
-  int incl = n;
+  constexpr int PER = 16;
+  __shared__ int sums[PER * 16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int base = 0;
+  for (int64_t r0 = 0; r0 < N; r0 += 1024 * PER) {
+    int64_t t[PER];
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int up = __shfl_up(incl, off, 64);
-    if ((tid & 63) >= off) incl += up;
-  }
-  if ((tid & 63) == 63) wsum[tid >> 6] = incl;
-  __syncthreads();
-  int at = incl - n;
-  for (int i = 0; i < (tid >> 6); ++i) at += wsum[i];
-  if (tid == 1023) *count = at + n;
-  for (int64_t r = lo; r < hi; ++r) {
-    const int64_t t = labels[r * st];
-    if (t != ignore) {
-      row[at] = static_cast<int>(r);
-      label[at] = t >= 0 && t < V ? static_cast<int>(t) : -1;
-      pos[r] = at++;
-    } else {
-      pos[r] = -1;
-      if (loss_rows) loss_rows[r] = 0.f;
+    for (int i = 0; i < PER; ++i) {
+      const int64_t r = r0 + i * 1024 + tid;
+      t[i] = r < N ? labels[r * st] : ignore;
     }
+    uint64_t has[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      has[i] = __ballot(t[i] != ignore);
+      if (lane == 0) sums[i * 16 + wave] = __popcll(has[i]);
+    }
+    __syncthreads();
+    if (wave == 0) {  // exclusive sums of the 256 groups of 64 labels, in their order
+      int v[4], n = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = sums[4 * lane + j], n += v[j];
+      int incl = n;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int up = __shfl_up(incl, off, 64);
+        if (lane >= off) incl += up;
+      }
+      int at = base + incl - n;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sums[4 * lane + j] = at, at += v[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int64_t r = r0 + i * 1024 + tid;
+      if (r >= N) continue;
+      if (t[i] != ignore) {
+        const int at = sums[i * 16 + wave] + __popcll(has[i] & ((uint64_t(1) << lane) - 1));
+        row[at] = static_cast<int>(r);
+        label[at] = t[i] >= 0 && t[i] < V ? static_cast<int>(t[i]) : -1;
+        pos[r] = at;
+      } else {
+        pos[r] = -1;
+        if (loss_rows) loss_rows[r] = 0.f;
+      }
+    }
+    // (the last group's start and size: labels behind N count as ignored)
+    base = sums[PER * 16 - 1];
+    __shared__ int last;
+    if (tid == 1023) last = __popcll(has[PER - 1]);
+    __syncthreads();
+    base += last;
+    __syncthreads();
   }
+  if (tid == 0) *count = base;
 }
 
 // One wave per labelled row: d elements, then zeros up to ldo (the products read whole 64-element steps).
@@ -66,27 +94,32 @@ __global__ void __launch_bounds__(256) lce_gather_kernel(const T *x, int64_t rs,
   }
 }
 
-// A row's parts joined: 64 rows a workgroup, a quarter of the parts to each wave.
-__global__ void __launch_bounds__(256) lce_combine_kernel(LceArgs a, int nparts, float *nll, float *loss_rows) {
-  __shared__ float sm[4][64], ss[4][64];
-  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int count = *a.count, t = blockIdx.x * 64 + l;
-  if (blockIdx.x * 64 >= count) return;
+// A row's parts joined: 32 rows a workgroup, 32 threads to each (250 parts of 4096 rows: 23 us with 64 rows and
+// four threads to each, whose loads followed each other).
+__global__ void __launch_bounds__(1024) lce_combine_kernel(LceArgs a, int nparts, float *nll, float *loss_rows) {
+  __shared__ float sm[32][33], ss[32][33];
+  const int l = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int count = *a.count, t = blockIdx.x * 32 + l;
+  if (blockIdx.x * 32 >= count) return;
   float m = -INFINITY, s = 0.f;
   if (t < count)
-    for (int p = w; p < nparts; p += 4) lse_merge(m, s, a.part_m[int64_t(p) * a.N + t], a.part_s[int64_t(p) * a.N + t]);
+    for (int p = w; p < nparts; p += 32) lse_merge(m, s, a.part_m[int64_t(p) * a.N + t], a.part_s[int64_t(p) * a.N + t]);
   sm[w][l] = m;
   ss[w][l] = s;
   __syncthreads();
-  if (w != 0 || t >= count) return;
+  // (a wave holds two rows: row w of 32 pairs, one a lane)
+  m = sm[l][w];
+  s = ss[l][w];
 #pragma unroll
-  for (int i = 1; i < 4; ++i) lse_merge(m, s, sm[i][l], ss[i][l]);
+  for (int off = 16; off > 0; off >>= 1) lse_merge(m, s, __shfl_xor(m, off, 64), __shfl_xor(s, off, 64));
+  const int r = blockIdx.x * 32 + w;
+  if (l != 0 || r >= count) return;
   const float lse = m + log2f(s);
-  a.lse[t] = lse;
-  const float z = a.label[t] < 0 ? __builtin_nanf("") : a.at_label[t];
+  a.lse[r] = lse;
+  const float z = a.label[r] < 0 ? __builtin_nanf("") : a.at_label[r];
   const float loss = (lse - z * kLog2e) * 0.6931471805599453f;
-  if (loss_rows) loss_rows[a.row[t]] = loss;
-  else nll[t] = loss;
+  if (loss_rows) loss_rows[a.row[r]] = loss;
+  else nll[r] = loss;
 }
 
 // The sum (or mean) of the rows' losses, in 64 bits.
@@ -105,17 +138,37 @@ __global__ void __launch_bounds__(1024) lce_loss_kernel(const float *nll, const 
   *loss = static_cast<float>(mean ? s / n : s);  // (no label at all: 0 / 0)
 }
 
-// dX rows: the partial sums of a labelled row, rounded once; zeros for the others.
-template <typename T>
+// dX rows: the partial sums of a labelled row times the common factor, rounded once; zeros for the others.  One wave
+// a row; E = 4 where d is a multiple of 4.
+template <typename T, int E>
 __global__ void __launch_bounds__(256) lce_dx_rows_kernel(LceArgs a, T *dx) {
-  const int64_t n = int64_t(a.N) * a.d;
-  for (int64_t e = int64_t(blockIdx.x) * 256 + threadIdx.x; e < n; e += int64_t(gridDim.x) * 256) {
-    const int64_t r = e / a.d;
-    const int c = static_cast<int>(e - r * a.d), i = a.pos[r];
-    float s = 0.f;
-    if (i >= 0)
-      for (int k = 0; k < a.dx_splits; ++k) s += a.dx_part[(k * a.n_pad + i) * a.d + c];
-    st(dx + e, s);
+  const int64_t r = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (r >= a.N) return;
+  const int i = a.pos[r];
+  const float f = lce_factor(a, *a.count);
+  const float *p = a.dx_part + int64_t(i < 0 ? 0 : i) * a.d;
+  const int64_t plane = a.n_pad * a.d;
+  for (int c = (threadIdx.x & 63) * E; c < a.d; c += 64 * E) {
+    float s[E] = {};
+    if (i >= 0) {
+      for (int k = 0; k < a.dx_splits; ++k) {
+        float v[E];
+        if (E == 4) {
+          const float4 u = *reinterpret_cast<const float4 *>(p + k * plane + c);
+          v[0] = u.x, v[1 % E] = u.y, v[2 % E] = u.z, v[3 % E] = u.w;
+        } else {
+          v[0] = p[k * plane + c];
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) s[e] += v[e];
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) s[e] *= f;
+    }
+    T o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) st(o + e, s[e]);
+    __builtin_memcpy(dx + r * a.d + c, o, sizeof(o));
   }
 }
 
@@ -127,8 +180,8 @@ int esize(int dtype) { return dtype == MOTIF_F32 ? 4 : 2; }
 // The forward's workspace: statistics of the vocabulary's parts, z at the labels, the rows' losses.
 struct FwdSpace {
   size_t m, s, z, nll, bytes;
-  FwdSpace(int64_t N, int V) {
-    const size_t parts = lce_general_parts(V), col = up(4 * N, kAlign);
+  FwdSpace(int N, int V) {
+    const size_t parts = lce_general_parts(V, N), col = up(4 * size_t(N), kAlign);
     m = 0;
     s = up(parts * 4 * N, kAlign);
     z = 2 * s;
@@ -149,7 +202,7 @@ struct BwdSpace {
     n_pad = static_cast<int64_t>(up(N, 256));
     const size_t rows = (size_t(1) << 28) / (n_pad * e) / 256 * 256;
     vc = static_cast<int>(std::min(std::max<size_t>(rows, 4096), up(V, 256)));
-    splits = 1;
+    splits = general ? lce_general_dx_splits(N, d, V, vc) : lce_bf16_dx_splits(N, d, V, vc);
     p = 0;
     dx = up(size_t(n_pad) * vc * e, kAlign);
     bytes = dx + size_t(splits) * n_pad * d * 4;
@@ -192,8 +245,8 @@ extern "C" size_t motif_linear_ce_rows_bytes(int N, int d, int dtype) {
 extern "C" size_t motif_linear_ce_workspace_bytes(int N, int d, int V, int dtype, int backward) {
   if (!sizes_ok(N, d, V)) return 0;
   if (!backward) return FwdSpace(N, V).bytes;
-  (void)dtype;
-  return BwdSpace(N, d, V, true).bytes;
+  const size_t g = BwdSpace(N, d, V, true).bytes;
+  return dtype == MOTIF_BF16 ? std::max(g, BwdSpace(N, d, V, false).bytes) : g;
 }
 
 extern "C" int motif_linear_ce_fwd(const void *x, int64_t x_rs, const void *w, int64_t w_rs, const int64_t *labels,
@@ -224,10 +277,11 @@ extern "C" int motif_linear_ce_fwd(const void *x, int64_t x_rs, const void *w, i
   int rc = check_launch("lce_plan_kernel");
   if (rc == MOTIF_OK) rc = dtype == MOTIF_F32 ? gather<float>(x, x_rs, a, rows, s) : gather<bf16_t>(x, x_rs, a, rows, s);
   if (rc != MOTIF_OK) return rc;
-  const int nparts = lce_general_parts(V);
-  rc = launch_lce_general_stats(a, dtype, s);
+  const bool fast = lce_bf16_serves(w, w_rs, d, dtype);
+  const int nparts = fast ? lce_bf16_parts(V) : lce_general_parts(V, N);
+  rc = fast ? launch_lce_bf16_stats(a, s) : launch_lce_general_stats(a, dtype, s);
   if (rc != MOTIF_OK) return rc;
-  lce_combine_kernel<<<(N + 63) / 64, 256, 0, s>>>(a, nparts, nll, loss_rows);
+  lce_combine_kernel<<<(N + 31) / 32, 1024, 0, s>>>(a, nparts, nll, loss_rows);
   rc = check_launch("lce_combine_kernel");
   if (rc != MOTIF_OK || reduction == 0) return rc;
   lce_loss_kernel<<<1, 1024, 0, s>>>(nll, a.count, reduction == 2, loss);
@@ -243,7 +297,8 @@ extern "C" int motif_linear_ce_bwd(const void *rows, const void *w, int64_t w_rs
   if (!rows || !w || !kept || !dloss || !workspace) return set_error(MOTIF_ERR_INVALID, "linear_ce_bwd: null pointer");
   if (V > 1 && w_rs < d) return set_error(MOTIF_ERR_INVALID, "linear_ce_bwd: rows overlap");
   if (!dx && !dw) return MOTIF_OK;
-  const BwdSpace b(N, d, V, true);
+  const bool fast = lce_bf16_serves(w, w_rs, d, dtype);
+  const BwdSpace b(N, d, V, !fast);
   if (workspace_bytes < b.bytes) return set_error(MOTIF_ERR_INVALID, "linear_ce_bwd: workspace too small");
   hipStream_t s = static_cast<hipStream_t>(stream);
   LceArgs a{};
@@ -251,7 +306,7 @@ extern "C" int motif_linear_ce_bwd(const void *rows, const void *w, int64_t w_rs
   a.x = rows, a.ldx = static_cast<int64_t>(up(d, 64));
   a.w = w, a.ldw = w_rs;
   bind_kept(a, const_cast<int *>(kept));
-  a.dloss = dloss, a.dl_st = reduction == 0 ? dloss_st : 0, a.mean = reduction == 2;
+  a.dloss = dloss, a.dl_st = dloss_st, a.reduction = reduction;
   char *ws = static_cast<char *>(workspace);
   a.p = ws + b.p;
   a.dx_part = reinterpret_cast<float *>(ws + b.dx);
@@ -259,14 +314,24 @@ extern "C" int motif_linear_ce_bwd(const void *rows, const void *w, int64_t w_rs
   int rc = MOTIF_OK;
   for (int v0 = 0; v0 < V && rc == MOTIF_OK; v0 += b.vc) {
     a.v0 = v0, a.vn = std::min(b.vc, V - v0), a.first = v0 == 0;
-    rc = launch_lce_general_grads(a, dtype, s);
-    if (rc == MOTIF_OK && dx) rc = launch_lce_general_dx(a, dtype, s);
-    if (rc == MOTIF_OK && dw) rc = launch_lce_general_dw(a, dtype, s);
+    rc = fast ? launch_lce_bf16_grads(a, s) : launch_lce_general_grads(a, dtype, s);
+    if (rc != MOTIF_OK) break;
+    if (fast) {
+      rc = launch_lce_bf16_products(a, dx, dw, s);
+    } else {
+      if (dx) rc = launch_lce_general_dx(a, dtype, s);
+      if (rc == MOTIF_OK && dw) rc = launch_lce_general_dw(a, dtype, s);
+    }
   }
   if (rc != MOTIF_OK || !dx) return rc;
-  const int64_t n = int64_t(N) * d;
-  const unsigned g = static_cast<unsigned>(std::min<int64_t>((n + 255) / 256, 4096));
-  if (dtype == MOTIF_F32) lce_dx_rows_kernel<float><<<g, 256, 0, s>>>(a, static_cast<float *>(dx));
-  else lce_dx_rows_kernel<bf16_t><<<g, 256, 0, s>>>(a, static_cast<bf16_t *>(dx));
+  const unsigned g = (N + 3) / 4;
+  const bool f32 = dtype == MOTIF_F32;
+  if (d % 4 == 0 && reinterpret_cast<uintptr_t>(dx) % 16 == 0) {
+    if (f32) lce_dx_rows_kernel<float, 4><<<g, 256, 0, s>>>(a, static_cast<float *>(dx));
+    else lce_dx_rows_kernel<bf16_t, 4><<<g, 256, 0, s>>>(a, static_cast<bf16_t *>(dx));
+  } else {
+    if (f32) lce_dx_rows_kernel<float, 1><<<g, 256, 0, s>>>(a, static_cast<float *>(dx));
+    else lce_dx_rows_kernel<bf16_t, 1><<<g, 256, 0, s>>>(a, static_cast<bf16_t *>(dx));
+  }
   return check_launch("lce_dx_rows_kernel");
 }
