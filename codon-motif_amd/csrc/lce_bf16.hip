@@ -23,9 +23,15 @@ namespace motif {
 
 namespace {
 
-constexpr int TM = 256, TN = 128, BK = 32, STAGES = 3;
-constexpr int A_BYTES = TM * BK * 2, B_BYTES = TN * BK * 2, STAGE = A_BYTES + B_BYTES;
-constexpr int LOADS = STAGE / 1024 / 4;  // 1 KB loads of a wave per stage
+// The shapes of a workgroup: TN right columns (64 a wave, two waves over each), BK k a stage, ST stages in LDS.
+template <int TN_, int BK_, int ST_> struct Shape {
+  static constexpr int TN = TN_, BK = BK_, ST = ST_, NW = 2 * (TN / 64), THREADS = 64 * NW;
+  static constexpr int A_BYTES = 256 * BK * 2, B_BYTES = TN * BK * 2, STAGE = A_BYTES + B_BYTES;
+  static constexpr int LOADS = STAGE / 1024 / NW;  // 1 KB loads of a wave per stage
+};
+constexpr int TM = 256;
+using Wide = Shape<256, 64, 2>;
+using Narrow = Shape<128, 32, 3>;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
@@ -50,38 +56,43 @@ __device__ __forceinline__ void load_lds(i32x4 r, uint32_t dst, uint32_t voff, u
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 __device__ __forceinline__ bf16x8 join(uint2 a, uint2 b) { return __builtin_bit_cast(bf16x8, uint4{a.x, a.y, b.x, b.y}); }
 
-// R rows of 32 k, k beside each other in memory (row stride ld): LDS row r is four 16-byte pieces, piece c at
-// c ^ (r / 2 % 4) (eight rows' reads of one piece meet 128 bytes of banks once).
-template <int R> struct RowsK {
-  static constexpr int NJ = R * 64 / 1024 / 4;
+// R rows of BK k, k beside each other in memory (row stride ld): LDS row r is BK / 8 pieces of 16 bytes, piece c at
+// c ^ swap(r): the LDS serves 16 lanes at a time, rows 0-3, 12-15, 20-23 and 24-27 or the others, from 64 banks,
+// and no two of them may meet (r / 2 % 4 for rows of four pieces: half of the reads' cycles were conflicts).
+template <typename C, int R> struct RowsK {
+  static constexpr int NP = C::BK / 8, RL = 64 / NP, NJ = R / RL / C::NW;
   i32x4 buf;
   uint32_t off[NJ];
-  int kc, K;
+  int K;
+  __device__ __forceinline__ static int swap(int r) { return NP == 4 ? (r >> 2) & 3 : (r >> 1) & 7; }
+  __device__ __forceinline__ static int kc(int j) {  // first k of this lane's piece
+    const int l = threadIdx.x & 63;
+    return ((l % NP) ^ swap((wave_id() * NJ + j) * RL + l / NP)) * 8;
+  }
   __device__ __forceinline__ RowsK(const bf16_t *p, int64_t ld, int rows, int K_) : K(K_) {
     const int l = threadIdx.x & 63, w = wave_id();
     const int n = min(rows, R);
     buf = make_rsrc(p, n > 0 ? ((n - 1) * ld + K) * 2 : 0);
-    kc = ((l & 3) ^ ((l >> 3) & 3)) * 8;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) off[j] = static_cast<uint32_t>(((w * NJ + j) * 16 + (l >> 2)) * ld * 2 + kc * 2);
+    for (int j = 0; j < NJ; ++j) off[j] = static_cast<uint32_t>(((w * NJ + j) * RL + l / NP) * ld * 2 + kc(j) * 2);
   }
   __device__ __forceinline__ void issue(uint32_t dst, int k0) const {
     const int w = wave_id();
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
-      load_lds(buf, dst + (w * NJ + j) * 1024, k0 + kc < K ? off[j] : 0xfffffff0u, k0 * 2);
+      load_lds(buf, dst + (w * NJ + j) * 1024, k0 + kc(j) < K ? off[j] : 0xfffffff0u, k0 * 2);
   }
   // operand of rows r0 .. r0 + 31 at k step s (16 k)
   __device__ __forceinline__ static bf16x8 frag(const char *src, int r0, int s) {
     const int l = threadIdx.x & 63, r = r0 + (l & 31), c = 2 * s + (l >> 5);
-    return __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4 *>(src + r * 64 + ((c ^ ((r >> 1) & 3)) * 16)));
+    return __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4 *>(src + r * (C::BK * 2) + ((c ^ swap(r)) * 16)));
   }
 };
 
-// 32 k rows of R columns (row stride ld): LDS row k is R / 8 pieces, piece c at c ^ swap(k).
+// BK k rows of R columns (row stride ld): LDS row k is R / 8 pieces, piece c at c ^ swap(k).
 __device__ __forceinline__ int tr_swap(int k) { return ((k & 1) << 2) | ((k & 2) ? 10 : 0); }
-template <int R> struct ColsK {
-  static constexpr int NJ = R * 64 / 1024 / 4, RP = 512 / R;
+template <typename C, int R> struct ColsK {
+  static constexpr int RP = 512 / R, NJ = C::BK / RP / C::NW;
   const bf16_t *p;
   int64_t ld;
   int cols, K;
@@ -95,7 +106,7 @@ template <int R> struct ColsK {
     }
   }
   __device__ __forceinline__ void issue(uint32_t dst, int k0) const {
-    const int w = wave_id(), n = min(K - k0, BK);
+    const int w = wave_id(), n = min(K - k0, C::BK);
     const i32x4 buf = make_rsrc(p + int64_t(k0) * ld, ((n - 1) * ld + cols) * 2);
 #pragma unroll
     for (int j = 0; j < NJ; ++j) load_lds(buf, dst + (w * NJ + j) * 1024, off[j], 0);
@@ -108,9 +119,9 @@ template <int R> struct ColsK {
   }
 };
 
-// P's blocks as the left side of dX: 256 tokens x 32 vocabulary rows, block (t / 32, v / 16) in order
-struct PTokens {
-  static constexpr int NJ = 4;
+// P's blocks as the left side of dX: 256 tokens x BK vocabulary rows, block (t / 32, v / 16) in order
+template <typename C> struct PTokens {
+  static constexpr int NB = C::BK / 16, NJ = 8 * NB / C::NW;
   const char *p;
   int nvc;
   uint32_t off[NJ];
@@ -120,24 +131,24 @@ struct PTokens {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int q = w * NJ + j;
-      off[j] = static_cast<uint32_t>(((q >> 1) * nvc + (q & 1)) * 1024 + l * 16);
+      off[j] = static_cast<uint32_t>(((q / NB) * nvc + q % NB) * 1024 + l * 16);
     }
   }
   __device__ __forceinline__ void issue(uint32_t dst, int k0) const {
     const int w = wave_id();
-    const i32x4 buf = make_rsrc(p + int64_t(k0 / 16) * 1024, (7 * nvc + 2) * 1024);
+    const i32x4 buf = make_rsrc(p + int64_t(k0 / 16) * 1024, (7 * nvc + NB) * 1024);
 #pragma unroll
     for (int j = 0; j < NJ; ++j) load_lds(buf, dst + (w * NJ + j) * 1024, off[j], 0);
   }
   __device__ __forceinline__ static bf16x8 frag(const char *src, int r0, int s) {
-    const int l = threadIdx.x & 63, q = (r0 >> 5) * 2 + s;
+    const int l = threadIdx.x & 63, q = (r0 >> 5) * NB + s;
     return __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4 *>(src + q * 1024 + (l ^ ((l >> 5) << 2) ^ ((s & 1) << 3)) * 16));
   }
 };
 
-// ... as the left side of dW: 256 vocabulary rows x 32 tokens
-struct PVocab {
-  static constexpr int NJ = 4;
+// ... as the left side of dW: 256 vocabulary rows x BK tokens
+template <typename C> struct PVocab {
+  static constexpr int NJ = 16 * (C::BK / 32) / C::NW;
   const char *p;
   int nvc;
   __device__ __forceinline__ PVocab(const void *p_, int r0, int vc) : nvc(vc / 16) {
@@ -145,59 +156,72 @@ struct PVocab {
   }
   __device__ __forceinline__ void issue(uint32_t dst, int k0) const {
     const int l = threadIdx.x & 63, w = wave_id();
-    const i32x4 buf = make_rsrc(p + int64_t(k0 / 32) * nvc * 1024, 16 * 1024);
+    const i32x4 buf = make_rsrc(p + int64_t(k0 / 32) * nvc * 1024, ((C::BK / 32 - 1) * nvc + 16) * 1024);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) load_lds(buf, dst + (w * NJ + j) * 1024, (w * NJ + j) * 1024 + l * 16, 0);
+    for (int j = 0; j < NJ; ++j) {
+      const int q = w * NJ + j;
+      load_lds(buf, dst + q * 1024, l * 16, ((q >> 4) * nvc + (q & 15)) * 1024);
+    }
   }
   __device__ __forceinline__ static bf16x8 frag(const char *src, int r0, int s) {
-    const int l = threadIdx.x & 63, g = (l >> 4) & 1, h = l & 1, t = 16 * s + 4 * (l >> 5) + ((l >> 2) & 3);
+    const int l = threadIdx.x & 63, g = (l >> 4) & 1, h = l & 1, t = 16 * (s & 1) + 4 * (l >> 5) + ((l >> 2) & 3);
     const int place = (t + 32 * h) ^ (h << 2) ^ (g << 3);
-    const char *q = src + ((r0 >> 4) + g) * 1024 + ((l >> 1) & 1) * 8;
+    const char *q = src + ((s >> 1) * 16 + (r0 >> 4) + g) * 1024 + ((l >> 1) & 1) * 8;
     return join(read_tr(q + place * 16), read_tr(q + (place ^ 8) * 16));
   }
 };
 
-template <typename A, typename B>
-__device__ __forceinline__ void product(const A &a, const B &b, int kb, int ke, char *lds, f32x16 (&acc)[4][2]) {
-  const int w = wave_id();
+__device__ __forceinline__ void zero(f32x16 (&acc)[4][2]) {
 #pragma unroll
   for (int mb = 0; mb < 4; ++mb)
 #pragma unroll
     for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[mb][nb][i] = 0.f;
-  const int n = (ke - kb + BK - 1) / BK;
+}
+
+// One stage's products of a wave
+template <typename C, typename A, typename B>
+__device__ __forceinline__ void multiply(const char *sa, f32x16 (&acc)[4][2]) {
+  const int w = wave_id();
+  const char *sb = sa + C::A_BYTES;
+#pragma unroll
+  for (int s = 0; s < C::BK / 16; ++s) {
+    bf16x8 fa[4], fb[2];
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb) fb[nb] = B::frag(sb, 64 * (w >> 1) + 32 * nb, s);
+#pragma unroll
+    for (int mb = 0; mb < 4; ++mb) fa[mb] = A::frag(sa, 128 * (w & 1) + 32 * mb, s);
+#pragma unroll
+    for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb)
+        acc[mb][nb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[mb], fb[nb], acc[mb][nb], 0, 0, 0);
+  }
+}
+
+template <typename C, typename A, typename B>
+__device__ __forceinline__ void product(const A &a, const B &b, int kb, int ke, char *lds, f32x16 (&acc)[4][2]) {
+  zero(acc);
+  const int n = (ke - kb + C::BK - 1) / C::BK;
   const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)lds));
   auto issue = [&](int i, uint32_t place) {
-    a.issue(base + place, kb + i * BK);
-    b.issue(base + place + A_BYTES, kb + i * BK);
+    a.issue(base + place, kb + i * C::BK);
+    b.issue(base + place + C::A_BYTES, kb + i * C::BK);
   };
-  for (int i = 0; i < STAGES - 1 && i < n; ++i) issue(i, i * STAGE);
-  uint32_t at = 0, next = (STAGES - 1) * STAGE;  // places of stage i and of the one loaded beside it
+  for (int i = 0; i < C::ST - 1 && i < n; ++i) issue(i, i * C::STAGE);
+  uint32_t at = 0, next = (C::ST - 1) * C::STAGE;  // places of stage i and of the one loaded beside it
   for (int i = 0; i < n; ++i) {
-    // this wave has read stage i - 1 and its loads of stage i have landed (those of i + 1 may fly); then all
-    // waves have, and stage i + 2 may take the place of i - 1
-    if (i + 1 < n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
+    // this wave has read stage i - 1 and its loads of stage i have landed (those of the later ones may fly, but for the last); then
+    // all waves have, and the stage to load may take the place of i - 1
+    if (C::ST > 2 && i + C::ST - 2 < n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((C::ST - 2) * C::LOADS) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (i + STAGES - 1 < n) issue(i + STAGES - 1, next);
-    const char *sa = lds + at, *sb = sa + A_BYTES;
+    if (i + C::ST - 1 < n) issue(i + C::ST - 1, next);
+    multiply<C, A, B>(lds + at, acc);
     next = at;
-    at = at == (STAGES - 1) * STAGE ? 0 : at + STAGE;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      bf16x8 fa[4], fb[2];
-#pragma unroll
-      for (int nb = 0; nb < 2; ++nb) fb[nb] = B::frag(sb, 64 * (w >> 1) + 32 * nb, s);
-#pragma unroll
-      for (int mb = 0; mb < 4; ++mb) fa[mb] = A::frag(sa, 128 * (w & 1) + 32 * mb, s);
-#pragma unroll
-      for (int mb = 0; mb < 4; ++mb)
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb)
-          acc[mb][nb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[mb], fb[nb], acc[mb][nb], 0, 0, 0);
-    }
+    at = at == (C::ST - 1) * C::STAGE ? 0 : at + C::STAGE;
   }
 }
 
@@ -214,24 +238,28 @@ __device__ __forceinline__ TilePos tile_at(int id, int nm, int nn, int G) {
   return {m0 + r % g, r / g};
 }
 
-template <bool GRADS>
-__global__ void __launch_bounds__(256, 2) lce_z_kernel(LceArgs a, int nm, int nn) {
-  __shared__ __align__(1024) char lds[STAGES * STAGE];
+// z = W X^T of 256 vocabulary rows x TN tokens, then its statistics or P.  (Workgroups that stay and load the next
+// tile's first stage beside an epilogue were no faster, 1113 against 1044 us for 15565 x 768 x 40960: the loop
+// over tiles costs 70 registers.)
+template <typename C, bool GRADS>
+__global__ void __launch_bounds__(C::THREADS, 2) lce_z_kernel(LceArgs a, int nm, int nn) {
+  __shared__ __align__(1024) char lds[C::ST * C::STAGE];
   const int count = __builtin_amdgcn_readfirstlane(*a.count);
   const TilePos at = tile_at(xcd_tile(blockIdx.x, gridDim.x), nm, nn, 4);
-  const int t0 = at.n * TN, v0 = (GRADS ? a.v0 : 0) + at.m * TM;
+  const int t0 = at.n * C::TN, v0 = (GRADS ? a.v0 : 0) + at.m * TM;
   if (t0 >= count) return;
-  const RowsK<TM> A(static_cast<const bf16_t *>(a.w) + int64_t(v0) * a.ldw, a.ldw, a.V - v0, a.d);
-  const RowsK<TN> B(static_cast<const bf16_t *>(a.x) + int64_t(t0) * a.ldx, a.ldx, count - t0, static_cast<int>(a.ldx));
+  const RowsK<C, TM> A(static_cast<const bf16_t *>(a.w) + int64_t(v0) * a.ldw, a.ldw, a.V - v0, a.d);
+  const RowsK<C, C::TN> B(static_cast<const bf16_t *>(a.x) + int64_t(t0) * a.ldx, a.ldx, count - t0, static_cast<int>(a.ldx));
   f32x16 acc[4][2];
-  product(A, B, 0, a.d, lds, acc);
+  product<C>(A, B, 0, a.d, lds, acc);
   const int l = threadIdx.x & 63, w = wave_id(), h = l >> 5;
   const int vw = v0 + 128 * (w & 1), tw = t0 + 64 * (w >> 1);
   if (!GRADS) {
     lce_row_stats<4, 2>(a, acc, vw, tw, count, 2 * at.m + (w & 1));
     return;
   }
-  lce_row_grads<4, 2>(a, acc, vw, tw, count);
+  bool live[2];
+  lce_row_grads<4, 2>(a, acc, vw, tw, count, live);
   const int nvc = a.vc / 16;
 #pragma unroll
   for (int nb = 0; nb < 2; ++nb)
@@ -241,27 +269,29 @@ __global__ void __launch_bounds__(256, 2) lce_z_kernel(LceArgs a, int nm, int nn
       for (int q = 0; q < 2; ++q) {
         uint32_t u[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) {
           u[i] = static_cast<uint32_t>(f32_to_bf16(acc[mb][nb][8 * q + 2 * i])) |
                  (static_cast<uint32_t>(f32_to_bf16(acc[mb][nb][8 * q + 2 * i + 1])) << 16);
+          if (!live[nb]) u[i] = 0;
+        }
         char *blk = static_cast<char *>(a.p) +
                     (int64_t(tw / 32 + nb) * nvc + (vw - a.v0) / 16 + 2 * mb + q) * 1024;
         *reinterpret_cast<uint4 *>(blk + (l ^ (h << 2) ^ (q << 3)) * 16) = uint4{u[0], u[1], u[2], u[3]};
       }
 }
 
-// dX: tile `at` of share `share` of the piece's vocabulary rows (dx_splits shares, each with its own partial sums)
-__device__ __forceinline__ void dx_tile(const LceArgs &a, TilePos at, int share, int count, char *lds) {
-  const int t0 = at.m * TM, c0 = at.n * TN;
-  if (t0 >= count) return;
-  const int steps = (a.vn + BK - 1) / BK, per = (steps + a.dx_splits - 1) / a.dx_splits;
-  const int kb = share * per * BK, ke = min(a.vn, kb + per * BK);
-  const PTokens A(a.p, t0, a.vc);
-  const ColsK<TN> B(static_cast<const bf16_t *>(a.w) + int64_t(a.v0) * a.ldw + c0, a.ldw, a.d - c0, a.vn);
+// dX: tile `at` of share `share` of the piece's vocabulary rows
+template <typename C>
+__device__ __forceinline__ void dx_tile(const LceArgs &a, TilePos at, int share, DxShares sh, char *lds) {
+  const int t0 = at.m * TM, c0 = at.n * C::TN;
+  const int steps = (a.vn + C::BK - 1) / C::BK, per = (steps + sh.n - 1) / sh.n;
+  const int kb = share * per * C::BK, ke = min(a.vn, kb + per * C::BK);
+  const PTokens<C> A(a.p, t0, a.vc);
+  const ColsK<C, C::TN> B(static_cast<const bf16_t *>(a.w) + int64_t(a.v0) * a.ldw + c0, a.ldw, a.d - c0, a.vn);
   f32x16 acc[4][2];
-  product(A, B, kb, ke, lds, acc);
+  product<C>(A, B, kb, ke, lds, acc);
   const int l = threadIdx.x & 63, w = wave_id(), h = l >> 5;
-  float *out = a.dx_part + int64_t(share) * a.n_pad * a.d;
+  float *out = a.dx_part + share * sh.rows * a.d;
 #pragma unroll
   for (int nb = 0; nb < 2; ++nb) {
     const int c = c0 + 64 * (w >> 1) + 32 * nb + (l & 31);
@@ -283,12 +313,13 @@ __device__ __forceinline__ void dx_tile(const LceArgs &a, TilePos at, int share,
   }
 }
 
+template <typename C>
 __device__ __forceinline__ void dw_tile(const LceArgs &a, TilePos at, int count, char *lds) {
-  const int r0 = at.m * TM, c0 = at.n * TN;
-  const PVocab A(a.p, r0, a.vc);
-  const ColsK<TN> B(static_cast<const bf16_t *>(a.x) + c0, a.ldx, static_cast<int>(a.ldx) - c0, count);
+  const int r0 = at.m * TM, c0 = at.n * C::TN;
+  const PVocab<C> A(a.p, r0, a.vc);
+  const ColsK<C, C::TN> B(static_cast<const bf16_t *>(a.x) + c0, a.ldx, static_cast<int>(a.ldx) - c0, count);
   f32x16 acc[4][2];
-  product(A, B, 0, count, lds, acc);
+  product<C>(A, B, 0, count, lds, acc);
   const float f = lce_factor(a, count);
   const int l = threadIdx.x & 63, w = wave_id(), h = l >> 5;
 #pragma unroll
@@ -305,21 +336,30 @@ __device__ __forceinline__ void dw_tile(const LceArgs &a, TilePos at, int count,
 }
 
 // Both products of a piece in one launch, so that neither's last round leaves the chip half idle: `ndx`
-// workgroups (a multiple of 8) for dX, then dW's.
-struct Grid { int xm, xn, ndx, wm, wn; };
-__global__ void __launch_bounds__(256, 2) lce_products_kernel(LceArgs a, Grid g) {
-  __shared__ __align__(1024) char lds[STAGES * STAGE];
-  const int count = __builtin_amdgcn_readfirstlane(*a.count);
-  const int b = blockIdx.x, tiles = g.xm * g.xn;
-  if (b < g.ndx) {
-    const int id = xcd_tile(b, g.ndx);
-    if (id < tiles * a.dx_splits) dx_tile(a, tile_at(id % tiles, g.xm, g.xn, 4), id / tiles, count, lds);
-  } else {
-    dw_tile(a, tile_at(xcd_tile(b - g.ndx, gridDim.x - g.ndx), g.wm, g.wn, 4), count, lds);
+// workgroups for dX and then `ndw` for dW (multiples of 8), or the other way round where dW's sums are longer.
+struct Grid { int xn, ndx, wm, wn, ndw; };
+template <typename C>
+__global__ void __launch_bounds__(C::THREADS, 2) lce_products_kernel(LceArgs a, Grid g) {
+  __shared__ __align__(1024) char lds[C::ST * C::STAGE];
+  const int count = __builtin_amdgcn_readfirstlane(*a.count), b = blockIdx.x;
+  const DxShares sh = lce_dx_shares(a, count);
+  const bool dw_first = int64_t(count) * sh.n > a.vn;
+  const int b_dx = dw_first ? b - g.ndw : b, b_dw = dw_first ? b : b - g.ndx;
+  if (dw_first ? b_dx >= 0 : b_dw < 0) {
+    const int xm = (count + TM - 1) / TM, tiles = xm * g.xn;
+    if (b_dx >= tiles * sh.n) return;
+    const int id = xcd_tile(b_dx, tiles * sh.n);
+    dx_tile<C>(a, tile_at(id % tiles, xm, g.xn, 4), id / tiles, sh, lds);
+  } else if (b_dw < g.wm * g.wn) {
+    dw_tile<C>(a, tile_at(xcd_tile(b_dw, g.wm * g.wn), g.wm, g.wn, 4), count, lds);
   }
 }
 
-template <typename T> T up(T a, int b) { return (a + b - 1) / b; }
+template <typename T> T up(T a, int64_t b) { return static_cast<T>((a + b - 1) / b); }
+
+// 256 tokens a tile: 244 and 260 us for the two z products of 4096 x 768 x 32000 where 128 take 270 and 290; from
+// 2048 tokens (517 tokens: 48 against 45, and half of a small batch's last tile is padding).
+bool wide(int64_t N) { return N >= 2048; }
 
 }  // namespace
 
@@ -330,30 +370,45 @@ bool lce_bf16_serves(const void *w, int64_t ldw, int d, int dtype) {
 int lce_bf16_parts(int V) { return 2 * up(V, TM); }
 
 // Shares of a piece's vocabulary rows in dX: so many that none takes longer than the launch's work spread
-// over 512 places (two workgroups per CU) does.  Each costs partial sums of N x d in fp32.
+// over the places (two workgroups per CU) does.  Each costs partial sums of N x d in fp32.
 int lce_bf16_dx_splits(int64_t N, int d, int V, int vc) {
-  const int64_t n = std::min(V, vc), tn = up(d, TN), steps = up(n, BK);
-  const int64_t all = up(N, TM) * tn * steps + up(n, TM) * tn * up(N, BK);
-  return static_cast<int>(std::min<int64_t>({int64_t(16), steps, (steps * 512 + all - 1) / all}));
+  const int64_t bk = Narrow::BK, tn = up(d, Narrow::TN), places = 512;
+  const int64_t n = std::min(V, vc), steps = up(n, bk);
+  const int64_t all = up(N, TM) * tn * steps + up(n, TM) * tn * up(N, bk);
+  return static_cast<int>(std::min<int64_t>({int64_t(16), steps, up(steps * places, all)}));
 }
 
+namespace {
+
+template <typename C, bool GRADS> void z_launch(const LceArgs &a, hipStream_t s) {
+  const int nm = up(GRADS ? a.vn : a.V, TM), nn = up(a.N, C::TN);
+  lce_z_kernel<C, GRADS><<<nm * nn, C::THREADS, 0, s>>>(a, nm, nn);
+}
+
+template <typename C> void products_launch(const LceArgs &a, bool dx, bool dw, hipStream_t s) {
+  const Grid g = [&] {
+    const int xn = up(a.d, C::TN), wm = up(a.vn, TM);
+    return Grid{xn, dx ? up(a.dx_tiles * xn * a.dx_splits, 8) * 8 : 0, wm, xn, dw ? up(wm * xn, 8) * 8 : 0};
+  }();
+  lce_products_kernel<C><<<g.ndx + g.ndw, C::THREADS, 0, s>>>(a, g);
+}
+
+}  // namespace
+
 int launch_lce_bf16_stats(const LceArgs &a, hipStream_t s) {
-  const int nm = up(a.V, TM), nn = up(a.N, TN);
-  lce_z_kernel<false><<<nm * nn, 256, 0, s>>>(a, nm, nn);
+  if (wide(a.N)) z_launch<Wide, false>(a, s);
+  else z_launch<Narrow, false>(a, s);
   return check_launch("lce_z_kernel (statistics)");
 }
 
 int launch_lce_bf16_grads(const LceArgs &a, hipStream_t s) {
-  const int nm = up(a.vn, TM), nn = up(a.N, TN);
-  lce_z_kernel<true><<<nm * nn, 256, 0, s>>>(a, nm, nn);
+  if (wide(a.N)) z_launch<Wide, true>(a, s);
+  else z_launch<Narrow, true>(a, s);
   return check_launch("lce_z_kernel (gradients)");
 }
 
 int launch_lce_bf16_products(const LceArgs &a, bool dx, bool dw, hipStream_t s) {
-  Grid g{};
-  g.xm = up(a.N, TM), g.xn = g.wn = up(a.d, TN), g.wm = up(a.vn, TM);
-  g.ndx = dx ? up(g.xm * g.xn * a.dx_splits, 8) * 8 : 0;
-  lce_products_kernel<<<g.ndx + (dw ? g.wm * g.wn : 0), 256, 0, s>>>(a, g);
+  products_launch<Narrow>(a, dx, dw, s);
   return check_launch("lce_products_kernel");
 }
 

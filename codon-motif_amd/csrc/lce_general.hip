@@ -107,12 +107,13 @@ __global__ void __launch_bounds__(256) lce_general_z_kernel(LceArgs a) {
     lce_row_stats<MB, MB>(a, acc, vw, tw, count, 2 * blockIdx.x + (w & 1));
     return;
   }
-  lce_row_grads<MB, MB>(a, acc, vw, tw, count);
+  bool live[MB];
+  lce_row_grads<MB, MB>(a, acc, vw, tw, count, live);
   float *p = static_cast<float *>(a.p) + (vw - a.v0);
 #pragma unroll
   for (int nb = 0; nb < MB; ++nb) {
     const int t = tw + 32 * nb + (l & 31);
-    if (t >= count) continue;
+    if (!live[nb]) continue;
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll

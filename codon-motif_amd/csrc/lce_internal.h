@@ -34,9 +34,9 @@ struct LceArgs {
   int reduction;       // 0: a gradient per row, 1: sum, 2: mean over count
   void *p;             // P of a vocabulary piece (layout: the kernels' own)
   int v0, vc, vn;      // the piece: first vocabulary row, rows laid out, rows of the vocabulary in it
-  float *dx_part;      // [dx_splits, n_pad, d] fp32
+  float *dx_part;      // partial dX, fp32: see lce_dx_shares
   int64_t n_pad;
-  int dx_splits, first;  // first: the first piece (nothing to add to)
+  int dx_splits, dx_tiles, first;  // first: the first piece (nothing to add to)
   void *dw;            // [V, d]
 };
 
@@ -50,6 +50,15 @@ __device__ __forceinline__ void lse_merge(float &m, float &s, float m2, float s2
   const float ref = top == -INFINITY ? 0.f : top;
   s = s * fast_exp2(m - ref) + s2 * fast_exp2(m2 - ref);
   m = top;
+}
+
+// dX in shares of a piece's vocabulary rows: `dx_splits` of [n_pad, d] partial sums, or (dx_tiles: the tiles of 256
+// that n_pad makes) as many of the labelled rows' as fit the same place.
+struct DxShares { int n; int64_t rows; };
+__device__ __forceinline__ DxShares lce_dx_shares(const LceArgs &a, int count) {
+  if (!a.dx_tiles) return {a.dx_splits, a.n_pad};
+  const int live = max(1, (count + 255) / 256);
+  return {min(16, a.dx_splits * a.dx_tiles / live), int64_t(live) * 256};
 }
 
 // Forward: the pair of a wave's MB x 32 vocabulary rows from v0 for each of its NB x 32 tokens from t0,
@@ -101,27 +110,26 @@ __device__ __forceinline__ void lce_row_stats(const LceArgs &a, f32x16 (&acc)[MB
   }
 }
 
-// What P holds of the gradient of labelled row t's loss (NaN for a label outside the vocabulary)
-__device__ __forceinline__ float lce_row_scale(const LceArgs &a, int t) {
-  const float s = a.reduction ? 1.f : a.dloss[int64_t(a.row[t]) * a.dl_st];
-  return a.label[t] < 0 ? __builtin_nanf("") : s;
-}
-// ... and what multiplies the products afterwards
+// What multiplies the products with P
 __device__ __forceinline__ float lce_factor(const LceArgs &a, int count) {
   if (!a.reduction) return 1.f;
   return a.reduction == 1 ? *a.dloss : count ? *a.dloss / static_cast<float>(count) : 0.f;
 }
 
-// Backward: P over the same accumulators, in place; 0 behind the last labelled row and the vocabulary.
+// Backward: P over the same accumulators, in place; 0 behind the vocabulary.  What it holds for tokens behind the
+// last labelled one (`live`: this lane's are not) is the caller's to leave out: a row of infinities in W times no
+// row is no number.
 template <int MB, int NB>
-__device__ __forceinline__ void lce_row_grads(const LceArgs &a, f32x16 (&acc)[MB][NB], int v0, int t0, int count) {
+__device__ __forceinline__ void lce_row_grads(const LceArgs &a, f32x16 (&acc)[MB][NB], int v0, int t0, int count,
+                                              bool (&live)[NB]) {
   const int l = threadIdx.x & 63, h = l >> 5;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     const int t = t0 + 32 * nb + (l & 31);
-    const bool live = t < count;
-    const float lse = live ? a.lse[t] : 0.f, scale = live ? lce_row_scale(a, t) : 0.f;
-    const int rel = live ? a.label[t] - v0 : -1;
+    live[nb] = t < count;
+    const int label = live[nb] ? a.label[t] : 0, rel = live[nb] ? label - v0 : -1;
+    float lse = live[nb] ? a.lse[t] : 0.f;
+    if (live[nb] && label < 0) lse = __builtin_nanf("");  // (a label outside the vocabulary)
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
@@ -133,13 +141,13 @@ __device__ __forceinline__ void lce_row_grads(const LceArgs &a, f32x16 (&acc)[MB
         for (int i = 0; i < 16; ++i)
           if (rel == 32 * mb + acc_row(i, h)) acc[mb][nb][i] -= 1.f;
     }
+    if (a.reduction == 0) {  // (a factor of each row; a common one multiplies the products)
+      const float s = live[nb] ? a.dloss[int64_t(a.row[t]) * a.dl_st] : 0.f;
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb)
+      for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float p = acc[mb][nb][i] * scale;
-        acc[mb][nb][i] = live ? p : 0.f;  // (a row of infinities in W times no row is no number)
-      }
+        for (int i = 0; i < 16; ++i) acc[mb][nb][i] *= s;
+    }
   }
   if (v0 + 32 * MB > a.V) {
 #pragma unroll

@@ -145,13 +145,16 @@ __global__ void __launch_bounds__(256) lce_dx_rows_kernel(LceArgs a, T *dx) {
   const int64_t r = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (r >= a.N) return;
   const int i = a.pos[r];
-  const float f = lce_factor(a, *a.count);
+  const int count = *a.count;
+  const float f = lce_factor(a, count);
+  const DxShares sh = lce_dx_shares(a, count);
   const float *p = a.dx_part + int64_t(i < 0 ? 0 : i) * a.d;
-  const int64_t plane = a.n_pad * a.d;
+  const int64_t plane = sh.rows * a.d;
   for (int c = (threadIdx.x & 63) * E; c < a.d; c += 64 * E) {
     float s[E] = {};
     if (i >= 0) {
-      for (int k = 0; k < a.dx_splits; ++k) {
+#pragma unroll 4
+      for (int k = 0; k < sh.n; ++k) {
         float v[E];
         if (E == 4) {
           const float4 u = *reinterpret_cast<const float4 *>(p + k * plane + c);
@@ -310,7 +313,7 @@ extern "C" int motif_linear_ce_bwd(const void *rows, const void *w, int64_t w_rs
   char *ws = static_cast<char *>(workspace);
   a.p = ws + b.p;
   a.dx_part = reinterpret_cast<float *>(ws + b.dx);
-  a.n_pad = b.n_pad, a.dx_splits = b.splits, a.vc = b.vc, a.dw = dw;
+  a.n_pad = b.n_pad, a.dx_splits = b.splits, a.dx_tiles = fast ? static_cast<int>(b.n_pad / 256) : 0, a.vc = b.vc, a.dw = dw;
   int rc = MOTIF_OK;
   for (int v0 = 0; v0 < V && rc == MOTIF_OK; v0 += b.vc) {
     a.v0 = v0, a.vn = std::min(b.vc, V - v0), a.first = v0 == 0;
