@@ -20,7 +20,7 @@ namespace motif {
 
 namespace {
 
-constexpr int kMaxGroups = 1024;
+constexpr int kMaxGroups = 512;
 constexpr int kMaxD = 16384;  // features of a row
 
 struct NormArgs {
@@ -35,36 +35,33 @@ struct NormArgs {
   int rows, D, groups;
 };
 
-template <typename T, int E> struct Access;
-template <typename T> struct Access<T, 1> {
-  __device__ __forceinline__ static void load(const T *p, float *v) { v[0] = ld(p); }
-  __device__ __forceinline__ static void store(T *p, const float *v) { st(p, v[0]); }
+// One access: E elements as they lie in memory, and as floats.
+template <typename T, int E> struct Raw {
+  T e[E];
+  __device__ __forceinline__ void load(const T *p) { e[0] = *p; }
 };
-template <> struct Access<float, 4> {
-  __device__ __forceinline__ static void load(const float *p, float *v) {
-    const float4 u = *reinterpret_cast<const float4 *>(p);
-    v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
-  }
-  __device__ __forceinline__ static void store(float *p, const float *v) {
-    *reinterpret_cast<float4 *>(p) = float4{v[0], v[1], v[2], v[3]};
-  }
+template <typename T> struct __align__(16) Raw<T, 8> {
+  T e[8];
+  __device__ __forceinline__ void load(const T *p) { *this = *reinterpret_cast<const Raw *>(p); }
 };
-template <typename T> struct Access<T, 8> {
-  __device__ __forceinline__ static void load(const T *p, float *v) {
-    union { uint4 u; T e[8]; } c;
-    c.u = *reinterpret_cast<const uint4 *>(p);
+template <> struct __align__(16) Raw<float, 4> {
+  float e[4];
+  __device__ __forceinline__ void load(const float *p) { *this = *reinterpret_cast<const Raw *>(p); }
+};
+template <typename T, int E> __device__ __forceinline__ void load_row(const T *p, float *v) {
+  Raw<T, E> r;
+  r.load(p);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = ld(&c.e[i]);
-  }
-  __device__ __forceinline__ static void store(T *p, const float *v) {
-    union { uint4 u; T e[8]; } c;
+  for (int e = 0; e < E; ++e) v[e] = ld(&r.e[e]);
+}
+template <typename T, int E> __device__ __forceinline__ void store_row(T *p, const float *v) {
+  Raw<T, E> r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) st(&c.e[i], v[i]);
-    *reinterpret_cast<uint4 *>(p) = c.u;
-  }
-};
+  for (int e = 0; e < E; ++e) st(&r.e[e], v[e]);
+  *reinterpret_cast<Raw<T, E> *>(p) = r;
+}
 
-// The sums of N values over a row's LPR lanes (LPR 256 or 1024: the whole workgroup, through LDS).
+// The sums of N values over a row's LPR lanes (more than a wave: through LDS, every lane of the workgroup with them).
 template <int LPR, int N>
 __device__ __forceinline__ void group_sum(float (&v)[N], float *lds) {
 #pragma unroll
@@ -81,7 +78,7 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float *lds) {
     for (int n = 0; n < N; ++n) {
       v[n] = 0.f;
 #pragma unroll
-      for (int i = 0; i < W; ++i) v[n] += lds[N * i + n];
+      for (int i = 0; i < W; ++i) v[n] += lds[N * (threadIdx.x / LPR * W + i) + n];
     }
     __syncthreads();
   }
@@ -102,7 +99,7 @@ __global__ void __launch_bounds__(block_size<LPR>()) row_norm_fwd_kernel(NormArg
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = (sub + j * LPR) * E;
-    if (c < a.D) Access<T, E>::load(x + c, v[j]);
+    if (c < a.D) load_row<T, E>(x + c, v[j]);
     else
 #pragma unroll
       for (int e = 0; e < E; ++e) v[j][e] = 0.f;
@@ -139,15 +136,15 @@ __global__ void __launch_bounds__(block_size<LPR>()) row_norm_fwd_kernel(NormArg
     const int c = (sub + j * LPR) * E;
     if (c >= a.D) continue;
     float w[E], b[E], o[E];
-    if (a.w) Access<T, E>::load(static_cast<const T *>(a.w) + c, w);
-    if (LAYER && a.b) Access<T, E>::load(static_cast<const T *>(a.b) + c, b);
+    if (a.w) load_row<T, E>(static_cast<const T *>(a.w) + c, w);
+    if (LAYER && a.b) load_row<T, E>(static_cast<const T *>(a.b) + c, b);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       o[e] = v[j][e] * r;
       if (a.w) o[e] *= w[e];
       if (LAYER && a.b) o[e] += b[e];
     }
-    Access<T, E>::store(y + c, o);
+    store_row<T, E>(y + c, o);
   }
 }
 
@@ -159,47 +156,61 @@ __global__ void __launch_bounds__(block_size<LPR>()) row_norm_bwd_kernel(NormArg
   __shared__ float lds[32];
   const int sub = threadIdx.x % LPR, grp = threadIdx.x / LPR;
   const float inv = 1.f / static_cast<float>(a.D);
-  float w[NV][E], dw[NV][E], db[NV][E];
+  float dw[NV][E], db[NV][E];
+  Raw<T, E> w[NV], xr[NV], gr[NV];  // w, and the next row's x and dy, in flight while this one is worked on
+  float next_r = 0.f, next_m = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = (sub + j * LPR) * E;
 #pragma unroll
-    for (int e = 0; e < E; ++e) w[j][e] = 1.f, dw[j][e] = db[j][e] = 0.f;
-    if (a.w && c < a.D) Access<T, E>::load(static_cast<const T *>(a.w) + c, w[j]);
+    for (int e = 0; e < E; ++e) {
+      dw[j][e] = db[j][e] = 0.f;
+      st(&w[j].e[e], 1.f);
+    }
+    if (a.w && c < a.D) w[j].load(static_cast<const T *>(a.w) + c);
   }
+  auto fetch = [&](int64_t row) {
+    if (row >= a.rows) return;
+    const T *x = static_cast<const T *>(a.x) + row * a.x_rs, *dy = static_cast<const T *>(a.dy) + row * a.dy_rs;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (sub + j * LPR) * E;
+      if (c < a.D) xr[j].load(x + c), gr[j].load(dy + c);
+    }
+    next_r = a.rstd[row];
+    if (LAYER) next_m = a.mean[row];
+  };
+  fetch(int64_t(blockIdx.x) * RPB + grp);
   // (every lane of a workgroup takes every step: the sums below meet at barriers)
   for (int64_t row0 = int64_t(blockIdx.x) * RPB; row0 < a.rows; row0 += int64_t(gridDim.x) * RPB) {
     const int64_t row = row0 + grp;
     const bool live = row < a.rows;
-    const int64_t rr = live ? row : 0;
-    const T *x = static_cast<const T *>(a.x) + rr * a.x_rs, *dy = static_cast<const T *>(a.dy) + rr * a.dy_rs;
-    const float r = a.rstd[rr], m = LAYER ? a.mean[rr] : 0.f;
+    const float r = next_r, m = next_m;
     float h[NV][E], g[NV][E], s[NS];
 #pragma unroll
     for (int n = 0; n < NS; ++n) s[n] = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (sub + j * LPR) * E;
-      if (live && c < a.D) {
-        Access<T, E>::load(x + c, h[j]);
-        Access<T, E>::load(dy + c, g[j]);
+      const bool in = live && (sub + j * LPR) * E < a.D;
 #pragma unroll
-        for (int e = 0; e < E; ++e) h[j][e] = (h[j][e] - m) * r;
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) h[j][e] = g[j][e] = 0.f;
+      for (int e = 0; e < E; ++e) {
+        h[j][e] = in ? (ld(&xr[j].e[e]) - m) * r : 0.f;
+        g[j][e] = in ? ld(&gr[j].e[e]) : 0.f;
       }
+    }
+    fetch(row + int64_t(gridDim.x) * RPB);
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         if (PARAMS) {
           dw[j][e] = fmaf(g[j][e], h[j][e], dw[j][e]);
           if (LAYER) db[j][e] += g[j][e];
         }
-        g[j][e] *= w[j][e];
+        g[j][e] *= ld(&w[j].e[e]);
         s[0] = fmaf(g[j][e], h[j][e], s[0]);
         if (LAYER) s[NS - 1] += g[j][e];
       }
-    }
     group_sum<LPR, NS>(s, lds);
     if (!live || !a.y) continue;
     const float c1 = s[0] * inv, c0 = LAYER ? s[NS - 1] * inv : 0.f;
@@ -211,13 +222,14 @@ __global__ void __launch_bounds__(block_size<LPR>()) row_norm_bwd_kernel(NormArg
       float o[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) o[e] = r * (fmaf(-c1, h[j][e], g[j][e]) - c0);
-      Access<T, E>::store(dx + c, o);
+      store_row<T, E>(dx + c, o);
     }
   }
   if (!PARAMS) return;
   // the row groups of the workgroup: within a wave by shuffles, over its waves through LDS
-  constexpr int WR = LPR > 64 ? 1 : BS / 64;  // waves that hold the same columns
-  __shared__ float acc[WR > 1 ? (WR - 1) * (LPR < 64 ? LPR : 64) * E : 1];
+  constexpr int CW = LPR > 64 ? LPR : 64, L = LPR < 64 ? LPR : CW, NC = BS / CW;  // NC groups of waves hold the same columns
+  __shared__ float acc[NC > 1 ? (NC - 1) * L * E : 1];
+  const int copy = threadIdx.x / CW, lane = threadIdx.x % CW;
 #pragma unroll
   for (int k = 0; k < (LAYER ? 2 : 1); ++k) {
     float *out = a.part + (int64_t(k) * a.groups + blockIdx.x) * a.D;
@@ -231,17 +243,15 @@ __global__ void __launch_bounds__(block_size<LPR>()) row_norm_bwd_kernel(NormArg
 #pragma unroll
           for (int off = 32; off >= LPR; off >>= 1) v[e] += __shfl_xor(v[e], off, 64);
       }
-      if (WR > 1) {
-        constexpr int L = LPR < 64 ? LPR : 64;
-        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+      if (NC > 1) {
         __syncthreads();
-        if (wave > 0 && lane < L)
+        if (copy > 0 && lane < L)
 #pragma unroll
-          for (int e = 0; e < E; ++e) acc[((wave - 1) * E + e) * L + lane] = v[e];
+          for (int e = 0; e < E; ++e) acc[((copy - 1) * E + e) * L + lane] = v[e];
         __syncthreads();
-        if (wave == 0 && lane < L)
+        if (copy == 0 && lane < L)
 #pragma unroll
-          for (int i = 0; i < WR - 1; ++i)
+          for (int i = 0; i < NC - 1; ++i)
 #pragma unroll
             for (int e = 0; e < E; ++e) v[e] += acc[(i * E + e) * L + lane];
       }
@@ -264,6 +274,7 @@ __global__ void __launch_bounds__(1024) row_norm_params_kernel(NormArgs a) {
   const float *p = a.part + int64_t(blockIdx.y) * a.groups * a.D;
   float v = 0.f;
   if (c < a.D)
+#pragma unroll 8
     for (int g = sl; g < a.groups; g += 32) v += p[int64_t(g) * a.D + c];
   lds[sl][cl] = v;
   __syncthreads();
@@ -285,7 +296,7 @@ template <int E, typename F> bool with_shape(int D, F &&f) {
     MOTIF_ROW(32, 1)
     MOTIF_ROW(32, 3)
     MOTIF_ROW(64, 2)
-    MOTIF_ROW(64, 4)
+    MOTIF_ROW(128, 2)
     MOTIF_ROW(256, 2)
     MOTIF_ROW(256, 4)
     MOTIF_ROW(1024, kMaxD / E / 1024)

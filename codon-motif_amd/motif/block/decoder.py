@@ -15,6 +15,7 @@ from motif.model.config import MotifChordConfig
 from motif.ops import RMSNorm
 from motif.ops.attn_res import apply_block_attn_res, attn_res_read_norms
 from motif.ops.autograd_path import wants_grad
+from motif.ops.dropout import dropout_add
 from motif.ops.epilogue import residual_fold, swiglu, usable
 from motif.ops.linear_rows import linear_rows_dual, linear_rows_pair, rows_eligible, sum_weights
 
@@ -33,6 +34,9 @@ class Decoder(nn.Module):
     def __init__(self, attn_type: Literal['gdn', 'chord'], config: MotifChordConfig):
         super().__init__()
         self.attn_type = attn_type.lower()
+        if not 0.0 <= config.dropout < 1.0:
+            raise ValueError(f'dropout must be in [0, 1), got {config.dropout}')
+        self.dropout = config.dropout
         self.attn_norm = RMSNorm(config.model_dim)
         if self.attn_type == 'chord':
             self.attn = ChordAttention(hidden_size=config.model_dim, num_heads=config.num_heads,
@@ -47,6 +51,16 @@ class Decoder(nn.Module):
     @property
     def cache_type(self):
         return KVLayerCache if self.attn_type == 'chord' else GatedDeltaAttentionLayerCache
+
+
+def _dropped_branches(p, attn, mlp):
+    '''f_h = drop(attn) + drop(mlp) of a training step: two passes, the second with the first as its
+    residual.  Their seeds come from the device's generator, so that a captured step draws
+    anew at every replay and torch.manual_seed repeats a run.'''
+    if not attn.is_cuda or attn.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        return nn.functional.dropout(attn, p) + nn.functional.dropout(mlp, p)
+    seeds = torch.randint(2 ** 63 - 1, (2,), device=attn.device)
+    return dropout_add(mlp, p, seeds[1:], residual=dropout_add(attn, p, seeds[:1]))
 
 
 def _split_step(decoder, x, m, layer_cache, mask, position, prev):
@@ -263,7 +277,8 @@ class DecoderBlock(nn.Module):
         # put-off add into one pass.
         for i, decoder in enumerate(self.features):
             x, m = self._read(attn_res, i, decoder)
-            if cu_seqlens is None:
+            drop = decoder.dropout if self.training else 0.0
+            if cu_seqlens is None and not drop:
                 layer_cache = cache.attn[i] if use_attn_cache else None
                 done = None
                 if use_attn_cache and decoder.mlp._fused(m):
@@ -288,9 +303,12 @@ class DecoderBlock(nn.Module):
                                         attention_mask=mask, embedding_start=position)
             else:
                 attn_out = decoder.attn(hidden_states=x, past_key_value=cache.attn[i] if use_attn_cache else None)
-            prev = attn_res.partial_block
-            prev = prev if prev is not None and prev.shape == attn_out.output.shape else None
-            f_h, partial = decoder.mlp.forward_residual(m, attn_out.output, prev)
+            if drop:
+                f_h, partial = _dropped_branches(drop, attn_out.output, decoder.mlp(m)), None
+            else:
+                prev = attn_res.partial_block
+                prev = prev if prev is not None and prev.shape == attn_out.output.shape else None
+                f_h, partial = decoder.mlp.forward_residual(m, attn_out.output, prev)
             if use_attn_cache:
                 cache.attn[i] = attn_out.past_key_value
             attn_res.update_increment(f_h, partial)

@@ -1,6 +1,7 @@
 '''Model hyper-parameters; same fields and defaults as the reference's
 motif/model/config.py:5-39, and (new) the Chord layers' sliding window: a query sees the
-keys less than `window` positions back (None: all of them) and the first `sinks` tokens.'''
+keys less than `window` positions back (None: all of them) and the first `sinks` tokens;
+`dropout`, the share of each decoder's attention and MLP outputs that training drops.'''
 from dataclasses import dataclass
 from typing import Literal, Optional, Tuple
 
@@ -17,3 +18,4 @@ class MotifChordConfig:
     block_n: int = 4
     window: Optional[int] = None
     sinks: int = 0
+    dropout: float = 0.0

@@ -18,7 +18,7 @@ import torch.nn.functional as F
 from motif.block.decoder import DecoderBlock
 from motif.model.cache import ModelCache, build_cache
 from motif.model.config import MotifChordConfig
-from motif.ops import RMSNorm
+from motif.ops import RMSNorm, linear_cross_entropy
 from motif.ops.packed import PackedSeqs
 
 
@@ -114,14 +114,19 @@ class MotifChordModel(nn.Module):
     def forward(self, input_ids: torch.Tensor, cache: Optional[ModelCache] = None,
                 labels: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
                 position: Optional[Union[int, torch.Tensor]] = None,
-                cu_seqlens: Optional[torch.Tensor] = None, logits: bool = True) -> ModelOutput:
+                cu_seqlens: Optional[torch.Tensor] = None, logits: bool = True,
+                fused_loss: bool = False) -> ModelOutput:
         '''Run the model over [B, T] ids.
 
         `cu_seqlens` (new): packed sequences, B == 1 -- every sequence starts from
         empty state; an int tensor (its host-side metadata is then built once, one read
         back from the device) or a motif.ops.packed.PackedSeqs built beforehand (the
         forward then reads nothing back and can be captured in a graph).  `logits=False`
-        skips the vocabulary projection.'''
+        skips the vocabulary projection.  `fused_loss` (new): the labels' loss straight from the
+        hidden states (motif.ops.linear_cross_entropy, an fp32 scalar); the logits are not
+        formed and not returned.'''
+        if fused_loss and labels is None:
+            raise ValueError('fused_loss needs labels')
         cached = cache.seq_len if cache is not None else 0
         if cu_seqlens is not None:
             cu_seqlens = PackedSeqs.of(cu_seqlens, input_ids.shape[1], input_ids.device)
@@ -140,6 +145,9 @@ class MotifChordModel(nn.Module):
             out = block(x, cache[i], mask, 0 if position is None else position, cu_seqlens=cu_seqlens)
             x = out.hidden_states
         x = self.norm(x)
+        if fused_loss:
+            loss = linear_cross_entropy(x, self.lm_head.weight, labels.reshape(x.shape[:-1]), ignore_index=-100)
+            return ModelOutput(hidden_states=x, loss=loss, cache=cache)
         out_logits = self.lm_head(x) if (logits or labels is not None) else None
         loss = None
         if labels is not None:

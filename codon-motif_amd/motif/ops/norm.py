@@ -37,8 +37,22 @@ def _launch(x2, weight, bias, y2, stats, eps, layer):
         _lib.check(rc, 'motif_row_norm_fwd')
 
 
+def _norm_torch(x, weight, bias, eps, layer):
+    '''The same in torch ops, for derivatives beyond the first.'''
+    h = x.float()
+    if layer:
+        h = h - h.mean(-1, keepdim=True)
+    h = h * torch.rsqrt(h.pow(2).mean(-1, keepdim=True) + eps)
+    if weight is not None:
+        h = h * weight.float()
+    if bias is not None:
+        h = h + bias.float()
+    return h.to(x.dtype)
+
+
 class RowNormFunction(torch.autograd.Function):
-    '''motif_row_norm_fwd / motif_row_norm_bwd: gradients for x, weight and bias.'''
+    '''motif_row_norm_fwd / motif_row_norm_bwd: gradients for x, weight and bias (their own derivatives, where
+    a graph of them is asked for, through torch ops).'''
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps, layer):
@@ -48,17 +62,19 @@ class RowNormFunction(torch.autograd.Function):
         stats = torch.empty((2 if layer else 1) * rows, dtype=torch.float32, device=x.device)
         if rows:
             _launch(x2, weight, bias, y.view(rows, D), stats, eps, layer)
-        ctx.save_for_backward(x, weight, stats)
-        ctx.layer = layer
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.layer, ctx.eps = layer, eps
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        if torch.is_grad_enabled():  # (create_graph: what the kernels give carries no graph)
-            raise RuntimeError('the row norms have no second derivatives')
-        x, weight, stats = ctx.saved_tensors
+        x, weight, bias, stats = ctx.saved_tensors
         layer = ctx.layer
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        if torch.is_grad_enabled():  # (create_graph: what the kernels give carries no graph)
+            leaves = [t for t, need in zip((x, weight, bias), ctx.needs_input_grad) if need]
+            got = iter(torch.autograd.grad(_norm_torch(x, weight, bias, ctx.eps, layer), leaves, dy, create_graph=True))
+            return next(got) if need_x else None, next(got) if need_w else None, next(got) if need_b else None, None, None
         x2, dy2 = _rows(x), _rows(dy)
         rows, D = x2.shape
         dev, dt = x.device, x.dtype
@@ -119,11 +135,11 @@ def _norm(x, weight, bias, eps, layer, what):
 def rms_norm_rows(x, weight=None, eps=1e-6):
     '''x / sqrt(mean(x^2) + eps) * weight over the last dimension of x [..., D] (fp32, bf16 or
     fp16, D at most 16384), in fp32, rounded once.  weight [D] of x's dtype, or None.
-    Differentiable once in x and weight.'''
+    Differentiable in x and weight.'''
     return _norm(x, weight, None, eps, 0, 'rms_norm_rows')
 
 
 def layer_norm_rows(x, weight=None, bias=None, eps=1e-5):
     '''(x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x [..., D], as
-    rms_norm_rows; bias [D] of x's dtype, or None.  Differentiable once in x, weight and bias.'''
+    rms_norm_rows; bias [D] of x's dtype, or None.  Differentiable in x, weight and bias.'''
     return _norm(x, weight, bias, eps, 1, 'layer_norm_rows')

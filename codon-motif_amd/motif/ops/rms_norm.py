@@ -2,15 +2,33 @@
 
 Same parameters and formulas as the reference (motif/ops/rms_norm.py:419-553):
 RMSNorm y = x / sqrt(mean(x^2) + eps) * weight; GatedRMSNorm takes
-[values || gate] and returns rms_norm(values) * SiLU(gate).
+[values || gate] and returns rms_norm(values) * SiLU(gate).  Where gradients are wanted,
+RMSNorm runs the HIP kernels of `rms_norm_rows` (the same formula, rounded once).
 '''
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import _lib
+from .autograd_path import wants_grad
+from .norm import MAX_FEATURES, rms_norm_rows
+
+_KERNEL_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _trains_on_kernels(x, weight):
+    '''A call whose gradients the kernels give: first derivatives in reverse mode, outside
+    autocast and function transforms, which keep torch's own op.'''
+    return (x.dtype in _KERNEL_DTYPES and weight.dtype == x.dtype and weight.device == x.device
+            and weight.dim() == 1 and x.shape[-1] <= MAX_FEATURES and wants_grad(x, weight)
+            and not torch.is_autocast_enabled('cuda') and not torch._C._are_functorch_transforms_active()
+            and torch.autograd.forward_ad._current_level < 0 and not torch.compiler.is_compiling() and _lib.available())
+
 
 def _rms(x, weight, eps):
     if x.is_cuda and weight is not None and weight.numel() == x.shape[-1]:
+        if _trains_on_kernels(x, weight):
+            return rms_norm_rows(x, weight, eps)
         return F.rms_norm(x, (x.shape[-1],), weight, eps)
     x_f = x.float()
     y = (x_f * torch.rsqrt(x_f.pow(2).mean(-1, keepdim=True) + eps)).to(x.dtype)

@@ -109,4 +109,33 @@ def test_workspace_sizes():
         for V in (1, 300, 50000):
             assert lib.motif_linear_ce_workspace_bytes(N, 64, V, 1, 1) > lib.motif_linear_ce_rows_bytes(N, 64, 1)
     assert lib.motif_row_norm_bwd_workspace_bytes(10, 64, 1) == 2 * 10 * 64 * 4
-    assert lib.motif_row_norm_bwd_workspace_bytes(10 ** 6, 64, 0) == 1024 * 64 * 4
+    assert lib.motif_row_norm_bwd_workspace_bytes(10 ** 6, 64, 0) <= 4096 * 64 * 4  # (no more rows than workgroups)
+
+
+def test_model_options():
+    import dataclasses
+
+    from motif.model.config import MotifChordConfig
+    from motif.model.motif import MotifChordModel
+    cfg = MotifChordConfig(vocab_size=32, model_dim=64, num_heads=2, num_kv_heads=1, head_k_dim=32, block=('gdn', 'chord'), block_n=1)
+    model = MotifChordModel(cfg)
+    assert cfg.dropout == 0.0 and all(d.dropout == 0.0 for b in model.blocks for d in b.features)
+    with pytest.raises(ValueError, match='fused_loss'):
+        model(torch.zeros(1, 4, dtype=torch.int64), fused_loss=True)
+    for p in (1.0, -0.5):
+        with pytest.raises(ValueError, match='dropout'):
+            MotifChordModel(dataclasses.replace(cfg, dropout=p))
+    with pytest.raises(TypeError):
+        MotifChordConfig(drop=0.1)
+
+
+def test_dropout_survives_a_checkpoint(tmp_path):
+    from motif.model.config import MotifChordConfig
+    from motif.model.motif import MotifChordModel
+    cfg = MotifChordConfig(vocab_size=32, model_dim=64, num_heads=2, num_kv_heads=1, head_k_dim=32, block=('gdn', 'chord'),
+                           block_n=1, dropout=0.25)
+    path = str(tmp_path / 'm.safetensors')
+    MotifChordModel(cfg).save_pretrained(path)
+    back = MotifChordModel.from_pretrained(path, verbose=False)
+    assert back.config.dropout == 0.25 and back.blocks[0].features[1].dropout == 0.25
+    assert MotifChordModel.from_pretrained(path, verbose=False, dropout=0.0).config.dropout == 0.0
