@@ -23,15 +23,16 @@ namespace motif {
 
 namespace {
 
-// The shapes of a workgroup: TN right columns (64 a wave, two waves over each), BK k a stage, ST stages in LDS.
-template <int TN_, int BK_, int ST_> struct Shape {
-  static constexpr int TN = TN_, BK = BK_, ST = ST_, NW = 2 * (TN / 64), THREADS = 64 * NW;
-  static constexpr int A_BYTES = 256 * BK * 2, B_BYTES = TN * BK * 2, STAGE = A_BYTES + B_BYTES;
+// The shapes of a workgroup: TM left rows (two waves over them, MB blocks of 32 each), TN right columns (64 a wave),
+// BK k a stage, ST stages in LDS; PER of them on a CU.
+template <int TM_, int TN_, int BK_, int ST_, int PER_> struct Shape {
+  static constexpr int TM = TM_, TN = TN_, BK = BK_, ST = ST_, PER = PER_, MB = TM / 64, NW = 2 * (TN / 64), THREADS = 64 * NW;
+  static constexpr int BOUND = PER * NW / 4;  // waves on a SIMD
+  static constexpr int A_BYTES = TM * BK * 2, B_BYTES = TN * BK * 2, STAGE = A_BYTES + B_BYTES;
   static constexpr int LOADS = STAGE / 1024 / NW;  // 1 KB loads of a wave per stage
 };
-constexpr int TM = 256;
-using Wide = Shape<256, 64, 2>;
-using Narrow = Shape<128, 32, 3>;
+using Wide = Shape<256, 256, 64, 2, 1>;
+using Narrow = Shape<256, 128, 32, 3, 2>;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
@@ -171,9 +172,9 @@ template <typename C> struct PVocab {
   }
 };
 
-__device__ __forceinline__ void zero(f32x16 (&acc)[4][2]) {
+template <int MB> __device__ __forceinline__ void zero(f32x16 (&acc)[MB][2]) {
 #pragma unroll
-  for (int mb = 0; mb < 4; ++mb)
+  for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
     for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
@@ -182,18 +183,18 @@ __device__ __forceinline__ void zero(f32x16 (&acc)[4][2]) {
 
 // One stage's products of a wave
 template <typename C, typename A, typename B>
-__device__ __forceinline__ void multiply(const char *sa, f32x16 (&acc)[4][2]) {
+__device__ __forceinline__ void multiply(const char *sa, f32x16 (&acc)[C::MB][2]) {
   const int w = wave_id();
   const char *sb = sa + C::A_BYTES;
 #pragma unroll
   for (int s = 0; s < C::BK / 16; ++s) {
-    bf16x8 fa[4], fb[2];
+    bf16x8 fa[C::MB], fb[2];
 #pragma unroll
     for (int nb = 0; nb < 2; ++nb) fb[nb] = B::frag(sb, 64 * (w >> 1) + 32 * nb, s);
 #pragma unroll
-    for (int mb = 0; mb < 4; ++mb) fa[mb] = A::frag(sa, 128 * (w & 1) + 32 * mb, s);
+    for (int mb = 0; mb < C::MB; ++mb) fa[mb] = A::frag(sa, C::TM / 2 * (w & 1) + 32 * mb, s);
 #pragma unroll
-    for (int mb = 0; mb < 4; ++mb)
+    for (int mb = 0; mb < C::MB; ++mb)
 #pragma unroll
       for (int nb = 0; nb < 2; ++nb)
         acc[mb][nb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[mb], fb[nb], acc[mb][nb], 0, 0, 0);
@@ -201,7 +202,7 @@ __device__ __forceinline__ void multiply(const char *sa, f32x16 (&acc)[4][2]) {
 }
 
 template <typename C, typename A, typename B>
-__device__ __forceinline__ void product(const A &a, const B &b, int kb, int ke, char *lds, f32x16 (&acc)[4][2]) {
+__device__ __forceinline__ void product(const A &a, const B &b, int kb, int ke, char *lds, f32x16 (&acc)[C::MB][2]) {
   zero(acc);
   const int n = (ke - kb + C::BK - 1) / C::BK;
   const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)lds));
@@ -242,29 +243,29 @@ __device__ __forceinline__ TilePos tile_at(int id, int nm, int nn, int G) {
 // tile's first stage beside an epilogue were no faster, 1113 against 1044 us for 15565 x 768 x 40960: the loop
 // over tiles costs 70 registers.)
 template <typename C, bool GRADS>
-__global__ void __launch_bounds__(C::THREADS, 2) lce_z_kernel(LceArgs a, int nm, int nn) {
+__global__ void __launch_bounds__(C::THREADS, C::BOUND) lce_z_kernel(LceArgs a, int nm, int nn) {
   __shared__ __align__(1024) char lds[C::ST * C::STAGE];
   const int count = __builtin_amdgcn_readfirstlane(*a.count);
   const TilePos at = tile_at(xcd_tile(blockIdx.x, gridDim.x), nm, nn, 4);
-  const int t0 = at.n * C::TN, v0 = (GRADS ? a.v0 : 0) + at.m * TM;
+  const int t0 = at.n * C::TN, v0 = (GRADS ? a.v0 : 0) + at.m * C::TM;
   if (t0 >= count) return;
-  const RowsK<C, TM> A(static_cast<const bf16_t *>(a.w) + int64_t(v0) * a.ldw, a.ldw, a.V - v0, a.d);
+  const RowsK<C, C::TM> A(static_cast<const bf16_t *>(a.w) + int64_t(v0) * a.ldw, a.ldw, a.V - v0, a.dk);
   const RowsK<C, C::TN> B(static_cast<const bf16_t *>(a.x) + int64_t(t0) * a.ldx, a.ldx, count - t0, static_cast<int>(a.ldx));
-  f32x16 acc[4][2];
-  product<C>(A, B, 0, a.d, lds, acc);
+  f32x16 acc[C::MB][2];
+  product<C>(A, B, 0, a.dk, lds, acc);
   const int l = threadIdx.x & 63, w = wave_id(), h = l >> 5;
-  const int vw = v0 + 128 * (w & 1), tw = t0 + 64 * (w >> 1);
+  const int vw = v0 + C::TM / 2 * (w & 1), tw = t0 + 64 * (w >> 1);
   if (!GRADS) {
-    lce_row_stats<4, 2>(a, acc, vw, tw, count, 2 * at.m + (w & 1));
+    lce_row_stats<C::MB, 2>(a, acc, vw, tw, count, 2 * at.m + (w & 1));
     return;
   }
   bool live[2];
-  lce_row_grads<4, 2>(a, acc, vw, tw, count, live);
+  lce_row_grads<C::MB, 2>(a, acc, vw, tw, count, live);
   const int nvc = a.vc / 16;
 #pragma unroll
   for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
-    for (int mb = 0; mb < 4; ++mb)
+    for (int mb = 0; mb < C::MB; ++mb)
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         uint32_t u[4];
@@ -283,11 +284,11 @@ __global__ void __launch_bounds__(C::THREADS, 2) lce_z_kernel(LceArgs a, int nm,
 // dX: tile `at` of share `share` of the piece's vocabulary rows
 template <typename C>
 __device__ __forceinline__ void dx_tile(const LceArgs &a, TilePos at, int share, DxShares sh, char *lds) {
-  const int t0 = at.m * TM, c0 = at.n * C::TN;
+  const int t0 = at.m * C::TM, c0 = at.n * C::TN;
   const int steps = (a.vn + C::BK - 1) / C::BK, per = (steps + sh.n - 1) / sh.n;
   const int kb = share * per * C::BK, ke = min(a.vn, kb + per * C::BK);
   const PTokens<C> A(a.p, t0, a.vc);
-  const ColsK<C, C::TN> B(static_cast<const bf16_t *>(a.w) + int64_t(a.v0) * a.ldw + c0, a.ldw, a.d - c0, a.vn);
+  const ColsK<C, C::TN> B(static_cast<const bf16_t *>(a.w) + int64_t(a.v0) * a.ldw + c0, a.ldw, a.dk - c0, a.vn);
   f32x16 acc[4][2];
   product<C>(A, B, kb, ke, lds, acc);
   const int l = threadIdx.x & 63, w = wave_id(), h = l >> 5;
@@ -315,22 +316,34 @@ __device__ __forceinline__ void dx_tile(const LceArgs &a, TilePos at, int share,
 
 template <typename C>
 __device__ __forceinline__ void dw_tile(const LceArgs &a, TilePos at, int count, char *lds) {
-  const int r0 = at.m * TM, c0 = at.n * C::TN;
+  const int r0 = at.m * C::TM, c0 = at.n * C::TN;
   const PVocab<C> A(a.p, r0, a.vc);
   const ColsK<C, C::TN> B(static_cast<const bf16_t *>(a.x) + c0, a.ldx, static_cast<int>(a.ldx) - c0, count);
   f32x16 acc[4][2];
   product<C>(A, B, 0, count, lds, acc);
   const float f = lce_factor(a, count);
   const int l = threadIdx.x & 63, w = wave_id(), h = l >> 5;
+  bf16_t *dw = static_cast<bf16_t *>(a.dw);
+  const bool pairs = a.d % 2 == 0 && reinterpret_cast<uintptr_t>(dw) % 4 == 0;
 #pragma unroll
   for (int mb = 0; mb < 4; ++mb)
 #pragma unroll
     for (int nb = 0; nb < 2; ++nb) {
       const int c = c0 + 64 * (w >> 1) + 32 * nb + (l & 31);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int i = 0; i < 16; i += 2) {
+        // neighbouring lanes swap, so that each stores two columns of one of two rows
         const int r = r0 + 128 * (w & 1) + 32 * mb + acc_row(i, h);
-        if (r < a.vn && c < a.d) st(static_cast<bf16_t *>(a.dw) + int64_t(a.v0 + r) * a.d + c, acc[mb][nb][i] * f);
+        const float v0 = acc[mb][nb][i] * f, v1 = acc[mb][nb][i + 1] * f;
+        if (pairs) {
+          const float other = __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, l & 1 ? v0 : v1), 0xb1, 0xf, 0xf, true));
+          const uint32_t u = static_cast<uint32_t>(f32_to_bf16(l & 1 ? other : v0)) |
+                             (static_cast<uint32_t>(f32_to_bf16(l & 1 ? v1 : other)) << 16);
+          if (r + (l & 1) < a.vn && c < a.d) *reinterpret_cast<uint32_t *>(dw + int64_t(a.v0 + r + (l & 1)) * a.d + (c & ~1)) = u;
+        } else if (c < a.d) {
+          if (r < a.vn) st(dw + int64_t(a.v0 + r) * a.d + c, v0);
+          if (r + 1 < a.vn) st(dw + int64_t(a.v0 + r + 1) * a.d + c, v1);
+        }
       }
     }
 }
@@ -339,14 +352,14 @@ __device__ __forceinline__ void dw_tile(const LceArgs &a, TilePos at, int count,
 // workgroups for dX and then `ndw` for dW (multiples of 8), or the other way round where dW's sums are longer.
 struct Grid { int xn, ndx, wm, wn, ndw; };
 template <typename C>
-__global__ void __launch_bounds__(C::THREADS, 2) lce_products_kernel(LceArgs a, Grid g) {
+__global__ void __launch_bounds__(C::THREADS, C::BOUND) lce_products_kernel(LceArgs a, Grid g) {
   __shared__ __align__(1024) char lds[C::ST * C::STAGE];
   const int count = __builtin_amdgcn_readfirstlane(*a.count), b = blockIdx.x;
   const DxShares sh = lce_dx_shares(a, count);
   const bool dw_first = int64_t(count) * sh.n > a.vn;
   const int b_dx = dw_first ? b - g.ndw : b, b_dw = dw_first ? b : b - g.ndx;
   if (dw_first ? b_dx >= 0 : b_dw < 0) {
-    const int xm = (count + TM - 1) / TM, tiles = xm * g.xn;
+    const int xm = (count + C::TM - 1) / C::TM, tiles = xm * g.xn;
     if (b_dx >= tiles * sh.n) return;
     const int id = xcd_tile(b_dx, tiles * sh.n);
     dx_tile<C>(a, tile_at(id % tiles, xm, g.xn, 4), id / tiles, sh, lds);
@@ -357,58 +370,52 @@ __global__ void __launch_bounds__(C::THREADS, 2) lce_products_kernel(LceArgs a, 
 
 template <typename T> T up(T a, int64_t b) { return static_cast<T>((a + b - 1) / b); }
 
-// 256 tokens a tile: 244 and 260 us for the two z products of 4096 x 768 x 32000 where 128 take 270 and 290; from
-// 2048 tokens (517 tokens: 48 against 45, and half of a small batch's last tile is padding).
-bool wide(int64_t N) { return N >= 2048; }
+// The tile of the logits' products: 256 x 256 moves the least through the caches (244 and 260 us for the two products of
+// 4096 x 768 x 32000 where 256 x 128 take 270 and 290); 256 x 128 for fewer tokens (517: 45 against 48 us).  128 x 128
+// gained 4 us of 55 with 64 tokens and lost with 256 and more.
+template <typename F> auto with_shape(int64_t N, F &&f) { return N >= 2048 ? f(Wide{}) : f(Narrow{}); }
 
 }  // namespace
 
-bool lce_bf16_serves(const void *w, int64_t ldw, int d, int dtype) {
-  return dtype == MOTIF_BF16 && d % 8 == 0 && ldw % 8 == 0 && ldw < (1 << 21) && reinterpret_cast<uintptr_t>(w) % 16 == 0;
+bool lce_bf16_direct(const void *w, int64_t ldw, int d) {
+  return d % 8 == 0 && ldw % 8 == 0 && ldw < (1 << 21) && reinterpret_cast<uintptr_t>(w) % 16 == 0;
 }
 
-int lce_bf16_parts(int V) { return 2 * up(V, TM); }
+int lce_bf16_parts(int V, int N) {
+  return with_shape(N, [&](auto c) { return 2 * up(V, decltype(c)::TM); });
+}
 
 // Shares of a piece's vocabulary rows in dX: so many that none takes longer than the launch's work spread
 // over the places (two workgroups per CU) does.  Each costs partial sums of N x d in fp32.
 int lce_bf16_dx_splits(int64_t N, int d, int V, int vc) {
   const int64_t bk = Narrow::BK, tn = up(d, Narrow::TN), places = 512;
   const int64_t n = std::min(V, vc), steps = up(n, bk);
-  const int64_t all = up(N, TM) * tn * steps + up(n, TM) * tn * up(N, bk);
-  return static_cast<int>(std::min<int64_t>({int64_t(16), steps, up(steps * places, all)}));
+  const int64_t all = up(N, Narrow::TM) * tn * steps + up(n, Narrow::TM) * tn * up(N, bk);
+  return static_cast<int>(std::min<int64_t>({int64_t(kMaxShares), steps, up(steps * places, all)}));
 }
 
 namespace {
 
-template <typename C, bool GRADS> void z_launch(const LceArgs &a, hipStream_t s) {
-  const int nm = up(GRADS ? a.vn : a.V, TM), nn = up(a.N, C::TN);
-  lce_z_kernel<C, GRADS><<<nm * nn, C::THREADS, 0, s>>>(a, nm, nn);
-}
-
-template <typename C> void products_launch(const LceArgs &a, bool dx, bool dw, hipStream_t s) {
-  const Grid g = [&] {
-    const int xn = up(a.d, C::TN), wm = up(a.vn, TM);
-    return Grid{xn, dx ? up(a.dx_tiles * xn * a.dx_splits, 8) * 8 : 0, wm, xn, dw ? up(wm * xn, 8) * 8 : 0};
-  }();
-  lce_products_kernel<C><<<g.ndx + g.ndw, C::THREADS, 0, s>>>(a, g);
+template <bool GRADS> int z_launch(const LceArgs &a, hipStream_t s) {
+  return with_shape(a.N, [&](auto c) {
+    using C = decltype(c);
+    const int nm = up(GRADS ? a.vn : a.V, C::TM), nn = up(a.N, C::TN);
+    lce_z_kernel<C, GRADS><<<nm * nn, C::THREADS, 0, s>>>(a, nm, nn);
+    return check_launch("lce_z_kernel");
+  });
 }
 
 }  // namespace
 
-int launch_lce_bf16_stats(const LceArgs &a, hipStream_t s) {
-  if (wide(a.N)) z_launch<Wide, false>(a, s);
-  else z_launch<Narrow, false>(a, s);
-  return check_launch("lce_z_kernel (statistics)");
-}
+int launch_lce_bf16_stats(const LceArgs &a, hipStream_t s) { return z_launch<false>(a, s); }
 
-int launch_lce_bf16_grads(const LceArgs &a, hipStream_t s) {
-  if (wide(a.N)) z_launch<Wide, true>(a, s);
-  else z_launch<Narrow, true>(a, s);
-  return check_launch("lce_z_kernel (gradients)");
-}
+int launch_lce_bf16_grads(const LceArgs &a, hipStream_t s) { return z_launch<true>(a, s); }
 
 int launch_lce_bf16_products(const LceArgs &a, bool dx, bool dw, hipStream_t s) {
-  products_launch<Narrow>(a, dx, dw, s);
+  using C = Narrow;
+  const int xn = up(a.d, C::TN), wm = up(a.vn, C::TM);
+  const Grid g{xn, dx ? up(a.dx_tiles * xn * a.dx_splits, 8) * 8 : 0, wm, xn, dw ? up(wm * xn, 8) * 8 : 0};
+  lce_products_kernel<C><<<g.ndx + g.ndw, C::THREADS, 0, s>>>(a, g);
   return check_launch("lce_products_kernel");
 }
 

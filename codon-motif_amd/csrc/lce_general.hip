@@ -1,5 +1,4 @@
-// Cross entropy from hidden states on the fp32 matrix instructions (v_mfma_f32_32x32x2_f32): fp32
-// inputs, and bf16 ones whose rows the bf16 kernels cannot load 16 bytes at a time.  One product,
+// Cross entropy from hidden states for fp32 inputs, on v_mfma_f32_32x32x2_f32.  One product,
 // C = A B^T over k, in four uses: z = W X^T (row statistics, or P), dX = P W, dW = P^T X.  A
 // workgroup of four waves owns 64 x 64 or 128 x 128 of C and stages 32 or 16 k of both sides in LDS
 // as fp32, k outermost, the next ones in registers meanwhile; the matrix instruction (64 cycles for two
@@ -20,9 +19,9 @@ template <int MB> struct Tile {
 constexpr int kChain = 512;  // k summed after each other
 
 // TM rows x BK k of an operand: element (m, k) at p[m ld + k] (KIN) or p[k ld + m]; zero outside.
-template <int MB, typename T, bool KIN> struct Side {
+template <int MB, bool KIN> struct Side {
   using X = Tile<MB>;
-  const T *p;
+  const float *p;
   int64_t ld;
   int m_max, k_max;  // elements from p on
   float r[8];
@@ -32,7 +31,7 @@ template <int MB, typename T, bool KIN> struct Side {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int m = m_of(i), k = k0 + k_of(i);
-      r[i] = m < m_max && k < k_max ? motif::ld(p + (KIN ? int64_t(m) * ld + k : int64_t(k) * ld + m)) : 0.f;
+      r[i] = m < m_max && k < k_max ? p[KIN ? int64_t(m) * ld + k : int64_t(k) * ld + m] : 0.f;
     }
   }
   __device__ __forceinline__ void store(float *s) const {
@@ -90,15 +89,15 @@ __device__ __forceinline__ void product(SA &A, SB &B, int kb, int ke, float *sa,
 }
 
 // z of TM vocabulary rows and TM tokens, then their statistics or P
-template <int MB, typename T, bool GRADS>
+template <int MB, bool GRADS>
 __global__ void __launch_bounds__(256) lce_general_z_kernel(LceArgs a) {
   using X = Tile<MB>;
   __shared__ float sa[X::SIZE], sb[X::SIZE];
   const int count = __builtin_amdgcn_readfirstlane(*a.count);
   const int t0 = blockIdx.y * X::TM, v0 = (GRADS ? a.v0 : 0) + blockIdx.x * X::TM;
   if (t0 >= count) return;
-  Side<MB, T, true> A{static_cast<const T *>(a.w) + int64_t(v0) * a.ldw, a.ldw, a.V - v0, a.d};
-  Side<MB, T, true> B{static_cast<const T *>(a.x) + int64_t(t0) * a.ldx, a.ldx, count - t0, a.d};
+  Side<MB, true> A{static_cast<const float *>(a.w) + int64_t(v0) * a.ldw, a.ldw, a.V - v0, a.d};
+  Side<MB, true> B{static_cast<const float *>(a.x) + int64_t(t0) * a.ldx, a.ldx, count - t0, a.d};
   f32x16 acc[MB][MB];
   product<MB>(A, B, 0, a.d, sa, sb, acc);
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6, h = l >> 5;
@@ -125,7 +124,7 @@ __global__ void __launch_bounds__(256) lce_general_z_kernel(LceArgs a) {
 }
 
 // Share blockIdx.z of dX [tokens, d] += P W over the piece
-template <int MB, typename T>
+template <int MB>
 __global__ void __launch_bounds__(256) lce_general_dx_kernel(LceArgs a) {
   using X = Tile<MB>;
   __shared__ float sa[X::SIZE], sb[X::SIZE];
@@ -134,8 +133,8 @@ __global__ void __launch_bounds__(256) lce_general_dx_kernel(LceArgs a) {
   if (t0 >= count) return;
   const int steps = (a.vn + X::BK - 1) / X::BK, per = (steps + a.dx_splits - 1) / a.dx_splits;
   const int kb = min(a.vn, int(blockIdx.z) * per * X::BK), ke = min(a.vn, kb + per * X::BK);
-  Side<MB, float, true> A{static_cast<const float *>(a.p) + int64_t(t0) * a.vc, a.vc, count - t0, a.vn};
-  Side<MB, T, false> B{static_cast<const T *>(a.w) + int64_t(a.v0) * a.ldw + c0, a.ldw, a.d - c0, a.vn};
+  Side<MB, true> A{static_cast<const float *>(a.p) + int64_t(t0) * a.vc, a.vc, count - t0, a.vn};
+  Side<MB, false> B{static_cast<const float *>(a.w) + int64_t(a.v0) * a.ldw + c0, a.ldw, a.d - c0, a.vn};
   f32x16 acc[MB][MB];
   product<MB>(A, B, kb, ke, sa, sb, acc);
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6, h = l >> 5;
@@ -157,14 +156,14 @@ __global__ void __launch_bounds__(256) lce_general_dx_kernel(LceArgs a) {
 }
 
 // dW rows of the piece = P^T X
-template <int MB, typename T>
+template <int MB>
 __global__ void __launch_bounds__(256) lce_general_dw_kernel(LceArgs a) {
   using X = Tile<MB>;
   __shared__ float sa[X::SIZE], sb[X::SIZE];
   const int count = __builtin_amdgcn_readfirstlane(*a.count);
   const int r0 = blockIdx.y * X::TM, c0 = blockIdx.x * X::TM;
-  Side<MB, float, false> A{static_cast<const float *>(a.p) + r0, a.vc, a.vn - r0, count};
-  Side<MB, T, false> B{static_cast<const T *>(a.x) + c0, a.ldx, a.d - c0, count};
+  Side<MB, false> A{static_cast<const float *>(a.p) + r0, a.vc, a.vn - r0, count};
+  Side<MB, false> B{static_cast<const float *>(a.x) + c0, a.ldx, a.d - c0, count};
   f32x16 acc[MB][MB];
   product<MB>(A, B, 0, count, sa, sb, acc);
   const float f = lce_factor(a, count);
@@ -177,7 +176,7 @@ __global__ void __launch_bounds__(256) lce_general_dw_kernel(LceArgs a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int r = r0 + 32 * MB * (w & 1) + 32 * mb + acc_row(i, h);
-        if (r < a.vn && c < a.d) st(static_cast<T *>(a.dw) + int64_t(a.v0 + r) * a.d + c, acc[mb][nb][i] * f);
+        if (r < a.vn && c < a.d) static_cast<float *>(a.dw)[int64_t(a.v0 + r) * a.d + c] = acc[mb][nb][i] * f;
       }
     }
 }
@@ -187,26 +186,6 @@ __global__ void __launch_bounds__(256) lce_general_dw_kernel(LceArgs a) {
 bool small(int x, int y, int z = 1) { return int64_t((x + 127) / 128) * ((y + 127) / 128) * z < 512; }
 template <int MB> dim3 tiles(int x, int y, int z = 1) {
   return dim3((x + Tile<MB>::TM - 1) / Tile<MB>::TM, (y + Tile<MB>::TM - 1) / Tile<MB>::TM, z);
-}
-
-template <typename T> void z_launch(const LceArgs &a, bool grads, hipStream_t s) {
-  if (grads) {
-    if (small(a.vn, a.N)) lce_general_z_kernel<1, T, true><<<tiles<1>(a.vn, a.N), 256, 0, s>>>(a);
-    else lce_general_z_kernel<2, T, true><<<tiles<2>(a.vn, a.N), 256, 0, s>>>(a);
-  } else {
-    if (small(a.V, a.N)) lce_general_z_kernel<1, T, false><<<tiles<1>(a.V, a.N), 256, 0, s>>>(a);
-    else lce_general_z_kernel<2, T, false><<<tiles<2>(a.V, a.N), 256, 0, s>>>(a);
-  }
-}
-
-template <typename T> void dx_launch(const LceArgs &a, hipStream_t s) {
-  if (small(a.d, a.N, a.dx_splits)) lce_general_dx_kernel<1, T><<<tiles<1>(a.d, a.N, a.dx_splits), 256, 0, s>>>(a);
-  else lce_general_dx_kernel<2, T><<<tiles<2>(a.d, a.N, a.dx_splits), 256, 0, s>>>(a);
-}
-
-template <typename T> void dw_launch(const LceArgs &a, hipStream_t s) {
-  if (small(a.d, a.vn)) lce_general_dw_kernel<1, T><<<tiles<1>(a.d, a.vn), 256, 0, s>>>(a);
-  else lce_general_dw_kernel<2, T><<<tiles<2>(a.d, a.vn), 256, 0, s>>>(a);
 }
 
 }  // namespace
@@ -223,27 +202,27 @@ int lce_general_dx_splits(int64_t N, int d, int V, int vc) {
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({512 / t, int64_t(most), int64_t(16)})));
 }
 
-int launch_lce_general_stats(const LceArgs &a, int dtype, hipStream_t s) {
-  if (dtype == MOTIF_F32) z_launch<float>(a, false, s);
-  else z_launch<bf16_t>(a, false, s);
+int launch_lce_general_stats(const LceArgs &a, hipStream_t s) {
+  if (small(a.V, a.N)) lce_general_z_kernel<1, false><<<tiles<1>(a.V, a.N), 256, 0, s>>>(a);
+  else lce_general_z_kernel<2, false><<<tiles<2>(a.V, a.N), 256, 0, s>>>(a);
   return check_launch("lce_general_z_kernel (statistics)");
 }
 
-int launch_lce_general_grads(const LceArgs &a, int dtype, hipStream_t s) {
-  if (dtype == MOTIF_F32) z_launch<float>(a, true, s);
-  else z_launch<bf16_t>(a, true, s);
+int launch_lce_general_grads(const LceArgs &a, hipStream_t s) {
+  if (small(a.vn, a.N)) lce_general_z_kernel<1, true><<<tiles<1>(a.vn, a.N), 256, 0, s>>>(a);
+  else lce_general_z_kernel<2, true><<<tiles<2>(a.vn, a.N), 256, 0, s>>>(a);
   return check_launch("lce_general_z_kernel (gradients)");
 }
 
-int launch_lce_general_dx(const LceArgs &a, int dtype, hipStream_t s) {
-  if (dtype == MOTIF_F32) dx_launch<float>(a, s);
-  else dx_launch<bf16_t>(a, s);
+int launch_lce_general_dx(const LceArgs &a, hipStream_t s) {
+  if (small(a.d, a.N, a.dx_splits)) lce_general_dx_kernel<1><<<tiles<1>(a.d, a.N, a.dx_splits), 256, 0, s>>>(a);
+  else lce_general_dx_kernel<2><<<tiles<2>(a.d, a.N, a.dx_splits), 256, 0, s>>>(a);
   return check_launch("lce_general_dx_kernel");
 }
 
-int launch_lce_general_dw(const LceArgs &a, int dtype, hipStream_t s) {
-  if (dtype == MOTIF_F32) dw_launch<float>(a, s);
-  else dw_launch<bf16_t>(a, s);
+int launch_lce_general_dw(const LceArgs &a, hipStream_t s) {
+  if (small(a.d, a.vn)) lce_general_dw_kernel<1><<<tiles<1>(a.d, a.vn), 256, 0, s>>>(a);
+  else lce_general_dw_kernel<2><<<tiles<2>(a.d, a.vn), 256, 0, s>>>(a);
   return check_launch("lce_general_dw_kernel");
 }
 

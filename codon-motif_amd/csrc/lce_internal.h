@@ -1,6 +1,6 @@
 // Softmax cross entropy straight from hidden states X [N, d] and the vocabulary's rows W [V, d]
-// (linear_ce.hip: the entries and the row kernels; lce_general.hip: fp32 matrix products for every
-// type, size and alignment; lce_bf16.hip: bf16 on the matrix instructions).
+// (linear_ce.hip: the entries and the row kernels; lce_general.hip: the products of fp32 inputs;
+// lce_bf16.hip: those of bf16).
 //
 // With z_iv = x_i . w_v, s_i the gradient of row i's loss and t_i its label:
 //   loss_i = log sum_v e^{z_iv} - z_{i t_i}
@@ -21,7 +21,7 @@ struct LceArgs {
   const void *x;       // [count, ldx]: the labelled rows
   const void *w;       // [V, d], row stride ldw
   int64_t ldx, ldw;
-  int N, d, V;
+  int N, d, V, dk;     // dk: columns of x and w that the bf16 kernels read (d, or with zeros up to a multiple of 8)
   const int *row;      // [N] original row of labelled row i
   const int *label;    // [N] its label (-1: outside the vocabulary; loss and gradient are NaN)
   const int *pos;      // [N] labelled position of original row r, or -1
@@ -54,11 +54,12 @@ __device__ __forceinline__ void lse_merge(float &m, float &s, float m2, float s2
 
 // dX in shares of a piece's vocabulary rows: `dx_splits` of [n_pad, d] partial sums, or (dx_tiles: the tiles of 256
 // that n_pad makes) as many of the labelled rows' as fit the same place.
+constexpr int kMaxShares = 32;
 struct DxShares { int n; int64_t rows; };
 __device__ __forceinline__ DxShares lce_dx_shares(const LceArgs &a, int count) {
   if (!a.dx_tiles) return {a.dx_splits, a.n_pad};
   const int live = max(1, (count + 255) / 256);
-  return {min(16, a.dx_splits * a.dx_tiles / live), int64_t(live) * 256};
+  return {min(kMaxShares, a.dx_splits * a.dx_tiles / live), int64_t(live) * 256};
 }
 
 // Forward: the pair of a wave's MB x 32 vocabulary rows from v0 for each of its NB x 32 tokens from t0,
@@ -160,17 +161,18 @@ __device__ __forceinline__ void lce_row_grads(const LceArgs &a, f32x16 (&acc)[MB
   }
 }
 
-// lce_general.hip: the products on fp32 matrix instructions, any alignment (P is fp32 [N, vc])
+// lce_general.hip: fp32 products, any alignment (P is fp32 [N, vc])
 int lce_general_parts(int V, int N);
-int launch_lce_general_stats(const LceArgs &a, int dtype, hipStream_t s);
-int launch_lce_general_grads(const LceArgs &a, int dtype, hipStream_t s);  // P of the piece
+int launch_lce_general_stats(const LceArgs &a, hipStream_t s);
+int launch_lce_general_grads(const LceArgs &a, hipStream_t s);  // P of the piece
 int lce_general_dx_splits(int64_t N, int d, int V, int vc);
-int launch_lce_general_dx(const LceArgs &a, int dtype, hipStream_t s);
-int launch_lce_general_dw(const LceArgs &a, int dtype, hipStream_t s);
+int launch_lce_general_dx(const LceArgs &a, hipStream_t s);
+int launch_lce_general_dw(const LceArgs &a, hipStream_t s);
 
-// lce_bf16.hip: bf16 whose vocabulary rows start on 16-byte boundaries (P is bf16 in blocks)
-bool lce_bf16_serves(const void *w, int64_t ldw, int d, int dtype);
-int lce_bf16_parts(int V);
+// lce_bf16.hip: bf16 (P is bf16 in blocks).  Vocabulary rows that do not start on 16-byte boundaries are
+// copied to some that do first (`direct`: no need).
+bool lce_bf16_direct(const void *w, int64_t ldw, int d);
+int lce_bf16_parts(int V, int N);
 int lce_bf16_dx_splits(int64_t N, int d, int V, int vc);
 int launch_lce_bf16_stats(const LceArgs &a, hipStream_t s);
 int launch_lce_bf16_grads(const LceArgs &a, hipStream_t s);

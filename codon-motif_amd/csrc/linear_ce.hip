@@ -94,6 +94,13 @@ __global__ void __launch_bounds__(256) lce_gather_kernel(const T *x, int64_t rs,
   }
 }
 
+// The vocabulary's rows on 16-byte boundaries with zeros up to ldo, one wave a row.
+__global__ void __launch_bounds__(256) lce_copy_kernel(const bf16_t *w, int64_t rs, bf16_t *out, int V, int d, int ldo) {
+  const int v = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (v >= V) return;
+  for (int c = threadIdx.x & 63; c < ldo; c += 64) out[int64_t(v) * ldo + c] = c < d ? w[v * rs + c] : bf16_t(0);
+}
+
 // A row's parts joined: 32 rows a workgroup, 32 threads to each (250 parts of 4096 rows: 23 us with 64 rows and
 // four threads to each, whose loads followed each other).
 __global__ void __launch_bounds__(1024) lce_combine_kernel(LceArgs a, int nparts, float *nll, float *loss_rows) {
@@ -138,41 +145,40 @@ __global__ void __launch_bounds__(1024) lce_loss_kernel(const float *nll, const 
   *loss = static_cast<float>(mean ? s / n : s);  // (no label at all: 0 / 0)
 }
 
-// dX rows: the partial sums of a labelled row times the common factor, rounded once; zeros for the others.  One wave
-// a row; E = 4 where d is a multiple of 4.
+// dX rows: the partial sums of a labelled row times the common factor, rounded once; zeros for the others.  A wave takes
+// 64 E columns of a row (`per` of them make a row); E = 4 where d is a multiple of 4.
 template <typename T, int E>
-__global__ void __launch_bounds__(256) lce_dx_rows_kernel(LceArgs a, T *dx) {
-  const int64_t r = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (r >= a.N) return;
-  const int i = a.pos[r];
-  const int count = *a.count;
-  const float f = lce_factor(a, count);
-  const DxShares sh = lce_dx_shares(a, count);
-  const float *p = a.dx_part + int64_t(i < 0 ? 0 : i) * a.d;
-  const int64_t plane = sh.rows * a.d;
-  for (int c = (threadIdx.x & 63) * E; c < a.d; c += 64 * E) {
-    float s[E] = {};
-    if (i >= 0) {
-#pragma unroll 4
-      for (int k = 0; k < sh.n; ++k) {
-        float v[E];
-        if (E == 4) {
-          const float4 u = *reinterpret_cast<const float4 *>(p + k * plane + c);
-          v[0] = u.x, v[1 % E] = u.y, v[2 % E] = u.z, v[3 % E] = u.w;
-        } else {
-          v[0] = p[k * plane + c];
-        }
-#pragma unroll
-        for (int e = 0; e < E; ++e) s[e] += v[e];
+__global__ void __launch_bounds__(256) lce_dx_rows_kernel(LceArgs a, T *dx, int per) {
+  const int64_t id = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t r = id / per;
+  const int c = (static_cast<int>(id - r * per) * 64 + (threadIdx.x & 63)) * E;
+  if (r >= a.N || c >= a.d) return;
+  const int i = a.pos[r], count = *a.count;
+  float s[E] = {};
+  if (i >= 0) {
+    const float f = lce_factor(a, count);
+    const DxShares sh = lce_dx_shares(a, count);
+    const float *p = a.dx_part + int64_t(i) * a.d + c;
+    const int64_t plane = sh.rows * a.d;
+#pragma unroll 8
+    for (int k = 0; k < sh.n; ++k) {
+      float v[E];
+      if (E == 4) {
+        const float4 u = *reinterpret_cast<const float4 *>(p + k * plane);
+        v[0] = u.x, v[1 % E] = u.y, v[2 % E] = u.z, v[3 % E] = u.w;
+      } else {
+        v[0] = p[k * plane];
       }
 #pragma unroll
-      for (int e = 0; e < E; ++e) s[e] *= f;
+      for (int e = 0; e < E; ++e) s[e] += v[e];
     }
-    T o[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) st(o + e, s[e]);
-    __builtin_memcpy(dx + r * a.d + c, o, sizeof(o));
+    for (int e = 0; e < E; ++e) s[e] *= f;
   }
+  T o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) st(o + e, s[e]);
+  __builtin_memcpy(dx + r * a.d + c, o, sizeof(o));
 }
 
 constexpr size_t kAlign = 256;
@@ -180,34 +186,41 @@ size_t up(size_t n, size_t m) { return (n + m - 1) / m * m; }
 
 int esize(int dtype) { return dtype == MOTIF_F32 ? 4 : 2; }
 
-// The forward's workspace: statistics of the vocabulary's parts, z at the labels, the rows' losses.
+// Copies of vocabulary rows (bf16 off 16-byte boundaries); 0: none
+size_t copy_bytes(const void *w, int64_t w_rs, int d, int V, int dtype) {
+  return dtype != MOTIF_BF16 || lce_bf16_direct(w, w_rs, d) ? 0 : up(size_t(V) * up(d, 64) * 2, kAlign);
+}
+
+// The forward's workspace: copied vocabulary rows, statistics of the vocabulary's parts, z at the labels, the rows' losses.
 struct FwdSpace {
+  int parts;
   size_t m, s, z, nll, bytes;
-  FwdSpace(int N, int V) {
-    const size_t parts = lce_general_parts(V, N), col = up(4 * size_t(N), kAlign);
-    m = 0;
-    s = up(parts * 4 * N, kAlign);
-    z = 2 * s;
+  FwdSpace(int N, int V, int dtype, size_t copy) {
+    parts = dtype == MOTIF_BF16 ? lce_bf16_parts(V, N) : lce_general_parts(V, N);
+    const size_t col = up(4 * size_t(N), kAlign), part = up(size_t(parts) * 4 * N, kAlign);
+    m = copy;
+    s = m + part;
+    z = s + part;
     nll = z + col;
     bytes = nll + col;
   }
 };
 
-// The backward's: P of a vocabulary piece and fp32 partial dX.  A piece holds P in 256 MB (so that it
-// stays in the memory-side cache between its three products), but no fewer than 4096 vocabulary rows:
-// every piece reads and writes the partial dX once.
+// The backward's: copied vocabulary rows, P of a vocabulary piece and fp32 partial dX.  A piece holds P in 256 MB (so that
+// it stays in the memory-side cache between its three products; 512 MB and 1 GB were no faster), but no fewer than 4096
+// vocabulary rows: every piece reads and writes the partial dX once.
 struct BwdSpace {
   int vc, splits;
   int64_t n_pad;
   size_t p, dx, bytes;
-  BwdSpace(int64_t N, int d, int V, bool general) {
-    const size_t e = general ? 4 : 2;
+  BwdSpace(int64_t N, int d, int V, int dtype, size_t copy) {
+    const size_t e = esize(dtype);
     n_pad = static_cast<int64_t>(up(N, 256));
     const size_t rows = (size_t(1) << 28) / (n_pad * e) / 256 * 256;
     vc = static_cast<int>(std::min(std::max<size_t>(rows, 4096), up(V, 256)));
-    splits = general ? lce_general_dx_splits(N, d, V, vc) : lce_bf16_dx_splits(N, d, V, vc);
-    p = 0;
-    dx = up(size_t(n_pad) * vc * e, kAlign);
+    splits = dtype == MOTIF_BF16 ? lce_bf16_dx_splits(N, d, V, vc) : lce_general_dx_splits(N, d, V, vc);
+    p = copy;
+    dx = p + up(size_t(n_pad) * vc * e, kAlign);
     bytes = dx + size_t(splits) * n_pad * d * 4;
   }
 };
@@ -222,6 +235,16 @@ void bind_kept(LceArgs &a, int *kept) {
   a.pos = kept + 2 * N;
   a.lse = reinterpret_cast<float *>(kept + 3 * N);
   a.count = kept + 4 * N;
+}
+
+// w, or its copy at `ws`
+int bind_weight(LceArgs &a, const void *w, int64_t w_rs, size_t copy, void *ws, hipStream_t s) {
+  a.w = w, a.ldw = w_rs, a.dk = static_cast<int>(up(a.d, 8));
+  if (!copy) return MOTIF_OK;
+  a.w = ws, a.ldw = static_cast<int64_t>(up(a.d, 64));
+  lce_copy_kernel<<<(a.V + 3) / 4, 256, 0, s>>>(static_cast<const bf16_t *>(w), w_rs, static_cast<bf16_t *>(ws), a.V, a.d,
+                                                 static_cast<int>(a.ldw));
+  return check_launch("lce_copy_kernel");
 }
 
 template <typename T> int gather(const void *x, int64_t rs, const LceArgs &a, void *out, hipStream_t s) {
@@ -245,11 +268,10 @@ extern "C" size_t motif_linear_ce_rows_bytes(int N, int d, int dtype) {
   return size_t(N) * up(d, 64) * esize(dtype);
 }
 
-extern "C" size_t motif_linear_ce_workspace_bytes(int N, int d, int V, int dtype, int backward) {
+extern "C" size_t motif_linear_ce_workspace_bytes(int N, int d, const void *w, int64_t w_rs, int V, int dtype, int backward) {
   if (!sizes_ok(N, d, V)) return 0;
-  if (!backward) return FwdSpace(N, V).bytes;
-  const size_t g = BwdSpace(N, d, V, true).bytes;
-  return dtype == MOTIF_BF16 ? std::max(g, BwdSpace(N, d, V, false).bytes) : g;
+  const size_t copy = copy_bytes(w, w_rs, d, V, dtype);
+  return backward ? BwdSpace(N, d, V, dtype, copy).bytes : FwdSpace(N, V, dtype, copy).bytes;
 }
 
 extern "C" int motif_linear_ce_fwd(const void *x, int64_t x_rs, const void *w, int64_t w_rs, const int64_t *labels,
@@ -262,13 +284,13 @@ extern "C" int motif_linear_ce_fwd(const void *x, int64_t x_rs, const void *w, i
   if (!x || !w || !labels || !rows || !kept || !loss || !workspace)
     return set_error(MOTIF_ERR_INVALID, "linear_ce_fwd: null pointer");
   if (x_rs < 0 || (V > 1 && w_rs < d)) return set_error(MOTIF_ERR_INVALID, "linear_ce_fwd: rows overlap");
-  const FwdSpace f(N, V);
+  const size_t copy = copy_bytes(w, w_rs, d, V, dtype);
+  const FwdSpace f(N, V, dtype, copy);
   if (workspace_bytes < f.bytes) return set_error(MOTIF_ERR_INVALID, "linear_ce_fwd: workspace too small");
   hipStream_t s = static_cast<hipStream_t>(stream);
   LceArgs a{};
   a.N = N, a.d = d, a.V = V;
   a.x = rows, a.ldx = static_cast<int64_t>(up(d, 64));
-  a.w = w, a.ldw = w_rs;
   bind_kept(a, kept);
   char *ws = static_cast<char *>(workspace);
   a.part_m = reinterpret_cast<float *>(ws + f.m);
@@ -279,12 +301,11 @@ extern "C" int motif_linear_ce_fwd(const void *x, int64_t x_rs, const void *w, i
                                      kept + 4 * int64_t(N), loss_rows);
   int rc = check_launch("lce_plan_kernel");
   if (rc == MOTIF_OK) rc = dtype == MOTIF_F32 ? gather<float>(x, x_rs, a, rows, s) : gather<bf16_t>(x, x_rs, a, rows, s);
+  if (rc == MOTIF_OK) rc = bind_weight(a, w, w_rs, copy, ws, s);
   if (rc != MOTIF_OK) return rc;
-  const bool fast = lce_bf16_serves(w, w_rs, d, dtype);
-  const int nparts = fast ? lce_bf16_parts(V) : lce_general_parts(V, N);
-  rc = fast ? launch_lce_bf16_stats(a, s) : launch_lce_general_stats(a, dtype, s);
+  rc = dtype == MOTIF_BF16 ? launch_lce_bf16_stats(a, s) : launch_lce_general_stats(a, s);
   if (rc != MOTIF_OK) return rc;
-  lce_combine_kernel<<<(N + 31) / 32, 1024, 0, s>>>(a, nparts, nll, loss_rows);
+  lce_combine_kernel<<<(N + 31) / 32, 1024, 0, s>>>(a, f.parts, nll, loss_rows);
   rc = check_launch("lce_combine_kernel");
   if (rc != MOTIF_OK || reduction == 0) return rc;
   lce_loss_kernel<<<1, 1024, 0, s>>>(nll, a.count, reduction == 2, loss);
@@ -300,41 +321,42 @@ extern "C" int motif_linear_ce_bwd(const void *rows, const void *w, int64_t w_rs
   if (!rows || !w || !kept || !dloss || !workspace) return set_error(MOTIF_ERR_INVALID, "linear_ce_bwd: null pointer");
   if (V > 1 && w_rs < d) return set_error(MOTIF_ERR_INVALID, "linear_ce_bwd: rows overlap");
   if (!dx && !dw) return MOTIF_OK;
-  const bool fast = lce_bf16_serves(w, w_rs, d, dtype);
-  const BwdSpace b(N, d, V, !fast);
+  const bool bf16 = dtype == MOTIF_BF16;
+  const size_t copy = copy_bytes(w, w_rs, d, V, dtype);
+  const BwdSpace b(N, d, V, dtype, copy);
   if (workspace_bytes < b.bytes) return set_error(MOTIF_ERR_INVALID, "linear_ce_bwd: workspace too small");
   hipStream_t s = static_cast<hipStream_t>(stream);
   LceArgs a{};
   a.N = N, a.d = d, a.V = V;
   a.x = rows, a.ldx = static_cast<int64_t>(up(d, 64));
-  a.w = w, a.ldw = w_rs;
   bind_kept(a, const_cast<int *>(kept));
   a.dloss = dloss, a.dl_st = dloss_st, a.reduction = reduction;
   char *ws = static_cast<char *>(workspace);
   a.p = ws + b.p;
   a.dx_part = reinterpret_cast<float *>(ws + b.dx);
-  a.n_pad = b.n_pad, a.dx_splits = b.splits, a.dx_tiles = fast ? static_cast<int>(b.n_pad / 256) : 0, a.vc = b.vc, a.dw = dw;
-  int rc = MOTIF_OK;
+  a.n_pad = b.n_pad, a.dx_splits = b.splits, a.dx_tiles = bf16 ? static_cast<int>(b.n_pad / 256) : 0, a.vc = b.vc, a.dw = dw;
+  int rc = bind_weight(a, w, w_rs, copy, ws, s);
   for (int v0 = 0; v0 < V && rc == MOTIF_OK; v0 += b.vc) {
     a.v0 = v0, a.vn = std::min(b.vc, V - v0), a.first = v0 == 0;
-    rc = fast ? launch_lce_bf16_grads(a, s) : launch_lce_general_grads(a, dtype, s);
+    rc = bf16 ? launch_lce_bf16_grads(a, s) : launch_lce_general_grads(a, s);
     if (rc != MOTIF_OK) break;
-    if (fast) {
+    if (bf16) {
       rc = launch_lce_bf16_products(a, dx, dw, s);
     } else {
-      if (dx) rc = launch_lce_general_dx(a, dtype, s);
-      if (rc == MOTIF_OK && dw) rc = launch_lce_general_dw(a, dtype, s);
+      if (dx) rc = launch_lce_general_dx(a, s);
+      if (rc == MOTIF_OK && dw) rc = launch_lce_general_dw(a, s);
     }
   }
   if (rc != MOTIF_OK || !dx) return rc;
-  const unsigned g = (N + 3) / 4;
-  const bool f32 = dtype == MOTIF_F32;
-  if (d % 4 == 0 && reinterpret_cast<uintptr_t>(dx) % 16 == 0) {
-    if (f32) lce_dx_rows_kernel<float, 4><<<g, 256, 0, s>>>(a, static_cast<float *>(dx));
-    else lce_dx_rows_kernel<bf16_t, 4><<<g, 256, 0, s>>>(a, static_cast<bf16_t *>(dx));
+  const bool four = d % 4 == 0 && reinterpret_cast<uintptr_t>(dx) % 16 == 0;
+  const int per = (d + (four ? 256 : 64) - 1) / (four ? 256 : 64);
+  const unsigned g = static_cast<unsigned>((int64_t(N) * per + 3) / 4);
+  if (four) {
+    if (bf16) lce_dx_rows_kernel<bf16_t, 4><<<g, 256, 0, s>>>(a, static_cast<bf16_t *>(dx), per);
+    else lce_dx_rows_kernel<float, 4><<<g, 256, 0, s>>>(a, static_cast<float *>(dx), per);
   } else {
-    if (f32) lce_dx_rows_kernel<float, 1><<<g, 256, 0, s>>>(a, static_cast<float *>(dx));
-    else lce_dx_rows_kernel<bf16_t, 1><<<g, 256, 0, s>>>(a, static_cast<bf16_t *>(dx));
+    if (bf16) lce_dx_rows_kernel<bf16_t, 1><<<g, 256, 0, s>>>(a, static_cast<bf16_t *>(dx), per);
+    else lce_dx_rows_kernel<float, 1><<<g, 256, 0, s>>>(a, static_cast<float *>(dx), per);
   }
   return check_launch("lce_dx_rows_kernel");
 }

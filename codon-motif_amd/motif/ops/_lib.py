@@ -125,7 +125,7 @@ _SIGNATURES = {
         _T4 * 5 + [_P] * 5 + [_P, _I64, _I64] + _T4 * 3 + [_P] + [_I32] * 7 + [_F32, _F32]
         + [_P, _SZ, _I32, _P], _I32),
     'motif_linear_ce_rows_bytes': ([_I32] * 3, _SZ),
-    'motif_linear_ce_workspace_bytes': ([_I32] * 5, _SZ),
+    'motif_linear_ce_workspace_bytes': ([_I32, _I32, _P, _I64, _I32, _I32, _I32], _SZ),
     'motif_linear_ce_fwd': (
         [_P, _I64, _P, _I64, _P, _I64, _I64] + [_I32] * 4 + [_P, _P, _P, _P, _SZ, _I32, _P], _I32),
     'motif_linear_ce_bwd': (

@@ -26,7 +26,7 @@ class LinearCEFunction(torch.autograd.Function):
         rows = torch.empty(lib.motif_linear_ce_rows_bytes(N, d, code), dtype=torch.uint8, device=dev)
         kept = torch.empty(4 * N + 1, dtype=torch.int32, device=dev)
         loss = torch.empty((N,) if reduction == 0 else (), dtype=torch.float32, device=dev)
-        nbytes = lib.motif_linear_ce_workspace_bytes(N, d, V, code, 0)
+        nbytes = lib.motif_linear_ce_workspace_bytes(N, d, weight.data_ptr(), weight.stride(0), V, code, 0)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         with _lib.on_device(dev):
             rc = lib.motif_linear_ce_fwd(
@@ -51,7 +51,7 @@ class LinearCEFunction(torch.autograd.Function):
         dx = torch.empty((N, d), dtype=dt, device=dev) if ctx.needs_input_grad[0] else None
         dw = torch.empty((V, d), dtype=dt, device=dev) if ctx.needs_input_grad[1] else None
         lib = _lib.lib()
-        nbytes = lib.motif_linear_ce_workspace_bytes(N, d, V, code, 1)
+        nbytes = lib.motif_linear_ce_workspace_bytes(N, d, weight.data_ptr(), weight.stride(0), V, code, 1)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         with _lib.on_device(dev):
             rc = lib.motif_linear_ce_bwd(

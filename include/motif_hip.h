@@ -805,10 +805,10 @@ int motif_mul_sigmoid(const void *x, int64_t x_rs, const void *g, int64_t g_rs, 
  *   log-sum-exps.
  * Backward: dloss fp32 ([N] at stride dloss_st for reduction 0, else one value); dx [N, d] and dw
  * [V, d], contiguous, dtype's type, either may be NULL.  Workspaces 16-byte aligned, of
- * motif_linear_ce_workspace_bytes(.., backward).  dtype: MOTIF_F32 or MOTIF_BF16.
+ * motif_linear_ce_workspace_bytes(.., backward) for that w (bf16 rows off 16-byte boundaries are copied).  dtype: MOTIF_F32 or MOTIF_BF16.
  */
 size_t motif_linear_ce_rows_bytes(int N, int d, int dtype);
-size_t motif_linear_ce_workspace_bytes(int N, int d, int V, int dtype, int backward);
+size_t motif_linear_ce_workspace_bytes(int N, int d, const void *w, int64_t w_rs, int V, int dtype, int backward);
 int motif_linear_ce_fwd(const void *x, int64_t x_rs, const void *w, int64_t w_rs, const int64_t *labels,
                         int64_t labels_st, int64_t ignore_index, int N, int d, int V, int reduction, void *rows,
                         int *kept, float *loss, void *workspace, size_t workspace_bytes, int dtype, void *stream);

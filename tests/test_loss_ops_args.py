@@ -104,10 +104,12 @@ def test_c_entries_check_their_arguments():
 def test_workspace_sizes():
     lib = _lib.lib()
     assert lib.motif_linear_ce_rows_bytes(5, 100, 1) == 5 * 128 * 2
-    assert lib.motif_linear_ce_rows_bytes(0, 100, 1) == 0 and lib.motif_linear_ce_workspace_bytes(5, 0, 3, 1, 0) == 0
+    assert lib.motif_linear_ce_rows_bytes(0, 100, 1) == 0 and lib.motif_linear_ce_workspace_bytes(5, 0, 16, 8, 3, 1, 0) == 0
     for N in (1, 300, 70000):
         for V in (1, 300, 50000):
-            assert lib.motif_linear_ce_workspace_bytes(N, 64, V, 1, 1) > lib.motif_linear_ce_rows_bytes(N, 64, 1)
+            aligned, off = (lib.motif_linear_ce_workspace_bytes(N, 64, at, 64, V, 1, 1) for at in (16, 18))
+            assert off >= aligned + V * 64 * 2 and aligned > lib.motif_linear_ce_rows_bytes(N, 64, 1)
+            assert lib.motif_linear_ce_workspace_bytes(N, 64, 18, 64, V, 0, 1) >= N * 64 * 4
     assert lib.motif_row_norm_bwd_workspace_bytes(10, 64, 1) == 2 * 10 * 64 * 4
     assert lib.motif_row_norm_bwd_workspace_bytes(10 ** 6, 64, 0) <= 4096 * 64 * 4  # (no more rows than workgroups)
 
