@@ -1,9 +1,13 @@
 // Cross entropy from hidden states for fp32 inputs, on v_mfma_f32_32x32x2_f32.  One product,
 // C = A B^T over k, in four uses: z = W X^T (row statistics, or P), dX = P W, dW = P^T X.  A
-// workgroup of four waves owns 64 x 64 or 128 x 128 of C and stages 32 or 16 k of both sides in LDS
-// as fp32, k outermost, the next ones in registers meanwhile; the matrix instruction (64 cycles for two
-// k) bounds it, so LDS reads of single words suffice.  Sums run over 512 k at a time, which are then added (one
-// chain over a vocabulary of 5000 lost a bit of dX: 1.3e-6 off where this is 7e-7).
+// workgroup of four waves owns 64 x 64 of C (32 x 32 a wave) and stages 32 k of both sides in LDS, k outermost,
+// twice: one place is filled, from registers loaded a step before, while the other is multiplied.  The matrix
+// instruction (64 cycles for two k) bounds it, so LDS reads of single words suffice.  (128 x 128 were slower
+// at every size: 512 x 1024 x 8192, dW 125 against 94 us.)  What is reached: 85-95 TFLOP/s at 2048 x 768 x 8192, where
+// a large library product reaches 154; a wave per SIMD and workgroup, its chain of one accumulator and its barriers
+// leave the rest.
+// Sums run over 512 k at a time, which are then added (one chain over a vocabulary of 5000 lost a bit of dX: 1.3e-6
+// off where this is 6e-7).
 #include "lce_internal.h"
 
 #include <algorithm>
@@ -12,217 +16,217 @@ namespace motif {
 
 namespace {
 
-// Tiles of TM x TM, TM = 64 MB: one or two blocks of 32 a side for each of the four waves.
-template <int MB> struct Tile {
-  static constexpr int TM = 64 * MB, BK = 2048 / TM, LD = TM + 4, SIZE = BK * LD;
-};
-constexpr int kChain = 512;  // k summed after each other
+constexpr int TM = 64, BK = 32, LD = TM + 4, SIZE = BK * LD;
+constexpr int kChain = 512;
 
-// TM rows x BK k of an operand: element (m, k) at p[m ld + k] (KIN) or p[k ld + m]; zero outside.
-template <int MB, bool KIN> struct Side {
-  using X = Tile<MB>;
+// TM rows x BK k of an operand: element (m, k) at p[m ld + k] (KIN) or p[k ld + m]; zero outside.  VEC: 16 bytes a load,
+// through a range-checked buffer (rows on 16-byte boundaries, k_max a multiple of 4 where KIN).
+template <bool KIN, bool VEC> struct Side {
+  static constexpr int E = VEC ? 4 : 1, N = 8 / E, ROW = (KIN ? BK : TM) / E;  // accesses of a thread, and along memory
   const float *p;
   int64_t ld;
   int m_max, k_max;  // elements from p on
   float r[8];
-  __device__ __forceinline__ static int m_of(int i) { return KIN ? threadIdx.x / X::BK + 256 / X::BK * i : threadIdx.x % X::TM; }
-  __device__ __forceinline__ static int k_of(int i) { return KIN ? threadIdx.x % X::BK : threadIdx.x / X::TM + 256 / X::TM * i; }
+  __device__ __forceinline__ static int along(int i) { return (threadIdx.x + 256 * i) % ROW * E; }
+  __device__ __forceinline__ static int across(int i) { return (threadIdx.x + 256 * i) / ROW; }
   __device__ __forceinline__ void load(int k0) {
+    if (VEC) {
+      const int n = KIN ? min(m_max, TM) : min(k_max - k0, BK);
+      const buf_t b = make_buf(KIN ? p : p + k0 * ld, n > 0 ? static_cast<uint32_t>(((n - 1) * ld + (KIN ? k_max : min(m_max, TM))) * 4) : 0u);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int m = m_of(i), k = k0 + k_of(i);
-      r[i] = m < m_max && k < k_max ? p[KIN ? int64_t(m) * ld + k : int64_t(k) * ld + m] : 0.f;
+      for (int i = 0; i < N; ++i) {
+        const int k = k0 + along(i);
+        const uint32_t off = static_cast<uint32_t>((across(i) * ld + (KIN ? k : along(i))) * 4);
+        const uint4 u = buf_ld16(b, !KIN || k < k_max ? off : 0xfffffff0u);
+        r[4 * i] = __uint_as_float(u.x), r[4 * i + 1] = __uint_as_float(u.y);
+        r[4 * i + 2] = __uint_as_float(u.z), r[4 * i + 3] = __uint_as_float(u.w);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int m = KIN ? across(i) : along(i), k = k0 + (KIN ? along(i) : across(i));
+        r[i] = m < m_max && k < k_max ? p[KIN ? int64_t(m) * ld + k : int64_t(k) * ld + m] : 0.f;
+      }
     }
   }
   __device__ __forceinline__ void store(float *s) const {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[k_of(i) * X::LD + m_of(i)] = r[i];
+    for (int i = 0; i < N; ++i) {
+      float *q = s + (KIN ? along(i) * LD + across(i) : across(i) * LD + along(i));
+      if (KIN || !VEC) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) q[e * LD] = r[E * i + e];
+      } else {
+        *reinterpret_cast<f32x4 *>(q) = f32x4{r[E * i], r[(E * i + 1) % 8], r[(E * i + 2) % 8], r[(E * i + 3) % 8]};
+      }
+    }
   }
 };
 
-template <int MB, typename SA, typename SB>
-__device__ __forceinline__ void product(SA &A, SB &B, int kb, int ke, float *sa, float *sb, f32x16 (&sum)[MB][MB]) {
-  using X = Tile<MB>;
+// C of the workgroup's tile over k in [kb, ke), this wave's 32 x 32 in sum[0][0]
+template <typename SA, typename SB>
+__device__ __forceinline__ void product(SA &A, SB &B, int kb, int ke, float *lds, f32x16 (&sum)[1][1]) {
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6, h = l >> 5;
-  f32x16 acc[MB][MB];
+  f32x16 acc;
 #pragma unroll
-  for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-    for (int nb = 0; nb < MB; ++nb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[mb][nb][i] = sum[mb][nb][i] = 0.f;
+  for (int i = 0; i < 16; ++i) acc[i] = sum[0][0][i] = 0.f;
   if (kb >= ke) return;
   A.load(kb);
   B.load(kb);
-  const float *pa = sa + 32 * MB * (w & 1) + (l & 31), *pb = sb + 32 * MB * (w >> 1) + (l & 31);
-  for (int k0 = kb; k0 < ke; k0 += X::BK) {
-    __syncthreads();
-    A.store(sa);
-    B.store(sb);
-    __syncthreads();
-    if (k0 + X::BK < ke) {
-      A.load(k0 + X::BK);
-      B.load(k0 + X::BK);
+  A.store(lds);
+  B.store(lds + SIZE);
+  int at = 0;
+  for (int k0 = kb; k0 < ke; k0 += BK) {
+    const bool more = k0 + BK < ke;
+    if (more) {
+      A.load(k0 + BK);
+      B.load(k0 + BK);
     }
+    __syncthreads();
+    const float *pa = lds + at + 32 * (w & 1) + (l & 31), *pb = lds + at + SIZE + 32 * (w >> 1) + (l & 31);
 #pragma unroll
-    for (int k = 0; k < X::BK; k += 2) {
-      float fa[MB], fb[MB];
+    for (int k = 0; k < BK; k += 2)
+      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(pa[(k + h) * LD], pb[(k + h) * LD], acc, 0, 0, 0);
+    if ((k0 - kb) % kChain == kChain - BK || !more)
 #pragma unroll
-      for (int b = 0; b < MB; ++b) fa[b] = pa[(k + h) * X::LD + 32 * b], fb[b] = pb[(k + h) * X::LD + 32 * b];
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-        for (int nb = 0; nb < MB; ++nb)
-          acc[mb][nb] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[mb], fb[nb], acc[mb][nb], 0, 0, 0);
+      for (int i = 0; i < 16; ++i) {
+        sum[0][0][i] += acc[i];
+        acc[i] = 0.f;
+      }
+    // (the other place was last read before this step's barrier)
+    at ^= 2 * SIZE;
+    if (more) {
+      A.store(lds + at);
+      B.store(lds + at + SIZE);
     }
-    if ((k0 - kb) % kChain == kChain - X::BK || k0 + X::BK >= ke)
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-        for (int nb = 0; nb < MB; ++nb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            sum[mb][nb][i] += acc[mb][nb][i];
-            acc[mb][nb][i] = 0.f;
-          }
   }
 }
 
 // z of TM vocabulary rows and TM tokens, then their statistics or P
-template <int MB, bool GRADS>
+template <bool VEC, bool GRADS>
 __global__ void __launch_bounds__(256) lce_general_z_kernel(LceArgs a) {
-  using X = Tile<MB>;
-  __shared__ float sa[X::SIZE], sb[X::SIZE];
+  __shared__ __align__(16) float lds[4 * SIZE];
   const int count = __builtin_amdgcn_readfirstlane(*a.count);
-  const int t0 = blockIdx.y * X::TM, v0 = (GRADS ? a.v0 : 0) + blockIdx.x * X::TM;
+  const int t0 = blockIdx.x * TM, v0 = (GRADS ? a.v0 : 0) + blockIdx.y * TM;
   if (t0 >= count) return;
-  Side<MB, true> A{static_cast<const float *>(a.w) + int64_t(v0) * a.ldw, a.ldw, a.V - v0, a.d};
-  Side<MB, true> B{static_cast<const float *>(a.x) + int64_t(t0) * a.ldx, a.ldx, count - t0, a.d};
-  f32x16 acc[MB][MB];
-  product<MB>(A, B, 0, a.d, sa, sb, acc);
+  Side<true, VEC> A{static_cast<const float *>(a.w) + int64_t(v0) * a.ldw, a.ldw, a.V - v0, a.d};
+  Side<true, VEC> B{static_cast<const float *>(a.x) + int64_t(t0) * a.ldx, a.ldx, count - t0, a.d};
+  f32x16 acc[1][1];
+  product(A, B, 0, a.d, lds, acc);
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6, h = l >> 5;
-  const int vw = v0 + 32 * MB * (w & 1), tw = t0 + 32 * MB * (w >> 1);
+  const int vw = v0 + 32 * (w & 1), tw = t0 + 32 * (w >> 1);
   if (!GRADS) {
-    lce_row_stats<MB, MB>(a, acc, vw, tw, count, 2 * blockIdx.x + (w & 1));
+    lce_row_stats<1, 1>(a, acc, vw, tw, count, 2 * blockIdx.y + (w & 1));
     return;
   }
-  bool live[MB];
-  lce_row_grads<MB, MB>(a, acc, vw, tw, count, live);
-  float *p = static_cast<float *>(a.p) + (vw - a.v0);
+  bool live[1];
+  lce_row_grads<1, 1>(a, acc, vw, tw, count, live);
+  if (!live[0]) return;
+  float *p = static_cast<float *>(a.p) + int64_t(tw + (l & 31)) * a.vc + (vw - a.v0);
 #pragma unroll
-  for (int nb = 0; nb < MB; ++nb) {
-    const int t = tw + 32 * nb + (l & 31);
-    if (!live[nb]) continue;
-#pragma unroll
-    for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        const f32x4 v = {acc[mb][nb][i], acc[mb][nb][i + 1], acc[mb][nb][i + 2], acc[mb][nb][i + 3]};
-        *reinterpret_cast<f32x4 *>(p + int64_t(t) * a.vc + 32 * mb + acc_row(i, h)) = v;
-      }
-  }
+  for (int i = 0; i < 16; i += 4)
+    *reinterpret_cast<f32x4 *>(p + acc_row(i, h)) = f32x4{acc[0][0][i], acc[0][0][i + 1], acc[0][0][i + 2], acc[0][0][i + 3]};
 }
 
 // Share blockIdx.z of dX [tokens, d] += P W over the piece
-template <int MB>
+template <bool VEC>
 __global__ void __launch_bounds__(256) lce_general_dx_kernel(LceArgs a) {
-  using X = Tile<MB>;
-  __shared__ float sa[X::SIZE], sb[X::SIZE];
+  __shared__ __align__(16) float lds[4 * SIZE];
   const int count = __builtin_amdgcn_readfirstlane(*a.count);
-  const int t0 = blockIdx.y * X::TM, c0 = blockIdx.x * X::TM;
+  const int t0 = blockIdx.x * TM, c0 = blockIdx.y * TM;
   if (t0 >= count) return;
-  const int steps = (a.vn + X::BK - 1) / X::BK, per = (steps + a.dx_splits - 1) / a.dx_splits;
-  const int kb = min(a.vn, int(blockIdx.z) * per * X::BK), ke = min(a.vn, kb + per * X::BK);
-  Side<MB, true> A{static_cast<const float *>(a.p) + int64_t(t0) * a.vc, a.vc, count - t0, a.vn};
-  Side<MB, false> B{static_cast<const float *>(a.w) + int64_t(a.v0) * a.ldw + c0, a.ldw, a.d - c0, a.vn};
-  f32x16 acc[MB][MB];
-  product<MB>(A, B, kb, ke, sa, sb, acc);
+  const int steps = (a.vn + BK - 1) / BK, per = (steps + a.dx_splits - 1) / a.dx_splits;
+  const int kb = min(a.vn, int(blockIdx.z) * per * BK), ke = min(a.vn, kb + per * BK);
+  // (P holds zeros behind the piece)
+  Side<true, VEC> A{static_cast<const float *>(a.p) + int64_t(t0) * a.vc, a.vc, count - t0, (a.vn + 3) & ~3};
+  Side<false, VEC> B{static_cast<const float *>(a.w) + int64_t(a.v0) * a.ldw + c0, a.ldw, a.d - c0, a.vn};
+  f32x16 acc[1][1];
+  product(A, B, kb, ke, lds, acc);
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6, h = l >> 5;
-  float *out = a.dx_part + int64_t(blockIdx.z) * a.n_pad * a.d;
+  const int c = c0 + 32 * (w >> 1) + (l & 31);
+  if (c >= a.d) return;
+  float *out = a.dx_part + int64_t(blockIdx.z) * a.n_pad * a.d + c;
 #pragma unroll
-  for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-    for (int nb = 0; nb < MB; ++nb) {
-      const int c = c0 + 32 * MB * (w >> 1) + 32 * nb + (l & 31);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int t = t0 + 32 * MB * (w & 1) + 32 * mb + acc_row(i, h);
-        if (t < count && c < a.d) {
-          float *o = out + int64_t(t) * a.d + c;
-          *o = a.first ? acc[mb][nb][i] : *o + acc[mb][nb][i];
-        }
-      }
+  for (int i = 0; i < 16; ++i) {
+    const int t = t0 + 32 * (w & 1) + acc_row(i, h);
+    if (t < count) {
+      float *o = out + int64_t(t) * a.d;
+      *o = a.first ? acc[0][0][i] : *o + acc[0][0][i];
     }
+  }
 }
 
 // dW rows of the piece = P^T X
-template <int MB>
+template <bool VEC>
 __global__ void __launch_bounds__(256) lce_general_dw_kernel(LceArgs a) {
-  using X = Tile<MB>;
-  __shared__ float sa[X::SIZE], sb[X::SIZE];
+  __shared__ __align__(16) float lds[4 * SIZE];
   const int count = __builtin_amdgcn_readfirstlane(*a.count);
-  const int r0 = blockIdx.y * X::TM, c0 = blockIdx.x * X::TM;
-  Side<MB, false> A{static_cast<const float *>(a.p) + r0, a.vc, a.vn - r0, count};
-  Side<MB, false> B{static_cast<const float *>(a.x) + c0, a.ldx, a.d - c0, count};
-  f32x16 acc[MB][MB];
-  product<MB>(A, B, 0, count, sa, sb, acc);
+  const int r0 = blockIdx.x * TM, c0 = blockIdx.y * TM;
+  Side<false, VEC> A{static_cast<const float *>(a.p) + r0, a.vc, a.vn - r0, count};
+  Side<false, VEC> B{static_cast<const float *>(a.x) + c0, a.ldx, a.d - c0, count};
+  f32x16 acc[1][1];
+  product(A, B, 0, count, lds, acc);
   const float f = lce_factor(a, count);
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6, h = l >> 5;
+  const int c = c0 + 32 * (w >> 1) + (l & 31);
+  if (c >= a.d) return;
+  float *out = static_cast<float *>(a.dw) + int64_t(a.v0) * a.d + c;
 #pragma unroll
-  for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-    for (int nb = 0; nb < MB; ++nb) {
-      const int c = c0 + 32 * MB * (w >> 1) + 32 * nb + (l & 31);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int r = r0 + 32 * MB * (w & 1) + 32 * mb + acc_row(i, h);
-        if (r < a.vn && c < a.d) static_cast<float *>(a.dw)[int64_t(a.v0 + r) * a.d + c] = acc[mb][nb][i] * f;
-      }
-    }
+  for (int i = 0; i < 16; ++i) {
+    const int r = r0 + 32 * (w & 1) + acc_row(i, h);
+    if (r < a.vn) out[int64_t(r) * a.d] = acc[0][0][i] * f;
+  }
 }
 
-// Tiles of 64 until tiles of 128 give two workgroups to every CU (301 rows, 256 features, 5003 words: the
-// three products 39, 40 and 597 us with 128, see the table's case for now).
-bool small(int x, int y, int z = 1) { return int64_t((x + 127) / 128) * ((y + 127) / 128) * z < 512; }
-template <int MB> dim3 tiles(int x, int y, int z = 1) {
-  return dim3((x + Tile<MB>::TM - 1) / Tile<MB>::TM, (y + Tile<MB>::TM - 1) / Tile<MB>::TM, z);
+unsigned tiles(int n) { return static_cast<unsigned>((n + TM - 1) / TM); }
+
+// 16 bytes a load where the vocabulary's rows allow it (the labelled rows and P are laid out for it)
+bool wide_rows(const LceArgs &a) {
+  return a.d % 4 == 0 && a.ldw % 4 == 0 && a.ldw < (1 << 21) && reinterpret_cast<uintptr_t>(a.w) % 16 == 0;
 }
 
 }  // namespace
 
-int lce_general_parts(int V, int N) {
-  const int tm = small(V, N) ? 64 : 128;
-  return 2 * ((V + tm - 1) / tm);
-}
+int lce_general_parts(int V) { return 2 * static_cast<int>(tiles(V)); }
 
-// Shares of a piece's vocabulary rows: until 512 workgroups of 64 x 64, each with 128 rows at least
+// Shares of a piece's vocabulary rows: rounds of two workgroups to a CU (0.8 us a step of 32) against the partial sums'
+// traffic (4 TB/s).
 int lce_general_dx_splits(int64_t N, int d, int V, int vc) {
-  const int64_t t = ((N + 63) / 64) * ((d + 63) / 64);
-  const int most = (std::min(V, vc) + 127) / 128;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({512 / t, int64_t(most), int64_t(16)})));
+  const int64_t t = (N + TM - 1) / TM * tiles(d), steps = (std::min(V, vc) + BK - 1) / BK;
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= 16 && s <= steps; ++s) {
+    const double cost = double((t * s + 511) / 512) * double((steps + s - 1) / s) * 0.8 + double(s) * N * d * 8 / 4e6;
+    if (s == 1 || cost < least) best = s, least = cost;
+  }
+  return best;
 }
 
 int launch_lce_general_stats(const LceArgs &a, hipStream_t s) {
-  if (small(a.V, a.N)) lce_general_z_kernel<1, false><<<tiles<1>(a.V, a.N), 256, 0, s>>>(a);
-  else lce_general_z_kernel<2, false><<<tiles<2>(a.V, a.N), 256, 0, s>>>(a);
+  const dim3 g(tiles(a.N), tiles(a.V));
+  if (wide_rows(a)) lce_general_z_kernel<true, false><<<g, 256, 0, s>>>(a);
+  else lce_general_z_kernel<false, false><<<g, 256, 0, s>>>(a);
   return check_launch("lce_general_z_kernel (statistics)");
 }
 
 int launch_lce_general_grads(const LceArgs &a, hipStream_t s) {
-  if (small(a.vn, a.N)) lce_general_z_kernel<1, true><<<tiles<1>(a.vn, a.N), 256, 0, s>>>(a);
-  else lce_general_z_kernel<2, true><<<tiles<2>(a.vn, a.N), 256, 0, s>>>(a);
+  const dim3 g(tiles(a.N), tiles(a.vn));
+  if (wide_rows(a)) lce_general_z_kernel<true, true><<<g, 256, 0, s>>>(a);
+  else lce_general_z_kernel<false, true><<<g, 256, 0, s>>>(a);
   return check_launch("lce_general_z_kernel (gradients)");
 }
 
 int launch_lce_general_dx(const LceArgs &a, hipStream_t s) {
-  if (small(a.d, a.N, a.dx_splits)) lce_general_dx_kernel<1><<<tiles<1>(a.d, a.N, a.dx_splits), 256, 0, s>>>(a);
-  else lce_general_dx_kernel<2><<<tiles<2>(a.d, a.N, a.dx_splits), 256, 0, s>>>(a);
+  const dim3 g(tiles(a.N), tiles(a.d), a.dx_splits);
+  if (wide_rows(a)) lce_general_dx_kernel<true><<<g, 256, 0, s>>>(a);
+  else lce_general_dx_kernel<false><<<g, 256, 0, s>>>(a);
   return check_launch("lce_general_dx_kernel");
 }
 
 int launch_lce_general_dw(const LceArgs &a, hipStream_t s) {
-  if (small(a.d, a.vn)) lce_general_dw_kernel<1><<<tiles<1>(a.d, a.vn), 256, 0, s>>>(a);
-  else lce_general_dw_kernel<2><<<tiles<2>(a.d, a.vn), 256, 0, s>>>(a);
+  const dim3 g(tiles(a.vn), tiles(a.d));
+  if (wide_rows(a)) lce_general_dw_kernel<true><<<g, 256, 0, s>>>(a);
+  else lce_general_dw_kernel<false><<<g, 256, 0, s>>>(a);
   return check_launch("lce_general_dw_kernel");
 }
 

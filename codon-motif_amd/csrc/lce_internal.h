@@ -162,7 +162,7 @@ __device__ __forceinline__ void lce_row_grads(const LceArgs &a, f32x16 (&acc)[MB
 }
 
 // lce_general.hip: fp32 products, any alignment (P is fp32 [N, vc])
-int lce_general_parts(int V, int N);
+int lce_general_parts(int V);
 int launch_lce_general_stats(const LceArgs &a, hipStream_t s);
 int launch_lce_general_grads(const LceArgs &a, hipStream_t s);  // P of the piece
 int lce_general_dx_splits(int64_t N, int d, int V, int vc);

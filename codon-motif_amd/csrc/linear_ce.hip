@@ -196,7 +196,7 @@ struct FwdSpace {
   int parts;
   size_t m, s, z, nll, bytes;
   FwdSpace(int N, int V, int dtype, size_t copy) {
-    parts = dtype == MOTIF_BF16 ? lce_bf16_parts(V, N) : lce_general_parts(V, N);
+    parts = dtype == MOTIF_BF16 ? lce_bf16_parts(V, N) : lce_general_parts(V);
     const size_t col = up(4 * size_t(N), kAlign), part = up(size_t(parts) * 4 * N, kAlign);
     m = copy;
     s = m + part;
@@ -225,7 +225,8 @@ struct BwdSpace {
   }
 };
 
-bool sizes_ok(int N, int d, int V) { return N > 0 && d > 0 && V > 0 && V <= (1 << 30) && d <= (1 << 20); }
+// (every launch's grid, and every 32-bit offset within a tile, fits these)
+bool sizes_ok(int N, int d, int V) { return N > 0 && N <= (1 << 23) && d > 0 && d <= (1 << 16) && V > 0 && V <= (1 << 22) - 64; }
 
 // kept: 4 N + 1 words: row, label, pos, lse, count
 void bind_kept(LceArgs &a, int *kept) {

@@ -7,6 +7,7 @@ import torch
 from . import _lib
 from .autograd_path import wants_grad
 
+MAX_ROWS, MAX_FEATURES, MAX_VOCABULARY = 2 ** 23, 2 ** 16, 2 ** 22 - 64
 _REDUCTIONS = {'none': 0, 'sum': 1, 'mean': 2}
 
 
@@ -97,7 +98,7 @@ def linear_cross_entropy(x, weight, labels, ignore_index=-100, reduction='mean')
         raise ValueError(f'linear_cross_entropy: x is {x.dtype}, weight {weight.dtype}')
     _lib.dtype_code(x.dtype)
     N, d = labels.numel(), x.shape[-1]
-    if N >= 2 ** 28 or weight.shape[0] > 2 ** 30 or d > 2 ** 20:
+    if N > MAX_ROWS or weight.shape[0] > MAX_VOCABULARY or d > MAX_FEATURES:
         raise ValueError(f'linear_cross_entropy: {N} rows of {d} features over {weight.shape[0]} are out of range')
     if not x.is_cuda:
         raise ValueError(f'linear_cross_entropy: x is on {x.device}, the kernels need a ROCm device')

@@ -21,6 +21,9 @@ X, W, T = torch.zeros(6, 8), torch.zeros(10, 8), torch.zeros(6, dtype=torch.int6
     ((X, W.bfloat16(), T), {}, ValueError),
     ((X.double(), W.double(), T), {}, NotImplementedError),
     ((X.half(), W.half(), T), {}, NotImplementedError),
+    ((X[:1].expand(2 ** 23 + 1, 8), W, T[:1].expand(2 ** 23 + 1)), {}, ValueError),
+    ((X, W[:1].expand(2 ** 22, 8), T), {}, ValueError),
+    ((torch.zeros(1, 65537), torch.zeros(2, 65537), T[:1]), {}, ValueError),
     ((X, W, T), {}, ValueError),  # (not on a GPU)
 ])
 def test_linear_cross_entropy(args, kw, err):
@@ -76,7 +79,7 @@ def test_c_entries_check_their_arguments():
 
     def ce_fwd(x=P, N=6, d=8, V=10, red=2, rs=8, ws=P, nbytes=big, dtype=0):
         return lib.motif_linear_ce_fwd(x, rs, P, rs, P, 1, -100, N, d, V, red, P, P, P, ws, nbytes, dtype, None)
-    for kw in (dict(x=None), dict(N=0), dict(d=0), dict(V=0), dict(red=3), dict(rs=7), dict(ws=None), dict(nbytes=16)):
+    for kw in (dict(x=None), dict(N=0), dict(d=0), dict(V=0), dict(N=2 ** 23 + 1), dict(V=2 ** 22), dict(d=65537, rs=65537), dict(red=3), dict(rs=7), dict(ws=None), dict(nbytes=16)):
         assert ce_fwd(**kw) == _lib.ERR_INVALID and 'linear_ce_fwd' in _err(), kw
     assert ce_fwd(dtype=2) == _lib.ERR_UNSUPPORTED
 
