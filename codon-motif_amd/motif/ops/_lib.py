@@ -180,6 +180,24 @@ def lib():
     return _lib
 
 
+_nodes = None
+
+
+def nodes():
+    '''The autograd nodes over the library (csrc/autograd_nodes.cpp); raises RuntimeError when
+    they cannot be loaded.'''
+    global _nodes
+    if _nodes is None:
+        lib()
+        try:
+            from motif import _autograd_nodes
+        except ImportError as exc:
+            raise RuntimeError(f'the motif autograd nodes are not available: {exc}. '
+                               'Build them with `python codon-motif_amd/csrc/build.py`.') from exc
+        _nodes = _autograd_nodes
+    return _nodes
+
+
 ERR_INVALID, ERR_UNSUPPORTED, ERR_HIP = 1, 2, 3
 
 

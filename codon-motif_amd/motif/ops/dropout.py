@@ -6,40 +6,6 @@ import torch
 from . import _lib
 
 
-def _launch(x, residual, p, seed):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    n = x.numel()
-    if n == 0:
-        return y
-    threshold = min(int(round(p * 2 ** 32)), 2 ** 32 - 1)
-    value, dev_seed = (0, seed.data_ptr()) if isinstance(seed, torch.Tensor) else (seed, None)
-    with _lib.on_device(x.device):
-        rc = _lib.lib().motif_dropout_add(x.data_ptr(), _lib.ptr(residual), y.data_ptr(), n, threshold, 1 / (1 - p),
-                                          value, dev_seed, _lib.chord_dtype_code(x.dtype), _lib.stream_ptr(x.device))
-    if rc:
-        _lib.check(rc, 'motif_dropout_add')
-    return y
-
-
-class DropoutAddFunction(torch.autograd.Function):
-    '''motif_dropout_add; its backward draws the forward's words again.'''
-
-    @staticmethod
-    def forward(ctx, x, residual, p, seed):
-        on_device = isinstance(seed, torch.Tensor)
-        ctx.save_for_backward(*((seed,) if on_device else ()))
-        ctx.p, ctx.seed = p, None if on_device else seed
-        return _launch(x.contiguous(), None if residual is None else residual.contiguous(), p, seed)
-
-    @staticmethod
-    def backward(ctx, dy):
-        if torch.is_grad_enabled():  # (create_graph: what the kernel gives carries no graph)
-            raise RuntimeError('dropout_add has no second derivatives')
-        seed = ctx.saved_tensors[0] if ctx.seed is None else ctx.seed
-        dx = _launch(dy.contiguous(), None, ctx.p, seed) if ctx.needs_input_grad[0] else None
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None
-
-
 def dropout_add(x, p, seed, residual=None):
     '''residual + x * keep / (1 - p) (without a residual: x * keep / (1 - p)), x and residual of
     one shape and dtype (fp32, bf16 or fp16), computed in fp32 and rounded once; a dropped
@@ -64,9 +30,11 @@ def dropout_add(x, p, seed, residual=None):
     elif isinstance(seed, int) and not isinstance(seed, bool):
         if not -2 ** 63 <= seed < 2 ** 64:
             raise ValueError('dropout_add: the seed has 64 bits')
-        seed &= 2 ** 64 - 1
+        seed = (seed + 2 ** 63) % 2 ** 64 - 2 ** 63  # (its 64 bits as an int64)
     else:
         raise TypeError(f'dropout_add: seed must be an int or an int64 tensor, got {type(seed).__name__}')
     if not x.is_cuda:
         raise ValueError(f'dropout_add: x is on {x.device}, the kernels need a ROCm device')
-    return DropoutAddFunction.apply(x, residual, p, seed)
+    if isinstance(seed, int):
+        return _lib.nodes().dropout_add(x, residual, p, seed, None)
+    return _lib.nodes().dropout_add(x, residual, p, 0, seed)

@@ -5,63 +5,9 @@ motif/model/motif.py:600-628).
 import torch
 
 from . import _lib
-from .autograd_path import wants_grad
 
 MAX_ROWS, MAX_FEATURES, MAX_VOCABULARY = 2 ** 23, 2 ** 16, 2 ** 22 - 64
 _REDUCTIONS = {'none': 0, 'sum': 1, 'mean': 2}
-
-
-class LinearCEFunction(torch.autograd.Function):
-    '''motif_linear_ce_fwd / motif_linear_ce_bwd: gradients for x [N, d] and weight [V, d].
-
-    What is kept for the backward: the labelled rows of x (a copy), the weight and 16 bytes a
-    row.  The backward's scratch is P in pieces of the vocabulary (256 MB, or 4096 vocabulary
-    rows where that is more) and the partial sums of x's gradient in fp32.'''
-
-    @staticmethod
-    def forward(ctx, x, weight, labels, ignore_index, reduction):
-        N, d = x.shape
-        V = weight.shape[0]
-        dev, code = x.device, _lib.dtype_code(x.dtype)
-        lib = _lib.lib()
-        rows = torch.empty(lib.motif_linear_ce_rows_bytes(N, d, code), dtype=torch.uint8, device=dev)
-        kept = torch.empty(4 * N + 1, dtype=torch.int32, device=dev)
-        loss = torch.empty((N,) if reduction == 0 else (), dtype=torch.float32, device=dev)
-        nbytes = lib.motif_linear_ce_workspace_bytes(N, d, weight.data_ptr(), weight.stride(0), V, code, 0)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        with _lib.on_device(dev):
-            rc = lib.motif_linear_ce_fwd(
-                x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), labels.data_ptr(), labels.stride(0),
-                ignore_index, N, d, V, reduction, rows.data_ptr(), kept.data_ptr(), loss.data_ptr(), ws.data_ptr(),
-                nbytes, code, _lib.stream_ptr(dev))
-        if rc:
-            _lib.check(rc, 'motif_linear_ce_fwd')
-        if ctx is not None:
-            ctx.save_for_backward(rows, weight, kept)
-            ctx.args = N, d, V, reduction
-        return loss
-
-    @staticmethod
-    def backward(ctx, dloss):
-        if torch.is_grad_enabled():  # (create_graph: what the kernels give carries no graph)
-            raise RuntimeError('linear_cross_entropy has no second derivatives')
-        rows, weight, kept = ctx.saved_tensors
-        N, d, V, reduction = ctx.args
-        dev, dt = weight.device, weight.dtype
-        code = _lib.dtype_code(dt)
-        dx = torch.empty((N, d), dtype=dt, device=dev) if ctx.needs_input_grad[0] else None
-        dw = torch.empty((V, d), dtype=dt, device=dev) if ctx.needs_input_grad[1] else None
-        lib = _lib.lib()
-        nbytes = lib.motif_linear_ce_workspace_bytes(N, d, weight.data_ptr(), weight.stride(0), V, code, 1)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        with _lib.on_device(dev):
-            rc = lib.motif_linear_ce_bwd(
-                rows.data_ptr(), weight.data_ptr(), weight.stride(0), kept.data_ptr(), dloss.data_ptr(),
-                dloss.stride(0) if reduction == 0 else 0, N, d, V, reduction, _lib.ptr(dx), _lib.ptr(dw),
-                ws.data_ptr(), nbytes, code, _lib.stream_ptr(dev))
-        if rc:
-            _lib.check(rc, 'motif_linear_ce_bwd')
-        return dx, dw, None, None, None
 
 
 def _row_major(t):
@@ -78,7 +24,11 @@ def linear_cross_entropy(x, weight, labels, ignore_index=-100, reduction='mean')
     Rows whose label is `ignore_index` are left out of every product: they get a zero
     gradient and nothing that they hold reaches the loss.  A label outside [0, V) that is not
     `ignore_index` gives NaN (loss and gradients).  Under autocast, x and weight are cast to its
-    dtype, as F.linear does.  Differentiable once in x and weight.'''
+    dtype, as F.linear does.  Differentiable once in x and weight.
+
+    For the backward a copy of the labelled rows, the weight and 16 bytes a row are kept.  Its scratch
+    is the gradient of the logits in pieces of the vocabulary (256 MB, or 4096 vocabulary rows where
+    that is more), and partial sums of x's gradient in fp32.'''
     if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction must be 'none', 'sum' or 'mean', got {reduction!r}")
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
@@ -108,9 +58,5 @@ def linear_cross_entropy(x, weight, labels, ignore_index=-100, reduction='mean')
     red = _REDUCTIONS[reduction]
     x2, lab = x.reshape(-1, d), labels.reshape(-1).to(torch.int64)
     x2 = x2 if x2.stride(1) == 1 else x2.contiguous()
-    w = _row_major(weight)
-    if wants_grad(x2, w):
-        loss = LinearCEFunction.apply(x2, w, lab, int(ignore_index), red)
-    else:
-        loss = LinearCEFunction.forward(None, x2, w, lab, int(ignore_index), red)
+    loss = _lib.nodes().linear_ce(x2, _row_major(weight), lab, int(ignore_index), red)
     return loss.view(labels.shape) if red == 0 else loss
