@@ -57,7 +57,8 @@ def _dropped_branches(p, attn, mlp):
     '''f_h = drop(attn) + drop(mlp) of a training step: two passes, the second with the first as its
     residual.  Their seeds come from the device's generator, so that a captured step draws
     anew at every replay and torch.manual_seed repeats a run.'''
-    if not attn.is_cuda or attn.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+    if (not attn.is_cuda or attn.dtype not in (torch.bfloat16, torch.float16, torch.float32)
+            or mlp.dtype != attn.dtype or mlp.shape != attn.shape):
         return nn.functional.dropout(attn, p) + nn.functional.dropout(mlp, p)
     seeds = torch.randint(2 ** 63 - 1, (2,), device=attn.device)
     return dropout_add(mlp, p, seeds[1:], residual=dropout_add(attn, p, seeds[:1]))

@@ -14,15 +14,17 @@ from .autograd_path import wants_grad
 from .norm import MAX_FEATURES, rms_norm_rows
 
 _KERNEL_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+_PLAIN = (torch.Tensor, nn.Parameter)
 
 
 def _trains_on_kernels(x, weight):
-    '''A call whose gradients the kernels give: first derivatives in reverse mode, outside
-    autocast and function transforms, which keep torch's own op.'''
-    return (x.dtype in _KERNEL_DTYPES and weight.dtype == x.dtype and weight.device == x.device
-            and weight.dim() == 1 and x.shape[-1] <= MAX_FEATURES and wants_grad(x, weight)
-            and not torch.is_autocast_enabled('cuda') and not torch._C._are_functorch_transforms_active()
-            and torch.autograd.forward_ad._current_level < 0 and not torch.compiler.is_compiling() and _lib.available())
+    '''A call whose gradients the kernels give: plain tensors in reverse mode.  Autocast, function
+    transforms, forward-mode derivatives, tracing and compiling keep torch's own op.'''
+    return (wants_grad(x, weight) and torch._C._get_tracing_state() is None and x.dtype in _KERNEL_DTYPES and weight.dtype == x.dtype
+            and weight.device == x.device and weight.dim() == 1 and x.shape[-1] <= MAX_FEATURES
+            and type(x) in _PLAIN and type(weight) in _PLAIN and not torch.is_autocast_enabled('cuda')
+            and not torch._C._are_functorch_transforms_active() and torch.autograd.forward_ad._current_level < 0
+            and not torch.compiler.is_compiling() and _lib.available())
 
 
 def _rms(x, weight, eps):

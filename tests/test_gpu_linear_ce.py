@@ -69,6 +69,10 @@ def test_large_training_step():
     _check(*_inputs(8192 + 77, 256, 40960, BF, ignored=0.1, seed=2))
 
 
+def test_several_pieces_in_fp32():
+    _check(*_inputs(8192 + 5, 64, 9001, F32, ignored=0.05, seed=4))
+
+
 def test_many_rows_of_a_small_vocabulary():
     _check(*_inputs(70001, 64, 500, BF, ignored=0.2, seed=3))
 
@@ -282,7 +286,7 @@ def test_no_rows():
     assert _op()(x, w, t, reduction='none').shape == (0,)
     s = _op()(x, w, t, reduction='sum')
     s.backward()
-    assert float(s) == 0 and not w.grad.any() and x.grad.shape == (0, 8)
+    assert float(s.detach()) == 0 and not w.grad.any() and x.grad.shape == (0, 8)
 
 
 def test_second_derivatives_are_refused():

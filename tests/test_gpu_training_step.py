@@ -65,6 +65,11 @@ def test_rms_norm_module_elsewhere():
     assert torch.allclose(g, want, rtol=1e-4, atol=1e-4)
     with torch.autocast('cuda', dtype=BF):
         assert norm(xr).shape == x.shape
+    traced = torch.jit.trace(norm, (x,))
+    assert torch.allclose(traced(2 * x + 1), norm(2 * x + 1), rtol=1e-5, atol=1e-5)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        assert norm(dual).shape == x.shape
     assert norm(x.to(BF).requires_grad_()).shape == x.shape
     assert norm(x[:, ::2].repeat(1, 2)).shape == x.shape
 
@@ -148,6 +153,7 @@ def test_dropped_branches():
     assert (f.double() - want).abs().max() <= 1e-6 * 10
     assert torch.equal((f == 0), ~(ka | km))
     assert _dropped_branches(0.5, a.cpu(), m.cpu()).shape == a.shape
+    assert _dropped_branches(0.5, a, m.to(BF)).dtype == F32
 
 
 def test_dropout_with_packed_sequences():
