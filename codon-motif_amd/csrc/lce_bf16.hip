@@ -33,6 +33,7 @@ template <int TM_, int TN_, int BK_, int ST_, int PER_> struct Shape {
 };
 using Wide = Shape<256, 256, 64, 2, 1>;
 using Narrow = Shape<256, 128, 32, 3, 2>;
+using Three = Shape<256, 128, 32, 2, 3>;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
@@ -371,9 +372,14 @@ __global__ void __launch_bounds__(C::THREADS, C::BOUND) lce_products_kernel(LceA
 template <typename T> T up(T a, int64_t b) { return static_cast<T>((a + b - 1) / b); }
 
 // The tile of the logits' products: 256 x 256 moves the least through the caches (244 and 260 us for the two products of
-// 4096 x 768 x 32000 where 256 x 128 take 270 and 290); 256 x 128 for fewer tokens (517: 45 against 48 us).  128 x 128
-// gained 4 us of 55 with 64 tokens and lost with 256 and more.
-template <typename F> auto with_shape(int64_t N, F &&f) { return N >= 2048 ? f(Wide{}) : f(Narrow{}); }
+// 4096 x 768 x 32000 where 256 x 128 take 270 and 290); 256 x 128 for fewer tokens, three workgroups to a CU with two
+// stages each where two with three would not hold all of them at once (517 tokens: 42.6 against 45 us; 2000 x 100 x 40000:
+// 46 against 54; 256 tokens the other way: 26.8 against 24.7).  128 x 128 gained 4 us of 55 with 64 tokens and lost with
+// 256 and more.
+template <typename F> auto with_shape(int64_t N, int64_t V, F &&f) {
+  if (N >= 2048) return f(Wide{});
+  return up(V, Narrow::TM) * up(N, Narrow::TN) <= 2 * 256 ? f(Narrow{}) : f(Three{});
+}
 
 }  // namespace
 
@@ -381,9 +387,7 @@ bool lce_bf16_direct(const void *w, int64_t ldw, int d) {
   return d % 8 == 0 && ldw % 8 == 0 && ldw < (1 << 21) && reinterpret_cast<uintptr_t>(w) % 16 == 0;
 }
 
-int lce_bf16_parts(int V, int N) {
-  return with_shape(N, [&](auto c) { return 2 * up(V, decltype(c)::TM); });
-}
+int lce_bf16_parts(int V) { return 2 * up(V, 256); }
 
 // Shares of a piece's vocabulary rows in dX: so many that none takes longer than the launch's work spread
 // over the places (two workgroups per CU) does.  Each costs partial sums of N x d in fp32.
@@ -397,8 +401,9 @@ int lce_bf16_dx_splits(int64_t N, int d, int V, int vc) {
 namespace {
 
 template <bool GRADS> int z_launch(const LceArgs &a, hipStream_t s) {
-  return with_shape(a.N, [&](auto c) {
+  return with_shape(a.N, GRADS ? a.vn : a.V, [&](auto c) {
     using C = decltype(c);
+    static_assert(C::TM == 256, "the vocabulary parts of the statistics");
     const int nm = up(GRADS ? a.vn : a.V, C::TM), nn = up(a.N, C::TN);
     lce_z_kernel<C, GRADS><<<nm * nn, C::THREADS, 0, s>>>(a, nm, nn);
     return check_launch("lce_z_kernel");

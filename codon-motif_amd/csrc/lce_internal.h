@@ -172,7 +172,7 @@ int launch_lce_general_dw(const LceArgs &a, hipStream_t s);
 // lce_bf16.hip: bf16 (P is bf16 in blocks).  Vocabulary rows that do not start on 16-byte boundaries are
 // copied to some that do first (`direct`: no need).
 bool lce_bf16_direct(const void *w, int64_t ldw, int d);
-int lce_bf16_parts(int V, int N);
+int lce_bf16_parts(int V);
 int lce_bf16_dx_splits(int64_t N, int d, int V, int vc);
 int launch_lce_bf16_stats(const LceArgs &a, hipStream_t s);
 int launch_lce_bf16_grads(const LceArgs &a, hipStream_t s);
