@@ -1,7 +1,7 @@
 // Autograd nodes of the training operators around the mixers (row norms, dropout, cross entropy from hidden
 // states), over the C ABI of libmotif_hip.so.  In C++ because a step calls them by the dozen: as
-// Python Functions a norm's forward and backward kept the host 106 us (64 x 768, on the box where torch's own
-// op keeps it 60), most of it in Python on the engine's thread.  Arguments are checked by the callers in
+// Python Functions a norm's forward and backward kept the host 106 us (64 x 768; torch's own op beside it 60), most of
+// it in Python on the engine's thread; so they keep it 59.  Arguments are checked by the callers in
 // motif/ops; here they are tensors of one device with features beside each other.
 #include <torch/extension.h>
 

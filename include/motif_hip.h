@@ -3,7 +3,8 @@
  * sequence-mixing hot path: the Gated DeltaNet (GDN) delta rule (token
  * recurrence and chunked prefill), its short causal conv front end, and Chord
  * GGD-biased softmax attention (prefill and split-K decode; under a sliding window, and
- * over a key / value cache held in 4 bits).
+ * over a key / value cache held in 4 bits), and of what surrounds them in a training step (row
+ * norms, dropout, the cross entropy from hidden states).
  *
  * Conventions
  *  - Every entry point is `extern "C"`, takes raw device pointers, element
@@ -13,8 +14,8 @@
  *    host, nothing allocates device memory (scratch comes in as `workspace`).
  *  - Return value: MOTIF_OK (0) or a motif_status code; `motif_last_error()`
  *    returns a message for the last failure on the calling thread.
- *  - dtype codes: MOTIF_F32 = 0, MOTIF_BF16 = 1, MOTIF_F16 = 2 (fp16: the Chord attention
- *    and 4-bit cache entries only).
+ *  - dtype codes: MOTIF_F32 = 0, MOTIF_BF16 = 1, MOTIF_F16 = 2 (fp16: the Chord attention,
+ *    4-bit cache, row norm and dropout entries only).
  *  - Recurrent state is always fp32, row-major [.., dk, dv], contiguous.
  */
 #ifndef MOTIF_HIP_H
