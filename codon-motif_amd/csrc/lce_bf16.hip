@@ -1,10 +1,12 @@
 // Cross entropy from hidden states in bf16 on v_mfma_f32_32x32x16_bf16: the three products of
-// lce_internal.h, one workgroup of four waves to a tile of 256 x 128 (128 x 64 a wave: 8 matrix
-// instructions for 6 LDS reads of 16 bytes a lane), 32 k at a time.  Both sides go straight from memory
-// to LDS (16 bytes a lane), three stages deep, 72 KB, so that two workgroups share a CU and one's
-// exponentials run beside the other's matrix instructions.
+// lce_internal.h.  A wave owns 128 x 64 of a product (8 matrix instructions for 6 LDS reads of 16 bytes a
+// lane), four or eight waves a tile of 256 x 128 or 256 x 256.  Both sides go straight from memory to LDS (16 bytes
+// a lane) in two or three stages of 32 or 64 k, one barrier a stage; LDS reads and writes meet no bank conflicts.
+// What bounds them: 4096 x 768 x 32000 reaches 860 (z with its epilogue) to 980 TFLOP/s (dX and dW) where the library's
+// bare products reach 920, 565 and 692; the clock falls to 1.75-2.1 GHz under them (matrix instructions busy 48-64% of
+// it), the loads alone take 300 of 415 us of dX and dW, the matrix instructions without loads 330.
 //
-//   z = W X^T    left: 256 vocabulary rows, right: 128 tokens; a lane holds one token's scores, so a
+//   z = W X^T    left: 256 vocabulary rows, right: 128 or 256 tokens; a lane holds one token's scores, so a
 //                row's maximum and sum are in-lane sums and one exchange
 //   dX = P W     left: 256 tokens, right: 128 features
 //   dW = P^T X   left: 256 vocabulary rows, right: 128 features
@@ -371,13 +373,14 @@ __global__ void __launch_bounds__(C::THREADS, C::BOUND) lce_products_kernel(LceA
 
 template <typename T> T up(T a, int64_t b) { return static_cast<T>((a + b - 1) / b); }
 
-// The tile of the logits' products: 256 x 256 moves the least through the caches (244 and 260 us for the two products of
-// 4096 x 768 x 32000 where 256 x 128 take 270 and 290); 256 x 128 for fewer tokens, three workgroups to a CU with two
-// stages each where two with three would not hold all of them at once (517 tokens: 42.6 against 45 us; 2000 x 100 x 40000:
-// 46 against 54; 256 tokens the other way: 26.8 against 24.7).  128 x 128 gained 4 us of 55 with 64 tokens and lost with
-// 256 and more.
-template <typename F> auto with_shape(int64_t N, int64_t V, F &&f) {
-  if (N >= 2048) return f(Wide{});
+// The tile of the logits' products.  256 x 256 moves the least through the caches, but its one workgroup a CU leaves the
+// matrix instructions idle through its epilogue: for many tokens and long sums (4096 x 768 x 32000: 236 and 256 us for the
+// two products where 256 x 128 take 255 and 271; 2111 tokens 136 and 149 against 134 and 144; 6000 x 256 x 32000: 150 and
+// 92 against 135 and 88).  256 x 128: three workgroups to a CU with two stages each where two with three would not
+// hold all of them at once (517 tokens: 42.6 against 45 us; 2000 x 100 x 40000: 46 against 54; 256 tokens the other way: 26.8
+// against 24.7).  128 x 128 gained 4 us of 55 with 64 tokens and lost with 256 and more.
+template <typename F> auto with_shape(int64_t N, int d, int64_t V, F &&f) {
+  if (N >= 2560 && d >= 512) return f(Wide{});
   return up(V, Narrow::TM) * up(N, Narrow::TN) <= 2 * 256 ? f(Narrow{}) : f(Three{});
 }
 
@@ -401,7 +404,7 @@ int lce_bf16_dx_splits(int64_t N, int d, int V, int vc) {
 namespace {
 
 template <bool GRADS> int z_launch(const LceArgs &a, hipStream_t s) {
-  return with_shape(a.N, GRADS ? a.vn : a.V, [&](auto c) {
+  return with_shape(a.N, a.d, GRADS ? a.vn : a.V, [&](auto c) {
     using C = decltype(c);
     static_assert(C::TM == 256, "the vocabulary parts of the statistics");
     const int nm = up(GRADS ? a.vn : a.V, C::TM), nn = up(a.N, C::TN);

@@ -3,9 +3,9 @@
 // workgroup of four waves owns 64 x 64 of C (32 x 32 a wave) and stages 32 k of both sides in LDS, k outermost,
 // twice: one place is filled, from registers loaded a step before, while the other is multiplied.  The matrix
 // instruction (64 cycles for two k) bounds it, so LDS reads of single words suffice.  (128 x 128 were slower
-// at every size: 512 x 1024 x 8192, dW 125 against 94 us.)  What is reached: 85-95 TFLOP/s at 2048 x 768 x 8192, where
-// a large library product reaches 154; a wave per SIMD and workgroup, its chain of one accumulator and its barriers
-// leave the rest.
+// at every size: 512 x 1024 x 8192, dW 125 against 94 us.)  dX and dW share a launch (189 against 203 us there; 27 against 37
+// for 271 x 256 x 5003).  What is reached: 88-95 TFLOP/s at 2048 x 768 x 8192, where a large library product reaches
+// 154; a wave per SIMD and workgroup, its chain of one accumulator and its barriers leave the rest.
 // Sums run over 512 k at a time, which are then added (one chain over a vocabulary of 5000 lost a bit of dX: 1.3e-6
 // off where this is 6e-7).
 #include "lce_internal.h"
@@ -128,46 +128,43 @@ __global__ void __launch_bounds__(256) lce_general_z_kernel(LceArgs a) {
     *reinterpret_cast<f32x4 *>(p + acc_row(i, h)) = f32x4{acc[0][0][i], acc[0][0][i + 1], acc[0][0][i + 2], acc[0][0][i + 3]};
 }
 
-// Share blockIdx.z of dX [tokens, d] += P W over the piece
+// Both products of a piece in one launch: `ndx` workgroups for dX (token tile, column tile, share of the vocabulary rows,
+// the first fastest), then dW's (vocabulary tile, column tile).
 template <bool VEC>
-__global__ void __launch_bounds__(256) lce_general_dx_kernel(LceArgs a) {
+__global__ void __launch_bounds__(256) lce_general_products_kernel(LceArgs a, int tt, int vt, int ndx) {
   __shared__ __align__(16) float lds[4 * SIZE];
   const int count = __builtin_amdgcn_readfirstlane(*a.count);
-  const int t0 = blockIdx.x * TM, c0 = blockIdx.y * TM;
-  if (t0 >= count) return;
-  const int steps = (a.vn + BK - 1) / BK, per = (steps + a.dx_splits - 1) / a.dx_splits;
-  const int kb = min(a.vn, int(blockIdx.z) * per * BK), ke = min(a.vn, kb + per * BK);
-  // (P holds zeros behind the piece)
-  Side<true, VEC> A{static_cast<const float *>(a.p) + int64_t(t0) * a.vc, a.vc, count - t0, (a.vn + 3) & ~3};
-  Side<false, VEC> B{static_cast<const float *>(a.w) + int64_t(a.v0) * a.ldw + c0, a.ldw, a.d - c0, a.vn};
-  f32x16 acc[1][1];
-  product(A, B, kb, ke, lds, acc);
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6, h = l >> 5;
-  const int c = c0 + 32 * (w >> 1) + (l & 31);
-  if (c >= a.d) return;
-  float *out = a.dx_part + int64_t(blockIdx.z) * a.n_pad * a.d + c;
+  f32x16 acc[1][1];
+  if (static_cast<int>(blockIdx.x) < ndx) {  // dX [tokens, d] += P W over the piece
+    const int ct = (a.d + TM - 1) / TM, b = blockIdx.x;
+    const int t0 = b % tt * TM, c0 = b / tt % ct * TM, share = b / tt / ct;
+    if (t0 >= count) return;
+    const int steps = (a.vn + BK - 1) / BK, per = (steps + a.dx_splits - 1) / a.dx_splits;
+    const int kb = min(a.vn, share * per * BK), ke = min(a.vn, kb + per * BK);
+    // (P holds zeros behind the piece)
+    Side<true, VEC> A{static_cast<const float *>(a.p) + int64_t(t0) * a.vc, a.vc, count - t0, (a.vn + 3) & ~3};
+    Side<false, VEC> B{static_cast<const float *>(a.w) + int64_t(a.v0) * a.ldw + c0, a.ldw, a.d - c0, a.vn};
+    product(A, B, kb, ke, lds, acc);
+    const int c = c0 + 32 * (w >> 1) + (l & 31);
+    if (c >= a.d) return;
+    float *out = a.dx_part + int64_t(share) * a.n_pad * a.d + c;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int t = t0 + 32 * (w & 1) + acc_row(i, h);
-    if (t < count) {
-      float *o = out + int64_t(t) * a.d;
-      *o = a.first ? acc[0][0][i] : *o + acc[0][0][i];
+    for (int i = 0; i < 16; ++i) {
+      const int t = t0 + 32 * (w & 1) + acc_row(i, h);
+      if (t < count) {
+        float *o = out + int64_t(t) * a.d;
+        *o = a.first ? acc[0][0][i] : *o + acc[0][0][i];
+      }
     }
+    return;
   }
-}
-
-// dW rows of the piece = P^T X
-template <bool VEC>
-__global__ void __launch_bounds__(256) lce_general_dw_kernel(LceArgs a) {
-  __shared__ __align__(16) float lds[4 * SIZE];
-  const int count = __builtin_amdgcn_readfirstlane(*a.count);
-  const int r0 = blockIdx.x * TM, c0 = blockIdx.y * TM;
+  // dW rows of the piece = P^T X
+  const int b = blockIdx.x - ndx, r0 = b % vt * TM, c0 = b / vt * TM;
   Side<false, VEC> A{static_cast<const float *>(a.p) + r0, a.vc, a.vn - r0, count};
   Side<false, VEC> B{static_cast<const float *>(a.x) + c0, a.ldx, a.d - c0, count};
-  f32x16 acc[1][1];
   product(A, B, 0, count, lds, acc);
   const float f = lce_factor(a, count);
-  const int l = threadIdx.x & 63, w = threadIdx.x >> 6, h = l >> 5;
   const int c = c0 + 32 * (w >> 1) + (l & 31);
   if (c >= a.d) return;
   float *out = static_cast<float *>(a.dw) + int64_t(a.v0) * a.d + c;
@@ -216,18 +213,13 @@ int launch_lce_general_grads(const LceArgs &a, hipStream_t s) {
   return check_launch("lce_general_z_kernel (gradients)");
 }
 
-int launch_lce_general_dx(const LceArgs &a, hipStream_t s) {
-  const dim3 g(tiles(a.N), tiles(a.d), a.dx_splits);
-  if (wide_rows(a)) lce_general_dx_kernel<true><<<g, 256, 0, s>>>(a);
-  else lce_general_dx_kernel<false><<<g, 256, 0, s>>>(a);
-  return check_launch("lce_general_dx_kernel");
-}
-
-int launch_lce_general_dw(const LceArgs &a, hipStream_t s) {
-  const dim3 g(tiles(a.vn), tiles(a.d));
-  if (wide_rows(a)) lce_general_dw_kernel<true><<<g, 256, 0, s>>>(a);
-  else lce_general_dw_kernel<false><<<g, 256, 0, s>>>(a);
-  return check_launch("lce_general_dw_kernel");
+int launch_lce_general_products(const LceArgs &a, bool dx, bool dw, hipStream_t s) {
+  const int tt = static_cast<int>(tiles(a.N)), vt = static_cast<int>(tiles(a.vn)), ct = static_cast<int>(tiles(a.d));
+  const int ndx = dx ? tt * ct * a.dx_splits : 0;
+  const dim3 g(ndx + (dw ? vt * ct : 0));
+  if (wide_rows(a)) lce_general_products_kernel<true><<<g, 256, 0, s>>>(a, tt, vt, ndx);
+  else lce_general_products_kernel<false><<<g, 256, 0, s>>>(a, tt, vt, ndx);
+  return check_launch("lce_general_products_kernel");
 }
 
 }  // namespace motif

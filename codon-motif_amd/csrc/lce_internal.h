@@ -166,8 +166,7 @@ int lce_general_parts(int V);
 int launch_lce_general_stats(const LceArgs &a, hipStream_t s);
 int launch_lce_general_grads(const LceArgs &a, hipStream_t s);  // P of the piece
 int lce_general_dx_splits(int64_t N, int d, int V, int vc);
-int launch_lce_general_dx(const LceArgs &a, hipStream_t s);
-int launch_lce_general_dw(const LceArgs &a, hipStream_t s);
+int launch_lce_general_products(const LceArgs &a, bool dx, bool dw, hipStream_t s);
 
 // lce_bf16.hip: bf16 (P is bf16 in blocks).  Vocabulary rows that do not start on 16-byte boundaries are
 // copied to some that do first (`direct`: no need).

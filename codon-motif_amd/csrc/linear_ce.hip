@@ -406,12 +406,7 @@ extern "C" int motif_linear_ce_bwd(const void *rows, const void *w, int64_t w_rs
     a.v0 = v0, a.vn = std::min(b.vc, V - v0), a.first = v0 == 0;
     rc = bf16 ? launch_lce_bf16_grads(a, s) : launch_lce_general_grads(a, s);
     if (rc != MOTIF_OK) break;
-    if (bf16) {
-      rc = launch_lce_bf16_products(a, dx, dw, s);
-    } else {
-      if (dx) rc = launch_lce_general_dx(a, s);
-      if (rc == MOTIF_OK && dw) rc = launch_lce_general_dw(a, s);
-    }
+    rc = bf16 ? launch_lce_bf16_products(a, dx, dw, s) : launch_lce_general_products(a, dx, dw, s);
   }
   if (rc != MOTIF_OK || !dx) return rc;
   const bool four = d % 4 == 0 && reinterpret_cast<uintptr_t>(dx) % 16 == 0;
