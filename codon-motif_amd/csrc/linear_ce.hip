@@ -258,8 +258,11 @@ struct FwdSpace {
 };
 
 // The backward's: copied vocabulary rows, P of a vocabulary piece and fp32 partial dX.  A piece holds P in 256 MB (so that
-// it stays in the memory-side cache between its three products; 512 MB and 1 GB were no faster), but no fewer than 4096
-// vocabulary rows: every piece reads and writes the partial dX once.
+// it stays in the memory-side cache between its three products: 16384 x 768 x 40960 in five of them 3.3 ms, in four 3.6), but
+// no fewer than 4096 vocabulary rows, since every piece reads and writes the partial dX once.  In bf16 a tile of dW sums
+// N / 32 steps, and the launch has N vc tn / 32768 of them for each of 512 places (tn column tiles); where that is half as
+// many or fewer, the piece grows, up to 1 GB, until they are as many (32768 x 768 x 32000: eight pieces 7.0 ms, three
+// 5.2).  The pieces of a vocabulary are made alike.
 struct BwdSpace {
   int vc, splits;
   int64_t n_pad;
@@ -267,8 +270,12 @@ struct BwdSpace {
   BwdSpace(int64_t N, int d, int V, int dtype, size_t copy) {
     const size_t e = esize(dtype);
     n_pad = static_cast<int64_t>(up(N, 256));
-    const size_t rows = (size_t(1) << 28) / (n_pad * e) / 256 * 256;
-    vc = static_cast<int>(std::min(std::max<size_t>(rows, 4096), up(V, 256)));
+    const size_t near = std::max<size_t>((size_t(1) << 28) / (n_pad * e), 4096), tn = (d + 127) / 128;
+    size_t rows = near;
+    if (dtype == MOTIF_BF16 && 65536 >= 2 * near * tn) rows = std::max(near, std::min(65536 / tn, (size_t(1) << 30) / (n_pad * e)));
+    rows = std::max<size_t>(rows / 256 * 256, 256);
+    const size_t pieces = (V + rows - 1) / rows;
+    vc = static_cast<int>(up((V + pieces - 1) / pieces, 256));
     splits = dtype == MOTIF_BF16 ? lce_bf16_dx_splits(N, d, V, vc) : lce_general_dx_splits(N, d, V, vc);
     p = copy;
     dx = p + up(size_t(n_pad) * vc * e, kAlign);
@@ -276,7 +283,6 @@ struct BwdSpace {
   }
 };
 
-// (every launch's grid, and every 32-bit offset within a tile, fits these)
 bool sizes_ok(int N, int d, int V) { return N > 0 && N <= (1 << 23) && d > 0 && d <= (1 << 16) && V > 0 && V <= (1 << 22) - 64; }
 
 // kept: 4 N + 1 words: row, label, pos, lse, count

@@ -27,8 +27,8 @@ def linear_cross_entropy(x, weight, labels, ignore_index=-100, reduction='mean')
     dtype, as F.linear does.  Differentiable once in x and weight.
 
     For the backward a copy of the labelled rows, the weight and 16 bytes a row are kept.  Its scratch
-    is the gradient of the logits in pieces of the vocabulary (256 MB, or 4096 vocabulary rows where
-    that is more), and partial sums of x's gradient in fp32.'''
+    is the gradient of the logits in pieces of the vocabulary (256 MB to 1 GB, or 4096 vocabulary
+    rows where that is more), and partial sums of x's gradient in fp32.'''
     if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction must be 'none', 'sum' or 'mean', got {reduction!r}")
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:

@@ -64,9 +64,10 @@ def test_sum_and_rows(N, d, V, dtype):
     _check(x, w, labels, 'none', torch.randn(2 * N, generator=g, device=DEV)[::2])
 
 
-def test_large_training_step():
-    '''Several vocabulary pieces (P of a piece holds 256 MB) and full tiles.'''
-    _check(*_inputs(8192 + 77, 256, 40960, BF, ignored=0.1, seed=2))
+@pytest.mark.parametrize('d,V', [(256, 40960), (768, 40001)])
+def test_large_training_step(d, V):
+    '''Several vocabulary pieces (P of a piece holds 256 MB and more) and full tiles.'''
+    _check(*_inputs(8192 + 77, d, V, BF, ignored=0.1, seed=2))
 
 
 def test_several_pieces_in_fp32():
