@@ -5,7 +5,12 @@
 // motif/ops; here they are tensors of one device with features beside each other.
 #include <torch/extension.h>
 
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
+#include <torch/csrc/autograd/graph_task.h>
+
+#include <unordered_set>
 
 #include "../../include/motif_hip.h"
 
@@ -32,6 +37,34 @@ void check(int rc, const char *what) {
   TORCH_CHECK_VALUE(rc != MOTIF_ERR_INVALID, msg);
   TORCH_CHECK_NOT_IMPLEMENTED(rc != MOTIF_ERR_UNSUPPORTED, msg);
   TORCH_CHECK(false, msg);
+}
+
+// Refuses a backward that is captured while a gradient of it would be summed up on the default stream.  A leaf's
+// summing node lives as long as any graph of that leaf and keeps the stream that it was made on: where an eager
+// loss of the same leaves is still held, the engine would make the default stream wait for the capturing one, which
+// breaks the capture and can end the process.  So this runs before a gradient is handed on, over the nodes that the pass will
+// reach, and only while capturing.
+void refuse_stale_leaves(const char *what) {
+  using namespace torch::autograd;
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const auto *wanted = get_current_graph_task_exec_info();  // (empty: every node)
+  std::vector<Node *> next = {get_current_node().get()};
+  std::unordered_set<Node *> seen;
+  while (!next.empty()) {
+    Node *node = next.back();
+    next.pop_back();
+    if (!node || !seen.insert(node).second) continue;
+    if (seen.size() > 1 && wanted && !wanted->empty()) {
+      const auto it = wanted->find(node);
+      if (it == wanted->end() || !it->second.should_execute()) continue;
+    }
+    if (dynamic_cast<AccumulateGrad *>(node)) {
+      const auto stream = node->stream();
+      TORCH_CHECK(!stream || stream->id() != 0, what, ": this backward is being captured while a loss of the same leaves, made on the "
+                  "default stream, is still held: delete it (and what else holds its graph) before the capture");
+    }
+    for (const auto &edge : node->next_edges()) next.push_back(edge.function.get());
+  }
 }
 
 void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -99,6 +132,7 @@ struct RowNorm : torch::autograd::Function<RowNorm> {
     const bool need[3] = {ctx->needs_input_grad(0), w.defined() && ctx->needs_input_grad(1),
                           b.defined() && ctx->needs_input_grad(w.defined() ? 2 : 1)};
     if (!grads[0].defined()) return variable_list(5);
+    refuse_stale_leaves("row norm");
     if (at::GradMode::is_enabled()) {  // (what the kernels give carries no graph)
       variable_list leaves, out(5);
       for (int i = 0; i < 3; ++i)
@@ -177,6 +211,7 @@ struct DropoutAdd : torch::autograd::Function<DropoutAdd> {
     const Tensor &dy = grads[0];
     variable_list out(5);
     if (!dy.defined()) return out;
+    refuse_stale_leaves("dropout_add");
     const c10::DeviceGuard guard(dy.device());
     if (ctx->needs_input_grad(0))
       out[0] = dropout_launch(dy.contiguous(), Tensor(), ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(), seed_dev);
@@ -222,6 +257,7 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
     const Tensor &rows = saved[0], &weight = saved[1], &kept = saved[2], &dloss = grads[0];
     variable_list out(5);
     if (!dloss.defined()) return out;
+    refuse_stale_leaves("linear_cross_entropy");
     const c10::DeviceGuard guard(weight.device());
     const int64_t N = ctx->saved_data["N"].toInt(), d = ctx->saved_data["d"].toInt(), V = weight.size(0);
     const int reduction = static_cast<int>(ctx->saved_data["reduction"].toInt()), code = dtype_code(weight);
