@@ -134,10 +134,14 @@ struct RowNorm : torch::autograd::Function<RowNorm> {
     if (!grads[0].defined()) return variable_list(5);
     refuse_stale_leaves("row norm");
     if (at::GradMode::is_enabled()) {  // (what the kernels give carries no graph)
-      variable_list leaves, out(5);
-      for (int i = 0; i < 3; ++i)
-        if (need[i]) leaves.push_back(saved[i]);
-      const Tensor y = norm_torch(x, w, b, ctx->saved_data["eps"].toDouble(), layer);
+      // With respect to views of the inputs, not to the inputs: where one of those was made from another, the way back
+      // through it belongs to the pass that called this.
+      variable_list in(3), leaves, out(5);
+      for (int i = 0; i < 3; ++i) {
+        if (saved[i].defined()) in[i] = saved[i].view_as(saved[i]);
+        if (need[i]) leaves.push_back(in[i]);
+      }
+      const Tensor y = norm_torch(in[0], in[1], in[2], ctx->saved_data["eps"].toDouble(), layer);
       const variable_list got = torch::autograd::grad({y}, leaves, {grads[0]}, std::nullopt, /*create_graph=*/true);
       for (int i = 0, k = 0; i < 3; ++i)
         if (need[i]) out[i] = got[k++];
