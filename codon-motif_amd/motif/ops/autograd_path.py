@@ -9,7 +9,10 @@ ops in float32, so autograd supplies the backward.  Inference never takes this p
 import math
 
 import torch
+import torch.autograd.forward_ad as fwAD
 import torch.nn.functional as F
+
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
 
 
 def wants_grad(*items) -> bool:
@@ -32,6 +35,21 @@ def wants_grad(*items) -> bool:
             if wants_grad(*it):
                 return True
     return False
+
+
+def refuse_transforms(what, *tensors):
+    '''Raises NotImplementedError where a call of kernels that write through raw pointers would
+    be lost: while torch.jit.trace or make_fx records (they would see an empty tensor), and for tensors
+    of a function transform or with a forward-mode tangent (the result would come without it).
+    None among `tensors` is skipped.'''
+    if torch._C._get_tracing_state() is not None or torch._C._get_dispatch_mode(_PROXY) is not None:
+        raise NotImplementedError(f'{what}: the kernels cannot be traced')
+    if torch._C._are_functorch_transforms_active():
+        if any(t is not None and torch._C._functorch.is_functorch_wrapped_tensor(t) for t in tensors):
+            raise NotImplementedError(f'{what}: not under a function transform')
+    if fwAD._current_level >= 0:
+        if any(t is not None and fwAD.unpack_dual(t).tangent is not None for t in tensors):
+            raise NotImplementedError(f'{what}: no forward-mode derivatives')
 
 
 def _cdt(t):

@@ -4,6 +4,7 @@
 import torch
 
 from . import _lib
+from .autograd_path import refuse_transforms
 
 
 def dropout_add(x, p, seed, residual=None):
@@ -15,7 +16,9 @@ def dropout_add(x, p, seed, residual=None):
     e div 4 under the 64-bit key `seed` is at least round(p 2^32), 0 <= p < 1.  `seed` is an int, or
     an int64 tensor of one element on x's device that is read when the kernel runs (so that a
     captured graph draws anew when it changes); it must stay as it is until the backward.
-    Differentiable once in x and residual.'''
+    Differentiable once in x and residual, in reverse mode; tracing, function transforms and
+    forward-mode tangents are refused.'''
+    refuse_transforms('dropout_add', x, residual, seed if isinstance(seed, torch.Tensor) else None)
     p = float(p)
     if not 0.0 <= p < 1.0:
         raise ValueError(f'dropout_add: p must be in [0, 1), got {p}')

@@ -5,6 +5,7 @@ motif/model/motif.py:600-628).
 import torch
 
 from . import _lib
+from .autograd_path import refuse_transforms
 
 MAX_ROWS, MAX_FEATURES, MAX_VOCABULARY = 2 ** 23, 2 ** 16, 2 ** 22 - 64
 _REDUCTIONS = {'none': 0, 'sum': 1, 'mean': 2}
@@ -24,11 +25,13 @@ def linear_cross_entropy(x, weight, labels, ignore_index=-100, reduction='mean')
     Rows whose label is `ignore_index` are left out of every product: they get a zero
     gradient and nothing that they hold reaches the loss.  A label outside [0, V) that is not
     `ignore_index` gives NaN (loss and gradients).  Under autocast, x and weight are cast to its
-    dtype, as F.linear does.  Differentiable once in x and weight.
+    dtype, as F.linear does.  Differentiable once in x and weight, in reverse mode; tracing,
+    function transforms and forward-mode tangents are refused.
 
     For the backward a copy of the labelled rows, the weight and 16 bytes a row are kept.  Its scratch
     is the gradient of the logits in pieces of the vocabulary (256 MB to 1 GB, or 4096 vocabulary
     rows where that is more), and partial sums of x's gradient in fp32.'''
+    refuse_transforms('linear_cross_entropy', x, weight, labels)
     if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction must be 'none', 'sum' or 'mean', got {reduction!r}")
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:

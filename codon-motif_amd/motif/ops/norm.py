@@ -7,12 +7,14 @@ summed in a fixed order.  `RMSNorm` calls `rms_norm_rows` where gradients are wa
 import torch
 
 from . import _lib
+from .autograd_path import refuse_transforms
 
 MAX_FEATURES = 16384
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def _check(x, params, what):
+    refuse_transforms(what, x, *(t for _, t in params))
     if x.dtype not in _DTYPES:
         raise NotImplementedError(f'{what}: unsupported dtype {x.dtype}')
     if x.dim() < 1 or x.shape[-1] < 1:
@@ -35,13 +37,15 @@ def _check(x, params, what):
 def rms_norm_rows(x, weight=None, eps=1e-6):
     '''x / sqrt(mean(x^2) + eps) * weight over the last dimension of x [..., D] (fp32, bf16 or
     fp16, D at most 16384), in fp32, rounded once.  weight [D] of x's dtype, or None.
-    Differentiable in x and weight.'''
+    Differentiable in x and weight, in
+    reverse mode; tracing, function transforms and forward-mode tangents are refused.'''
     _check(x, (('weight', weight),), 'rms_norm_rows')
     return _lib.nodes().row_norm(x, weight, None, eps, False)
 
 
 def layer_norm_rows(x, weight=None, bias=None, eps=1e-5):
     '''(x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x [..., D], as
-    rms_norm_rows; bias [D] of x's dtype, or None.  Differentiable in x, weight and bias.'''
+    rms_norm_rows; bias [D] of x's dtype, or None.  Differentiable in x, weight and bias in
+    the same way.'''
     _check(x, (('weight', weight), ('bias', bias)), 'layer_norm_rows')
     return _lib.nodes().row_norm(x, weight, bias, eps, True)
