@@ -7,6 +7,7 @@ hipStream_t handles and device pointers torch hands out are valid for it.
 import contextlib
 import ctypes
 import os
+import warnings
 
 import torch
 
@@ -181,6 +182,7 @@ def lib():
 
 
 _nodes = None
+_nodes_found = None
 
 
 def nodes():
@@ -196,6 +198,20 @@ def nodes():
                                'Build them with `python codon-motif_amd/csrc/build.py`.') from exc
         _nodes = _autograd_nodes
     return _nodes
+
+
+def nodes_available() -> bool:
+    '''True when the autograd nodes loaded too and a ROCm device is visible: for calls that have torch's own
+    op to fall back to.  The nodes are built against one torch; where they do not load, that is said once.'''
+    global _nodes_found
+    if _nodes_found is None and available():
+        try:
+            nodes()
+            _nodes_found = True
+        except RuntimeError as exc:
+            _nodes_found = False
+            warnings.warn(f'{exc} Until then RMSNorm trains on torch\'s own op.', stacklevel=2)
+    return bool(_nodes_found) and available()
 
 
 ERR_INVALID, ERR_UNSUPPORTED, ERR_HIP = 1, 2, 3

@@ -19,12 +19,13 @@ _PLAIN = (torch.Tensor, nn.Parameter)
 
 def _trains_on_kernels(x, weight):
     '''A call whose gradients the kernels give: plain tensors in reverse mode.  Autocast, function
-    transforms, forward-mode derivatives, tracing and compiling keep torch's own op.'''
+    transforms, forward-mode derivatives, tracing and compiling keep torch's own op, and so does an
+    installation whose autograd nodes do not load.'''
     return (wants_grad(x, weight) and torch._C._get_tracing_state() is None and x.dtype in _KERNEL_DTYPES and weight.dtype == x.dtype
             and weight.device == x.device and weight.dim() == 1 and x.shape[-1] <= MAX_FEATURES
             and type(x) in _PLAIN and type(weight) in _PLAIN and not torch.is_autocast_enabled('cuda')
             and not torch._C._are_functorch_transforms_active() and torch.autograd.forward_ad._current_level < 0
-            and not torch.compiler.is_compiling() and _lib.available())
+            and not torch.compiler.is_compiling() and _lib.nodes_available())
 
 
 def _rms(x, weight, eps):
