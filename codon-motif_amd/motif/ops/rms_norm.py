@@ -30,7 +30,7 @@ def _trains_on_kernels(x, weight):
 
 def _rms(x, weight, eps):
     if x.is_cuda and weight is not None and weight.numel() == x.shape[-1]:
-        if _trains_on_kernels(x, weight):
+        if eps is not None and _trains_on_kernels(x, weight):  # (torch's op takes the type's own then)
             return rms_norm_rows(x, weight, eps)
         return F.rms_norm(x, (x.shape[-1],), weight, eps)
     x_f = x.float()
