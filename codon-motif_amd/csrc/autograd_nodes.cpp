@@ -192,8 +192,8 @@ Tensor row_norm(const Tensor &x, const OptTensor &weight, const OptTensor &bias,
 Tensor dropout_launch(const Tensor &x, const Tensor &residual, double p, int64_t seed, const Tensor &seed_dev) {
   const Tensor y = at::empty(x.sizes(), x.options());
   const double t = std::nearbyint(p * 4294967296.0);  // (half to even, as Python's round)
-  const uint32_t threshold = t >= 4294967295.0 ? 4294967295u : static_cast<uint32_t>(t);
-  check(motif_dropout_add(ptr(x), ptr(residual), ptr(y), x.numel(), threshold, static_cast<float>(1 / (1 - p)),
+  const bool none = t >= 4294967296.0;  // (no word is as large: a scale of 0 drops every element)
+  check(motif_dropout_add(ptr(x), ptr(residual), ptr(y), x.numel(), none ? 0 : static_cast<uint32_t>(t), none ? 0.f : static_cast<float>(1 / (1 - p)),
                           static_cast<uint64_t>(seed), static_cast<const int64_t *>(ptr(seed_dev)), dtype_code(x), stream_of(x)),
         "motif_dropout_add");
   return y;

@@ -4,6 +4,7 @@
 // "Parallel random numbers: as easy as 1, 2, 3", SC 2011) at the counter (e / 4 as two 32-bit
 // words, 0, 0) under the 64-bit key `seed` is at least T = round(p 2^32).  The backward pass draws the
 // same words again.  Computed in fp32, rounded once; a dropped element adds nothing, whatever it holds.
+// T = 2^32 (p within 2^-33 of 1), which no word reaches, is a scale of 0: every element is dropped.
 //
 // Bound by memory (x, the residual and y once each) while the ten rounds, two 32 x 32 -> 64 bit products
 // each for four elements, stay below it.  One thread draws for two (16-bit types) or one counter
@@ -50,6 +51,7 @@ template <typename T, bool RES, bool VEC>
 __global__ void __launch_bounds__(256) dropout_kernel(DropArgs a) {
   constexpr int E = 16 / sizeof(T);
   const uint64_t key = a.seed_dev ? static_cast<uint64_t>(*a.seed_dev) : a.seed;
+  const bool some = a.scale != 0.f;
   const T *x = static_cast<const T *>(a.x), *res = static_cast<const T *>(a.res);
   T *y = static_cast<T *>(a.y);
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i * E < a.n; i += int64_t(gridDim.x) * 256) {
@@ -73,7 +75,7 @@ __global__ void __launch_bounds__(256) dropout_kernel(DropArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int e = 4 * q + j;
-        const bool keep = wd.w[j] >= a.threshold;
+        const bool keep = some && wd.w[j] >= a.threshold;
         const float xv = ld(&px.e[e]);
         float v;
         if (RES) {

@@ -836,7 +836,7 @@ int motif_row_norm_bwd(const void *dy, int64_t dy_rs, const void *x, int64_t x_r
 /*
  * Dropout of a branch: y_e = residual_e + x_e * scale where word e mod 4 of Philox4x32-10 at counter
  * (e / 4 as two words, 0, 0) under the 64-bit key is >= threshold, else residual_e (0 without a
- * residual).  n contiguous elements; the key is *seed_dev, or `seed` when seed_dev is NULL.  The
+ * residual); a scale of 0 drops every element.  n contiguous elements; the key is *seed_dev, or `seed` when seed_dev is NULL.  The
  * gradient for x is the same call on dy without a residual.
  */
 int motif_dropout_add(const void *x, const void *residual, void *y, int64_t n, uint32_t threshold, float scale,
