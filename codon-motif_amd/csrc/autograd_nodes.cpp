@@ -70,6 +70,9 @@ void refuse_stale_leaves(const char *what) {
 void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor given(const OptTensor &t) { return t.has_value() ? *t : Tensor(); }
 
+// t as it lies in memory: torch's negative views (the imaginary part of a conjugate, say) hold their sign beside it
+Tensor plain(const Tensor &t) { return t.defined() ? t.resolve_neg() : t; }
+
 // ------------------------------------------------------------ row norms
 // x as rows of D: its stride where the leading dimensions lie regularly, else a contiguous copy
 struct Rows {
@@ -148,7 +151,7 @@ struct RowNorm : torch::autograd::Function<RowNorm> {
       return out;
     }
     const c10::DeviceGuard guard(x.device());
-    const Rows r(x), dy(grads[0]);
+    const Rows r(x), dy(plain(grads[0]));
     const Tensor dx = need[0] ? at::empty(x.sizes(), x.options()) : Tensor();
     const Tensor dw = need[1] ? at::empty({r.D}, x.options()) : Tensor(), db = need[2] ? at::empty({r.D}, x.options()) : Tensor();
     if (r.n == 0) {
@@ -178,8 +181,8 @@ bool wants_grad(std::initializer_list<const Tensor *> ts) {
   return false;
 }
 
-Tensor row_norm(const Tensor &x, const OptTensor &weight, const OptTensor &bias, double eps, bool layer) {
-  const Tensor w = weight ? weight->contiguous() : Tensor(), b = bias ? bias->contiguous() : Tensor();
+Tensor row_norm(const Tensor &input, const OptTensor &weight, const OptTensor &bias, double eps, bool layer) {
+  const Tensor x = plain(input), w = weight ? plain(weight->contiguous()) : Tensor(), b = bias ? plain(bias->contiguous()) : Tensor();
   if (wants_grad({&x, &w, &b}))
     return RowNorm::apply(x, w.defined() ? OptTensor(w) : OptTensor(), b.defined() ? OptTensor(b) : OptTensor(), eps, layer);
   const c10::DeviceGuard guard(x.device());
@@ -218,14 +221,15 @@ struct DropoutAdd : torch::autograd::Function<DropoutAdd> {
     refuse_stale_leaves("dropout_add");
     const c10::DeviceGuard guard(dy.device());
     if (ctx->needs_input_grad(0))
-      out[0] = dropout_launch(dy.contiguous(), Tensor(), ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(), seed_dev);
+      out[0] = dropout_launch(plain(dy.contiguous()), Tensor(), ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(), seed_dev);
     if (ctx->saved_data["added"].toBool() && ctx->needs_input_grad(1)) out[1] = dy;
     return out;
   }
 };
 
 Tensor dropout_add(const Tensor &x, const OptTensor &residual, double p, int64_t seed, const OptTensor &seed_dev) {
-  return DropoutAdd::apply(x, residual, p, seed, seed_dev);
+  return DropoutAdd::apply(plain(x), residual ? OptTensor(plain(*residual)) : OptTensor(), p, seed,
+                           seed_dev ? OptTensor(plain(*seed_dev)) : OptTensor());
 }
 
 // ------------------------------------------------------------ cross entropy
@@ -258,7 +262,8 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "linear_cross_entropy has no second derivatives");
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &rows = saved[0], &weight = saved[1], &kept = saved[2], &dloss = grads[0];
+    const Tensor &rows = saved[0], &weight = saved[1], &kept = saved[2];
+    const Tensor dloss = plain(grads[0]);
     variable_list out(5);
     if (!dloss.defined()) return out;
     refuse_stale_leaves("linear_cross_entropy");
@@ -280,7 +285,8 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
   }
 };
 
-Tensor linear_ce(const Tensor &x, const Tensor &weight, const Tensor &labels, int64_t ignore, int64_t reduction) {
+Tensor linear_ce(const Tensor &states, const Tensor &vocabulary, const Tensor &targets, int64_t ignore, int64_t reduction) {
+  const Tensor x = plain(states), weight = plain(vocabulary), labels = plain(targets);
   if (wants_grad({&x, &weight})) return LinearCE::apply(x, weight, labels, ignore, reduction);
   return LinearCE::forward(nullptr, x, weight, labels, ignore, reduction);
 }
