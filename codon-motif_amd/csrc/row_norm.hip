@@ -368,9 +368,17 @@ template <typename T, int E> int launch_fwd(const NormArgs &a, bool layer, hipSt
   const bool ok = with_shape<E>(a.D, [&](auto lpr, auto nv) {
     constexpr int LPR = decltype(lpr)::value, NV = decltype(nv)::value;
     const int rpb = rows_per_block<LPR>();
-    const dim3 g(static_cast<unsigned>((int64_t(a.rows) + rpb - 1) / rpb)), b(block_size<LPR>());
-    if (layer) row_norm_fwd_kernel<T, E, LPR, NV, true><<<g, b, 0, s>>>(a);
-    else row_norm_fwd_kernel<T, E, LPR, NV, false><<<g, b, 0, s>>>(a);
+    // (a launch has less than 2^32 threads: 2^29 rows of 8 lanes, 2^24 of 256)
+    const int64_t most = int64_t(UINT32_MAX / block_size<LPR>()) * rpb;
+    for (int64_t r0 = 0; r0 < a.rows; r0 += most) {
+      NormArgs c = a;
+      c.rows = static_cast<int>(std::min<int64_t>(most, a.rows - r0));
+      c.x = static_cast<const T *>(a.x) + r0 * a.x_rs, c.y = static_cast<T *>(a.y) + r0 * a.y_rs;
+      c.rstd = a.rstd ? a.rstd + r0 : nullptr, c.mean = a.mean ? a.mean + r0 : nullptr;
+      const dim3 g(static_cast<unsigned>((int64_t(c.rows) + rpb - 1) / rpb)), b(block_size<LPR>());
+      if (layer) row_norm_fwd_kernel<T, E, LPR, NV, true><<<g, b, 0, s>>>(c);
+      else row_norm_fwd_kernel<T, E, LPR, NV, false><<<g, b, 0, s>>>(c);
+    }
   });
   if (!ok) return set_error(MOTIF_ERR_UNSUPPORTED, "row_norm: rows longer than the kernels hold");
   return check_launch("row_norm_fwd_kernel");
