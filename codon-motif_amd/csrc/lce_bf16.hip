@@ -249,7 +249,9 @@ template <typename C, bool GRADS>
 __global__ void __launch_bounds__(C::THREADS, C::BOUND) lce_z_kernel(LceArgs a, int nm, int nn) {
   __shared__ __align__(1024) char lds[C::ST * C::STAGE];
   const int count = __builtin_amdgcn_readfirstlane(*a.count);
-  const TilePos at = tile_at(xcd_tile(blockIdx.x, gridDim.x), nm, nn, 4);
+  const int b = static_cast<int>(lce_block());  // (at most 2^14 x 2^16 tiles)
+  if (b >= nm * nn) return;
+  const TilePos at = tile_at(xcd_tile(b, nm * nn), nm, nn, 4);
   const int t0 = at.n * C::TN, v0 = (GRADS ? a.v0 : 0) + at.m * C::TM;
   if (t0 >= count) return;
   const RowsK<C, C::TM> A(static_cast<const bf16_t *>(a.w) + int64_t(v0) * a.ldw, a.ldw, a.V - v0, a.dk);
@@ -408,7 +410,7 @@ template <bool GRADS> int z_launch(const LceArgs &a, hipStream_t s) {
     using C = decltype(c);
     static_assert(C::TM == 256, "the vocabulary parts of the statistics");
     const int nm = up(GRADS ? a.vn : a.V, C::TM), nn = up(a.N, C::TN);
-    lce_z_kernel<C, GRADS><<<nm * nn, C::THREADS, 0, s>>>(a, nm, nn);
+    lce_z_kernel<C, GRADS><<<lce_grid(int64_t(nm) * nn), C::THREADS, 0, s>>>(a, nm, nn);
     return check_launch("lce_z_kernel");
   });
 }

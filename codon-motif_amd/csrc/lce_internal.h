@@ -40,6 +40,14 @@ struct LceArgs {
   void *dw;            // [V, d]
 };
 
+// A launch has less than 2^32 threads along x: workgroups beyond kGridX go along y, in the same order.
+constexpr int64_t kGridX = 1 << 21;
+inline dim3 lce_grid(int64_t n) {
+  const int64_t x = n < kGridX ? n : kGridX;
+  return dim3(static_cast<unsigned>(x), static_cast<unsigned>((n + x - 1) / x));
+}
+__device__ __forceinline__ int64_t lce_block() { return int64_t(blockIdx.y) * gridDim.x + blockIdx.x; }
+
 // A wave's accumulators of 32 x 32 products with the vocabulary (or P's rows) on the left: register
 // i of lane l is row 8 (i / 4) + 4 (l / 32) + i % 4, column l % 32.
 __device__ __forceinline__ int acc_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }

@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(1024) lce_loss_kernel(const float *nll, const 
 // 64 E columns of a row (`per` of them make a row); E = 4 where d is a multiple of 4.
 template <typename T, int E>
 __global__ void __launch_bounds__(256) lce_dx_rows_kernel(LceArgs a, T *dx, int per) {
-  const int64_t id = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t id = lce_block() * 4 + (threadIdx.x >> 6);
   const int64_t r = id / per;
   const int c = (static_cast<int>(id - r * per) * 64 + (threadIdx.x & 63)) * E;
   if (r >= a.N || c >= a.d) return;
@@ -283,7 +283,13 @@ struct BwdSpace {
   }
 };
 
-bool sizes_ok(int N, int d, int V) { return N > 0 && N <= (1 << 23) && d > 0 && d <= (1 << 16) && V > 0 && V <= (1 << 22) - 64; }
+// Each size by itself, and the tiles of dX and dW together, which are one launch of 256 threads each (2^24 tiles: x and w of 1 TB
+// in bf16, 275 GB in fp32; a small dX has up to 512 more in its shares).
+bool sizes_ok(int N, int d, int V, int dtype) {
+  if (N < 1 || N > (1 << 23) || d < 1 || d > (1 << 16) || V < 1 || V > (1 << 22) - 64) return false;
+  const int64_t tm = dtype == MOTIF_BF16 ? 256 : 64, tn = dtype == MOTIF_BF16 ? 128 : 64;
+  return ((N + tm - 1) / tm + (V + tm - 1) / tm) * ((d + tn - 1) / tn) <= (1 << 24) - 1024;
+}
 
 // kept: 4 N + 1 words: row, label, pos, lse, count
 void bind_kept(LceArgs &a, int *kept) {
@@ -338,12 +344,12 @@ template <typename T> int gather(const void *x, int64_t rs, const LceArgs &a, co
 using namespace motif;
 
 extern "C" size_t motif_linear_ce_rows_bytes(int N, int d, int dtype) {
-  if (!sizes_ok(N, d, 1)) return 0;
+  if (!sizes_ok(N, d, 1, dtype)) return 0;
   return size_t(N) * up(d, 64) * esize(dtype);
 }
 
 extern "C" size_t motif_linear_ce_workspace_bytes(int N, int d, const void *w, int64_t w_rs, int V, int dtype, int backward) {
-  if (!sizes_ok(N, d, V)) return 0;
+  if (!sizes_ok(N, d, V, dtype)) return 0;
   const size_t copy = copy_bytes(w, w_rs, d, V, dtype);
   return backward ? BwdSpace(N, d, V, dtype, copy).bytes : FwdSpace(N, V, dtype, copy).bytes;
 }
@@ -353,7 +359,7 @@ extern "C" int motif_linear_ce_fwd(const void *x, int64_t x_rs, const void *w, i
                                    void *rows, int *kept, float *loss, void *workspace, size_t workspace_bytes, int dtype,
                                    void *stream) {
   if (dtype != MOTIF_F32 && dtype != MOTIF_BF16) return set_error(MOTIF_ERR_UNSUPPORTED, "linear_ce_fwd: fp32 or bf16");
-  if (!sizes_ok(N, d, V)) return set_error(MOTIF_ERR_INVALID, "linear_ce_fwd: N, d, V out of range");
+  if (!sizes_ok(N, d, V, dtype)) return set_error(MOTIF_ERR_INVALID, "linear_ce_fwd: N, d, V out of range");
   if (reduction < 0 || reduction > 2) return set_error(MOTIF_ERR_INVALID, "linear_ce_fwd: reduction is 0, 1 or 2");
   if (!x || !w || !labels || !rows || !kept || !loss || !workspace)
     return set_error(MOTIF_ERR_INVALID, "linear_ce_fwd: null pointer");
@@ -388,7 +394,7 @@ extern "C" int motif_linear_ce_bwd(const void *rows, const void *w, int64_t w_rs
                                    int64_t dloss_st, int N, int d, int V, int reduction, void *dx, void *dw,
                                    void *workspace, size_t workspace_bytes, int dtype, void *stream) {
   if (dtype != MOTIF_F32 && dtype != MOTIF_BF16) return set_error(MOTIF_ERR_UNSUPPORTED, "linear_ce_bwd: fp32 or bf16");
-  if (!sizes_ok(N, d, V)) return set_error(MOTIF_ERR_INVALID, "linear_ce_bwd: N, d, V out of range");
+  if (!sizes_ok(N, d, V, dtype)) return set_error(MOTIF_ERR_INVALID, "linear_ce_bwd: N, d, V out of range");
   if (reduction < 0 || reduction > 2) return set_error(MOTIF_ERR_INVALID, "linear_ce_bwd: reduction is 0, 1 or 2");
   if (!rows || !w || !kept || !dloss || !workspace) return set_error(MOTIF_ERR_INVALID, "linear_ce_bwd: null pointer");
   if (V > 1 && w_rs < d) return set_error(MOTIF_ERR_INVALID, "linear_ce_bwd: rows overlap");
@@ -417,7 +423,7 @@ extern "C" int motif_linear_ce_bwd(const void *rows, const void *w, int64_t w_rs
   if (rc != MOTIF_OK || !dx) return rc;
   const bool four = d % 4 == 0 && reinterpret_cast<uintptr_t>(dx) % 16 == 0;
   const int per = (d + (four ? 256 : 64) - 1) / (four ? 256 : 64);
-  const unsigned g = static_cast<unsigned>((int64_t(N) * per + 3) / 4);
+  const dim3 g = lce_grid((int64_t(N) * per + 3) / 4);
   if (four) {
     if (bf16) lce_dx_rows_kernel<bf16_t, 4><<<g, 256, 0, s>>>(a, static_cast<bf16_t *>(dx), per);
     else lce_dx_rows_kernel<float, 4><<<g, 256, 0, s>>>(a, static_cast<float *>(dx), per);

@@ -796,7 +796,7 @@ int motif_mul_sigmoid(const void *x, int64_t x_rs, const void *g, int64_t g_rs, 
  * Softmax cross entropy straight from hidden states x [N, d] and the vocabulary's rows w [V, d]
  * (the reference computes the logits and then F.cross_entropy, motif/model/motif.py:600-628), the
  * logits never stored: loss_i = log sum_v exp(x_i . w_v) - x_i . w_{t_i} in fp32.
- *   N at most 2^23, d 2^16, V 2^22 - 64.  x row stride x_rs, w row stride w_rs >= d, features beside each other; labels int64, stride
+ *   N at most 2^23, d 2^16, V 2^22 - 64, and (N + V) d at most about 2^39 in bf16 and 2^36 in fp32.  x row stride x_rs, w row stride w_rs >= d, features beside each other; labels int64, stride
  *   labels_st.  A row whose label is ignore_index has no loss and no gradient, whatever it holds; a
  *   label outside [0, V) gives a loss and gradients of NaN.
  *   reduction 0: loss [N] fp32 (0 where ignored); 1: the sum; 2: the mean over the labelled rows
