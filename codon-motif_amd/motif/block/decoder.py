@@ -31,6 +31,8 @@ class DecoderBlockOutput:
 
 
 class Decoder(nn.Module):
+    dropout = 0.0  # (of decoders pickled without it)
+
     def __init__(self, attn_type: Literal['gdn', 'chord'], config: MotifChordConfig):
         super().__init__()
         self.attn_type = attn_type.lower()
