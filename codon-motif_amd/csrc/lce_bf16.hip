@@ -46,17 +46,20 @@ __device__ __forceinline__ uint2 read_tr(const char *p) {
 
 // 16 bytes a lane from buffer r at byte voff + soff into LDS at dst + 16 lane (dst the same for the wave).  The
 // builtin for it makes the compiler wait for every load in flight before each transposed LDS read, which
-// would empty the pipeline at every step; here `product` does all the waiting itself.  (m0 holds the place; nothing
-// else in these kernels uses it.)
+// would empty the pipeline at every step; here `product` does all the waiting itself.  (m0 holds the place.  It is no
+// register that the compiler keeps values in, which it warns of; said here, it sets m0 anew for whatever else may need it.)
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ i32x4 make_rsrc(const void *p, int64_t bytes) {
   const uint64_t a = reinterpret_cast<uint64_t>(p);
   return i32x4{static_cast<int>(a), static_cast<int>((a >> 32) & 0xffff), static_cast<int>(bytes), 0x00020000};
 }
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_lds(i32x4 r, uint32_t dst, uint32_t voff, uint32_t soff) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-               ::"s"(dst), "v"(voff), "s"(r), "s"(soff) : "memory");
+               ::"s"(dst), "v"(voff), "s"(r), "s"(soff) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 __device__ __forceinline__ bf16x8 join(uint2 a, uint2 b) { return __builtin_bit_cast(bf16x8, uint4{a.x, a.y, b.x, b.y}); }
 
