@@ -67,7 +67,14 @@ void refuse_stale_leaves(const char *what) {
   }
 }
 
-void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+// Null for an argument left out, and for nothing else: subclasses without memory of their own (distributed tensors, fake
+// ones) have null pointers too.
+void *ptr(const Tensor &t) {
+  if (!t.defined()) return nullptr;
+  void *p = t.data_ptr();
+  TORCH_CHECK_VALUE(p || t.numel() == 0, "the kernels take tensors with memory of their own: this one has no memory (a distributed or fake tensor)");
+  return p;
+}
 Tensor given(const OptTensor &t) { return t.has_value() ? *t : Tensor(); }
 
 // t as it lies in memory: torch's negative views (the imaginary part of a conjugate, say) hold their sign beside it
@@ -99,7 +106,7 @@ struct Rows {
 void norm_forward(const Rows &r, const Tensor &w, const Tensor &b, const Tensor &y, const Tensor &stats, double eps, bool layer) {
   if (r.n == 0) return;
   float *rstd = stats.defined() ? stats.data_ptr<float>() : nullptr;
-  check(motif_row_norm_fwd(r.t.data_ptr(), r.stride, ptr(w), ptr(b), y.data_ptr(), r.D, rstd, layer && rstd ? rstd + r.n : nullptr,
+  check(motif_row_norm_fwd(ptr(r.t), r.stride, ptr(w), ptr(b), y.data_ptr(), r.D, rstd, layer && rstd ? rstd + r.n : nullptr,
                            static_cast<int>(r.n), static_cast<int>(r.D), static_cast<float>(eps), layer, dtype_code(y), stream_of(y)),
         "motif_row_norm_fwd");
 }
@@ -166,7 +173,7 @@ struct RowNorm : torch::autograd::Function<RowNorm> {
       ws = at::empty({static_cast<int64_t>(bytes / 4)}, stats.options());
     }
     const float *rstd = stats.data_ptr<float>();
-    check(motif_row_norm_bwd(dy.t.data_ptr(), dy.stride, r.t.data_ptr(), r.stride, ptr(w), rstd, layer ? rstd + r.n : nullptr, ptr(dx),
+    check(motif_row_norm_bwd(ptr(dy.t), dy.stride, ptr(r.t), r.stride, ptr(w), rstd, layer ? rstd + r.n : nullptr, ptr(dx),
                              r.D, ptr(dw), ptr(db), static_cast<int>(r.n), static_cast<int>(r.D), layer, ptr(ws), bytes,
                              dtype_code(x), stream_of(x)),
           "motif_row_norm_bwd");
@@ -244,9 +251,9 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
     const Tensor rows = at::empty({static_cast<int64_t>(motif_linear_ce_rows_bytes(N, d, code))}, bytes);
     const Tensor kept = at::empty({4 * int64_t(N) + 1}, x.options().dtype(at::kInt));
     const Tensor loss = reduction == 0 ? at::empty({N}, x.options().dtype(at::kFloat)) : at::empty({}, x.options().dtype(at::kFloat));
-    const size_t need = motif_linear_ce_workspace_bytes(N, d, weight.data_ptr(), weight.stride(0), V, code, 0);
+    const size_t need = motif_linear_ce_workspace_bytes(N, d, ptr(weight), weight.stride(0), V, code, 0);
     const Tensor ws = at::empty({static_cast<int64_t>(need)}, bytes);
-    check(motif_linear_ce_fwd(x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), labels.data_ptr<int64_t>(),
+    check(motif_linear_ce_fwd(ptr(x), x.stride(0), ptr(weight), weight.stride(0), static_cast<const int64_t *>(ptr(labels)),
                               labels.stride(0), ignore, N, d, V, static_cast<int>(reduction), rows.data_ptr(), kept.data_ptr<int>(),
                               loss.data_ptr<float>(), ws.data_ptr(), need, code, stream_of(x)),
           "motif_linear_ce_fwd");
@@ -272,10 +279,10 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
     const int reduction = static_cast<int>(ctx->saved_data["reduction"].toInt()), code = dtype_code(weight);
     const Tensor dx = ctx->needs_input_grad(0) ? at::empty({N, d}, weight.options()) : Tensor();
     const Tensor dw = ctx->needs_input_grad(1) ? at::empty({V, d}, weight.options()) : Tensor();
-    const size_t need = motif_linear_ce_workspace_bytes(static_cast<int>(N), static_cast<int>(d), weight.data_ptr(), weight.stride(0),
+    const size_t need = motif_linear_ce_workspace_bytes(static_cast<int>(N), static_cast<int>(d), ptr(weight), weight.stride(0),
                                                         static_cast<int>(V), code, 1);
     const Tensor ws = at::empty({static_cast<int64_t>(need)}, weight.options().dtype(at::kByte));
-    check(motif_linear_ce_bwd(rows.data_ptr(), weight.data_ptr(), weight.stride(0), kept.data_ptr<int>(), dloss.data_ptr<float>(),
+    check(motif_linear_ce_bwd(rows.data_ptr(), ptr(weight), weight.stride(0), kept.data_ptr<int>(), static_cast<const float *>(ptr(dloss)),
                               reduction == 0 ? dloss.stride(0) : 0, static_cast<int>(N), static_cast<int>(d), static_cast<int>(V),
                               reduction, ptr(dx), ptr(dw), ws.data_ptr(), need, code, stream_of(weight)),
           "motif_linear_ce_bwd");
