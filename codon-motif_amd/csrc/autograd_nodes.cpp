@@ -111,14 +111,24 @@ void norm_forward(const Rows &r, const Tensor &w, const Tensor &b, const Tensor 
         "motif_row_norm_fwd");
 }
 
-// The same in torch ops, for derivatives beyond the first
-Tensor norm_torch(const Tensor &x, const Tensor &w, const Tensor &b, double eps, bool layer) {
+// The gradients in torch ops, all in fp32: where they have to carry a graph of their own (create_graph), which the kernels'
+// do not, and for several gradients at once (is_grads_batched), which have no memory for a kernel to read.
+variable_list norm_grads_torch(const Tensor &x, const Tensor &w, const Tensor &grad, double eps, bool layer, const bool (&need)[3]) {
   Tensor h = x.to(at::kFloat);
   if (layer) h = h - h.mean(-1, true);
-  h = h * (h.square().mean(-1, true) + eps).rsqrt();
-  if (w.defined()) h = h * w.to(at::kFloat);
-  if (b.defined()) h = h + b.to(at::kFloat);
-  return h.to(x.scalar_type());
+  const Tensor r = (h.square().mean(-1, true) + eps).rsqrt(), dy = grad.to(at::kFloat);
+  h = h * r;
+  variable_list out(5);
+  if (need[0]) {
+    const Tensor g = w.defined() ? dy * w.to(at::kFloat) : dy;
+    Tensor dx = g - h * (g * h).mean(-1, true);
+    if (layer) dx = dx - g.mean(-1, true);
+    out[0] = (dx * r).to(x.scalar_type());
+  }
+  const auto rows = [&](const Tensor &t) { return t.reshape({-1, x.size(-1)}).sum(0).to(x.scalar_type()); };
+  if (need[1]) out[1] = rows(dy * h);
+  if (need[2]) out[2] = rows(dy);
+  return out;
 }
 
 struct RowNorm : torch::autograd::Function<RowNorm> {
@@ -143,20 +153,8 @@ struct RowNorm : torch::autograd::Function<RowNorm> {
                           b.defined() && ctx->needs_input_grad(w.defined() ? 2 : 1)};
     if (!grads[0].defined()) return variable_list(5);
     refuse_stale_leaves("row norm");
-    if (at::GradMode::is_enabled()) {  // (what the kernels give carries no graph)
-      // With respect to views of the inputs, not to the inputs: where one of those was made from another, the way back
-      // through it belongs to the pass that called this.
-      variable_list in(3), leaves, out(5);
-      for (int i = 0; i < 3; ++i) {
-        if (saved[i].defined()) in[i] = saved[i].view_as(saved[i]);
-        if (need[i]) leaves.push_back(in[i]);
-      }
-      const Tensor y = norm_torch(in[0], in[1], in[2], ctx->saved_data["eps"].toDouble(), layer);
-      const variable_list got = torch::autograd::grad({y}, leaves, {grads[0]}, std::nullopt, /*create_graph=*/true);
-      for (int i = 0, k = 0; i < 3; ++i)
-        if (need[i]) out[i] = got[k++];
-      return out;
-    }
+    if (at::GradMode::is_enabled() || !grads[0].has_storage())
+      return norm_grads_torch(x, w, grads[0], ctx->saved_data["eps"].toDouble(), layer, need);
     const c10::DeviceGuard guard(x.device());
     const Rows r(x), dy(plain(grads[0]));
     const Tensor dx = need[0] ? at::empty(x.sizes(), x.options()) : Tensor();
