@@ -67,6 +67,9 @@ void refuse_stale_leaves(const char *what) {
   }
 }
 
+// A gradient that came in with a forward-mode tangent, which the kernels would lose
+bool has_tangent(const Tensor &t) { return t._fw_grad(/*level=*/0).defined(); }
+
 // Null for an argument left out, and for nothing else: subclasses without memory of their own (distributed tensors, fake
 // ones) have null pointers too.
 void *ptr(const Tensor &t) {
@@ -111,8 +114,8 @@ void norm_forward(const Rows &r, const Tensor &w, const Tensor &b, const Tensor 
         "motif_row_norm_fwd");
 }
 
-// The gradients in torch ops, all in fp32: where they have to carry a graph of their own (create_graph), which the kernels'
-// do not, and for several gradients at once (is_grads_batched), which have no memory for a kernel to read.
+// The gradients in torch ops, all in fp32: where they have to carry a graph of their own (create_graph) or a tangent, which
+// the kernels' do not, and for several gradients at once (is_grads_batched), which have no memory for a kernel to read.
 variable_list norm_grads_torch(const Tensor &x, const Tensor &w, const Tensor &grad, double eps, bool layer, const bool (&need)[3]) {
   Tensor h = x.to(at::kFloat);
   if (layer) h = h - h.mean(-1, true);
@@ -153,7 +156,7 @@ struct RowNorm : torch::autograd::Function<RowNorm> {
                           b.defined() && ctx->needs_input_grad(w.defined() ? 2 : 1)};
     if (!grads[0].defined()) return variable_list(5);
     refuse_stale_leaves("row norm");
-    if (at::GradMode::is_enabled() || !grads[0].has_storage())
+    if (at::GradMode::is_enabled() || !grads[0].has_storage() || has_tangent(grads[0]))
       return norm_grads_torch(x, w, grads[0], ctx->saved_data["eps"].toDouble(), layer, need);
     const c10::DeviceGuard guard(x.device());
     const Rows r(x), dy(plain(grads[0]));
@@ -223,6 +226,7 @@ struct DropoutAdd : torch::autograd::Function<DropoutAdd> {
     const Tensor &dy = grads[0];
     variable_list out(5);
     if (!dy.defined()) return out;
+    TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(dy), "dropout_add: no forward-mode derivatives");
     refuse_stale_leaves("dropout_add");
     const c10::DeviceGuard guard(dy.device());
     if (ctx->needs_input_grad(0))
@@ -271,6 +275,7 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
     const Tensor dloss = plain(grads[0]);
     variable_list out(5);
     if (!dloss.defined()) return out;
+    TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(dloss), "linear_cross_entropy: no forward-mode derivatives");
     refuse_stale_leaves("linear_cross_entropy");
     const c10::DeviceGuard guard(weight.device());
     const int64_t N = ctx->saved_data["N"].toInt(), d = ctx->saved_data["d"].toInt(), V = weight.size(0);

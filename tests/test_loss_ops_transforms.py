@@ -98,6 +98,25 @@ def test_norm_module_keeps_its_tangent():
 
 
 @pytest.mark.gpu
+@NAMES
+def test_a_gradient_with_a_tangent(name):
+    '''A forward-mode tangent on the gradient that comes in, its input without one: linear through the norms, refused by the others.'''
+    x = _x('cuda').requires_grad_()
+    y = OPS[name](x)
+    dy, t = torch.full_like(y, 0.5), torch.full_like(y, -2.0) if y.dim() == 0 else torch.cos(torch.arange(y.numel(), device='cuda') * 1.0).view(y.shape)
+    want, = torch.autograd.grad(y, x, t, retain_graph=True)
+    with fwAD.dual_level():
+        dual = fwAD.make_dual(dy, t)
+        if 'norm' not in name:
+            with pytest.raises(NotImplementedError, match=f'{name}.*forward-mode'):
+                torch.autograd.grad(y, x, dual)
+            return
+        got = fwAD.unpack_dual(torch.autograd.grad(y, x, dual)[0]).tangent
+    # fp32 on both ways: two sums of eight terms and some twenty operations
+    assert got is not None and (got - want).abs().max() <= 60 * 2.0 ** -24 * want.abs().max()
+
+
+@pytest.mark.gpu
 def test_model_loss_is_not_traced():
     from motif.model.config import MotifChordConfig
     from motif.model.motif import MotifChordModel
