@@ -98,13 +98,15 @@ template <typename C, int R> struct RowsK {
 
 // BK k rows of R columns (row stride ld): LDS row k is R / 8 pieces, piece c at c ^ swap(k).
 __device__ __forceinline__ int tr_swap(int k) { return ((k & 1) << 2) | ((k & 2) ? 10 : 0); }
-template <typename C, int R> struct ColsK {
+// FOLD: the rows are gone through a second time, from k = `fold` on.
+template <typename C, int R, bool FOLD = false> struct ColsK {
   static constexpr int RP = 512 / R, NJ = C::BK / RP / C::NW;
   const bf16_t *p;
   int64_t ld;
-  int cols, K;
+  int cols, K, fold;
   uint32_t off[NJ];
-  __device__ __forceinline__ ColsK(const bf16_t *p_, int64_t ld_, int cols_, int K_) : p(p_), ld(ld_), cols(cols_), K(K_) {
+  __device__ __forceinline__ ColsK(const bf16_t *p_, int64_t ld_, int cols_, int K_, int fold_ = 0)
+      : p(p_), ld(ld_), cols(cols_), K(K_), fold(fold_) {
     const int l = threadIdx.x & 63, w = wave_id();
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
@@ -113,6 +115,7 @@ template <typename C, int R> struct ColsK {
     }
   }
   __device__ __forceinline__ void issue(uint32_t dst, int k0) const {
+    if (FOLD && k0 >= fold) k0 -= fold;
     const int w = wave_id(), n = min(K - k0, C::BK);
     const i32x4 buf = make_rsrc(p + int64_t(k0) * ld, ((n - 1) * ld + cols) * 2);
 #pragma unroll
@@ -153,16 +156,17 @@ template <typename C> struct PTokens {
   }
 };
 
-// ... as the left side of dW: 256 vocabulary rows x BK tokens
-template <typename C> struct PVocab {
+// ... as the left side of dW: 256 vocabulary rows x BK tokens (FOLD: from k = `fold` on the rows that hold remainders)
+template <typename C, bool FOLD = false> struct PVocab {
   static constexpr int NJ = 16 * (C::BK / 32) / C::NW;
   const char *p;
-  int nvc;
-  __device__ __forceinline__ PVocab(const void *p_, int r0, int vc) : nvc(vc / 16) {
+  int nvc, fold;
+  __device__ __forceinline__ PVocab(const void *p_, int r0, int vc, int fold_ = 0) : nvc(vc / 16), fold(fold_) {
     p = static_cast<const char *>(p_) + int64_t(r0 / 16) * 1024;
   }
   __device__ __forceinline__ void issue(uint32_t dst, int k0) const {
     const int l = threadIdx.x & 63, w = wave_id();
+    if (FOLD && k0 >= fold) k0 += kRestAt - fold;
     const i32x4 buf = make_rsrc(p + int64_t(k0 / 32) * nvc * 1024, ((C::BK / 32 - 1) * nvc + 16) * 1024);
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
@@ -177,6 +181,11 @@ template <typename C> struct PVocab {
     return join(read_tr(q + place * 16), read_tr(q + (place ^ 8) * 16));
   }
 };
+
+// What bf16 b leaves of p (nothing of what is no finite number)
+__device__ __forceinline__ bf16_t remainder(float p, uint32_t b) {
+  return f32_to_bf16((b & 0x7f80u) == 0x7f80u ? 0.f : p - __uint_as_float(b << 16));
+}
 
 template <int MB> __device__ __forceinline__ void zero(f32x16 (&acc)[MB][2]) {
 #pragma unroll
@@ -270,12 +279,17 @@ __global__ void __launch_bounds__(C::THREADS, C::BOUND) lce_z_kernel(LceArgs a, 
   bool live[2];
   lce_row_grads<C::MB, 2>(a, acc, vw, tw, count, live);
   const int nvc = a.vc / 16;
+  const bool few = count <= kFewRows;
+  if (few && tw >= kRestAt) return;  // (behind the last row; the remainders of the first take these places)
+  const int64_t rest = int64_t(kRestAt / 32) * nvc * 1024;
 #pragma unroll
   for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
     for (int mb = 0; mb < C::MB; ++mb)
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
+        char *blk = static_cast<char *>(a.p) +
+                    (int64_t(tw / 32 + nb) * nvc + (vw - a.v0) / 16 + 2 * mb + q) * 1024 + (l ^ (h << 2) ^ (q << 3)) * 16;
         uint32_t u[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -283,9 +297,15 @@ __global__ void __launch_bounds__(C::THREADS, C::BOUND) lce_z_kernel(LceArgs a, 
                  (static_cast<uint32_t>(f32_to_bf16(acc[mb][nb][8 * q + 2 * i + 1])) << 16);
           if (!live[nb]) u[i] = 0;
         }
-        char *blk = static_cast<char *>(a.p) +
-                    (int64_t(tw / 32 + nb) * nvc + (vw - a.v0) / 16 + 2 * mb + q) * 1024;
-        *reinterpret_cast<uint4 *>(blk + (l ^ (h << 2) ^ (q << 3)) * 16) = uint4{u[0], u[1], u[2], u[3]};
+        *reinterpret_cast<uint4 *>(blk) = uint4{u[0], u[1], u[2], u[3]};
+        if (!few || tw + 32 * nb >= kFewRows) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          u[i] = static_cast<uint32_t>(remainder(acc[mb][nb][8 * q + 2 * i], u[i] & 0xffffu)) |
+                 (static_cast<uint32_t>(remainder(acc[mb][nb][8 * q + 2 * i + 1], u[i] >> 16)) << 16);
+          if (!live[nb]) u[i] = 0;
+        }
+        *reinterpret_cast<uint4 *>(blk + rest) = uint4{u[0], u[1], u[2], u[3]};
       }
 }
 
@@ -322,13 +342,14 @@ __device__ __forceinline__ void dx_tile(const LceArgs &a, TilePos at, int share,
   }
 }
 
-template <typename C>
+template <typename C, bool FEW>
 __device__ __forceinline__ void dw_tile(const LceArgs &a, TilePos at, int count, char *lds) {
   const int r0 = at.m * C::TM, c0 = at.n * C::TN;
-  const PVocab<C> A(a.p, r0, a.vc);
-  const ColsK<C, C::TN> B(static_cast<const bf16_t *>(a.x) + c0, a.ldx, static_cast<int>(a.ldx) - c0, count);
+  const int fold = (count + C::BK - 1) / C::BK * C::BK;
+  const PVocab<C, FEW> A(a.p, r0, a.vc, fold);
+  const ColsK<C, C::TN, FEW> B(static_cast<const bf16_t *>(a.x) + c0, a.ldx, static_cast<int>(a.ldx) - c0, count, fold);
   f32x16 acc[4][2];
-  product<C>(A, B, 0, count, lds, acc);
+  product<C>(A, B, 0, FEW ? 2 * fold : count, lds, acc);
   const float f = lce_factor(a, count);
   const int l = threadIdx.x & 63, w = wave_id(), h = l >> 5;
   bf16_t *dw = static_cast<bf16_t *>(a.dw);
@@ -372,7 +393,9 @@ __global__ void __launch_bounds__(C::THREADS, C::BOUND) lce_products_kernel(LceA
     const int id = xcd_tile(b_dx, tiles * sh.n);
     dx_tile<C>(a, tile_at(id % tiles, xm, g.xn, 4), id / tiles, sh, lds);
   } else if (b_dw < g.wm * g.wn) {
-    dw_tile<C>(a, tile_at(xcd_tile(b_dw, g.wm * g.wn), g.wm, g.wn, 4), count, lds);
+    const TilePos at = tile_at(xcd_tile(b_dw, g.wm * g.wn), g.wm, g.wn, 4);
+    if (count <= kFewRows) dw_tile<C, true>(a, at, count, lds);
+    else dw_tile<C, false>(a, at, count, lds);
   }
 }
 

@@ -60,6 +60,13 @@ __device__ __forceinline__ void lse_merge(float &m, float &s, float m2, float s2
   m = top;
 }
 
+// bf16: P is rounded to bf16 for its products.  Over many rows those roundings add up to less than the results' own (dx and dw
+// are 1.15 to 1.35 times as far from 64 bits as without them); with a row or two they do not (up to 1.7 times).  Up to kFewRows
+// labelled rows, what the rounding left over takes the places kRestAt further on, as rows of its own, for which the tiles have
+// room (16 x 768 x 32000: 90 us with and without, 30 x 1024 x 40000: 115 and 108; up to 128 rows it would be 107 where 98 do
+// for 128 x 768 x 32000).
+constexpr int kFewRows = 32, kRestAt = 128;
+
 // dX in shares of a piece's vocabulary rows: `dx_splits` of [n_pad, d] partial sums, or (dx_tiles: the tiles of 256
 // that n_pad makes) as many of the labelled rows' as fit the same place.
 constexpr int kMaxShares = 32;

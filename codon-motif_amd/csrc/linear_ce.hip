@@ -211,18 +211,22 @@ __global__ void __launch_bounds__(256) lce_dx_rows_kernel(LceArgs a, T *dx, int 
     const DxShares sh = lce_dx_shares(a, count);
     const float *p = a.dx_part + int64_t(i) * a.d + c;
     const int64_t plane = sh.rows * a.d;
-#pragma unroll 8
-    for (int k = 0; k < sh.n; ++k) {
+    auto add = [&](const float *p) {
       float v[E];
       if (E == 4) {
-        const float4 u = *reinterpret_cast<const float4 *>(p + k * plane);
+        const float4 u = *reinterpret_cast<const float4 *>(p);
         v[0] = u.x, v[1 % E] = u.y, v[2 % E] = u.z, v[3 % E] = u.w;
       } else {
-        v[0] = p[k * plane];
+        v[0] = *p;
       }
 #pragma unroll
       for (int e = 0; e < E; ++e) s[e] += v[e];
-    }
+    };
+#pragma unroll 8
+    for (int k = 0; k < sh.n; ++k) add(p + k * plane);
+    if (a.dx_tiles && count <= kFewRows)  // (the rows of P's remainders)
+#pragma unroll 8
+      for (int k = 0; k < sh.n; ++k) add(p + k * plane + int64_t(kRestAt) * a.d);
 #pragma unroll
     for (int e = 0; e < E; ++e) s[e] *= f;
   }
