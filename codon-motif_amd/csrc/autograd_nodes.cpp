@@ -81,7 +81,7 @@ void *ptr(const Tensor &t) {
 Tensor given(const OptTensor &t) { return t.has_value() ? *t : Tensor(); }
 
 // t as it lies in memory: torch's negative views (the imaginary part of a conjugate, say) hold their sign beside it
-Tensor plain(const Tensor &t) { return t.defined() ? t.resolve_neg() : t; }
+Tensor plain(const Tensor &t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
 
 // ------------------------------------------------------------ row norms
 // x as rows of D: its stride where the leading dimensions lie regularly, else a contiguous copy

@@ -13,6 +13,8 @@ import torch.autograd.forward_ad as fwAD
 import torch.nn.functional as F
 
 _PROXY = torch._C._TorchDispatchModeKey.PROXY
+_tracing, _dispatch_mode, _transforms = (
+    torch._C._get_tracing_state, torch._C._get_dispatch_mode, torch._C._are_functorch_transforms_active)
 
 
 def wants_grad(*items) -> bool:
@@ -42,9 +44,9 @@ def refuse_transforms(what, *tensors):
     be lost: while torch.jit.trace or make_fx records (they would see an empty tensor), and for tensors
     of a function transform or with a forward-mode tangent (the result would come without it).
     None among `tensors` is skipped.'''
-    if torch._C._get_tracing_state() is not None or torch._C._get_dispatch_mode(_PROXY) is not None:
+    if _tracing() is not None or _dispatch_mode(_PROXY) is not None:
         raise NotImplementedError(f'{what}: the kernels cannot be traced')
-    if torch._C._are_functorch_transforms_active():
+    if _transforms():
         if any(t is not None and torch._C._functorch.is_functorch_wrapped_tensor(t) for t in tensors):
             raise NotImplementedError(f'{what}: not under a function transform')
     if fwAD._current_level >= 0:
