@@ -2,9 +2,10 @@
 // lce_internal.h.  A wave owns 128 x 64 of a product (8 matrix instructions for 6 LDS reads of 16 bytes a
 // lane), four or eight waves a tile of 256 x 128 or 256 x 256.  Both sides go straight from memory to LDS (16 bytes
 // a lane) in two or three stages of 32 or 64 k, one barrier a stage; LDS reads and writes meet no bank conflicts.
-// What bounds them: 4096 x 768 x 32000 reaches 860 (z with its epilogue) to 980 TFLOP/s (dX and dW) where the library's
-// bare products reach 920, 565 and 692; the clock falls to 1.75-2.1 GHz under them (matrix instructions busy 48-64% of
-// it), the loads alone take 300 of 415 us of dX and dW, the matrix instructions without loads 330.
+// What bounds them: at 4096 x 768 x 32000 z with its statistics reaches 850-910 TFLOP/s, with P 760-830, dX and dW 970-1020,
+// where the library's bare products reach 920, 565 and 692.  Each stage's latency and the epilogues: matrix instructions are
+// busy 52, 47 and 66% of the cycles, at a clock that falls to 1.75-2.1 GHz; the loads of dX and dW alone take 300 of 415 us, the
+// matrix instructions without loads 330.
 //
 //   z = W X^T    left: 256 vocabulary rows, right: 128 or 256 tokens; a lane holds one token's scores, so a
 //                row's maximum and sum are in-lane sums and one exchange

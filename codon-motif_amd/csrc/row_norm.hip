@@ -358,7 +358,8 @@ template <int E, typename F> bool with_shape(int D, F &&f) {
 
 template <int LPR> int rows_per_block() { return (LPR > 256 ? LPR : 256) / LPR; }
 
-// Workgroups of the backward: four or more rows each where there are enough
+// Workgroups of the backward: one for each set of rows that a workgroup takes at a time, at most kMaxGroups, which then go
+// through the sets in turn
 int bwd_groups(int rows, int rpb) {
   const int64_t blocks = (int64_t(rows) + rpb - 1) / rpb;
   return static_cast<int>(std::min<int64_t>(blocks, kMaxGroups));

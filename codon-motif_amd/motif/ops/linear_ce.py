@@ -30,7 +30,10 @@ def linear_cross_entropy(x, weight, labels, ignore_index=-100, reduction='mean')
 
     For the backward a copy of the labelled rows, the weight and 16 bytes a row are kept.  Its scratch
     is the gradient of the logits in pieces of the vocabulary (256 MB to 1 GB, or 4096 vocabulary
-    rows where that is more), and partial sums of x's gradient in fp32.'''
+    rows where that is more; for all rows, labelled or not), and partial sums of x's gradient in
+    fp32.  The forward's is two fp32 numbers for each row and 128 (bf16) or 32 (fp32) vocabulary rows.
+
+    In bf16 the logits' gradient is rounded to bf16 for its products, but for steps of up to 32 labelled rows.'''
     refuse_transforms('linear_cross_entropy', x, weight, labels)
     if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction must be 'none', 'sum' or 'mean', got {reduction!r}")

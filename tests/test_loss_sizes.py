@@ -34,3 +34,9 @@ def test_what_it_holds(N, d, V, dtype):
     # a forward has two numbers for each row and 128 (bf16) or 32 (fp32) words, a backward P of 256 words and dX once
     words = 128 if dtype else 32
     assert space[0] >= 8 * N * (V // words) and space[1] >= N * 256 * (2 if dtype else 4) + 4 * N * d
+
+
+def test_norm_workgroups():
+    '''A partial row for each of at most 512 workgroups, twice for LayerNorm.'''
+    need = _lib.lib().motif_row_norm_bwd_workspace_bytes
+    assert need(511, 64, 0) == 511 * 64 * 4 and need(10 ** 6, 64, 0) == 512 * 64 * 4 and need(2 ** 31 - 1, 16384, 1) == 2 * 512 * 16384 * 4
