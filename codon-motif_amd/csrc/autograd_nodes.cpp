@@ -80,8 +80,12 @@ void *ptr(const Tensor &t) {
 }
 Tensor given(const OptTensor &t) { return t.has_value() ? *t : Tensor(); }
 
-// t as it lies in memory: torch's negative views (the imaginary part of a conjugate, say) hold their sign beside it
-Tensor plain(const Tensor &t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+// t as it lies in memory: torch's negative views (the imaginary part of a conjugate, say) hold their sign beside it, its
+// zero tensors (which come up in derivatives) have no memory
+Tensor plain(const Tensor &t) {
+  if (!t.defined()) return t;
+  return t._is_zerotensor() ? t.clone() : t.is_neg() ? t.resolve_neg() : t;
+}
 
 // ------------------------------------------------------------ row norms
 // x as rows of D: its stride where the leading dimensions lie regularly, else a contiguous copy

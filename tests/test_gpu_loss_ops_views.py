@@ -70,3 +70,17 @@ def test_imaginary_parts_of_rows_of_one_feature():
     x = z.conj().imag
     assert x.is_neg()
     assert torch.equal(rms_norm_rows(x), rms_norm_rows(-z.imag)) and torch.equal(dropout_add(x, 0.0, 1), -z.imag)
+
+
+@pytest.mark.parametrize('op', [_rms, _layer, _module, _dropout, _loss])
+def test_zero_tensors(op):
+    '''torch's zeros without memory (they come up in its derivatives), as an input and as the gradient that comes in.'''
+    g = gen(4)
+    x, w, b, res = (torch.randn(s, generator=g).to(DEV) for s in ((20, 64), (64,), (64,), (20, 64)))
+    zero = torch._efficientzerotensor((20, 64), device=DEV)
+    assert torch.equal(op(x, w, b, zero), op(x, w, b, torch.zeros_like(x)))
+    assert torch.equal(op(zero, w, b, res), op(torch.zeros_like(x), w, b, res))
+    leaf = x.clone().requires_grad_()
+    y = op(leaf, w, b, res)
+    dx, = torch.autograd.grad(y, leaf, torch._efficientzerotensor(tuple(y.shape), device=DEV))
+    assert dx.shape == x.shape and not dx.any()
